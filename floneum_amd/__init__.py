@@ -105,6 +105,26 @@ class CRmsNorm(ctypes.Structure):
     _fields_ = [("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("dtype", ctypes.c_int), ("eps", ctypes.c_float)]
 
 
+class CQ8Tensor(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("offset", ctypes.c_uint64), ("scale_offset", ctypes.c_uint64),
+                ("shape", ctypes.c_uint32 * 4), ("stride", ctypes.c_int64 * 3), ("scale_stride", ctypes.c_int64 * 2),
+                ("block_tokens", ctypes.c_uint32), ("first", ctypes.c_uint32), ("format", ctypes.c_int)]
+
+
+class CQ8AppendArgs(ctypes.Structure):
+    _fields_ = [("k", CQ8Tensor), ("v", CQ8Tensor), ("row", ctypes.c_uint64), ("lens", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+                ("k_new", CTensor4), ("v_new", CTensor4), ("in_dtype", ctypes.c_int), ("rope", ctypes.POINTER(CRopeTables)),
+                ("k_norm", ctypes.POINTER(CRmsNorm)), ("q", CTensor4), ("q_out", CTensor4), ("q_dtype", ctypes.c_int),
+                ("q_out_dtype", ctypes.c_int), ("q_norm", ctypes.POINTER(CRmsNorm))]
+
+
+class CQ8AttnArgs(ctypes.Structure):
+    _fields_ = [("q", CTensor4), ("out", CTensor4), ("k", CQ8Tensor), ("v", CQ8Tensor), ("dtype", ctypes.c_int),
+                ("out_dtype", ctypes.c_int), ("scale", ctypes.c_float), ("mask_kind", ctypes.c_int), ("mask", CTensor2),
+                ("analytic", CAnalyticMask), ("kv_lens", ctypes.c_void_p), ("q_positions", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
 SYMBOLS = {
     "fhip_last_error": (ctypes.c_char_p, []),
     "fhip_version": (ctypes.c_char_p, []),
@@ -175,6 +195,17 @@ SYMBOLS = {
     "fhip_kv_cache_norm_rope_append": (ctypes.c_int, [_P, _P, ctypes.POINTER(CRmsNorm), ctypes.POINTER(CRopeTables),
                                                       ctypes.POINTER(CTensor4), ctypes.POINTER(CTensor4), ctypes.c_int,
                                                       ctypes.POINTER(CTensor4), ctypes.POINTER(CTensor4)]),
+    "fhip_q8_append": (ctypes.c_int, [_P, ctypes.POINTER(CQ8AppendArgs)]),
+    "fhip_q8_dequantize": (ctypes.c_int, [_P, ctypes.POINTER(CQ8Tensor), ctypes.c_uint64, _P, ctypes.POINTER(CTensor4), ctypes.c_int]),
+    "fhip_q8_attention_validate": (ctypes.c_int, [ctypes.POINTER(CQ8AttnArgs)]),
+    "fhip_q8_attention_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(CQ8AttnArgs), ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
+    "fhip_q8_attention": (ctypes.c_int, [_P, ctypes.POINTER(CQ8AttnArgs)]),
+    "fhip_q8_cache_create": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, _PP]),
+    "fhip_q8_cache_destroy": (ctypes.c_int, [_P]),
+    "fhip_q8_cache_reset": (ctypes.c_int, [_P]),
+    "fhip_q8_cache_current_seq_len": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_uint64)]),
+    "fhip_q8_cache_allocated_seq_len": (ctypes.c_int, [_P, ctypes.POINTER(ctypes.c_uint64)]),
+    "fhip_q8_cache_append": (ctypes.c_int, [_P, _P, ctypes.POINTER(CQ8AppendArgs), ctypes.POINTER(CQ8Tensor), ctypes.POINTER(CQ8Tensor)]),
 }
 
 _LIB = None
@@ -576,15 +607,22 @@ class Tensor:
 
     # -- the operator -------------------------------------------------------------------------------
     def flash_attention(self, k, v, scale, mask=None, *, analytic=None, kv_lens=None, out_dtype=None,
-                        force_kernel=KERNEL_AUTO, out=None):
+                        force_kernel=KERNEL_AUTO, out=None, q_positions=None):
         """fusor::Tensor<4,D>::flash_attention(&self, k, v, scale, mask) -> Self.
 
         self [B,H,Sq,D]; k, v [B,Hkv,Skv,D]; mask = None or (Tensor<2>, MaskKind).  Keyword-only
         arguments are the C ABI's extensions: `analytic` = (causal, q_pos_offset, window) or an
         AnalyticMask from MaskCache.get_analytic; `kv_lens` = device int32 [B] tensor of valid key
         counts; `out_dtype` F32 for 16-bit inputs.  Raises InvalidArgument (an AssertionError)
-        where the reference panics."""
+        where the reference panics.
+
+        k and v may be an 8-bit cache's (Q8Tensor): fhip_q8_attention, which also takes `q_positions`, a
+        device int32 [B] tensor added to the analytic mask's q_pos_offset, sequence by sequence."""
         L = _LIB or lib()
+        if type(k) is Q8Tensor or type(v) is Q8Tensor:
+            return _q8_attention(self, k, v, scale, mask, analytic, kv_lens, q_positions, out_dtype, force_kernel, out)
+        if q_positions is not None:
+            raise InvalidArgument(ERR_INVALID_ARG, "q_positions is for 8-bit keys and values")
         if _native is not None:
             done = _native.attention(self, k, v, scale, mask, analytic, kv_lens, out_dtype, force_kernel, out, Buffer)
             if done is not None:
@@ -885,6 +923,224 @@ def _kv_step(self, rope, q, k, v, start_pos, interleaved=False, q_norm=None, k_n
 
 
 KvCache.qkv_rope_append = _kv_step
+
+
+# ---- 8-bit key / value cache ----------------------------------------------------------------------------
+
+class Q8Format(enum.IntEnum):
+    """Codes of the 8-bit cache (fhip_q8_format)."""
+    INT8 = 0
+    E4M3 = 1
+
+
+def _q8_pitch(head_dim):
+    return (head_dim + 15) & ~15
+
+
+def _lens_ptr(t, batch, name):
+    if t is None:
+        return None
+    if t.dtype != "i32" or t.shape != (batch,):
+        raise InvalidArgument(ERR_INVALID_ARG, f"{name} is a device int32 tensor of the batch's size")
+    return t.buffer.ptr + t.offset * 4
+
+
+class Q8Tensor:
+    """Keys or values [batch, kv heads, rows, head_dim] in 8 bits (fhip_q8_tensor): a code per element and an f32 scale per
+    (batch, kv head, block of `block_tokens` rows).  `codes` and `scales` are buffers; strides and offset in bytes, of the scales in elements;
+    `first` is row 0's place in its block."""
+
+    __slots__ = ("codes", "scales", "shape", "format", "block_tokens", "strides", "offset", "scale_strides", "scale_offset", "first",
+                 "__weakref__")
+
+    def __init__(self, codes, scales, shape, format, block_tokens, strides=None, offset=0, scale_strides=None, scale_offset=0, first=0):
+        self.codes, self.scales = codes, scales
+        self.shape = tuple(map(int, shape))
+        self.format, self.block_tokens, self.first = Q8Format(format), int(block_tokens), int(first)
+        if strides is None or scale_strides is None:
+            _, heads, rows, dim = self.shape
+            pitch, blocks = _q8_pitch(dim), -(-rows // max(1, self.block_tokens))
+            strides = (heads * rows * pitch, rows * pitch, pitch) if strides is None else strides
+            scale_strides = (heads * blocks, blocks) if scale_strides is None else scale_strides
+        self.strides, self.scale_strides = tuple(map(int, strides)), tuple(map(int, scale_strides))
+        self.offset, self.scale_offset = int(offset), int(scale_offset)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @classmethod
+    def empty(cls, device, shape, format=Q8Format.INT8, block_tokens=1):
+        """Room for `shape` rows; all codes are 0, the scales too."""
+        batch, heads, rows, dim = map(int, shape)
+        n, blocks = batch * heads * rows * _q8_pitch(dim), batch * heads * -(-rows // max(1, block_tokens))
+        codes, scales = Buffer(device, n), Buffer(device, 4 * blocks)
+        for b, size in ((codes, n), (scales, 4 * blocks)):
+            if size:
+                check(lib().fhip_memset(device.stream, ctypes.c_void_p(b.ptr), 0, size))
+        return cls(codes, scales, shape, format, block_tokens)
+
+    def narrow(self, dim, start, length):
+        """Part of the batch (0), the heads (1) or the rows (2), without a copy."""
+        assert dim in (0, 1, 2) and 0 <= start and start + length <= self.shape[dim]
+        shape = list(self.shape)
+        shape[dim] = length
+        offset, scale_offset, first = self.offset + start * self.strides[dim], self.scale_offset, self.first
+        if dim == 2:
+            scale_offset += (first + start) // self.block_tokens
+            first = (first + start) % self.block_tokens
+        else:
+            scale_offset += start * self.scale_strides[dim]
+        return Q8Tensor(self.codes, self.scales, shape, self.format, self.block_tokens, self.strides, offset, self.scale_strides,
+                        scale_offset, first)
+
+    def _c(self):
+        t = CQ8Tensor(self.codes.ptr, self.scales.ptr, self.offset, self.scale_offset)
+        t.shape[:], t.stride[:], t.scale_stride[:] = self.shape, self.strides, self.scale_strides
+        t.block_tokens, t.first, t.format = self.block_tokens, self.first, int(self.format)
+        return t
+
+    def append(self, v_cache, k, v, row=0, *, lens=None, counts=None, rope=None, start_pos=0, interleaved=False, k_norm=None, q=None,
+               q_norm=None, q_out=None, q_out_dtype=None):
+        """New keys `k` into this tensor and new values `v` into `v_cache`, from row `row` on (fhip_q8_append): normalised (k_norm, an
+        RmsNorm) and rotated (rope, a RopeCache) on the way, the values as they are, and q, if given, normalised (q_norm) and rotated
+        into q_out, in one launch.  lens, counts: device int32 [B] tensors, see the C header.  Returns q_out (None without q)."""
+        a, q_out, keep = _q8_append_args(self.device, k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out, q_out_dtype)
+        a.k, a.v, a.row = self._c(), v_cache._c(), int(row)
+        check(lib().fhip_q8_append(self.device.stream, ctypes.byref(a)))
+        del keep
+        return q_out
+
+    def dequantize(self, out_dtype=F32, *, out=None, row=0, rows=None, lens=None):
+        """Rows row .. row + rows (of sequence b: row + lens[b] ..) as numbers of out_dtype (fhip_q8_dequantize)."""
+        if out is None:
+            count = self.shape[2] - row if rows is None else rows
+            out = Tensor.empty(self.device, (self.shape[0], self.shape[1], count, self.shape[3]), out_dtype)
+        elif rows is not None and rows != out.shape[2]:
+            raise InvalidArgument(ERR_INVALID_ARG, "rows differs from out's")
+        if out.device is not self.device:
+            raise AssertionError("Cannot mix tensors of different devices")
+        x, co = self._c(), out._c4()
+        check(lib().fhip_q8_dequantize(self.device.stream, ctypes.byref(x), int(row), _lens_ptr(lens, self.shape[0], "lens"),
+                                       ctypes.byref(co), out.dtype))
+        return out
+
+
+def _q8_append_args(device, k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out, q_out_dtype):
+    if k.dtype != v.dtype:
+        raise InvalidArgument(ERR_INVALID_ARG, "new keys and values must share one element type")
+    for t in (k, v, q, q_out):
+        if t is not None and t.device is not device:
+            raise AssertionError("Cannot mix tensors of different devices")
+    a = CQ8AppendArgs()
+    a.k_new, a.v_new, a.in_dtype = k._c4(), v._c4(), k.dtype
+    batch, keep = k.shape[0], []
+    a.lens, a.counts = _lens_ptr(lens, batch, "lens"), _lens_ptr(counts, batch, "counts")
+    if rope is not None:
+        keep.append(rope._tables(int(start_pos), interleaved))
+        a.rope = ctypes.pointer(keep[-1])
+    for name, norm in (("k_norm", k_norm), ("q_norm", q_norm)):
+        if norm is not None:
+            keep.append(norm._c())
+            setattr(a, name, ctypes.pointer(keep[-1]))
+    if q is not None:
+        if q_out is None:
+            q_out = Tensor.empty(device, q.shape, q.dtype if q_out_dtype is None else q_out_dtype)
+        a.q, a.q_out, a.q_dtype, a.q_out_dtype = q._c4(), q_out._c4(), q.dtype, q_out.dtype
+    elif q_out is not None or q_norm is not None:
+        raise InvalidArgument(ERR_INVALID_ARG, "q_out and q_norm need q")
+    return a, q_out, keep
+
+
+def _q8_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, out_dtype, force_kernel, out):
+    if type(k) is not Q8Tensor or type(v) is not Q8Tensor:
+        raise InvalidArgument(ERR_INVALID_ARG, "keys and values must both be 8-bit tensors")
+    if not (k.device is q.device and v.device is q.device):
+        raise AssertionError("Cannot mix tensors of different devices")
+    if len(q.shape) != 4:
+        raise InvalidArgument(ERR_INVALID_ARG, "flash_attention takes rank-4 tensors")
+    if force_kernel != KERNEL_AUTO:
+        raise InvalidArgument(ERR_INVALID_ARG, "force_kernel does not apply to 8-bit keys and values")
+    dev = q.device
+    if out is None:
+        out = Tensor.empty(dev, q.shape, q.dtype if out_dtype is None else out_dtype)
+    elif out_dtype is not None and out_dtype != out.dtype:
+        raise InvalidArgument(ERR_INVALID_ARG, "out_dtype differs from out's")
+    a = CQ8AttnArgs()
+    a.q, a.out, a.k, a.v = q._c4(), out._c4(), k._c(), v._c()
+    a.dtype, a.out_dtype, a.scale = q.dtype, out.dtype, float(np.float32(scale))
+    if mask is not None:
+        m, kind, *_ = mask  # (an interval table describes the mask for other kernels)
+        if m.device is not dev:
+            raise AssertionError("Mask must be on the same device as other tensors")
+        if m.dtype != q.dtype:
+            raise InvalidArgument(ERR_INVALID_ARG, "mask must have the element type of q")
+        a.mask, a.mask_kind = m._c2(), int(kind)
+    if isinstance(analytic, CAnalyticMask):
+        a.analytic = analytic
+    elif analytic is not None:
+        causal, off, window = analytic
+        a.analytic = CAnalyticMask(1, 1 if causal else 0, int(off), int(window or 0))
+    a.kv_lens, a.q_positions = _lens_ptr(kv_lens, q.shape[0], "kv_lens"), _lens_ptr(q_positions, q.shape[0], "q_positions")
+    need = ctypes.c_size_t()
+    check(lib().fhip_q8_attention_workspace_bytes(ctypes.byref(a), dev.compute_units, ctypes.byref(need)))
+    if need.value:
+        a.workspace, a.workspace_bytes = dev.workspace(need.value)
+    check(lib().fhip_q8_attention(dev.stream, ctypes.byref(a)))
+    return out
+
+
+class Q8KvCache:
+    """KvCache in 8 bits (fhip_q8_cache): append and qkv_rope_append return the whole cache as Q8Tensors, which
+    Tensor.flash_attention takes as keys and values."""
+
+    def __init__(self, concat_dim, max_sequence_len, format=Q8Format.INT8, block_tokens=1, device=None):
+        if concat_dim != 2:
+            raise FhipError(ERR_UNSUPPORTED, "the device KV cache concatenates along dim 2 ([B,Hkv,seq,D]), "
+                                             "the layout kalosm-llama uses")
+        self.device = device or Device.default()
+        h = ctypes.c_void_p()
+        check(lib().fhip_q8_cache_create(self.device.handle, int(format), block_tokens, max_sequence_len, ctypes.byref(h)))
+        self.handle = h
+
+    def __del__(self):
+        try:
+            if self.handle:
+                lib().fhip_q8_cache_destroy(self.handle)
+                self.handle = None
+        except Exception:
+            pass
+
+    def reset(self):
+        check(lib().fhip_q8_cache_reset(self.handle))
+
+    def current_seq_len(self):
+        n = ctypes.c_uint64()
+        check(lib().fhip_q8_cache_current_seq_len(self.handle, ctypes.byref(n)))
+        return n.value
+
+    def allocated_seq_len(self):
+        n = ctypes.c_uint64()
+        check(lib().fhip_q8_cache_allocated_seq_len(self.handle, ctypes.byref(n)))
+        return n.value
+
+    def _append(self, k, v, rope, start_pos, interleaved, k_norm, q, q_norm, q_out_dtype):
+        a, q_out, keep = _q8_append_args(self.device, k, v, None, None, rope, start_pos, interleaved, k_norm, q, q_norm, None, q_out_dtype)
+        ka, va = CQ8Tensor(), CQ8Tensor()
+        check(lib().fhip_q8_cache_append(self.handle, self.device.stream, ctypes.byref(a), ctypes.byref(ka), ctypes.byref(va)))
+        del keep
+        return (q_out, *(Q8Tensor(_View(self.device, c.codes, self), _View(self.device, c.scales, self), c.shape, c.format, c.block_tokens,
+                                  c.stride, c.offset, c.scale_stride, c.scale_offset, c.first) for c in (ka, va)))
+
+    def append(self, device, k, v):
+        return self._append(k, v, None, 0, False, None, None, None, None)[1:]
+
+    def append_rope(self, rope, k, v, start_pos, interleaved=False, k_norm=None):
+        return self._append(k, v, rope, start_pos, interleaved, k_norm, None, None, None)[1:]
+
+    def qkv_rope_append(self, rope, q, k, v, start_pos, interleaved=False, q_norm=None, k_norm=None, q_out_dtype=None):
+        """rope(norm(q)) and append(rope(norm(k)), v) in one launch; returns (q_rotated, k_all, v_all)."""
+        return self._append(k, v, rope, start_pos, interleaved, k_norm, q, q_norm, q_out_dtype)
 
 
 def base_inverse_frequency(dim, rope_theta):

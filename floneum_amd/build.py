@@ -9,7 +9,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ["api.hip", "attn_generic.hip", "attn_decode.hip", "attn_prefill_mfma.hip", "attn_prefill_mfma_wide.hip", "attn_prefill_mfma_rows32.hip", "attn_prefill_mfma_rows64.hip",
            "attn_prefill_f32.hip", "attn_prefill_f32_terms.hip",
-           "kv_cache.hip", "mask_intervals.hip", "rope.hip", "calibration.hip"]
+           "kv_cache.hip", "mask_intervals.hip", "rope.hip", "calibration.hip",
+           "api_q8.hip", "kv_q8.hip", "attn_q8_decode.hip"]
 LIB = os.path.join(HERE, "libfusor_hip.so")
 HOST = os.path.join(HERE, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))  # (no other interpreter takes it for its own)
 STATIC = os.path.join(HERE, "libfusor_hip.a")
@@ -20,7 +21,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", 
 
 
 # the rotary embedding must round every product and sum on its own (bit parity with the reference's CPU path)
-PER_FILE = {"rope.hip": ["-ffp-contract=off"]}
+PER_FILE = {"rope.hip": ["-ffp-contract=off"], "kv_q8.hip": ["-ffp-contract=off"]}
 
 
 def _compile(src):
@@ -49,13 +50,14 @@ def build(verbose=True):
     subprocess.check_call(["g++", "-std=c++17", "-O2", "-Wall", "-Wno-missing-field-initializers", "-fPIC", "-shared", "-fvisibility=hidden",
                            "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, "host_python.cpp"), "-o", HOST, "-L", HERE,
                            "-lfusor_hip", "-Wl,-rpath,$ORIGIN"])
-    # the C++ host mirror's test program (needs a GPU, started by tests/test_host_mirror_gpu.py)
+    # the C++ host mirror's test programs (need a GPU, started by tests/test_host_mirror_gpu.py and tests/test_q8_host_mirror_gpu.py)
     root = os.path.dirname(HERE)
-    cpp = os.path.join(root, "tests", "cpp", "test_host_mirror.cpp")
-    if os.path.exists(cpp):
-        subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-I", os.path.join(root, "include"), cpp,
-                               "-o", os.path.join(root, "tests", "cpp", "test_host_mirror"),
-                               "-L", HERE, "-lfusor_hip", "-Wl,-rpath,$ORIGIN/../../floneum_amd"])
+    for name in ("test_host_mirror", "test_host_mirror_q8"):
+        cpp = os.path.join(root, "tests", "cpp", name + ".cpp")
+        if os.path.exists(cpp):
+            subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-I", os.path.join(root, "include"), cpp,
+                                   "-o", os.path.join(root, "tests", "cpp", name),
+                                   "-L", HERE, "-lfusor_hip", "-Wl,-rpath,$ORIGIN/../../floneum_amd"])
     if verbose:
         print(f"built {LIB}")
     return LIB

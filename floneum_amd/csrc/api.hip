@@ -10,6 +10,7 @@
 
 #include "common.h"
 #include "decode_marks.h"
+#include "handles.h"
 
 // Workspace of fhip_flash_attention_noalloc: device memory the library itself holds, so that the call needs no
 // allocation by anyone.  Each GPU the library runs on has its own copy of the array at its own address, looked
@@ -19,22 +20,6 @@
 // to start at zero.
 constexpr size_t STATIC_WORKSPACE_BYTES = (size_t)FHIP_NOALLOC_WORKSPACE_BYTES;
 static __device__ __align__(256) unsigned char scratch[STATIC_WORKSPACE_BYTES];
-
-struct fhip_device {
-    int ordinal;
-    hipDeviceProp_t prop;
-    void *scratch_ptr;  // this device's address of `scratch`
-    // Sources of the per-call marks of masked prefill calls (AttnParams::bad_tag) and of decode calls (dec_tag): the state a
-    // device handle changes after its creation.
-    std::atomic<uint32_t> next_tag;
-    std::atomic<uint64_t> next_mark;
-    // The fused split-KV merge needs workgroups L of a one-dimensional launch with the same L % 8 to share an XCD (and
-    // with it an L2).  Probed once per handle.  `trip` is a word of pinned host memory the decode kernels set when the
-    // workgroups of a unit find themselves on different XCDs all the same: the next decode call then fails once and the
-    // form stays off for the handle.
-    std::atomic<bool> xcd_grouped;
-    int32_t *trip_host, *trip_dev;
-};
 
 // Do workgroups with the same number modulo 8 run on one XCD?  (The hardware deals the workgroups of a launch to its
 // XCDs round-robin in launch order, starting wherever the previous launch of the queue left off: true for 8, 4, 2 or 1
@@ -59,20 +44,6 @@ static void probe_xcd_grouping(fhip_device *d) {
     }
     d->xcd_grouped.store(true);
 }
-struct fhip_stream {
-    fhip_device *dev;
-    hipStream_t s;
-};
-struct fhip_event {
-    fhip_device *dev;
-    hipEvent_t e;
-};
-struct fhip_graph {
-    fhip_device *dev;
-    hipGraph_t graph;
-    hipGraphExec_t exec;
-};
-
 namespace fhip {
 
 static thread_local char g_err[512] = "";

@@ -452,6 +452,120 @@ int fhip_kv_cache_qkv_rope_append(fhip_kv_cache *c, fhip_stream *s, const fhip_r
                                   const fhip_tensor4 *k_new, const fhip_tensor4 *v_new, fhip_dtype in_dtype,
                                   fhip_tensor4 *k_all, fhip_tensor4 *v_all);
 
+/* ---- key / value cache in 8 bits -----------------------------------------------------------------
+ * The reference keeps its cache in the tensors' own type (fusor-ml/fusor/src/cache/kv_cache.rs:13-68); this is the same
+ * cache at a quarter of f32's bytes, half of f16's.  Rows are held as one code of 8 bits per element and one f32 scale per
+ * (tensor, batch, kv head, block of `block_tokens` rows); a row reads back as code * scale.
+ *   scale = max(largest |x| of the block's rows * (1 / largest code), 2^-100), in f32, the reciprocal rounded to f32 too
+ *   code  = the format's value nearest to x / scale (the exact quotient), ties to even
+ * with x the row in f32 (after the norm and the rotation).  Rows that join a block that holds earlier ones can only raise
+ * its scale; if they do, the earlier rows are coded again, from what they read back as (f32).  With block_tokens 1 that
+ * never happens and a row's codes depend on the row alone.  A NaN or an infinity in a row makes its block's scale NaN: the
+ * block's rows of that head read back as NaN, and so does attention that sees them, but not attention that masks them. */
+typedef enum {
+    FHIP_Q8_INT8 = 0, /* two's complement, -127..127                                                   */
+    FHIP_Q8_E4M3 = 1  /* float of 4 exponent and 3 mantissa bits, no infinities, largest 448: for rows whose largest element
+                         is far from the rest                                                          */
+} fhip_q8_format;
+
+/* View [batch, kv heads, rows, head_dim] of such a cache.  Code (b,h,r,d) is the byte
+ * codes[offset + b*stride[0] + h*stride[1] + r*stride[2] + d], its scale
+ * scales[scale_offset + b*scale_stride[0] + h*scale_stride[1] + (first + r) / block_tokens].
+ * Rows are read in pieces of 16 bytes: codes + offset and the strides are multiples of 16, and the bytes from head_dim up to the
+ * next multiple of 16 are zero (nothing here writes them).  head_dim: a multiple of 8 up to 256. */
+typedef struct {
+    void *codes;
+    void *scales;            /* f32                                                                    */
+    uint64_t offset;         /* bytes                                                                  */
+    uint64_t scale_offset;   /* elements                                                               */
+    uint32_t shape[4];
+    int64_t stride[3];       /* bytes: batch, head, row                                                */
+    int64_t scale_stride[2]; /* elements: batch, head                                                  */
+    uint32_t block_tokens;   /* 1, 8, 16, 32 or 64                                                     */
+    uint32_t first;          /* place of row 0 in its block, < block_tokens                            */
+    fhip_q8_format format;
+} fhip_q8_tensor;
+
+/* Arguments of fhip_q8_append.  Zero-initialise, then fill. */
+typedef struct {
+    fhip_q8_tensor k;             /* where the rows go: the whole memory that may be written             */
+    fhip_q8_tensor v;
+    uint64_t row;                 /* place of the first new row                                        */
+    const int32_t *lens;          /* optional device [B]: sequence b's first new row goes to row + lens[b], and its position in
+                                     the rotation is moved by lens[b] too (a batch whose sequences hold different numbers of
+                                     tokens; the contents may change between replays of a graph)       */
+    const int32_t *counts;        /* optional device [B]: sequence b brings only its first counts[b] new rows */
+    fhip_tensor4 k_new;           /* [B, Hkv, n, D] of in_dtype, any strides                            */
+    fhip_tensor4 v_new;
+    fhip_dtype in_dtype;
+    const fhip_rope_tables *rope; /* NULL: keys (and q) are not rotated                                */
+    const fhip_rms_norm *k_norm;  /* NULL: keys are not normalised                                     */
+    fhip_tensor4 q;               /* q.ptr NULL: none.  [B, H, n, D]: normalised and rotated on the way, as fhip_norm_rope does */
+    fhip_tensor4 q_out;           /* the same shape; may be q                                          */
+    fhip_dtype q_dtype;
+    fhip_dtype q_out_dtype;
+    const fhip_rms_norm *q_norm;
+} fhip_q8_append_args;
+
+/* One step's preparation in ONE launch: the new keys normalised, rotated and written to the cache in 8 bits, the new values
+ * likewise without norm and rotation, q normalised and rotated into q_out (the counterpart of fhip_kv_cache_qkv_rope_append).  Keys that
+ * were rotated and normalised are the f32 values that call rounds to its cache's type.  Rows whose place lies outside the view, or whose
+ * position outside the tables, are left out (with `lens` only the device knows them), and so are rows from counts[b] on: neither the
+ * cache nor q_out is written there.  Rows of a block behind the new ones count as absent: what they held is lost with the
+ * scale.  Asynchronous on `s`; may be captured. */
+int fhip_q8_append(fhip_stream *s, const fhip_q8_append_args *args);
+
+/* out[b,h,i,:] = row `row` + lens[b] + i of x (lens NULL: row + i), code * scale in f32, rounded to out_dtype.  out: [B, Hkv, n, D], any
+ * strides.  Rows outside the view are left out: out is not written there.  Asynchronous on `s`; may be captured. */
+int fhip_q8_dequantize(fhip_stream *s, const fhip_q8_tensor *x, uint64_t row, const int32_t *lens, const fhip_tensor4 *out,
+                       fhip_dtype out_dtype);
+
+/* Arguments of one attention call over an 8-bit cache.  Zero-initialise, then fill. */
+typedef struct {
+    fhip_tensor4 q;          /* [B, H,   Sq,  D] of dtype, any strides                                  */
+    fhip_tensor4 out;        /* the same shape, of out_dtype (dtype, or FHIP_F32)                       */
+    fhip_q8_tensor k;        /* [B, Hkv, Skv, D]; v: the same shape, format and block_tokens             */
+    fhip_q8_tensor v;
+    fhip_dtype dtype;
+    fhip_dtype out_dtype;
+    float scale;
+    fhip_mask_kind mask_kind;
+    fhip_tensor2 mask;       /* of dtype, added to the scores as in fhip_flash_attention                */
+    fhip_analytic_mask analytic;
+    const int32_t *kv_lens;     /* optional device [B], as in fhip_attn_args                            */
+    const int32_t *q_positions; /* optional device [B]: added to analytic.q_pos_offset for sequence b (sequences of different
+                                   lengths under a causal mask or a window; the contents may change between replays) */
+    void *workspace;
+    size_t workspace_bytes;
+} fhip_q8_attn_args;
+
+/* Host-only check of the arguments: the status and message that fhip_q8_attention would return. */
+int fhip_q8_attention_validate(const fhip_q8_attn_args *args);
+/* Bytes of device workspace (16-byte aligned) the call needs on a device of `compute_units`; 0: none. */
+int fhip_q8_attention_workspace_bytes(const fhip_q8_attn_args *args, int32_t compute_units, size_t *bytes);
+/* out = softmax(q k^T * scale + mask) v over the values that k and v stand for, with the head mapping, masks and special
+ * cases of fhip_flash_attention: rows whose keys are all masked come out NaN, no keys at all give zeros.  Scores, softmax
+ * statistics and sums are f32; codes enter the matrix products exactly, f32 queries and probabilities as two 16-bit terms
+ * each (f32 precision), 16-bit queries exactly and their probabilities rounded to 11 bits.  Rows of the cache that a mask hides by
+ * position or length may hold anything.  Asynchronous on `s`; may be captured. */
+int fhip_q8_attention(fhip_stream *s, const fhip_q8_attn_args *args);
+
+/* Growable 8-bit cache of keys and values: fhip_kv_cache with the same observable lengths and growth (the allocation grows to
+ * the next power of two; beyond max_sequence_len only the last max_sequence_len rows stay), k_all / v_all being 8-bit views. */
+typedef struct fhip_q8_cache fhip_q8_cache;
+int fhip_q8_cache_create(fhip_device *dev, fhip_q8_format format, uint32_t block_tokens, uint64_t max_sequence_len,
+                         fhip_q8_cache **out);
+int fhip_q8_cache_destroy(fhip_q8_cache *c);
+/* The cache is empty again; its memory stays with it, as in fhip_kv_cache_reset. */
+int fhip_q8_cache_reset(fhip_q8_cache *c);
+int fhip_q8_cache_current_seq_len(const fhip_q8_cache *c, uint64_t *len);
+int fhip_q8_cache_allocated_seq_len(const fhip_q8_cache *c, uint64_t *len);
+/* Appends args->k_new / v_new (rotated, normalised, with q, as fhip_q8_append does; args->k, v and row are the cache's own and
+ * ignored, lens and counts must be NULL).  k_all / v_all: views of all rows, valid until the next append / reset / destroy.  An append
+ * that fails leaves the cache as it was.  An append that grows or moves the rows cannot be captured when it allocates. */
+int fhip_q8_cache_append(fhip_q8_cache *c, fhip_stream *s, const fhip_q8_append_args *args, fhip_q8_tensor *k_all,
+                         fhip_q8_tensor *v_all);
+
 /* Library version string, e.g. "fusor-hip 0.1 (gfx950)". */
 const char *fhip_version(void);
 

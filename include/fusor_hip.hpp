@@ -434,6 +434,104 @@ class KvCache {
     }
 };
 
+/// Codes of the 8-bit cache (fhip_q8_format)
+enum class Q8Format { INT8 = FHIP_Q8_INT8, E4M3 = FHIP_Q8_E4M3 };
+
+/// Keys or values in 8 bits: a view of codes and scales that a Q8KvCache owns.
+class Q8Tensor {
+    Device dev_;
+    fhip_q8_tensor view_;
+    std::shared_ptr<void> keepalive_;
+
+   public:
+    Q8Tensor(const Device &dev, const fhip_q8_tensor &view, std::shared_ptr<void> keepalive)
+        : dev_(dev), view_(view), keepalive_(std::move(keepalive)) {}
+    const uint32_t *shape() const { return view_.shape; }
+    const Device &device() const { return dev_; }
+    const fhip_q8_tensor &c() const { return view_; }
+    /// the rows as numbers of type `dt`
+    Tensor<4> dequantize(DType dt = DType::F32) const {
+        Tensor<4> out = Tensor<4>::empty(dev_, dt, view_.shape);
+        const fhip_tensor4 o = out.c4();
+        check(fhip_q8_dequantize(dev_.stream(), &view_, 0, nullptr, &o, (fhip_dtype)dt));
+        return out;
+    }
+};
+
+/// KvCache in 8 bits (fhip_q8_cache).
+class Q8KvCache {
+    struct Inner {
+        fhip_q8_cache *c = nullptr;
+        ~Inner() {
+            if (c) fhip_q8_cache_destroy(c);
+        }
+    };
+    std::shared_ptr<Inner> in_;
+    Device dev_;
+
+   public:
+    Q8KvCache(const Device &dev, int concat_dim, uint64_t max_sequence_len, Q8Format format = Q8Format::INT8, uint32_t block_tokens = 1)
+        : in_(std::make_shared<Inner>()), dev_(dev) {
+        if (concat_dim != 2) throw GpuError("the device KV cache concatenates [B, Hkv, seq, D] along dim 2");
+        check(fhip_q8_cache_create(dev.handle(), (fhip_q8_format)format, block_tokens, max_sequence_len, &in_->c));
+    }
+    void reset() { check(fhip_q8_cache_reset(in_->c)); }
+    uint64_t current_seq_len() const {
+        uint64_t n;
+        check(fhip_q8_cache_current_seq_len(in_->c, &n));
+        return n;
+    }
+    /// append(k, v) with the keys normalised (k_norm) and rotated (tables) on the way, and q, if given, normalised and rotated into q_out,
+    /// in one launch; returns (k_all, v_all)
+    std::pair<Q8Tensor, Q8Tensor> append(const Tensor<4> &k, const Tensor<4> &v, const fhip_rope_tables *tables = nullptr,
+                                         const fhip_rms_norm *k_norm = nullptr, const Tensor<4> *q = nullptr, Tensor<4> *q_out = nullptr,
+                                         const fhip_rms_norm *q_norm = nullptr) {
+        if (k.dtype() != v.dtype()) throw Panic("append: keys and values differ in element type");
+        if ((q == nullptr) != (q_out == nullptr)) throw Panic("append: q and q_out come together");
+        fhip_q8_append_args a{};
+        a.k_new = k.c4(), a.v_new = v.c4();
+        a.in_dtype = (fhip_dtype)k.dtype();
+        a.rope = tables, a.k_norm = k_norm, a.q_norm = q_norm;
+        if (q) a.q = q->c4(), a.q_out = q_out->c4(), a.q_dtype = (fhip_dtype)q->dtype(), a.q_out_dtype = (fhip_dtype)q_out->dtype();
+        fhip_q8_tensor ka{}, va{};
+        check(fhip_q8_cache_append(in_->c, dev_.stream(), &a, &ka, &va));
+        return {Q8Tensor(dev_, ka, in_), Q8Tensor(dev_, va, in_)};
+    }
+};
+
+/// q.flash_attention(k, v, scale, mask) over an 8-bit cache's keys and values (fhip_q8_attention)
+inline Tensor<4> flash_attention(const Tensor<4> &q, const Q8Tensor &k, const Q8Tensor &v, float scale,
+                                 std::optional<std::pair<const Tensor<2> *, MaskKind>> mask = std::nullopt,
+                                 const fhip_analytic_mask *analytic = nullptr, const int32_t *kv_lens = nullptr,
+                                 const int32_t *q_positions = nullptr) {
+    const Device &dev = q.device();
+    if (!dev.same(k.device()) || !dev.same(v.device())) throw Panic("Cannot mix tensors of different devices");
+    uint32_t shape[4];
+    for (int i = 0; i < 4; i++) shape[i] = q.shape()[i];
+    Tensor<4> out = Tensor<4>::empty(dev, q.dtype(), shape);
+    fhip_q8_attn_args a{};
+    a.q = q.c4(), a.out = out.c4(), a.k = k.c(), a.v = v.c();
+    a.dtype = a.out_dtype = (fhip_dtype)q.dtype();
+    a.scale = scale;
+    if (mask) {
+        if (!dev.same(mask->first->device())) throw Panic("Mask must be on the same device as other tensors");
+        if (mask->first->dtype() != q.dtype()) throw Panic("mask must have the element type of q");
+        a.mask = mask->first->c2();
+        a.mask_kind = (fhip_mask_kind)mask->second;
+    }
+    if (analytic) a.analytic = *analytic;
+    a.kv_lens = kv_lens;
+    a.q_positions = q_positions;
+    size_t need = 0;
+    check(fhip_q8_attention_workspace_bytes(&a, dev.info().compute_units, &need));
+    if (need) {
+        a.workspace = dev.workspace(need);
+        a.workspace_bytes = dev.workspace_bytes();
+    }
+    check(fhip_q8_attention(dev.stream(), &a));
+    return out;
+}
+
 /// fusor::RopeCache (fusor-ml/fusor/src/composite/rope.rs:180-265): [context_length, head_dim/2] f32
 /// cos/sin tables on the device, applied by one fused kernel per tensor.
 class RopeCache {

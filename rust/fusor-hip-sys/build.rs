@@ -24,6 +24,9 @@ const SOURCES: &[&str] = &[
     "mask_intervals.hip",
     "rope.hip",
     "calibration.hip",
+    "api_q8.hip",
+    "kv_q8.hip",
+    "attn_q8_decode.hip",
 ];
 
 // the flags floneum_amd/build.py uses; packed-f32 VALU forms are kept out of the generated code on purpose
@@ -54,7 +57,7 @@ fn compile(root: &Path, out_dir: &Path) {
         let obj = out_dir.join(src.replace(".hip", ".o"));
         let mut cmd = Command::new(&hipcc);
         cmd.args(FLAGS);
-        if *src == "rope.hip" {
+        if *src == "rope.hip" || *src == "kv_q8.hip" {
             // the rotary embedding rounds every product and sum on its own (bit parity with fusor's CPU ops)
             cmd.arg("-ffp-contract=off");
         }

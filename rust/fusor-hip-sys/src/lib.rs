@@ -41,6 +41,10 @@ pub struct fhip_graph {
 pub struct fhip_kv_cache {
     _private: [u8; 0],
 }
+#[repr(C)]
+pub struct fhip_q8_cache {
+    _private: [u8; 0],
+}
 
 // ---- enums (C enums without negative values: `unsigned int`) ------------------------------------
 /// Element types (reference: `DataTypeEnum`, fusor-ml/core/src/tensor.rs:110-134).
@@ -136,6 +140,70 @@ pub struct fhip_decode_plan_info {
     pub chunk: i32,
     pub wavefronts: i32,
     pub kernels: i32,
+}
+
+/// Codes of the 8-bit cache.
+pub type fhip_q8_format = c_uint;
+/// Two's complement, -127..127.
+pub const FHIP_Q8_INT8: fhip_q8_format = 0;
+/// Float of 4 exponent and 3 mantissa bits, largest 448.
+pub const FHIP_Q8_E4M3: fhip_q8_format = 1;
+
+/// View `[batch, kv heads, rows, head_dim]` of an 8-bit cache: codes (strides and offset in bytes) and f32 scales.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct fhip_q8_tensor {
+    pub codes: *mut c_void,
+    pub scales: *mut c_void,
+    pub offset: u64,
+    pub scale_offset: u64,
+    pub shape: [u32; 4],
+    pub stride: [i64; 3],
+    pub scale_stride: [i64; 2],
+    pub block_tokens: u32,
+    pub first: u32,
+    pub format: fhip_q8_format,
+}
+
+/// Arguments of `fhip_q8_append`.  Zero-initialise, then fill.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct fhip_q8_append_args {
+    pub k: fhip_q8_tensor,
+    pub v: fhip_q8_tensor,
+    pub row: u64,
+    pub lens: *const i32,
+    pub counts: *const i32,
+    pub k_new: fhip_tensor4,
+    pub v_new: fhip_tensor4,
+    pub in_dtype: fhip_dtype,
+    pub rope: *const fhip_rope_tables,
+    pub k_norm: *const fhip_rms_norm,
+    pub q: fhip_tensor4,
+    pub q_out: fhip_tensor4,
+    pub q_dtype: fhip_dtype,
+    pub q_out_dtype: fhip_dtype,
+    pub q_norm: *const fhip_rms_norm,
+}
+
+/// Arguments of one attention call over an 8-bit cache.  Zero-initialise, then fill.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct fhip_q8_attn_args {
+    pub q: fhip_tensor4,
+    pub out: fhip_tensor4,
+    pub k: fhip_q8_tensor,
+    pub v: fhip_q8_tensor,
+    pub dtype: fhip_dtype,
+    pub out_dtype: fhip_dtype,
+    pub scale: f32,
+    pub mask_kind: fhip_mask_kind,
+    pub mask: fhip_tensor2,
+    pub analytic: fhip_analytic_mask,
+    pub kv_lens: *const i32,
+    pub q_positions: *const i32,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: usize,
 }
 
 #[repr(C)]
@@ -365,6 +433,38 @@ unsafe extern "C" {
         v_all: *mut fhip_tensor4,
     ) -> c_int;
 
+    // 8-bit KV cache
+    pub fn fhip_q8_append(s: *mut fhip_stream, args: *const fhip_q8_append_args) -> c_int;
+    pub fn fhip_q8_dequantize(
+        s: *mut fhip_stream,
+        x: *const fhip_q8_tensor,
+        row: u64,
+        lens: *const i32,
+        out: *const fhip_tensor4,
+        out_dtype: fhip_dtype,
+    ) -> c_int;
+    pub fn fhip_q8_attention_validate(args: *const fhip_q8_attn_args) -> c_int;
+    pub fn fhip_q8_attention_workspace_bytes(args: *const fhip_q8_attn_args, compute_units: i32, bytes: *mut usize) -> c_int;
+    pub fn fhip_q8_attention(s: *mut fhip_stream, args: *const fhip_q8_attn_args) -> c_int;
+    pub fn fhip_q8_cache_create(
+        dev: *mut fhip_device,
+        format: fhip_q8_format,
+        block_tokens: u32,
+        max_sequence_len: u64,
+        out: *mut *mut fhip_q8_cache,
+    ) -> c_int;
+    pub fn fhip_q8_cache_destroy(c: *mut fhip_q8_cache) -> c_int;
+    pub fn fhip_q8_cache_reset(c: *mut fhip_q8_cache) -> c_int;
+    pub fn fhip_q8_cache_current_seq_len(c: *const fhip_q8_cache, len: *mut u64) -> c_int;
+    pub fn fhip_q8_cache_allocated_seq_len(c: *const fhip_q8_cache, len: *mut u64) -> c_int;
+    pub fn fhip_q8_cache_append(
+        c: *mut fhip_q8_cache,
+        s: *mut fhip_stream,
+        args: *const fhip_q8_append_args,
+        k_all: *mut fhip_q8_tensor,
+        v_all: *mut fhip_q8_tensor,
+    ) -> c_int;
+
     pub fn fhip_version() -> *const c_char;
 }
 
@@ -378,4 +478,7 @@ const _: () = {
     assert!(core::mem::size_of::<fhip_decode_plan_info>() == 20);
     assert!(core::mem::size_of::<fhip_rope_tables>() == 40);
     assert!(core::mem::size_of::<fhip_rms_norm>() == 24);
+    assert!(core::mem::size_of::<fhip_q8_tensor>() == 104);
+    assert!(core::mem::size_of::<fhip_q8_append_args>() == 528);
+    assert!(core::mem::size_of::<fhip_q8_attn_args>() == 448);
 };

@@ -8,7 +8,8 @@
 //!     `TensorLayoutInfo` already has (fusor-ml/core/src/mir/inputs.rs:164-173, fusor-ml/types/src/layout.rs:88-129);
 //!   * [`HipTensor::flash_attention`]: same signature as `fusor_core::Tensor::flash_attention`
 //!     (fusor-ml/core/src/composite/flash_attention.rs:28-52), plus `MaskKind::BatchKeyMask` natively;
-//!   * [`KvCache`], [`MaskCache`]: device-side counterparts of fusor-ml/fusor/src/cache/{kv_cache,mask_cache}.rs.
+//!   * [`KvCache`], [`MaskCache`]: device-side counterparts of fusor-ml/fusor/src/cache/{kv_cache,mask_cache}.rs;
+//!   * [`Q8KvCache`], [`HipTensor::flash_attention_q8`]: the cache in 8 bits and attention over it (no counterpart there).
 //!
 //! Failures that are `assert!` panics in the reference (head divisibility, mask shape) panic here with the same
 //! text, so `#[should_panic(expected = ...)]` tests keep holding; HIP failures are `Error::Hip`.
@@ -366,6 +367,47 @@ impl<D: HipDataType> HipTensor<4, D> {
         check(unsafe { fhip_flash_attention(dev.stream(), &a) }).expect("flash_attention");
         out
     }
+
+    /// [`HipTensor::flash_attention`] over an 8-bit cache's keys and values (`fhip_q8_attention`).
+    pub fn flash_attention_q8(&self, k: &Q8Tensor, v: &Q8Tensor, scale: f32, mask: Option<(&HipTensor<2, D>, MaskKind)>) -> Self {
+        let dev = self.device().clone();
+        let out = Self::uninit(&dev, self.shape).expect("output allocation");
+        let mut a: fhip_q8_attn_args = unsafe { std::mem::zeroed() };
+        a.q = self.as_ffi();
+        a.out = out.as_ffi();
+        a.k = k.view;
+        a.v = v.view;
+        a.dtype = D::FHIP_DTYPE;
+        a.out_dtype = D::FHIP_DTYPE;
+        a.scale = scale;
+        if let Some((m, kind)) = mask {
+            match m.analytic {
+                Some(desc) if kind == MaskKind::QKMask => a.analytic = desc,
+                _ => {
+                    a.mask = m.as_ffi();
+                    a.mask_kind = kind.ffi();
+                }
+            }
+        }
+        let mut need = 0usize;
+        check(unsafe { fhip_q8_attention_workspace_bytes(&a, dev.compute_units(), &mut need) }).expect("workspace query");
+        let mut ws = dev.0.workspace.lock().unwrap();
+        if need > ws.1 {
+            unsafe {
+                if !ws.0.is_null() {
+                    fhip_stream_synchronize(dev.stream());
+                    fhip_free(dev.raw(), ws.0);
+                }
+                let mut p = ptr::null_mut();
+                check(fhip_malloc(dev.raw(), need, &mut p)).expect("workspace allocation");
+                *ws = (p, need);
+            }
+        }
+        a.workspace = ws.0;
+        a.workspace_bytes = ws.1;
+        check(unsafe { fhip_q8_attention(dev.stream(), &a) }).expect("flash_attention_q8");
+        out
+    }
 }
 
 impl<D: HipDataType> HipTensor<2, D> {
@@ -454,6 +496,79 @@ impl<D> Drop for KvCache<D> {
         unsafe {
             fhip_stream_synchronize(self.device.stream());
             fhip_kv_cache_destroy(self.raw);
+        }
+    }
+}
+
+/// Codes of the 8-bit cache.
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum Q8Format {
+    Int8,
+    E4m3,
+}
+
+/// Keys or values in 8 bits: a view into a [`Q8KvCache`], valid until its next append / reset.
+#[derive(Clone)]
+pub struct Q8Tensor {
+    device: Device,
+    view: fhip_q8_tensor,
+}
+
+impl Q8Tensor {
+    pub fn shape(&self) -> [usize; 4] {
+        self.view.shape.map(|x| x as usize)
+    }
+    /// The rows as numbers.
+    pub fn dequantize<D: HipDataType>(&self) -> Result<HipTensor<4, D>> {
+        let out = HipTensor::<4, D>::uninit(&self.device, self.shape())?;
+        let o = out.as_ffi();
+        check(unsafe { fhip_q8_dequantize(self.device.stream(), &self.view, 0, ptr::null(), &o, D::FHIP_DTYPE) })?;
+        Ok(out)
+    }
+}
+
+/// [`KvCache`] in 8 bits, with one scale per head and block of `block_tokens` rows.
+pub struct Q8KvCache {
+    device: Device,
+    raw: *mut fhip_q8_cache,
+}
+unsafe impl Send for Q8KvCache {}
+
+impl Q8KvCache {
+    pub fn new(device: &Device, max_sequence_len: usize, format: Q8Format, block_tokens: u32) -> Result<Self> {
+        let mut raw = ptr::null_mut();
+        let format = match format {
+            Q8Format::Int8 => FHIP_Q8_INT8,
+            Q8Format::E4m3 => FHIP_Q8_E4M3,
+        };
+        check(unsafe { fhip_q8_cache_create(device.raw(), format, block_tokens, max_sequence_len as u64, &mut raw) })?;
+        Ok(Q8KvCache { device: device.clone(), raw })
+    }
+    pub fn reset(&mut self) -> Result<()> {
+        check(unsafe { fhip_q8_cache_reset(self.raw) })
+    }
+    pub fn current_seq_len(&self) -> usize {
+        let mut n = 0u64;
+        unsafe { fhip_q8_cache_current_seq_len(self.raw, &mut n) };
+        n as usize
+    }
+    /// Appends `[B, Hkv, n, D]` rows and returns the cached keys and values including them.
+    pub fn append<D: HipDataType>(&mut self, k: &HipTensor<4, D>, v: &HipTensor<4, D>) -> Result<(Q8Tensor, Q8Tensor)> {
+        let mut a: fhip_q8_append_args = unsafe { std::mem::zeroed() };
+        a.k_new = k.as_ffi();
+        a.v_new = v.as_ffi();
+        a.in_dtype = D::FHIP_DTYPE;
+        let mut k_all: fhip_q8_tensor = unsafe { std::mem::zeroed() };
+        let mut v_all: fhip_q8_tensor = unsafe { std::mem::zeroed() };
+        check(unsafe { fhip_q8_cache_append(self.raw, self.device.stream(), &a, &mut k_all, &mut v_all) })?;
+        Ok((Q8Tensor { device: self.device.clone(), view: k_all }, Q8Tensor { device: self.device.clone(), view: v_all }))
+    }
+}
+impl Drop for Q8KvCache {
+    fn drop(&mut self) {
+        unsafe {
+            fhip_stream_synchronize(self.device.stream());
+            fhip_q8_cache_destroy(self.raw);
         }
     }
 }
