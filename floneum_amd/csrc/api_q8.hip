@@ -298,6 +298,8 @@ static void fill_attention(const fhip_q8_attn_args *a, int cus, Q8AttnParams *p)
     p->q = (const char *)a->q.ptr + a->q.offset * (uint64_t)bytes_of(a->dtype);
     p->out = (char *)a->out.ptr + a->out.offset * (uint64_t)bytes_of(a->out_dtype);
     for (int i = 0; i < 4; i++) p->qs[i] = a->q.stride[i], p->os[i] = a->out.stride[i];
+    p->q_vec = fours(a->q, bytes_of(a->dtype));
+    p->out_vec = fours(a->out, bytes_of(a->out_dtype));
     p->q_dtype = a->dtype;
     p->out_dtype = a->out_dtype;
     p->k = view_of(a->k), p->v = view_of(a->v);
@@ -319,6 +321,11 @@ static void fill_attention(const fhip_q8_attn_args *a, int cus, Q8AttnParams *p)
     }
     p->scale = a->scale;
     p->cus = cus > 0 ? cus : 256;
+}
+
+// Few columns ((query row, head of the group) pairs) per KV head: the kernel that streams the codes into registers.
+static Q8AttnPlan attention_plan(const Q8AttnParams &p) {
+    return (int64_t)p.G * p.Sq <= 32 ? q8_decode_plan(p) : q8_prefill_plan(p);
 }
 
 }  // namespace fhip
@@ -394,7 +401,7 @@ int fhip_q8_attention_workspace_bytes(const fhip_q8_attn_args *args, int32_t com
     if (rc || empty(args->q.shape) || args->k.shape[2] == 0) return rc;
     Q8AttnParams p;
     fill_attention(args, compute_units, &p);
-    *bytes = q8_decode_plan(p).bytes;
+    *bytes = attention_plan(p).bytes;
     return FHIP_OK;
 }
 
@@ -409,7 +416,7 @@ int fhip_q8_attention(fhip_stream *s, const fhip_q8_attn_args *args) {
     }
     Q8AttnParams p;
     fill_attention(args, s->dev->prop.multiProcessorCount, &p);
-    const Q8AttnPlan plan = q8_decode_plan(p);
+    const Q8AttnPlan plan = attention_plan(p);
     if (plan.bytes && (!args->workspace || ((uintptr_t)args->workspace & 15) != 0 || args->workspace_bytes < plan.bytes)) {
         set_error("q8_attention: needs %zu bytes of 16-byte aligned workspace, got %zu", plan.bytes, args->workspace ? args->workspace_bytes : 0);
         return FHIP_ERR_WORKSPACE;
@@ -417,7 +424,7 @@ int fhip_q8_attention(fhip_stream *s, const fhip_q8_attn_args *args) {
     p.nsplit = plan.nsplit;
     p.min_chunk = plan.min_chunk;
     p.partials = (float *)args->workspace;
-    return launch_q8_decode(p, plan, s->s);
+    return plan.prefill ? launch_q8_prefill(p, plan, s->s) : launch_q8_decode(p, plan, s->s);
 }
 
 }  // extern "C"

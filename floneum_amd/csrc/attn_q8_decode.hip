@@ -20,11 +20,10 @@
 #include <algorithm>
 
 #include "q8.h"
+#include "q8_attention.h"
 #include "q8_device.h"
 
 namespace fhip {
-
-constexpr float Q8_LOG2E = 1.4426950408889634f;
 
 template <int DV>
 struct Q8Dims {
@@ -40,14 +39,6 @@ struct Q8Dims {
     }
 };
 
-__device__ __forceinline__ float xor16(float x) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
-}
-__device__ __forceinline__ float xor32(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-}
 __device__ __forceinline__ float quads_max(float x) {
     x = fmaxf(x, xor16(x));
     return fmaxf(x, xor32(x));
@@ -56,40 +47,6 @@ __device__ __forceinline__ float quads_sum(float x) {
     x += xor16(x);
     return x + xor32(x);
 }
-__device__ __forceinline__ float q8_load_any(const void *p, int64_t idx, int dtype) {
-    if (dtype == FHIP_F32) return ((const float *)p)[idx];
-    if (dtype == FHIP_F16) return (float)((const half_t *)p)[idx];
-    return to_float(((const bf16_t *)p)[idx]);
-}
-__device__ __forceinline__ void q8_store_any(void *p, int64_t idx, int dtype, float v) {
-    if (dtype == FHIP_F32) ((float *)p)[idx] = v;
-    else if (dtype == FHIP_F16) ((half_t *)p)[idx] = (half_t)v;
-    else ((bf16_t *)p)[idx] = from_float<bf16_t>(v);
-}
-// Score and additive mask (both times log2 e).  What a finite mask value puts below -2^22 (the type's lowest value, which overflows in the
-// log2 domain) counts as that: the exponent of the value's scale, which is added next, has to keep its weight beside it, and a row whose keys
-// are all that far down weighs them alike, as f32 scores that vanish beside the mask do.
-__device__ __forceinline__ float q8_with_mask(float s, float add) {
-    const float t = s + add;
-    return t < -0x1p22f ? -0x1p22f : t;
-}
-
-// The keys [lo, hi) that some column of the workgroup sees, from the analytic mask and the lengths.
-struct Q8Range {
-    int lo, hi;
-    int64_t pos0;  // position of query row 0
-};
-__device__ __forceinline__ Q8Range q8_visible(const Q8AttnParams &p, int b, int row0, int row1) {
-    int64_t lo = 0, hi = p.Skv, pos0 = p.q_pos_offset + (p.q_positions ? p.q_positions[b] : 0);
-    if (p.kv_lens) hi = min(hi, (int64_t)p.kv_lens[b]);
-    if (p.causal) hi = min(hi, pos0 + row1 + 1);
-    if (p.window > 0) lo = max(lo, pos0 + row0 - p.window + 1);
-    hi = max(hi, (int64_t)0);
-    Q8Range r;
-    r.lo = (int)min(lo, hi), r.hi = (int)hi, r.pos0 = pos0;
-    return r;
-}
-
 template <int DV, int TERMS, int FMT, int CB>
 __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8AttnParams p) {
     using Dims = Q8Dims<DV>;
@@ -401,8 +358,7 @@ __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8Att
                 if (p.nsplit > 1) {
                     *(float4_t *)(p.partials + share * DV + d) = v;
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) q8_store_any(p.out, o + (d + e) * p.os[3], p.out_dtype, v[e] / L);
+                    q8_store4_any(p, o + d * p.os[3], v / L);
                 }
             }
             if (p.nsplit > 1 && sub == 0) {
@@ -437,16 +393,28 @@ __global__ __launch_bounds__(64) void q8_merge_kernel(Q8AttnParams p) {
     if (4 * lane >= p.D) return;
     const int b = (int)(bg / p.Hkv), head = (int)(bg % p.Hkv) * p.G + c % p.G;
     const int64_t o = (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)(c / p.G) * p.os[2];
-#pragma unroll
-    for (int e = 0; e < 4; e++) q8_store_any(p.out, o + (4 * lane + e) * p.os[3], p.out_dtype, v[e] / L);
+    q8_store4_any(p, o + 4 * lane * p.os[3], v / L);
 }
 
 static int q8_padded_dim(int D) { return (D + 63) / 64 * 64; }
 
+int launch_q8_merge(const Q8AttnParams &p, hipStream_t stream) {
+    const dim3 grid((unsigned)((int64_t)p.B * p.H * p.Sq));
+    switch (q8_padded_dim(p.D)) {
+        case 64: hipLaunchKernelGGL(q8_merge_kernel<64>, grid, dim3(64), 0, stream, p); break;
+        case 128: hipLaunchKernelGGL(q8_merge_kernel<128>, grid, dim3(64), 0, stream, p); break;
+        case 192: hipLaunchKernelGGL(q8_merge_kernel<192>, grid, dim3(64), 0, stream, p); break;
+        default: hipLaunchKernelGGL(q8_merge_kernel<256>, grid, dim3(64), 0, stream, p);
+    }
+    FHIP_HIP_CHECK(hipGetLastError());
+    return FHIP_OK;
+}
+
 Q8AttnPlan q8_decode_plan(const Q8AttnParams &p) {
     Q8AttnPlan plan;
     const int NC = p.G * p.Sq;
-    plan.column_blocks = 1;
+    plan.prefill = false;
+    plan.waves = 4;
     const int64_t units = (int64_t)p.B * p.Hkv * ((NC + 15) / 16);
     int64_t seen = p.Skv;
     if (p.window > 0) seen = std::min<int64_t>(seen, p.window + p.Sq - 1);
@@ -466,11 +434,7 @@ static int launch_decode_dims(const Q8AttnParams &p, const Q8AttnPlan &plan, hip
     const int64_t y = std::min<int64_t>(units, 32768), z = (units + y - 1) / y;
     hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1>), dim3(p.nsplit, (unsigned)y, (unsigned)z), dim3(256), 0, stream, p);
     FHIP_HIP_CHECK(hipGetLastError());
-    if (p.nsplit > 1) {
-        hipLaunchKernelGGL(q8_merge_kernel<DV>, dim3((unsigned)((int64_t)p.B * p.Hkv * NC)), dim3(64), 0, stream, p);
-        FHIP_HIP_CHECK(hipGetLastError());
-    }
-    return FHIP_OK;
+    return p.nsplit > 1 ? launch_q8_merge(p, stream) : FHIP_OK;
 }
 template <int DV>
 static int launch_decode_types(const Q8AttnParams &p, const Q8AttnPlan &plan, hipStream_t stream) {

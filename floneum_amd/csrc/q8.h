@@ -69,6 +69,7 @@ struct Q8AttnParams {
     void *out;
     int64_t qs[4], os[4];
     int32_t q_dtype, out_dtype;
+    int32_t q_vec, out_vec;  // query / output rows in pieces of four elements
     Q8View k, v;
     int32_t B, H, Hkv, G, Sq, Skv, D, format;
     int32_t causal;
@@ -84,11 +85,15 @@ struct Q8AttnParams {
     int32_t cus;
 };
 struct Q8AttnPlan {
-    int column_blocks;  // of 16 columns ((query row, head of the group) pairs) per workgroup
+    bool prefill;  // the kernel for many rows (attn_q8_prefill.hip), else the one for few (attn_q8_decode.hip)
+    int waves;     // per workgroup of the former
     int nsplit, min_chunk;
-    size_t bytes;
+    size_t bytes;  // of workspace
 };
 Q8AttnPlan q8_decode_plan(const Q8AttnParams &p);
 int launch_q8_decode(const Q8AttnParams &p, const Q8AttnPlan &plan, hipStream_t stream);
+Q8AttnPlan q8_prefill_plan(const Q8AttnParams &p);
+int launch_q8_prefill(const Q8AttnParams &p, const Q8AttnPlan &plan, hipStream_t stream);
+int launch_q8_merge(const Q8AttnParams &p, hipStream_t stream);  // joins the shares in p.partials
 
 }  // namespace fhip

@@ -1,0 +1,116 @@
+// Device code that the attention kernels of the 8-bit cache share.
+#pragma once
+#include "q8.h"
+#include "q8_device.h"
+
+namespace fhip {
+
+constexpr float Q8_LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float xor16(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float xor32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float q8_load_any(const void *p, int64_t idx, int dtype) {
+    if (dtype == FHIP_F32) return ((const float *)p)[idx];
+    if (dtype == FHIP_F16) return (float)((const half_t *)p)[idx];
+    return to_float(((const bf16_t *)p)[idx]);
+}
+__device__ __forceinline__ void q8_store_any(void *p, int64_t idx, int dtype, float v) {
+    if (dtype == FHIP_F32) ((float *)p)[idx] = v;
+    else if (dtype == FHIP_F16) ((half_t *)p)[idx] = (half_t)v;
+    else ((bf16_t *)p)[idx] = from_float<bf16_t>(v);
+}
+// four consecutive dims of an output row
+__device__ __forceinline__ void q8_store4_any(const Q8AttnParams &p, int64_t idx, float4_t v) {
+    if (!p.out_vec) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) q8_store_any(p.out, idx + e * p.os[3], p.out_dtype, v[e]);
+    } else if (p.out_dtype == FHIP_F32) {
+        *(float4_t *)((float *)p.out + idx) = v;
+    } else {
+        uint16_t bits[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) bits[e] = p.out_dtype == FHIP_F16 ? __builtin_bit_cast(uint16_t, (half_t)v[e]) : from_float<bf16_t>(v[e]).bits;
+        *(uint2_t *)((uint16_t *)p.out + idx) = uint2_t{bits[0] | (uint32_t)bits[1] << 16, bits[2] | (uint32_t)bits[3] << 16};
+    }
+}
+
+// Score and additive mask (both times log2 e).  What a finite mask value puts below -2^22 (the type's lowest value, which overflows in the
+// log2 domain) counts as that: the exponent of the value's scale, which the kernel for few rows adds next, has to keep its weight beside it, and
+// a row whose keys are all that far down weighs them alike, as f32 scores that vanish beside the mask do.
+__device__ __forceinline__ float q8_with_mask(float s, float add) {
+    const float t = s + add;
+    return t < -0x1p22f ? -0x1p22f : t;
+}
+
+// The keys [lo, hi) that some row of row0 .. row1 sees, from the analytic mask and the lengths.
+struct Q8Range {
+    int lo, hi;
+    int64_t pos0;  // position of query row 0
+};
+__device__ __forceinline__ Q8Range q8_visible(const Q8AttnParams &p, int b, int row0, int row1) {
+    int64_t lo = 0, hi = p.Skv, pos0 = p.q_pos_offset + (p.q_positions ? p.q_positions[b] : 0);
+    if (p.kv_lens) hi = min(hi, (int64_t)p.kv_lens[b]);
+    if (p.causal) hi = min(hi, pos0 + row1 + 1);
+    if (p.window > 0) lo = max(lo, pos0 + row0 - p.window + 1);
+    hi = max(hi, (int64_t)0);
+    Q8Range r;
+    r.lo = (int)min(lo, hi), r.hi = (int)hi, r.pos0 = pos0;
+    return r;
+}
+
+// The operands of a query row (of a 32x32x16 product: lane half h holds dims 16 i + 8 h .. + 7 of step i), scaled by a power of two that brings its
+// largest element to [2^14, 2^15).  Returns what takes a product with codes to the log2 domain.
+template <int TERMS, int STEPS>
+__device__ __forceinline__ float q8_load_queries(const Q8AttnParams &p, int64_t base, int h, half8_t (&q)[TERMS][STEPS]) {
+    float x[STEPS][8], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+        const int d0 = 16 * i + 8 * h;
+        if (d0 >= p.D) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+        } else if (p.q_vec && p.q_dtype == FHIP_F32) {
+            const float4_t a = *(const float4_t *)((const float *)p.q + base + d0), b = *(const float4_t *)((const float *)p.q + base + d0 + 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[i][e] = a[e], x[i][4 + e] = b[e];
+        } else if (p.q_vec) {
+            const uint2_t a = *(const uint2_t *)((const uint16_t *)p.q + base + d0), b = *(const uint2_t *)((const uint16_t *)p.q + base + d0 + 4);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t w = e < 4 ? a[e >> 1] : b[(e - 4) >> 1], bits = e & 1 ? w >> 16 : w & 0xffffu;
+                x[i][e] = p.q_dtype == FHIP_F16 ? (float)__builtin_bit_cast(half_t, (uint16_t)bits) : __uint_as_float(bits << 16);
+            }
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < 8; e++) {
+                const float v = q8_load_any(p.q, base + (d0 + e) * p.qs[3], p.q_dtype);
+#pragma unroll
+                for (int y = 0; y < 8; y++) x[i][y] = y == e ? v : x[i][y];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[i][e]));
+    }
+    top = fmaxf(top, xor32(top));
+    // zeros, infinities and NaN stay as they are
+    const int shift = top > 0.0f && top <= 3.402823466e38f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            // a scale of 0 or below goes with the queries: the one of the scores is positive
+            const float v = __builtin_ldexpf(p.scale > 0.0f ? x[i][e] : p.scale < 0.0f ? -x[i][e] : 0.0f * x[i][e], shift);
+            const half_t high = (half_t)v;
+            q[0][i][e] = high;
+            if constexpr (TERMS == 2) q[1][i][e] = (half_t)(v - (float)high);
+        }
+    return __builtin_ldexpf((p.scale != 0.0f ? __builtin_fabsf(p.scale) : 1.0f) * Q8_LOG2E, -shift);
+}
+
+}  // namespace fhip

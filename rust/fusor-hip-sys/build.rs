@@ -27,6 +27,7 @@ const SOURCES: &[&str] = &[
     "api_q8.hip",
     "kv_q8.hip",
     "attn_q8_decode.hip",
+    "attn_q8_prefill.hip",
 ];
 
 // the flags floneum_amd/build.py uses; packed-f32 VALU forms are kept out of the generated code on purpose
