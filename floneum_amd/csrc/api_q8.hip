@@ -323,9 +323,9 @@ static void fill_attention(const fhip_q8_attn_args *a, int cus, Q8AttnParams *p)
     p->cus = cus > 0 ? cus : 256;
 }
 
-// Few columns ((query row, head of the group) pairs) per KV head: the kernel that streams the codes into registers.
+// Few columns ((query row, head of the group) pairs) per KV head: the kernel that streams the codes into registers (32 rows at a time).
 static Q8AttnPlan attention_plan(const Q8AttnParams &p) {
-    return (int64_t)p.G * p.Sq <= 32 ? q8_decode_plan(p) : q8_prefill_plan(p);
+    return (int64_t)p.G * p.Sq <= 32 && p.Skv >= 32 ? q8_decode_plan(p) : q8_prefill_plan(p);
 }
 
 }  // namespace fhip

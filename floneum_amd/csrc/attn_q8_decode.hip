@@ -47,10 +47,10 @@ __device__ __forceinline__ float quads_sum(float x) {
     x += xor16(x);
     return x + xor32(x);
 }
-template <int DV, int TERMS, int FMT, int CB>
-__global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8AttnParams p) {
+template <int DV, int TERMS, int FMT, int CB, bool MASK, bool BLOCKS>
+__global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8AttnParams p) {
     using Dims = Q8Dims<DV>;
-    constexpr int VW = Dims::VW, KS = Dims::KS, TILES = Dims::TILES, COLS = 16 * CB;
+    constexpr int VW = Dims::VW, KS = Dims::KS, TILES = Dims::TILES, COLS = 16 * CB, NBUF = DV <= 128 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float lds_acc[4][16][DV + 4];
     __shared__ float lds_m[4][COLS], lds_l[4][COLS];
 
@@ -69,44 +69,6 @@ __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8Att
     const int chunk = (max(p.min_chunk, (int)(((int64_t)len + p.nsplit - 1) / p.nsplit)) + 127) / 128 * 128;
     const int64_t lo64 = vis.lo + (int64_t)split * chunk;
     const int lo = (int)min(lo64, (int64_t)vis.hi), hi = (int)min((int64_t)vis.hi, lo64 + chunk);
-
-    // queries: column c is row c / G, head c % G of the group
-    half8_t q[CB][TERMS][KS][2];
-    float colscale[CB];
-    int limit[CB], start[CB];  // keys [start, limit) of the column
-    int row[CB];
-#pragma unroll
-    for (int cbk = 0; cbk < CB; cbk++) {
-        const int c = min(c0 + cbk * 16 + n, NC - 1);
-        row[cbk] = c / p.G;
-        const int head = kvh * p.G + c % p.G;
-        const int64_t base = (int64_t)b * p.qs[0] + (int64_t)head * p.qs[1] + (int64_t)row[cbk] * p.qs[2];
-        float x[KS][16], top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int d = 64 * s + 16 * g + e;
-                x[s][e] = d < p.D ? q8_load_any(p.q, base + d * p.qs[3], p.q_dtype) : 0.0f;
-                top = fmaxf(top, __builtin_fabsf(x[s][e]));
-            }
-        top = quads_max(top);
-        // the largest element to [2^14, 2^15); zeros, infinities and NaN stay as they are
-        const int shift = top > 0.0f && top <= 3.402823466e38f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float v = __builtin_ldexpf(x[s][e], shift);
-                const half_t high = (half_t)v;
-                q[cbk][0][s][e >> 3][e & 7] = high;
-                if constexpr (TERMS == 2) q[cbk][1][s][e >> 3][e & 7] = (half_t)(v - (float)high);
-            }
-        colscale[cbk] = __builtin_ldexpf(p.scale * Q8_LOG2E, -shift);
-        const int64_t at = vis.pos0 + row[cbk];
-        limit[cbk] = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);
-        start[cbk] = (int)(p.window > 0 ? min((int64_t)hi, max((int64_t)0, at - p.window + 1)) : 0);
-    }
 
     float4_t acc[CB][TILES];
     float m[CB], l[CB];
@@ -128,81 +90,83 @@ __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8Att
     const int voff = (VW == 3 ? 8 : 4 * VW) * n < pitch ? (VW == 3 ? 8 : 4 * VW) * n : 0, vlast = 128 + 4 * n < pitch ? 128 + 4 * n : 0;
     const int kkey = 8 * (n >> 2) + (n & 3), vkey = 8 * g;  // the lane's first key of a step
 
-    uint4_t kc[2][KS];
-    uint32_t vc[8][VW];
-    float ks[8], vs[8];
-    auto load_k_rows = [&](int u, const uint8_t *r, int at) {
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const int off = s == KS - 1 ? klast : 64 * s + 16 * g;
-            kc[u][s] = __builtin_nontemporal_load((const uint4_t *)(r + (uint32_t)(at + off)));
-        }
+    // queries: column c is row c / G, head c % G of the group
+    half8_t q[CB][TERMS][KS][2];
+    float colscale[CB];
+    int limit[CB], start[CB];  // keys [start, limit) of the column
+    int row[CB];
+    // What a wavefront holds of a step's keys.  Steps are loaded NBUF ahead, without a branch (behind one the compiler would wait for all
+    // loads): the last step of a share starts 32 keys before its end and leaves out those of the step before, and steps beyond it load that
+    // one again.  A tensor has at least 32 rows here.
+    struct Step {
+        uint4_t kc[2][KS];
+        uint32_t vc[8][VW];
+        float ks[8], vs[8];
     };
-    auto load_v_rows = [&](int i, const uint8_t *r, int at) {
-        if constexpr (VW == 1) {
-            vc[i][0] = __builtin_nontemporal_load((const uint32_t *)(r + (uint32_t)(at + voff)));
-        } else if constexpr (VW == 4) {
-            const uint4_t w = __builtin_nontemporal_load((const uint4_t *)(r + (uint32_t)(at + voff)));
+    const uint32_t klane = (uint32_t)(kkey * krow), vlane = (uint32_t)(vkey * vrow);
+    auto first_key = [&](int k0) { return max(0, min(k0, hi - 32)); };
+    auto load_k = [&](Step &x, int k0) {
+        const uint8_t *r = kbase + (int64_t)first_key(k0) * krow;
 #pragma unroll
-            for (int e = 0; e < 4; e++) vc[i][e] = w[e];
-        } else {
-            const uint2_t w = __builtin_nontemporal_load((const uint2_t *)(r + (uint32_t)(at + voff)));
-            vc[i][0] = w[0], vc[i][1] = w[1];
-            if constexpr (VW == 3) vc[i][2] = __builtin_nontemporal_load((const uint32_t *)(r + (uint32_t)(at + vlast)));
-        }
+        for (int u = 0; u < 2; u++, r += 4 * krow)
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+                x.kc[u][s] = *(const uint4_t *)((r + (klane + (s == KS - 1 ? klast : 64 * s + 16 * g))));
     };
-    // Keys beyond the share are loaded as its last one: what lies there may be anything, 8-bit NaN among it.
-    auto load_k = [&](int k0) {
-        const uint8_t *const r = kbase + (int64_t)k0 * krow;
-        if (k0 + 32 <= hi) {
+    auto load_v = [&](Step &x, int k0) {
+        const uint8_t *r = vbase + (int64_t)first_key(k0) * vrow;
 #pragma unroll
-            for (int u = 0; u < 2; u++) load_k_rows(u, r + 4 * u * krow, kkey * krow);
-        } else {
+        for (int i = 0; i < 8; i++, r += vrow) {
+            if constexpr (VW == 1) {
+                x.vc[i][0] = *(const uint32_t *)((r + (vlane + voff)));
+            } else if constexpr (VW == 4) {
+                const uint4_t w = *(const uint4_t *)((r + (vlane + voff)));
 #pragma unroll
-            for (int u = 0; u < 2; u++) load_k_rows(u, r, min(kkey + 4 * u, hi - 1 - k0) * krow);
-        }
-    };
-    auto load_v = [&](int k0) {
-        const uint8_t *const r = vbase + (int64_t)k0 * vrow;
-        if (k0 + 32 <= hi) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) load_v_rows(i, r + i * vrow, vkey * vrow);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) load_v_rows(i, r, min(vkey + i, hi - 1 - k0) * vrow);
-        }
-    };
-    // scales of the lane's eight keys
-    auto load_scales = [&](float (&out)[8], const float *s, const Q8View &v, int k0) {
-        if (v.log2_block == 0) {
-            if (k0 + 32 <= hi) {
-                typedef float float4_at4_t __attribute__((ext_vector_type(4), aligned(4)));
-                const float4_at4_t a = *(const float4_at4_t *)(s + k0 + vkey), c = *(const float4_at4_t *)(s + k0 + vkey + 4);
-#pragma unroll
-                for (int i = 0; i < 4; i++) out[i] = a[i], out[4 + i] = c[i];
+                for (int e = 0; e < 4; e++) x.vc[i][e] = w[e];
             } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) out[i] = s[min(k0 + vkey + i, hi - 1)];
+                const uint2_t w = *(const uint2_t *)((r + (vlane + voff)));
+                x.vc[i][0] = w[0], x.vc[i][1] = w[1];
+                if constexpr (VW == 3) x.vc[i][2] = *(const uint32_t *)((r + (vlane + vlast)));
             }
-        } else {  // blocks of 8 keys or more: two at most
-            const int at = v.first + k0 + vkey, last = v.first + hi - 1, T = 1 << v.log2_block;
-            const float a = s[min(at, last) >> v.log2_block], c = s[min(at + 7, last) >> v.log2_block];
-            const int phase = at & (T - 1);
-#pragma unroll
-            for (int i = 0; i < 8; i++) out[i] = phase + i < T ? a : c;
         }
+    };
+    // scales of the lane's eight keys: one each, or with blocks of eight and more two at most
+    auto load_scale8 = [&](float (&out)[8], const float *s, const Q8View &v, int k0) {
+        const int at = v.first + first_key(k0) + vkey;
+        if constexpr (BLOCKS) {
+            out[0] = s[at >> v.log2_block], out[7] = s[(at + 7) >> v.log2_block];
+        } else {
+            typedef float float4_at4_t __attribute__((ext_vector_type(4), aligned(4)));
+            const float4_at4_t a = *(const float4_at4_t *)(s + at), c = *(const float4_at4_t *)(s + at + 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[i] = a[i], out[4 + i] = c[i];
+        }
+    };
+    auto spread_scale8 = [&](float (&x)[8], const Q8View &v, int k0) {
+        if constexpr (BLOCKS) {
+            const int T = 1 << v.log2_block, phase = (v.first + first_key(k0) + vkey) & (T - 1);
+            const float a = x[0], c = x[7];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = phase + i < T ? a : c;
+        }
+    };
+    auto load_scales = [&](Step &x, int k0) {
+        load_scale8(x.ks, kscale, p.k, k0);
+        load_scale8(x.vs, vscale, p.v, k0);
     };
 
-    int k0 = lo + 32 * wave;
-    if (k0 < hi) load_k(k0);
-    for (; k0 < hi; k0 += 128) {
-        load_scales(ks, kscale, p.k, k0);
-        load_scales(vs, vscale, p.v, k0);
-        load_v(k0);
-        // NaN among the values' scales goes by way of the scores, where rows that a mask hides are taken out
+    // the step at k0, and the loads of the step that takes its registers next
+    auto step = [&](Step &x, int k0) {
+        const int at = first_key(k0), next = k0 + NBUF * 128;
+        spread_scale8(x.ks, p.k, k0);
+        spread_scale8(x.vs, p.v, k0);
+        float exf[8], back[8], vs[8], ks[8];  // e_j, 2^-e_j
         bool lost = false;
 #pragma unroll
+        for (int i = 0; i < 8; i++) ks[i] = x.ks[i], vs[i] = x.vs[i];
+#pragma unroll
         for (int i = 0; i < 8; i += 2) lost = lost || __builtin_isunordered(vs[i], vs[i + 1]);
+        // NaN among the values' scales goes by way of the scores, where rows that a mask hides are taken out
         if (__builtin_amdgcn_ballot_w64(lost) != 0) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -222,24 +186,22 @@ __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8Att
                     half8_t kf;
 #pragma unroll
                     for (int w = 0; w < 2; w++) {
-                        const uint32_t word = kc[u][s][2 * a + w];
-                        const half2_t x = q8_pair_low<FMT>(word), y = q8_pair_high<FMT>(word);
-                        kf[4 * w] = x[0], kf[4 * w + 1] = x[1], kf[4 * w + 2] = y[0], kf[4 * w + 3] = y[1];
+                        const uint32_t word = x.kc[u][s][2 * a + w];
+                        const half2_t y = q8_pair_low<FMT>(word), z = q8_pair_high<FMT>(word);
+                        kf[4 * w] = y[0], kf[4 * w + 1] = y[1], kf[4 * w + 2] = z[0], kf[4 * w + 3] = z[1];
                     }
 #pragma unroll
-                    for (int cbk = 0; cbk < CB; cbk++) {
+                    for (int cbk = 0; cbk < CB; cbk++)
 #pragma unroll
-                        for (int x = TERMS - 1; x >= 0; x--)
-                            s4[cbk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[cbk][x][s][a], s4[cbk], 0, 0, 0);
-                    }
+                        for (int t = TERMS - 1; t >= 0; t--)
+                            s4[cbk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[cbk][t][s][a], s4[cbk], 0, 0, 0);
                 }
 #pragma unroll
             for (int cbk = 0; cbk < CB; cbk++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) sc[cbk][4 * u + r] = s4[cbk][r];
         }
-        if (k0 + 128 < hi) load_k(k0 + 128);
-        float exf[8], back[8];  // e_j, 2^-e_j
+        load_k(x, next);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int e = __builtin_amdgcn_frexp_expf(fmaxf(vs[i], Q8_LEAST_SCALE));
@@ -250,23 +212,23 @@ __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8Att
 #pragma unroll
         for (int cbk = 0; cbk < CB; cbk++) {
             float top = -INFINITY;
-            if (p.mask == nullptr) {
+            if constexpr (!MASK) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) sc[cbk][i] = __builtin_fmaf(sc[cbk][i], ks[i] * colscale[cbk], exf[i]);
                 // the step reaches beyond what some column sees
-                if (__builtin_amdgcn_ballot_w64(k0 + 32 > limit[cbk] || k0 < start[cbk]) != 0) {
+                if (__builtin_amdgcn_ballot_w64(at + 32 > limit[cbk] || at < start[cbk] || at < k0) != 0) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int key = k0 + vkey + i;
-                        if (key >= limit[cbk] || key < start[cbk]) sc[cbk][i] = -INFINITY;
+                        const int key = at + vkey + i;
+                        if (key >= limit[cbk] || key < start[cbk] || key < k0) sc[cbk][i] = -INFINITY;
                     }
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const int key = k0 + vkey + i;
+                    const int key = at + vkey + i;
                     float add = -INFINITY;
-                    if (key < limit[cbk])
+                    if (key < limit[cbk] && key >= k0)
                         add = q8_load_any(p.mask, (p.mask_kind == FHIP_MASK_QK ? row[cbk] : b) * p.ms0 + key * p.ms1, p.q_dtype);
                     const float s = q8_with_mask(sc[cbk][i] * (ks[i] * colscale[cbk]), add * Q8_LOG2E);
                     sc[cbk][i] = add == -INFINITY ? -INFINITY : s + exf[i];
@@ -294,13 +256,22 @@ __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8Att
                 if constexpr (TERMS == 2) pw[cbk][1][i] = (half_t)(w - (float)hi16);
             }
         }
+        load_scales(x, next);
+        // rows that are no keys of this step's may hold anything, 8-bit NaN among it
+        if (at < k0 || at + 32 > hi) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (at + vkey + i < k0 || at + vkey + i >= hi)
+#pragma unroll
+                    for (int w = 0; w < VW; w++) x.vc[i][w] = 0;
+        }
         // values: byte t of the eight keys' words w is dim(n, w, t)
 #pragma unroll
         for (int w = 0; w < VW; w++) {
             half8_t vf[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const uint32_t a = vc[2 * i][w], c = vc[2 * i + 1][w];
+                const uint32_t a = x.vc[2 * i][w], c = x.vc[2 * i + 1][w];
                 const uint32_t t01 = __builtin_amdgcn_perm(c, a, 0x05010400u), t23 = __builtin_amdgcn_perm(c, a, 0x07030602u);
                 const half2_t h0 = q8_pair_low<FMT>(t01), h1 = q8_pair_high<FMT>(t01), h2 = q8_pair_low<FMT>(t23), h3 = q8_pair_high<FMT>(t23);
                 vf[0][2 * i] = h0[0], vf[0][2 * i + 1] = h0[1];
@@ -311,12 +282,63 @@ __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8Att
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int cbk = 0; cbk < CB; cbk++) {
-                    float4_t &a = acc[cbk][4 * w + t];
+                for (int cbk = 0; cbk < CB; cbk++)
 #pragma unroll
-                    for (int x = TERMS - 1; x >= 0; x--)
-                        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[t], pw[cbk][x], a, 0, 0, 0);
+                    for (int y = TERMS - 1; y >= 0; y--)
+                        acc[cbk][4 * w + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[t], pw[cbk][y], acc[cbk][4 * w + t], 0, 0, 0);
+        }
+        load_v(x, next);
+    };
+
+    Step steps[NBUF];
+    int k0 = lo + 32 * wave;
+    if (k0 < hi) {
+#pragma unroll
+        for (int i = 0; i < NBUF; i++) {
+            load_k(steps[i], k0 + 128 * i);
+            load_scales(steps[i], k0 + 128 * i);
+            load_v(steps[i], k0 + 128 * i);
+        }
+    }
+#pragma unroll
+    for (int cbk = 0; cbk < CB; cbk++) {
+        const int c = min(c0 + cbk * 16 + n, NC - 1);
+        row[cbk] = c / p.G;
+        const int head = kvh * p.G + c % p.G;
+        const int64_t base = (int64_t)b * p.qs[0] + (int64_t)head * p.qs[1] + (int64_t)row[cbk] * p.qs[2];
+        float x[KS][2][8], top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+                q8_load_query8(p, base, 64 * s + 16 * g + 8 * a, x[s][a]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[s][a][e]));
+            }
+        const int shift = q8_query_shift(quads_max(top));
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    half_t high, low;
+                    q8_query_terms<TERMS>(p, x[s][a][e], shift, high, low);
+                    q[cbk][0][s][a][e] = high;
+                    if constexpr (TERMS == 2) q[cbk][1][s][a][e] = low;
                 }
+        colscale[cbk] = q8_score_scale(p, shift);
+        const int64_t at = vis.pos0 + row[cbk];
+        limit[cbk] = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);
+        start[cbk] = (int)(p.window > 0 ? min((int64_t)hi, max((int64_t)0, at - p.window + 1)) : 0);
+    }
+
+    while (k0 < hi) {
+#pragma unroll
+        for (int i = 0; i < NBUF; i++) {
+            step(steps[i], k0);
+            k0 += 128;
+            if (i + 1 < NBUF && k0 >= hi) break;
         }
     }
 
@@ -369,31 +391,57 @@ __global__ __launch_bounds__(256, DV <= 128 ? 3 : 2) void q8_decode_kernel(Q8Att
     }
 }
 
-// Joins the shares: a wavefront per (batch, kv head, column), four dims a lane.
+// Joins the shares of a (batch, kv head, column).  A workgroup of 256 lanes per column: the shares' maxima and sums are read at once, one a lane, and
+// their weights kept in LDS; then groups of DV / 4 lanes, four dims each, add up every GROUPS-th share.
 template <int DV>
-__global__ __launch_bounds__(64) void q8_merge_kernel(Q8AttnParams p) {
-    const int NC = p.G * p.Sq, lane = threadIdx.x;
-    const int64_t at = blockIdx.x;
-    const int c = (int)(at % NC);
-    const int64_t bg = at / NC;
+__global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
+    constexpr int LPG = DV == 192 ? 64 : DV / 4, GROUPS = 256 / LPG;
+    __shared__ float weight[Q8_MAX_SHARES], red[8];
+    __shared__ __attribute__((aligned(16))) float sums[GROUPS][4 * LPG];
+    const int NC = p.G * p.Sq, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t at = blockIdx.x, bg = at / NC;
+    const int c = (int)(at - bg * NC);
     const float *const ml = p.partials + (int64_t)p.B * p.Hkv * p.nsplit * NC * DV;
-    float M = -INFINITY;
-    for (int s = 0; s < p.nsplit; s++) M = fmaxf(M, ml[((bg * p.nsplit + s) * NC + c) * 2]);
+    const int64_t first = bg * p.nsplit * NC + c;
+    float m[Q8_MAX_SHARES / 256], l[Q8_MAX_SHARES / 256], M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < Q8_MAX_SHARES / 256; i++) {
+        const int s = tid + 256 * i;
+        m[i] = -INFINITY, l[i] = 0.0f;
+        if (s < p.nsplit) m[i] = ml[2 * (first + (int64_t)s * NC)], l[i] = ml[2 * (first + (int64_t)s * NC) + 1];
+        M = fmaxf(M, m[i]);
+    }
+    M = wave_max(M);
+    if (lane == 0) red[wave] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float ref = M == -INFINITY ? 0.0f : M;
     float L = 0.0f;
-    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < p.nsplit; s++) {
-        const int64_t i = (bg * p.nsplit + s) * NC + c;
-        const float sm = ml[2 * i];
-        if (sm == -INFINITY) continue;  // (NaN goes on)
-        const float f = __builtin_amdgcn_exp2f(sm - ref);
-        L += ml[2 * i + 1] * f;
-        if (4 * lane < p.D) v += *(const float4_t *)(p.partials + i * DV + 4 * lane) * f;
+#pragma unroll
+    for (int i = 0; i < Q8_MAX_SHARES / 256; i++) {
+        const float f = __builtin_amdgcn_exp2f(m[i] - ref);
+        if (tid + 256 * i < p.nsplit) weight[tid + 256 * i] = f;
+        L += l[i] * f;
     }
-    if (4 * lane >= p.D) return;
+    L = wave_sum(L);
+    if (lane == 0) red[4 + wave] = L;
+    __syncthreads();
+    L = (red[4] + red[5]) + (red[6] + red[7]);
+    const int group = tid / LPG, d = 4 * (tid % LPG);
+    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (d < p.D) {
+        const float *const part = p.partials + first * DV + d;
+        const int64_t step = (int64_t)NC * DV;
+#pragma unroll 4
+        for (int s = group; s < p.nsplit; s += GROUPS) v += *(const float4_t *)(part + s * step) * weight[s];
+    }
+    *(float4_t *)&sums[group][d] = v;
+    __syncthreads();
+    if (tid >= LPG || d >= p.D) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; g++) v += *(const float4_t *)&sums[g][d];
     const int b = (int)(bg / p.Hkv), head = (int)(bg % p.Hkv) * p.G + c % p.G;
-    const int64_t o = (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)(c / p.G) * p.os[2];
-    q8_store4_any(p, o + 4 * lane * p.os[3], v / L);
+    q8_store4_any(p, (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)(c / p.G) * p.os[2] + d * p.os[3], v / L);
 }
 
 static int q8_padded_dim(int D) { return (D + 63) / 64 * 64; }
@@ -401,10 +449,10 @@ static int q8_padded_dim(int D) { return (D + 63) / 64 * 64; }
 int launch_q8_merge(const Q8AttnParams &p, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)p.B * p.H * p.Sq));
     switch (q8_padded_dim(p.D)) {
-        case 64: hipLaunchKernelGGL(q8_merge_kernel<64>, grid, dim3(64), 0, stream, p); break;
-        case 128: hipLaunchKernelGGL(q8_merge_kernel<128>, grid, dim3(64), 0, stream, p); break;
-        case 192: hipLaunchKernelGGL(q8_merge_kernel<192>, grid, dim3(64), 0, stream, p); break;
-        default: hipLaunchKernelGGL(q8_merge_kernel<256>, grid, dim3(64), 0, stream, p);
+        case 64: hipLaunchKernelGGL(q8_merge_kernel<64>, grid, dim3(256), 0, stream, p); break;
+        case 128: hipLaunchKernelGGL(q8_merge_kernel<128>, grid, dim3(256), 0, stream, p); break;
+        case 192: hipLaunchKernelGGL(q8_merge_kernel<192>, grid, dim3(256), 0, stream, p); break;
+        default: hipLaunchKernelGGL(q8_merge_kernel<256>, grid, dim3(256), 0, stream, p);
     }
     FHIP_HIP_CHECK(hipGetLastError());
     return FHIP_OK;
@@ -418,10 +466,13 @@ Q8AttnPlan q8_decode_plan(const Q8AttnParams &p) {
     const int64_t units = (int64_t)p.B * p.Hkv * ((NC + 15) / 16);
     int64_t seen = p.Skv;
     if (p.window > 0) seen = std::min<int64_t>(seen, p.window + p.Sq - 1);
-    const int64_t target = 3 * (int64_t)p.cus;
+    // As many workgroups as the chip holds at once; four times as many shorter shares where the sequences have lengths of their own, which the
+    // host does not know: the long ones are spread (us, 16 of 128 to 16384 keys, 32/32 heads at 96: shares for 2, 4, 8 and 16 workgroups
+    // per CU 209, 189, 175 and 188).
+    const int64_t target = (p.kv_lens || p.q_positions ? 8 : 2) * (int64_t)p.cus;
     plan.min_chunk = 128;
     int64_t ns = std::min((target + units - 1) / units, (seen + 127) / 128);
-    ns = std::max<int64_t>(1, std::min<int64_t>(ns, 1024));
+    ns = std::max<int64_t>(1, std::min<int64_t>(ns, Q8_MAX_SHARES));
     plan.nsplit = (int)ns;
     plan.bytes = ns > 1 ? (size_t)p.B * p.Hkv * ns * NC * (q8_padded_dim(p.D) + 2) * sizeof(float) : 0;
     return plan;
@@ -432,7 +483,12 @@ static int launch_decode_dims(const Q8AttnParams &p, const Q8AttnPlan &plan, hip
     const int NC = p.G * p.Sq;
     const int64_t units = (int64_t)p.B * p.Hkv * ((NC + 15) / 16);
     const int64_t y = std::min<int64_t>(units, 32768), z = (units + y - 1) / y;
-    hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1>), dim3(p.nsplit, (unsigned)y, (unsigned)z), dim3(256), 0, stream, p);
+    const dim3 grid(p.nsplit, (unsigned)y, (unsigned)z);
+    const bool blocks = p.k.log2_block > 0;
+    if (p.mask && blocks) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1, true, true>), grid, dim3(256), 0, stream, p);
+    else if (p.mask) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1, true, false>), grid, dim3(256), 0, stream, p);
+    else if (blocks) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1, false, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1, false, false>), grid, dim3(256), 0, stream, p);
     FHIP_HIP_CHECK(hipGetLastError());
     return p.nsplit > 1 ? launch_q8_merge(p, stream) : FHIP_OK;
 }

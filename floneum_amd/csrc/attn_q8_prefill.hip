@@ -70,7 +70,28 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
     const int c = min(c0 + wave * 32 + n, NC - 1);
     const int row = c / p.G, head = kvh * p.G + c % p.G;
     half8_t q[TERMS][STEPS];
-    const float colscale = q8_load_queries<TERMS, STEPS>(p, (int64_t)b * p.qs[0] + (int64_t)head * p.qs[1] + (int64_t)row * p.qs[2], h, q);
+    float colscale;
+    {  // lane half h holds dims 16 i + 8 h .. + 7 of step i
+        const int64_t base = (int64_t)b * p.qs[0] + (int64_t)head * p.qs[1] + (int64_t)row * p.qs[2];
+        float x[STEPS][8], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            q8_load_query8(p, base, 16 * i + 8 * h, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[i][e]));
+        }
+        const int shift = q8_query_shift(fmaxf(top, xor32(top)));
+#pragma unroll
+        for (int i = 0; i < STEPS; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                half_t high, low;
+                q8_query_terms<TERMS>(p, x[i][e], shift, high, low);
+                q[0][i][e] = high;
+                if constexpr (TERMS == 2) q[1][i][e] = low;
+            }
+        colscale = q8_score_scale(p, shift);
+    }
     const int64_t at = vis.pos0 + row;
     const int limit = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);
     const int start = (int)(p.window > 0 ? min((int64_t)hi, max((int64_t)0, at - p.window + 1)) : 0);

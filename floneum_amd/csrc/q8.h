@@ -6,6 +6,7 @@ namespace fhip {
 
 constexpr int Q8_MAX_DIM = 256;
 constexpr int Q8_MAX_BLOCK = 64;
+constexpr int Q8_MAX_SHARES = 512;  // of the keys of a call
 
 // A view of codes and scales: pointers with the offsets applied, strides in bytes / elements.
 struct Q8View {

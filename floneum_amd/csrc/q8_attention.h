@@ -64,52 +64,42 @@ __device__ __forceinline__ Q8Range q8_visible(const Q8AttnParams &p, int b, int 
     return r;
 }
 
-// The operands of a query row (of a 32x32x16 product: lane half h holds dims 16 i + 8 h .. + 7 of step i), scaled by a power of two that brings its
-// largest element to [2^14, 2^15).  Returns what takes a product with codes to the log2 domain.
-template <int TERMS, int STEPS>
-__device__ __forceinline__ float q8_load_queries(const Q8AttnParams &p, int64_t base, int h, half8_t (&q)[TERMS][STEPS]) {
-    float x[STEPS][8], top = 0.0f;
+// eight consecutive dims of a query row, zeros beyond head_dim
+__device__ __forceinline__ void q8_load_query8(const Q8AttnParams &p, int64_t base, int d0, float (&x)[8]) {
+    if (d0 >= p.D) {
 #pragma unroll
-    for (int i = 0; i < STEPS; i++) {
-        const int d0 = 16 * i + 8 * h;
-        if (d0 >= p.D) {
+        for (int e = 0; e < 8; e++) x[e] = 0.0f;
+    } else if (p.q_vec && p.q_dtype == FHIP_F32) {
+        const float4_t a = *(const float4_t *)((const float *)p.q + base + d0), b = *(const float4_t *)((const float *)p.q + base + d0 + 4);
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
-        } else if (p.q_vec && p.q_dtype == FHIP_F32) {
-            const float4_t a = *(const float4_t *)((const float *)p.q + base + d0), b = *(const float4_t *)((const float *)p.q + base + d0 + 4);
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[i][e] = a[e], x[i][4 + e] = b[e];
-        } else if (p.q_vec) {
-            const uint2_t a = *(const uint2_t *)((const uint16_t *)p.q + base + d0), b = *(const uint2_t *)((const uint16_t *)p.q + base + d0 + 4);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t w = e < 4 ? a[e >> 1] : b[(e - 4) >> 1], bits = e & 1 ? w >> 16 : w & 0xffffu;
-                x[i][e] = p.q_dtype == FHIP_F16 ? (float)__builtin_bit_cast(half_t, (uint16_t)bits) : __uint_as_float(bits << 16);
-            }
-        } else {
-#pragma unroll 1
-            for (int e = 0; e < 8; e++) {
-                const float v = q8_load_any(p.q, base + (d0 + e) * p.qs[3], p.q_dtype);
-#pragma unroll
-                for (int y = 0; y < 8; y++) x[i][y] = y == e ? v : x[i][y];
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[i][e]));
-    }
-    top = fmaxf(top, xor32(top));
-    // zeros, infinities and NaN stay as they are
-    const int shift = top > 0.0f && top <= 3.402823466e38f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-#pragma unroll
-    for (int i = 0; i < STEPS; i++)
+        for (int e = 0; e < 4; e++) x[e] = a[e], x[4 + e] = b[e];
+    } else if (p.q_vec) {
+        const uint2_t a = *(const uint2_t *)((const uint16_t *)p.q + base + d0), b = *(const uint2_t *)((const uint16_t *)p.q + base + d0 + 4);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            // a scale of 0 or below goes with the queries: the one of the scores is positive
-            const float v = __builtin_ldexpf(p.scale > 0.0f ? x[i][e] : p.scale < 0.0f ? -x[i][e] : 0.0f * x[i][e], shift);
-            const half_t high = (half_t)v;
-            q[0][i][e] = high;
-            if constexpr (TERMS == 2) q[1][i][e] = (half_t)(v - (float)high);
+            const uint32_t w = e < 4 ? a[e >> 1] : b[(e - 4) >> 1], bits = e & 1 ? w >> 16 : w & 0xffffu;
+            x[e] = p.q_dtype == FHIP_F16 ? (float)__builtin_bit_cast(half_t, (uint16_t)bits) : __uint_as_float(bits << 16);
         }
+    } else {
+#pragma unroll 1
+        for (int e = 0; e < 8; e++) {
+            const float v = q8_load_any(p.q, base + (d0 + e) * p.qs[3], p.q_dtype);
+#pragma unroll
+            for (int y = 0; y < 8; y++) x[y] = y == e ? v : x[y];
+        }
+    }
+}
+// The power of two that brings a row's largest element to [2^14, 2^15); zeros, infinities and NaN stay as they are.
+__device__ __forceinline__ int q8_query_shift(float top) { return top > 0.0f && top <= 3.402823466e38f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; }
+// An element as one term or two.  A scale of 0 or below goes with the queries: the one of the scores (q8_score_scale) is positive.
+template <int TERMS>
+__device__ __forceinline__ void q8_query_terms(const Q8AttnParams &p, float x, int shift, half_t &high, half_t &low) {
+    const float v = __builtin_ldexpf(p.scale > 0.0f ? x : p.scale < 0.0f ? -x : 0.0f * x, shift);
+    high = (half_t)v;
+    if constexpr (TERMS == 2) low = (half_t)(v - (float)high);
+}
+// what takes a product of such a query with codes times their scale to the log2 domain
+__device__ __forceinline__ float q8_score_scale(const Q8AttnParams &p, int shift) {
     return __builtin_ldexpf((p.scale != 0.0f ? __builtin_fabsf(p.scale) : 1.0f) * Q8_LOG2E, -shift);
 }
 
