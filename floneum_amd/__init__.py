@@ -238,6 +238,7 @@ def _bind_native():
     except ModuleNotFoundError:
         return
     _host.bind(Tensor, _View, KvCache, RopeCache, RmsNorm, IntTensor)
+    _host.bind_q8(Q8Tensor, Q8KvCache)
     _native = _host
 
 
@@ -982,6 +983,9 @@ class Q8Tensor:
 
     def narrow(self, dim, start, length):
         """Part of the batch (0), the heads (1) or the rows (2), without a copy."""
+        done = _native.q8_narrow(self, dim, start, length) if _native is not None else None
+        if done is not None:
+            return done
         assert dim in (0, 1, 2) and 0 <= start and start + length <= self.shape[dim]
         shape = list(self.shape)
         shape[dim] = length
@@ -1005,7 +1009,15 @@ class Q8Tensor:
         """New keys `k` into this tensor and new values `v` into `v_cache`, from row `row` on (fhip_q8_append): normalised (k_norm, an
         RmsNorm) and rotated (rope, a RopeCache) on the way, the values as they are, and q, if given, normalised (q_norm) and rotated
         into q_out, in one launch.  lens, counts: device int32 [B] tensors, see the C header.  Returns q_out (None without q)."""
-        a, q_out, keep = _q8_append_args(self.device, k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out, q_out_dtype)
+        if q is not None and q_out is None:
+            q_out = Tensor.empty(self.device, q.shape, q.dtype if q_out_dtype is None else q_out_dtype)
+        if _native is not None:
+            done = _native.q8_append(self, v_cache, row, k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out)
+            if done is not None:
+                if done != OK:
+                    check(done)
+                return q_out
+        a, q_out, keep = _q8_append_args(self.device, k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out)
         a.k, a.v, a.row = self._c(), v_cache._c(), int(row)
         check(lib().fhip_q8_append(self.device.stream, ctypes.byref(a)))
         del keep
@@ -1018,6 +1030,12 @@ class Q8Tensor:
             out = Tensor.empty(self.device, (self.shape[0], self.shape[1], count, self.shape[3]), out_dtype)
         elif rows is not None and rows != out.shape[2]:
             raise InvalidArgument(ERR_INVALID_ARG, "rows differs from out's")
+        if _native is not None:
+            done = _native.q8_dequantize(self, out, row, lens)
+            if done is not None:
+                if done != OK:
+                    check(done)
+                return out
         if out.device is not self.device:
             raise AssertionError("Cannot mix tensors of different devices")
         x, co = self._c(), out._c4()
@@ -1026,7 +1044,7 @@ class Q8Tensor:
         return out
 
 
-def _q8_append_args(device, k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out, q_out_dtype):
+def _q8_append_args(device, k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out):
     if k.dtype != v.dtype:
         raise InvalidArgument(ERR_INVALID_ARG, "new keys and values must share one element type")
     for t in (k, v, q, q_out):
@@ -1044,8 +1062,6 @@ def _q8_append_args(device, k, v, lens, counts, rope, start_pos, interleaved, k_
             keep.append(norm._c())
             setattr(a, name, ctypes.pointer(keep[-1]))
     if q is not None:
-        if q_out is None:
-            q_out = Tensor.empty(device, q.shape, q.dtype if q_out_dtype is None else q_out_dtype)
         a.q, a.q_out, a.q_dtype, a.q_out_dtype = q._c4(), q_out._c4(), q.dtype, q_out.dtype
     elif q_out is not None or q_norm is not None:
         raise InvalidArgument(ERR_INVALID_ARG, "q_out and q_norm need q")
@@ -1066,6 +1082,12 @@ def _q8_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, out_dtyp
         out = Tensor.empty(dev, q.shape, q.dtype if out_dtype is None else out_dtype)
     elif out_dtype is not None and out_dtype != out.dtype:
         raise InvalidArgument(ERR_INVALID_ARG, "out_dtype differs from out's")
+    if _native is not None:
+        done = _native.q8_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, out)
+        if done is not None:
+            if done != OK:
+                check(done)
+            return out
     a = CQ8AttnArgs()
     a.q, a.out, a.k, a.v = q._c4(), out._c4(), k._c(), v._c()
     a.dtype, a.out_dtype, a.scale = q.dtype, out.dtype, float(np.float32(scale))
@@ -1099,6 +1121,7 @@ class Q8KvCache:
             raise FhipError(ERR_UNSUPPORTED, "the device KV cache concatenates along dim 2 ([B,Hkv,seq,D]), "
                                              "the layout kalosm-llama uses")
         self.device = device or Device.default()
+        self.format, self.block_tokens = Q8Format(format), int(block_tokens)
         h = ctypes.c_void_p()
         check(lib().fhip_q8_cache_create(self.device.handle, int(format), block_tokens, max_sequence_len, ctypes.byref(h)))
         self.handle = h
@@ -1125,7 +1148,14 @@ class Q8KvCache:
         return n.value
 
     def _append(self, k, v, rope, start_pos, interleaved, k_norm, q, q_norm, q_out_dtype):
-        a, q_out, keep = _q8_append_args(self.device, k, v, None, None, rope, start_pos, interleaved, k_norm, q, q_norm, None, q_out_dtype)
+        q_out = None if q is None else Tensor.empty(self.device, q.shape, q.dtype if q_out_dtype is None else q_out_dtype)
+        if _native is not None:
+            done = _native.q8_cache_append(self, self.format, self.block_tokens, k, v, None, None, rope, start_pos, interleaved, k_norm, q, q_norm, q_out)
+            if done is not None:
+                if done[0] != OK:
+                    check(done[0])
+                return q_out, done[1], done[2]
+        a, q_out, keep = _q8_append_args(self.device, k, v, None, None, rope, start_pos, interleaved, k_norm, q, q_norm, q_out)
         ka, va = CQ8Tensor(), CQ8Tensor()
         check(lib().fhip_q8_cache_append(self.handle, self.device.stream, ctypes.byref(a), ctypes.byref(ka), ctypes.byref(va)))
         del keep

@@ -25,6 +25,8 @@
 
 namespace fhip {
 
+typedef float float2_at8_t __attribute__((ext_vector_type(2)));
+
 template <int DV>
 struct Q8Dims {
     static constexpr int VW = DV / 64;   // 32-bit words of V per lane and key
@@ -49,6 +51,7 @@ __device__ __forceinline__ float quads_sum(float x) {
 }
 template <int DV, int TERMS, int FMT, int CB, bool MASK, bool BLOCKS>
 __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8AttnParams p) {
+    request_arguments<Q8AttnParams>();
     using Dims = Q8Dims<DV>;
     constexpr int VW = Dims::VW, KS = Dims::KS, TILES = Dims::TILES, COLS = 16 * CB, NBUF = DV <= 128 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float lds_acc[4][16][DV + 4];
@@ -58,15 +61,14 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     const int NC = p.G * p.Sq, blocks = (NC + COLS - 1) / COLS;
     const int split = blockIdx.x;
     const uint32_t unit = blockIdx.y + blockIdx.z * gridDim.y;
-    const int cb = unit % blocks;
-    const int bg = unit / blocks, kvh = bg % p.Hkv, b = bg / p.Hkv;
+    const int bg = blocks == 1 ? unit : unit / blocks, cb = unit - bg * blocks, b = (uint32_t)bg / (uint32_t)p.Hkv, kvh = bg - b * p.Hkv;
     if (b >= p.B) return;
     const int c0 = cb * COLS, c1 = min(c0 + COLS, NC) - 1;
 
     const Q8Range vis = q8_visible(p, b, c0 / p.G, c1 / p.G);
     // this share of the keys
     const int len = vis.hi - vis.lo;
-    const int chunk = (max(p.min_chunk, (int)(((int64_t)len + p.nsplit - 1) / p.nsplit)) + 127) / 128 * 128;
+    const int chunk = (max(p.min_chunk, (int)(((uint32_t)len + p.nsplit - 1) / (uint32_t)p.nsplit)) + 127) / 128 * 128;
     const int64_t lo64 = vis.lo + (int64_t)split * chunk;
     const int lo = (int)min(lo64, (int64_t)vis.hi), hi = (int)min((int64_t)vis.hi, lo64 + chunk);
 
@@ -290,6 +292,20 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         load_v(x, next);
     };
 
+    Q8Query8<TERMS> raw[CB][KS][2];
+#pragma unroll
+    for (int cbk = 0; cbk < CB; cbk++) {
+        const int c = min(c0 + cbk * 16 + n, NC - 1);
+        row[cbk] = c / p.G;
+        const int64_t base = (int64_t)b * p.qs[0] + (int64_t)(kvh * p.G + c - row[cbk] * p.G) * p.qs[1] + (int64_t)row[cbk] * p.qs[2];
+        if (p.q_vec) {
+#pragma unroll
+            for (int s = 0; s < 2 * KS; s++) raw[cbk][s >> 1][s & 1].load(p, base, 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2 * KS; s++) raw[cbk][s >> 1][s & 1].gather(p, base, 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+        }
+    }
     Step steps[NBUF];
     int k0 = lo + 32 * wave;
     if (k0 < hi) {
@@ -302,32 +318,36 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     }
 #pragma unroll
     for (int cbk = 0; cbk < CB; cbk++) {
-        const int c = min(c0 + cbk * 16 + n, NC - 1);
-        row[cbk] = c / p.G;
-        const int head = kvh * p.G + c % p.G;
-        const int64_t base = (int64_t)b * p.qs[0] + (int64_t)head * p.qs[1] + (int64_t)row[cbk] * p.qs[2];
-        float x[KS][2][8], top = 0.0f;
+        if (TERMS == 1 && p.q_dtype == FHIP_F16 && p.scale != 0.0f) {  // as they are
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+            for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int a = 0; a < 2; a++) {
-                q8_load_query8(p, base, 64 * s + 16 * g + 8 * a, x[s][a]);
+                for (int a = 0; a < 2; a++) q[cbk][0][s][a] = raw[cbk][s][a].halves(p, 64 * s + 16 * g + 8 * a);
+            colscale[cbk] = q8_score_scale(p, 0);
+        } else {
+            float x[KS][2][8], top = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[s][a][e]));
-            }
-        const int shift = q8_query_shift(quads_max(top));
+            for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+                for (int a = 0; a < 2; a++) {
+                    raw[cbk][s][a].widen(p, 64 * s + 16 * g + 8 * a, x[s][a]);
 #pragma unroll
-            for (int a = 0; a < 2; a++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    half_t high, low;
-                    q8_query_terms<TERMS>(p, x[s][a][e], shift, high, low);
-                    q[cbk][0][s][a][e] = high;
-                    if constexpr (TERMS == 2) q[cbk][1][s][a][e] = low;
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[s][a][e]));
                 }
-        colscale[cbk] = q8_score_scale(p, shift);
+            const int shift = q8_query_shift(quads_max(top));
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int a = 0; a < 2; a++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        half_t high, low;
+                        q8_query_terms<TERMS>(p, x[s][a][e], shift, high, low);
+                        q[cbk][0][s][a][e] = high;
+                        if constexpr (TERMS == 2) q[cbk][1][s][a][e] = low;
+                    }
+            colscale[cbk] = q8_score_scale(p, shift);
+        }
         const int64_t at = vis.pos0 + row[cbk];
         limit[cbk] = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);
         start[cbk] = (int)(p.window > 0 ? min((int64_t)hi, max((int64_t)0, at - p.window + 1)) : 0);
@@ -350,7 +370,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     }
 #pragma unroll
     for (int cbk = 0; cbk < CB; cbk++) {
-        __syncthreads();
+        lds_barrier();  // (the loads of steps beyond the last one may still be on their way)
 #pragma unroll
         for (int w = 0; w < VW; w++)
 #pragma unroll
@@ -358,7 +378,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                 const float4_t v = {acc[cbk][4 * w][r], acc[cbk][4 * w + 1][r], acc[cbk][4 * w + 2][r], acc[cbk][4 * w + 3][r]};
                 *(float4_t *)&lds_acc[wave][n][Dims::dim(4 * g + r, w, 0)] = v;
             }
-        __syncthreads();
+        lds_barrier();
         const int col = threadIdx.x >> 4, sub = threadIdx.x & 15, c = c0 + cbk * 16 + col;
         if (c < NC) {
             float M = -INFINITY, L = 0.0f, f[4];
@@ -370,9 +390,10 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                 f[x] = __builtin_amdgcn_exp2f(lds_m[x][cbk * 16 + col] - ref);
                 L += lds_l[x][cbk * 16 + col] * f[x];
             }
-            const int head = kvh * p.G + c % p.G;
-            const int64_t o = (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)(c / p.G) * p.os[2];
+            const int at = c / p.G;
+            const int64_t o = (int64_t)b * p.os[0] + (int64_t)(kvh * p.G + c - at * p.G) * p.os[1] + (int64_t)at * p.os[2];
             const int64_t share = ((int64_t)bg * p.nsplit + split) * NC + c;
+            const float inv = 1.0f / L;
             for (int d = 4 * sub; d < p.D; d += 64) {
                 float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -380,7 +401,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                 if (p.nsplit > 1) {
                     *(float4_t *)(p.partials + share * DV + d) = v;
                 } else {
-                    q8_store4_any(p, o + d * p.os[3], v / L);
+                    q8_store4_any(p, o + d * p.os[3], v * inv);
                 }
             }
             if (p.nsplit > 1 && sub == 0) {
@@ -391,47 +412,62 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     }
 }
 
-// Joins the shares of a (batch, kv head, column).  A workgroup of 256 lanes per column: the shares' maxima and sums are read at once, one a lane, and
-// their weights kept in LDS; then groups of DV / 4 lanes, four dims each, add up every GROUPS-th share.
-template <int DV>
+// Joins the shares of a (batch, kv head, column): groups of lanes, four dims a lane, add up every GROUPS-th share.  Bound by one memory latency after
+// another, so up to 64 shares are requested at once: a lane's sums of its shares, and by every wavefront the shares' maxima and sums, one a lane, whose
+// weights it keeps to itself.
+template <int DV, bool FEW>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
-    constexpr int LPG = DV == 192 ? 64 : DV / 4, GROUPS = 256 / LPG;
-    __shared__ float weight[Q8_MAX_SHARES], red[8];
+    request_arguments<Q8AttnParams>();
+    constexpr int LPG = DV == 192 ? 64 : DV / 4, GROUPS = 256 / LPG, MOST = 64 / GROUPS;
+    __shared__ float weight[FEW ? 4 * 64 : Q8_MAX_SHARES], red[8];
     __shared__ __attribute__((aligned(16))) float sums[GROUPS][4 * LPG];
     const int NC = p.G * p.Sq, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t at = blockIdx.x, bg = at / NC;
+    const uint32_t at = blockIdx.x, bg = at / (uint32_t)NC;
     const int c = (int)(at - bg * NC);
     const float *const ml = p.partials + (int64_t)p.B * p.Hkv * p.nsplit * NC * DV;
-    const int64_t first = bg * p.nsplit * NC + c;
-    float m[Q8_MAX_SHARES / 256], l[Q8_MAX_SHARES / 256], M = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < Q8_MAX_SHARES / 256; i++) {
-        const int s = tid + 256 * i;
-        m[i] = -INFINITY, l[i] = 0.0f;
-        if (s < p.nsplit) m[i] = ml[2 * (first + (int64_t)s * NC)], l[i] = ml[2 * (first + (int64_t)s * NC) + 1];
-        M = fmaxf(M, m[i]);
-    }
-    M = wave_max(M);
-    if (lane == 0) red[wave] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
-#pragma unroll
-    for (int i = 0; i < Q8_MAX_SHARES / 256; i++) {
-        const float f = __builtin_amdgcn_exp2f(m[i] - ref);
-        if (tid + 256 * i < p.nsplit) weight[tid + 256 * i] = f;
-        L += l[i] * f;
-    }
-    L = wave_sum(L);
-    if (lane == 0) red[4 + wave] = L;
-    __syncthreads();
-    L = (red[4] + red[5]) + (red[6] + red[7]);
+    const int64_t first = (int64_t)bg * p.nsplit * NC + c, step = (int64_t)NC * DV;
     const int group = tid / LPG, d = 4 * (tid % LPG);
+    const float *const part = p.partials + first * DV + (d < p.D ? d : 0);
     float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (d < p.D) {
-        const float *const part = p.partials + first * DV + d;
-        const int64_t step = (int64_t)NC * DV;
+    float L;
+    if constexpr (FEW) {
+        const float2_at8_t own = *(const float2_at8_t *)(ml + 2 * (first + (int64_t)min(lane, p.nsplit - 1) * NC));
+        float4_t x[MOST];
+#pragma unroll
+        for (int i = 0; i < MOST; i++) x[i] = *(const float4_t *)(part + min(group + i * GROUPS, p.nsplit - 1) * step);
+        const float M = wave_max(own[0]), ref = M == -INFINITY ? 0.0f : M;
+        const float f = lane < p.nsplit ? __builtin_amdgcn_exp2f(own[0] - ref) : 0.0f;
+        weight[64 * wave + lane] = f;
+        L = wave_sum(own[1] * f);
+        wave_lds_sync();
+#pragma unroll
+        for (int i = 0; i < MOST; i++)
+            if (group + i * GROUPS < p.nsplit) v += x[i] * weight[64 * wave + group + i * GROUPS];
+    } else {
+        float m[Q8_MAX_SHARES / 256], l[Q8_MAX_SHARES / 256], M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < Q8_MAX_SHARES / 256; i++) {
+            const int s = tid + 256 * i;
+            m[i] = -INFINITY, l[i] = 0.0f;
+            if (s < p.nsplit) m[i] = ml[2 * (first + (int64_t)s * NC)], l[i] = ml[2 * (first + (int64_t)s * NC) + 1];
+            M = fmaxf(M, m[i]);
+        }
+        M = wave_max(M);
+        if (lane == 0) red[wave] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float ref = M == -INFINITY ? 0.0f : M;
+        L = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Q8_MAX_SHARES / 256; i++) {
+            const float f = __builtin_amdgcn_exp2f(m[i] - ref);
+            if (tid + 256 * i < p.nsplit) weight[tid + 256 * i] = f;
+            L += l[i] * f;
+        }
+        L = wave_sum(L);
+        if (lane == 0) red[4 + wave] = L;
+        __syncthreads();
+        L = (red[4] + red[5]) + (red[6] + red[7]);
 #pragma unroll 4
         for (int s = group; s < p.nsplit; s += GROUPS) v += *(const float4_t *)(part + s * step) * weight[s];
     }
@@ -440,19 +476,24 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
     if (tid >= LPG || d >= p.D) return;
 #pragma unroll
     for (int g = 1; g < GROUPS; g++) v += *(const float4_t *)&sums[g][d];
-    const int b = (int)(bg / p.Hkv), head = (int)(bg % p.Hkv) * p.G + c % p.G;
-    q8_store4_any(p, (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)(c / p.G) * p.os[2] + d * p.os[3], v / L);
+    const int b = (int)(bg / p.Hkv), row = c / p.G, head = (int)(bg - b * p.Hkv) * p.G + c - row * p.G;
+    q8_store4_any(p, (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)row * p.os[2] + d * p.os[3], v * (1.0f / L));
 }
 
 static int q8_padded_dim(int D) { return (D + 63) / 64 * 64; }
 
-int launch_q8_merge(const Q8AttnParams &p, hipStream_t stream) {
+template <int DV>
+static void launch_merge_dims(const Q8AttnParams &p, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)p.B * p.H * p.Sq));
+    if (p.nsplit <= 64) hipLaunchKernelGGL((q8_merge_kernel<DV, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((q8_merge_kernel<DV, false>), grid, dim3(256), 0, stream, p);
+}
+int launch_q8_merge(const Q8AttnParams &p, hipStream_t stream) {
     switch (q8_padded_dim(p.D)) {
-        case 64: hipLaunchKernelGGL(q8_merge_kernel<64>, grid, dim3(256), 0, stream, p); break;
-        case 128: hipLaunchKernelGGL(q8_merge_kernel<128>, grid, dim3(256), 0, stream, p); break;
-        case 192: hipLaunchKernelGGL(q8_merge_kernel<192>, grid, dim3(256), 0, stream, p); break;
-        default: hipLaunchKernelGGL(q8_merge_kernel<256>, grid, dim3(256), 0, stream, p);
+        case 64: launch_merge_dims<64>(p, stream); break;
+        case 128: launch_merge_dims<128>(p, stream); break;
+        case 192: launch_merge_dims<192>(p, stream); break;
+        default: launch_merge_dims<256>(p, stream);
     }
     FHIP_HIP_CHECK(hipGetLastError());
     return FHIP_OK;

@@ -41,6 +41,7 @@ __device__ __forceinline__ half8_t q8_widen8_pairs(half2_t a, half2_t b, half2_t
 // Waits: `WAVES_PER_SIMD` wavefronts share a SIMD's registers.
 template <int DV, int TERMS, int FMT, int WAVES, bool MASK>
 __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kernel(Q8AttnParams p) {
+    request_arguments<Q8AttnParams>();
     constexpr int COLS = 32 * WAVES, STEPS = DV / 16, DT = DV / 32, UNITS = DV / 16, CHUNKS = DV / 8;
     // LDS, 16-byte chunks: K [key][chunk of 8 dims], V [dim][chunk of 8 keys]; the chunk is turned by the row so that 16 rows' pieces lie in
     // different banks
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
 
     const Q8Range vis = q8_visible(p, b, c0 / p.G, c1 / p.G);
     const int len = vis.hi - vis.lo;
-    const int share = (max(p.min_chunk, (int)(((int64_t)len + p.nsplit - 1) / p.nsplit)) + 63) / 64 * 64;
+    const int share = (max(p.min_chunk, (int)(((uint32_t)len + p.nsplit - 1) / (uint32_t)p.nsplit)) + 63) / 64 * 64;
     const int64_t lo64 = vis.lo + (int64_t)split * share;
     const int lo = (int)min(lo64, (int64_t)vis.hi), hi = (int)min((int64_t)vis.hi, lo64 + share);
 
@@ -73,24 +74,38 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
     float colscale;
     {  // lane half h holds dims 16 i + 8 h .. + 7 of step i
         const int64_t base = (int64_t)b * p.qs[0] + (int64_t)head * p.qs[1] + (int64_t)row * p.qs[2];
-        float x[STEPS][8], top = 0.0f;
+        Q8Query8<TERMS> raw[STEPS];
+        if (p.q_vec) {
 #pragma unroll
-        for (int i = 0; i < STEPS; i++) {
-            q8_load_query8(p, base, 16 * i + 8 * h, x[i]);
+            for (int i = 0; i < STEPS; i++) raw[i].load(p, base, 16 * i + 8 * h);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[i][e]));
+            for (int i = 0; i < STEPS; i++) raw[i].gather(p, base, 16 * i + 8 * h);
         }
-        const int shift = q8_query_shift(fmaxf(top, xor32(top)));
+        if (TERMS == 1 && p.q_dtype == FHIP_F16 && p.scale != 0.0f) {  // as they are
 #pragma unroll
-        for (int i = 0; i < STEPS; i++)
+            for (int i = 0; i < STEPS; i++) q[0][i] = raw[i].halves(p, 16 * i + 8 * h);
+            colscale = q8_score_scale(p, 0);
+        } else {
+            float x[STEPS][8], top = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                half_t high, low;
-                q8_query_terms<TERMS>(p, x[i][e], shift, high, low);
-                q[0][i][e] = high;
-                if constexpr (TERMS == 2) q[1][i][e] = low;
+            for (int i = 0; i < STEPS; i++) {
+                raw[i].widen(p, 16 * i + 8 * h, x[i]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[i][e]));
             }
-        colscale = q8_score_scale(p, shift);
+            const int shift = q8_query_shift(fmaxf(top, xor32(top)));
+#pragma unroll
+            for (int i = 0; i < STEPS; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    half_t high, low;
+                    q8_query_terms<TERMS>(p, x[i][e], shift, high, low);
+                    q[0][i][e] = high;
+                    if constexpr (TERMS == 2) q[1][i][e] = low;
+                }
+            colscale = q8_score_scale(p, shift);
+        }
     }
     const int64_t at = vis.pos0 + row;
     const int limit = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);

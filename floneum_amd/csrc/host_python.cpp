@@ -21,10 +21,11 @@ namespace {
 // The classes of the mirror and where their instances keep what is read here (set by `bind`).
 struct Slots {
     PyTypeObject *type = nullptr;
-    Py_ssize_t at[5] = {};
+    Py_ssize_t at[10] = {};
 };
 Slots tensor, view;  // Tensor: buffer, dtype, shape, strides, offset; _View: device, ptr, keepalive
-PyTypeObject *cache_type, *rope_type, *norm_type, *lens_type;
+Slots q8;            // Q8Tensor: codes, scales, shape, format, block_tokens, strides, offset, scale_strides, scale_offset, first
+PyTypeObject *cache_type, *rope_type, *norm_type, *lens_type, *q8_cache_type;
 
 PyObject *n_ptr, *n_device, *n_buffer, *n_offset, *n_shape, *n_dtype, *n_stream, *n_value, *n_compute_units, *n_workspace, *n_handle, *n_cos,
     *n_sin, *n_rows, *n_weight, *n_bias, *n_eps, *s_i32;
@@ -116,9 +117,9 @@ PyObject *instance(const Slots &s, int n, PyObject *const *values) {
     return o;
 }
 
-PyObject *tuple4(const uint32_t *u, const int64_t *i) {
-    PyObject *t = PyTuple_New(4);
-    for (int n = 0; t && n < 4; n++) {
+PyObject *tuple_of(int count, const uint32_t *u, const int64_t *i) {
+    PyObject *t = PyTuple_New(count);
+    for (int n = 0; t && n < count; n++) {
         PyObject *v = u ? PyLong_FromUnsignedLong(u[n]) : PyLong_FromLongLong(i[n]);
         if (!v) {
             Py_DECREF(t);
@@ -128,6 +129,8 @@ PyObject *tuple4(const uint32_t *u, const int64_t *i) {
     }
     return t;
 }
+
+PyObject *tuple4(const uint32_t *u, const int64_t *i) { return tuple_of(4, u, i); }
 
 // the tensor that a descriptor the library filled in describes: a view of `cache`'s memory
 PyObject *cache_tensor(PyObject *cache, PyObject *device, PyObject *dtype, const fhip_tensor4 &c) {
@@ -139,6 +142,30 @@ PyObject *cache_tensor(PyObject *cache, PyObject *device, PyObject *dtype, const
     if (!v.o || !shape.o || !strides.o || !offset.o) return nullptr;
     PyObject *tv[5] = {v.o, dtype, shape.o, strides.o, offset.o};
     return instance(tensor, 5, tv);
+}
+
+// (causal, q_pos_offset, window)
+bool analytic_of(PyObject *o, fhip_analytic_mask *m) {
+    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 3 || !PyBool_Check(PyTuple_GET_ITEM(o, 0)) ||
+        !as_i64(PyTuple_GET_ITEM(o, 1), &m->q_pos_offset) || !as_i64(PyTuple_GET_ITEM(o, 2), &m->window))
+        return false;
+    m->enabled = 1;
+    m->causal = PyTuple_GET_ITEM(o, 0) == Py_True;
+    return true;
+}
+
+// an IntTensor of so many sequences
+bool lens_of(PyObject *o, uint32_t sequences, const int32_t **out) {
+    if (Py_TYPE(o) != lens_type) return false;
+    Ref dtype(PyObject_GetAttr(o, n_dtype)), shape(PyObject_GetAttr(o, n_shape)), memory(PyObject_GetAttr(o, n_buffer));
+    uint64_t ptr, offset;
+    uint32_t count;
+    if (!dtype.o || !shape.o || !memory.o || !PyUnicode_Check(dtype.o) || PyUnicode_Compare(dtype.o, s_i32) != 0 ||
+        !PyTuple_CheckExact(shape.o) || PyTuple_GET_SIZE(shape.o) != 1 || !as_narrow(PyTuple_GET_ITEM(shape.o, 0), &count) ||
+        count != sequences || !attr_u64(memory.o, n_ptr, &ptr) || !attr_u64(o, n_offset, &offset))
+        return not_plain();
+    *out = (const int32_t *)(uintptr_t)ptr + offset;
+    return true;
 }
 
 // The descriptor of attention(q, k, v, scale, mask, analytic, kv_lens, out_dtype, force_kernel, out), without a workspace (and without a
@@ -180,26 +207,8 @@ PyObject *attention_args(PyObject *const *a, fhip_attn_args *args) {
             args->mask_intervals = (const void *)(uintptr_t)ptr;
         }
     }
-    if (a[5] != Py_None) {
-        if (!PyTuple_CheckExact(a[5]) || PyTuple_GET_SIZE(a[5]) != 3 || !PyBool_Check(PyTuple_GET_ITEM(a[5], 0)) ||
-            !as_i64(PyTuple_GET_ITEM(a[5], 1), &args->analytic.q_pos_offset) || !as_i64(PyTuple_GET_ITEM(a[5], 2), &args->analytic.window))
-            return nullptr;
-        args->analytic.enabled = 1;
-        args->analytic.causal = PyTuple_GET_ITEM(a[5], 0) == Py_True;
-    }
-    if (a[6] != Py_None) {
-        if (Py_TYPE(a[6]) != lens_type) return nullptr;
-        Ref dtype(PyObject_GetAttr(a[6], n_dtype)), shape(PyObject_GetAttr(a[6], n_shape)), memory(PyObject_GetAttr(a[6], n_buffer));
-        uint64_t ptr, offset;
-        uint32_t sequences;
-        if (!dtype.o || !shape.o || !memory.o || !PyUnicode_Check(dtype.o) || PyUnicode_Compare(dtype.o, s_i32) != 0 ||
-            !PyTuple_CheckExact(shape.o) || PyTuple_GET_SIZE(shape.o) != 1 || !as_narrow(PyTuple_GET_ITEM(shape.o, 0), &sequences) ||
-            sequences != args->q.shape[0] || !attr_u64(memory.o, n_ptr, &ptr) || !attr_u64(a[6], n_offset, &offset)) {
-            not_plain();
-            return nullptr;
-        }
-        args->kv_lens = (const int32_t *)(uintptr_t)ptr + offset;
-    }
+    if (a[5] != Py_None && !analytic_of(a[5], &args->analytic)) return nullptr;
+    if (a[6] != Py_None && !lens_of(a[6], args->q.shape[0], &args->kv_lens)) return nullptr;
     Py_INCREF(device.o);
     return device.o;
 }
@@ -351,6 +360,227 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return PyLong_FromLong(rc);
 }
 
+// ---- the 8-bit cache -------------------------------------------------------------------------------------------------------
+
+bool memory_of(PyObject *o, PyObject *device, void **out) {
+    uint64_t ptr;
+    if (!o || !attr_u64(o, n_ptr, &ptr)) return false;
+    *out = (void *)(uintptr_t)ptr;
+    Ref d(PyObject_GetAttr(o, n_device));
+    return d.o ? d.o == device : not_plain();
+}
+template <int N, typename T>
+bool numbers(PyObject *t, T *out) {
+    if (!t || !PyTuple_CheckExact(t) || PyTuple_GET_SIZE(t) != N) return false;
+    for (int i = 0; i < N; i++)
+        if (!as_narrow(PyTuple_GET_ITEM(t, i), &out[i])) return false;
+    return true;
+}
+bool describe_q8(PyObject *t, fhip_q8_tensor *c, PyObject *device) {
+    memset(c, 0, sizeof(*c));
+    if (Py_TYPE(t) != q8.type) return false;
+    const Ref codes(Py_XNewRef(slot(q8, t, 0))), scales(Py_XNewRef(slot(q8, t, 1))), shape(Py_XNewRef(slot(q8, t, 2))),
+        strides(Py_XNewRef(slot(q8, t, 5))), steps(Py_XNewRef(slot(q8, t, 7)));
+    int32_t format;
+    if (!memory_of(codes.o, device, &c->codes) || !memory_of(scales.o, device, &c->scales) || !numbers<4>(shape.o, c->shape) ||
+        !numbers<3>(strides.o, c->stride) || !numbers<2>(steps.o, c->scale_stride) || !as_narrow(slot(q8, t, 3), &format) ||
+        !as_narrow(slot(q8, t, 4), &c->block_tokens) || !as_u64(slot(q8, t, 6), &c->offset) || !as_u64(slot(q8, t, 8), &c->scale_offset) ||
+        !as_narrow(slot(q8, t, 9), &c->first))
+        return false;
+    c->format = (fhip_q8_format)format;
+    return true;
+}
+
+// q8_narrow(tensor, dim, start, length): a Q8Tensor, or None
+PyObject *q8_narrow(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    uint32_t dim, start, length, shape[4], block, first;
+    int64_t strides[3], steps[2];
+    uint64_t offset, scale_offset;
+    if (n != 4 || Py_TYPE(a[0]) != q8.type || !as_narrow(a[1], &dim) || dim > 2 || !as_narrow(a[2], &start) || !as_narrow(a[3], &length) ||
+        !numbers<4>(slot(q8, a[0], 2), shape) || (uint64_t)start + length > shape[dim] || !numbers<3>(slot(q8, a[0], 5), strides) ||
+        !numbers<2>(slot(q8, a[0], 7), steps) || !as_narrow(slot(q8, a[0], 4), &block) || block == 0 || !as_u64(slot(q8, a[0], 6), &offset) ||
+        !as_u64(slot(q8, a[0], 8), &scale_offset) || !as_narrow(slot(q8, a[0], 9), &first))
+        Py_RETURN_NONE;
+    shape[dim] = length;
+    offset += (uint64_t)((int64_t)start * strides[dim]);
+    if (dim == 2) {
+        scale_offset += ((uint64_t)first + start) / block;
+        first = (uint32_t)(((uint64_t)first + start) % block);
+    } else {
+        scale_offset += (uint64_t)((int64_t)start * steps[dim]);
+    }
+    Ref extents(tuple4(shape, nullptr)), at(PyLong_FromUnsignedLongLong(offset)), scale_at(PyLong_FromUnsignedLongLong(scale_offset)),
+        place(PyLong_FromUnsignedLong(first));
+    if (!extents.o || !at.o || !scale_at.o || !place.o) return nullptr;
+    PyObject *const values[10] = {slot(q8, a[0], 0), slot(q8, a[0], 1), extents.o, slot(q8, a[0], 3), slot(q8, a[0], 4),
+                                  slot(q8, a[0], 5), at.o, slot(q8, a[0], 7), scale_at.o, place.o};
+    return instance(q8, 10, values);
+}
+
+// q8_dequantize(tensor, out, row, lens): the library's status, or None
+PyObject *q8_dequantize(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 4 || Py_TYPE(a[1]) != tensor.type || !slot(tensor, a[1], 0)) Py_RETURN_NONE;
+    const Ref memory(Py_NewRef(slot(tensor, a[1], 0)));
+    Ref device(PyObject_GetAttr(memory.o, n_device));
+    fhip_q8_tensor x;
+    fhip_tensor4 out;
+    int32_t dtype;
+    uint64_t row;
+    const int32_t *lens = nullptr;
+    void *stream;
+    if (!device.o || !describe_q8(a[0], &x, device.o) || !describe<4>(a[1], &out, &dtype, nullptr) || !as_u64(a[2], &row) ||
+        (a[3] != Py_None && !lens_of(a[3], x.shape[0], &lens)) || !attr_handle(device.o, n_stream, &stream)) {
+        not_plain();
+        Py_RETURN_NONE;
+    }
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = fhip_q8_dequantize((fhip_stream *)stream, &x, row, lens, &out, (fhip_dtype)dtype);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+struct Q8NewRows {
+    fhip_q8_append_args args;
+    fhip_rope_tables tables;
+    fhip_rms_norm q_norm, k_norm;
+};
+// k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out
+bool q8_new_rows(PyObject *const *a, PyObject *device, Q8NewRows *c) {
+    memset(c, 0, sizeof(*c));
+    int32_t k_dtype, v_dtype, q_dtype, out_dtype;
+    if (!describe<4>(a[0], &c->args.k_new, &k_dtype, device) || !describe<4>(a[1], &c->args.v_new, &v_dtype, device) || k_dtype != v_dtype) return false;
+    c->args.in_dtype = (fhip_dtype)k_dtype;
+    const uint32_t B = c->args.k_new.shape[0];
+    if ((a[2] != Py_None && !lens_of(a[2], B, &c->args.lens)) || (a[3] != Py_None && !lens_of(a[3], B, &c->args.counts))) return false;
+    if (a[4] != Py_None) {
+        void *cos, *sin;
+        if (Py_TYPE(a[4]) != rope_type || !PyBool_Check(a[6]) || !attr_memory(a[4], n_cos, &cos) || !attr_memory(a[4], n_sin, &sin) ||
+            !attr_u64(a[4], n_rows, &c->tables.table_rows) || !as_u64(a[5], &c->tables.start_pos))
+            return false;
+        c->tables.cos = (const float *)cos, c->tables.sin = (const float *)sin, c->tables.interleaved = a[6] == Py_True;
+        c->args.rope = &c->tables;
+    }
+    if (a[7] != Py_None) {
+        if (!norm_of(a[7], &c->k_norm)) return false;
+        c->args.k_norm = &c->k_norm;
+    }
+    if (a[8] == Py_None) return a[9] == Py_None && a[10] == Py_None;
+    if (!describe<4>(a[8], &c->args.q, &q_dtype, device) || !describe<4>(a[10], &c->args.q_out, &out_dtype, device)) return false;
+    c->args.q_dtype = (fhip_dtype)q_dtype, c->args.q_out_dtype = (fhip_dtype)out_dtype;
+    if (a[9] != Py_None) {
+        if (!norm_of(a[9], &c->q_norm)) return false;
+        c->args.q_norm = &c->q_norm;
+    }
+    return true;
+}
+
+// q8_append(keys, values, row, and what q8_new_rows takes): the library's status, or None
+PyObject *q8_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 14 || Py_TYPE(a[0]) != q8.type || !slot(q8, a[0], 0)) Py_RETURN_NONE;
+    const Ref memory(Py_NewRef(slot(q8, a[0], 0)));
+    Ref device(PyObject_GetAttr(memory.o, n_device));
+    Q8NewRows c;
+    void *stream;
+    if (!device.o || !q8_new_rows(a + 3, device.o, &c) || !describe_q8(a[0], &c.args.k, device.o) || !describe_q8(a[1], &c.args.v, device.o) ||
+        !as_u64(a[2], &c.args.row) || !attr_handle(device.o, n_stream, &stream)) {
+        not_plain();
+        Py_RETURN_NONE;
+    }
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = fhip_q8_append((fhip_stream *)stream, &c.args);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+// the Q8Tensor that a descriptor the library filled in describes: a view of `cache`'s memory
+PyObject *q8_cache_tensor(PyObject *cache, PyObject *device, PyObject *format, PyObject *block, const fhip_q8_tensor &c) {
+    Ref codes_at(PyLong_FromUnsignedLongLong((uintptr_t)c.codes)), scales_at(PyLong_FromUnsignedLongLong((uintptr_t)c.scales));
+    if (!codes_at.o || !scales_at.o) return nullptr;
+    PyObject *const cv[3] = {device, codes_at.o, cache}, *const sv[3] = {device, scales_at.o, cache};
+    Ref codes(instance(view, 3, cv)), scales(instance(view, 3, sv)), shape(tuple4(c.shape, nullptr)), strides(tuple_of(3, nullptr, c.stride)),
+        offset(PyLong_FromUnsignedLongLong(c.offset)), steps(tuple_of(2, nullptr, c.scale_stride)),
+        scale_offset(PyLong_FromUnsignedLongLong(c.scale_offset)), first(PyLong_FromUnsignedLong(c.first));
+    if (!codes.o || !scales.o || !shape.o || !strides.o || !offset.o || !steps.o || !scale_offset.o || !first.o) return nullptr;
+    PyObject *const values[10] = {codes.o, scales.o, shape.o, format, block, strides.o, offset.o, steps.o, scale_offset.o, first.o};
+    return instance(q8, 10, values);
+}
+
+// q8_cache_append(cache, format, block_tokens, and what q8_new_rows takes): (status, keys, values), or None
+PyObject *q8_cache_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 14 || Py_TYPE(a[0]) != q8_cache_type) Py_RETURN_NONE;
+    Ref device(PyObject_GetAttr(a[0], n_device));
+    Q8NewRows c;
+    void *handle, *stream;
+    if (!device.o || !q8_new_rows(a + 3, device.o, &c) || !attr_handle(a[0], n_handle, &handle) || !attr_handle(device.o, n_stream, &stream)) {
+        not_plain();
+        Py_RETURN_NONE;
+    }
+    fhip_q8_tensor keys, values;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = fhip_q8_cache_append((fhip_q8_cache *)handle, (fhip_stream *)stream, &c.args, &keys, &values);
+    Py_END_ALLOW_THREADS
+    if (rc != FHIP_OK) return Py_BuildValue("iOO", rc, Py_None, Py_None);
+    Ref k(q8_cache_tensor(a[0], device.o, a[1], a[2], keys)), v(q8_cache_tensor(a[0], device.o, a[1], a[2], values));
+    if (!k.o || !v.o) return nullptr;
+    return Py_BuildValue("iOO", rc, k.o, v.o);
+}
+
+// the scratch that a call needs, from device.workspace: 1, 0 where the general way has to take the call, -1 with an exception
+int workspace_of(PyObject *device, size_t need, void **ptr, size_t *bytes) {
+    Ref size(PyLong_FromSize_t(need));
+    if (!size.o) return -1;
+    Ref ws(PyObject_CallMethodOneArg(device, n_workspace, size.o));
+    if (!ws.o) return -1;
+    uint64_t p, b;
+    if (!PyTuple_CheckExact(ws.o) || PyTuple_GET_SIZE(ws.o) != 2 || !as_u64(PyTuple_GET_ITEM(ws.o, 0), &p) || !as_u64(PyTuple_GET_ITEM(ws.o, 1), &b)) return 0;
+    *ptr = (void *)(uintptr_t)p, *bytes = b;
+    return 1;
+}
+
+// q8_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, out): the library's status, or None
+PyObject *q8_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 9 || Py_TYPE(a[0]) != tensor.type || !slot(tensor, a[0], 0)) Py_RETURN_NONE;
+    const Ref memory(Py_NewRef(slot(tensor, a[0], 0)));
+    Ref device(PyObject_GetAttr(memory.o, n_device));
+    fhip_q8_attn_args args;
+    memset(&args, 0, sizeof(args));
+    int32_t dtype, out_dtype, mask_dtype, kind;
+    void *stream;
+    uint64_t cus;
+    if (!device.o || !describe<4>(a[0], &args.q, &dtype, nullptr) || !describe_q8(a[1], &args.k, device.o) || !describe_q8(a[2], &args.v, device.o) ||
+        !describe<4>(a[8], &args.out, &out_dtype, nullptr) || !PyFloat_Check(a[3]) || !(std::fabs(PyFloat_AS_DOUBLE(a[3])) < 1e38)) {
+        not_plain();
+        Py_RETURN_NONE;
+    }
+    args.dtype = (fhip_dtype)dtype, args.out_dtype = (fhip_dtype)out_dtype, args.scale = (float)PyFloat_AS_DOUBLE(a[3]);
+    if (a[4] != Py_None) {
+        if (!PyTuple_CheckExact(a[4]) || PyTuple_GET_SIZE(a[4]) < 2 || !describe<2>(PyTuple_GET_ITEM(a[4], 0), &args.mask, &mask_dtype, device.o) ||
+            mask_dtype != dtype || !as_narrow(PyTuple_GET_ITEM(a[4], 1), &kind))
+            Py_RETURN_NONE;
+        args.mask_kind = (fhip_mask_kind)kind;
+    }
+    if ((a[5] != Py_None && !analytic_of(a[5], &args.analytic)) || (a[6] != Py_None && !lens_of(a[6], args.q.shape[0], &args.kv_lens)) ||
+        (a[7] != Py_None && !lens_of(a[7], args.q.shape[0], &args.q_positions)) || !attr_handle(device.o, n_stream, &stream) ||
+        !attr_u64(device.o, n_compute_units, &cus))
+        Py_RETURN_NONE;
+    size_t need = 0;
+    int rc = fhip_q8_attention_workspace_bytes(&args, (int32_t)cus, &need);
+    if (rc == FHIP_OK && need) {
+        const int got = workspace_of(device.o, need, &args.workspace, &args.workspace_bytes);
+        if (got < 0) return nullptr;
+        if (got == 0) Py_RETURN_NONE;
+    }
+    if (rc == FHIP_OK) {
+        Py_BEGIN_ALLOW_THREADS
+        rc = fhip_q8_attention((fhip_stream *)stream, &args);
+        Py_END_ALLOW_THREADS
+    }
+    return PyLong_FromLong(rc);
+}
+
 bool find(Slots *s, PyObject *type, int n, const char *const *names) {
     s->type = (PyTypeObject *)type;
     for (int i = 0; i < n; i++) {
@@ -378,7 +608,23 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+// bind_q8(Q8Tensor, Q8KvCache): the same for the 8-bit cache
+PyObject *bind_q8(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    static const char *const of_q8[] = {"codes", "scales", "shape", "format", "block_tokens", "strides", "offset", "scale_strides", "scale_offset", "first"};
+    if (n != 2 || !PyType_Check(a[0]) || !PyType_Check(a[1])) return PyErr_Format(PyExc_TypeError, "bind_q8 takes two classes");
+    Py_INCREF(a[0]), Py_INCREF(a[1]);
+    if (!find(&q8, a[0], 10, of_q8)) return nullptr;
+    q8_cache_type = (PyTypeObject *)a[1];
+    Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
+    {"bind_q8", (PyCFunction)(void *)bind_q8, METH_FASTCALL, nullptr},
+    {"q8_narrow", (PyCFunction)(void *)q8_narrow, METH_FASTCALL, nullptr},
+    {"q8_dequantize", (PyCFunction)(void *)q8_dequantize, METH_FASTCALL, nullptr},
+    {"q8_append", (PyCFunction)(void *)q8_append, METH_FASTCALL, nullptr},
+    {"q8_cache_append", (PyCFunction)(void *)q8_cache_append, METH_FASTCALL, nullptr},
+    {"q8_attention", (PyCFunction)(void *)q8_attention, METH_FASTCALL, nullptr},
     {"bind", (PyCFunction)(void *)bind, METH_FASTCALL, nullptr},
     {"attention", (PyCFunction)(void *)attention, METH_FASTCALL, nullptr},
     {"contiguous", (PyCFunction)(void *)contiguous, METH_FASTCALL, nullptr},

@@ -64,31 +64,56 @@ __device__ __forceinline__ Q8Range q8_visible(const Q8AttnParams &p, int b, int 
     return r;
 }
 
-// eight consecutive dims of a query row, zeros beyond head_dim
-__device__ __forceinline__ void q8_load_query8(const Q8AttnParams &p, int64_t base, int d0, float (&x)[8]) {
-    if (d0 >= p.D) {
+// Eight consecutive dims of a query row as they lie in memory: f32 (TERMS 2) or 16-bit ones.
+template <int TERMS>
+struct Q8Query8 {
+    uint32_t w[4 * TERMS];
+    // d0: the first of them; pieces beyond head_dim are read from the row's start
+    __device__ __forceinline__ void load(const Q8AttnParams &p, int64_t base, int d0) {
+        const int d = d0 < p.D ? d0 : 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = 0.0f;
-    } else if (p.q_vec && p.q_dtype == FHIP_F32) {
-        const float4_t a = *(const float4_t *)((const float *)p.q + base + d0), b = *(const float4_t *)((const float *)p.q + base + d0 + 4);
+        for (int i = 0; i < 2; i++) {
+            if constexpr (TERMS == 2) {
+                const uint4_t v = *(const uint4_t *)((const float *)p.q + base + d + 4 * i);
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = a[e], x[4 + e] = b[e];
-    } else if (p.q_vec) {
-        const uint2_t a = *(const uint2_t *)((const uint16_t *)p.q + base + d0), b = *(const uint2_t *)((const uint16_t *)p.q + base + d0 + 4);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint32_t w = e < 4 ? a[e >> 1] : b[(e - 4) >> 1], bits = e & 1 ? w >> 16 : w & 0xffffu;
-            x[e] = p.q_dtype == FHIP_F16 ? (float)__builtin_bit_cast(half_t, (uint16_t)bits) : __uint_as_float(bits << 16);
-        }
-    } else {
-#pragma unroll 1
-        for (int e = 0; e < 8; e++) {
-            const float v = q8_load_any(p.q, base + (d0 + e) * p.qs[3], p.q_dtype);
-#pragma unroll
-            for (int y = 0; y < 8; y++) x[y] = y == e ? v : x[y];
+                for (int e = 0; e < 4; e++) w[4 * i + e] = v[e];
+            } else {
+                const uint2_t v = *(const uint2_t *)((const uint16_t *)p.q + base + d + 4 * i);
+                w[2 * i] = v[0], w[2 * i + 1] = v[1];
+            }
         }
     }
-}
+    // the same of rows with any stride
+    __device__ __forceinline__ void gather(const Q8AttnParams &p, int64_t base, int d0) {
+        const int d = d0 < p.D ? d0 : 0;
+        if constexpr (TERMS == 2) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = ((const uint32_t *)p.q)[base + (d + e) * p.qs[3]];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                w[e] = (uint32_t)((const uint16_t *)p.q)[base + (d + 2 * e) * p.qs[3]] |
+                       (uint32_t)((const uint16_t *)p.q)[base + (d + 2 * e + 1) * p.qs[3]] << 16;
+        }
+    }
+    // f16 queries as they are; a scale below 0 goes with them
+    __device__ __forceinline__ half8_t halves(const Q8AttnParams &p, int d0) const {
+        const uint32_t keep = d0 < p.D ? ~0u : 0u, turn = p.scale < 0.0f ? 0x80008000u : 0u;
+        return __builtin_bit_cast(half8_t, uint4_t{(w[0] & keep) ^ turn, (w[1] & keep) ^ turn, (w[2] & keep) ^ turn, (w[3] & keep) ^ turn});
+    }
+    __device__ __forceinline__ void widen(const Q8AttnParams &p, int d0, float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if constexpr (TERMS == 2) {
+                x[e] = __uint_as_float(w[e]);
+            } else {
+                const uint32_t bits = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
+                x[e] = p.q_dtype == FHIP_F16 ? (float)__builtin_bit_cast(half_t, (uint16_t)bits) : __uint_as_float(bits << 16);
+            }
+            if (d0 >= p.D) x[e] = 0.0f;
+        }
+    }
+};
 // The power of two that brings a row's largest element to [2^14, 2^15); zeros, infinities and NaN stay as they are.
 __device__ __forceinline__ int q8_query_shift(float top) { return top > 0.0f && top <= 3.402823466e38f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0; }
 // An element as one term or two.  A scale of 0 or below goes with the queries: the one of the scores (q8_score_scale) is positive.

@@ -446,3 +446,59 @@ def test_too_little_workspace(device):
     a.workspace, a.workspace_bytes = memory.ptr, need.value
     assert fa.lib().fhip_q8_attention(device.stream, ctypes.byref(a)) == fa.OK
     c.check(got=out.to_numpy())
+
+
+@pytest.mark.parametrize("with_native", [True, False])
+def test_both_ways_to_the_library(device, monkeypatch, with_native):
+    """The mirror's calls through its native half and through ctypes."""
+    assert fa._native is not None
+    if not with_native:
+        monkeypatch.setattr(fa, "_native", None)
+    rng = np.random.default_rng(30)
+    rope = fa.RopeCache(64, 64, 10000.0, device)
+    norm = fa.RmsNorm(rng.normal(1, 0.2, 64).astype(np.float32), None, 1e-6, F32, device)
+    cache = fa.Q8KvCache(2, 64, fa.Q8Format.INT8, 8, device)
+    q, k, v = (rng.standard_normal((2, h, 9, 64)).astype(np.float32) for h in (4, 2, 2))
+    t = [upload(device, x, F32) for x in (q, k, v)]
+    turned, k8, v8 = cache.qkv_rope_append(rope, *t, 3, q_norm=norm, k_norm=norm)
+    mask = (upload(device, np.zeros((9, 9)), F32), fa.MaskKind.QKMask)
+    got = [turned.flash_attention(k8, v8, 0.125, m, analytic=a, kv_lens=n, q_positions=x) for m, a, n, x in
+           ((None, None, None, None), (mask, None, None, None), (None, (True, 0, 4), fa.IntTensor(device, [9, 5]), fa.IntTensor(device, [0, 1])))]
+    own = fa.Q8Tensor.empty(device, (2, 2, 20, 64), fa.Q8Format.INT8, 8)
+    own2 = fa.Q8Tensor.empty(device, (2, 2, 20, 64), fa.Q8Format.INT8, 8)
+    turned2 = own.append(own2, t[1], t[2], 1, lens=fa.IntTensor(device, [2, 2]), counts=fa.IntTensor(device, [9, 9]), rope=rope, start_pos=1, k_norm=norm,
+                         q=t[0], q_norm=norm)
+    assert np.array_equal(turned.to_numpy(), turned2.to_numpy())
+    back = own.narrow(2, 3, 9).dequantize(F32), own2.dequantize(F32, row=1, rows=9, lens=fa.IntTensor(device, [2, 2]))
+    for a, b in zip(back, (k8, v8)):
+        # (blocks lie elsewhere: 8-bit codes of other scales)
+        assert np.abs(a.to_numpy() - b.dequantize(F32).to_numpy()).max() < 5.0 / 127
+    want = [turned.flash_attention(k8.dequantize(F32), v8.dequantize(F32), 0.125, m, analytic=a, kv_lens=n) for m, a, n in
+            ((None, None, None), (mask, None, None))]
+    for a, b in zip(got, want):
+        assert np.abs(a.to_numpy() - b.to_numpy()).max() < 1e-5
+    windowed = got[2].to_numpy()  # row r of sequence 1 sees keys r - 2 .. r + 1 below 5
+    assert np.isnan(windowed[1, :, 7:]).all() and np.isfinite(windowed[1, :, :7]).all() and np.isfinite(windowed[0]).all()
+    assert not np.array_equal(windowed[0], got[0].to_numpy()[0])
+
+
+def test_shares_in_any_workspace(device):
+    """A workspace that starts with anything, calls of different shapes that follow each other in it, and a recorded call replayed."""
+    import ctypes
+    for D, Skv, Sq, B in ((64, 3000, 1, 2), (128, 1500, 3, 1), (256, 2000, 1, 3), (192, 9000, 1, 1)):
+        c = Call(device, B, 8, 2, Sq, Skv, D, F16, INT8, 1)
+        q, kv = upload(device, c.q, F16), c.tensors()
+        ws, size = device.workspace(1 << 24)
+        for fill in (0, 0xFF, 0x55):
+            fa.check(fa.lib().fhip_memset(device.stream, ctypes.c_void_p(ws), fill, size))
+            c.check(got=q.flash_attention(*kv, c.scale).to_numpy())
+        out = upload(device, c.q, F16)
+        with device.capture() as cap:
+            q.flash_attention(*kv, c.scale, out=out)
+        first = q.flash_attention(*kv, c.scale).to_numpy()
+        for _ in range(4):
+            fa.check(fa.lib().fhip_memset(device.stream, ctypes.c_void_p(out.buffer.ptr), 0, out.buffer.nbytes))
+            cap.graph.launch()
+            assert np.array_equal(out.to_numpy(), first)
+            q.flash_attention(*kv, c.scale)
+        del cap
