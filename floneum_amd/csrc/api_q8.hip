@@ -184,6 +184,7 @@ static int append_rows(hipStream_t stream, const fhip_q8_append_args *a, const A
         mode = a->rope->interleaved ? 1 : 0;
     }
     const uint32_t T = k.block_tokens, n = s.n - skip;
+    const bool alone = T == 1 || s.n == 1;  // new rows in blocks of their own
     auto job = [&](const fhip_tensor4 &src, fhip_dtype dtype, uint32_t heads, int md, const fhip_rms_norm *norm) -> Q8Rows & {
         Q8Rows &j = p.job[p.jobs++];
         j.src = (const char *)src.ptr + src.offset * (uint64_t)bytes_of(dtype);
@@ -215,10 +216,10 @@ static int append_rows(hipStream_t stream, const fhip_q8_append_args *a, const A
         j.n = (int32_t)n;
         j.pos0 = pos0 + skip;
         j.out = view_of(side == 0 ? k : v);
-        j.span = T == 1 ? n : (n + 2 * (T - 1)) / T * T;
+        j.span = alone ? n : (n + 2 * (T - 1)) / T * T;
         j.total = s.B * s.Hkv * j.span;
     }
-    return launch_q8_append(p, (int)T, a->q_norm || a->k_norm, stream);
+    return launch_q8_append(p, (int)T, alone, a->q_norm || a->k_norm, stream);
 }
 
 // ---- attention --------------------------------------------------------------------------------------------------------------------------

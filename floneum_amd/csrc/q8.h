@@ -38,7 +38,8 @@ struct Q8Rows {
     int64_t d[4];            // q only
     Q8View out;              // keys and values; of q only `rows`, which bounds the places of its rows
     uint32_t span;           // row slots per (batch, head): n, or whole blocks for any place of the first row in its own
-    uint32_t total;          // slots of the job
+    uint32_t total;          // slots of the job (both are counted in groups of rows by the launcher of rows on their own)
+    uint32_t by_heads[2], by_rows[2];  // factor and shift that divide numbers below 2^31 by heads and span (factor 0: by 1), set by the launcher
 };
 struct Q8AppendParams {
     Q8Rows job[3];
@@ -50,8 +51,8 @@ struct Q8AppendParams {
     const float *cos, *sin;
     int64_t table_rows;
 };
-// max_block: the larger of the jobs' block_tokens (1 for q alone); normed: some job has a norm
-int launch_q8_append(Q8AppendParams &p, int max_block, bool normed, hipStream_t stream);
+// max_block: the cache's block_tokens; rows_alone: no two new rows share a block, and the jobs' slots are their rows; normed: some job has a norm
+int launch_q8_append(Q8AppendParams &p, int max_block, bool rows_alone, bool normed, hipStream_t stream);
 
 struct Q8ReadParams {
     Q8View x;
@@ -61,6 +62,9 @@ struct Q8ReadParams {
     int32_t B, H, n, D, format;
     int64_t row;
     const int32_t *lens;
+};
+struct Q8ReadDivisors {
+    uint32_t pieces[2], rows[2], heads[2];  // as Q8Rows::by_heads
 };
 int launch_q8_dequantize(const Q8ReadParams &p, hipStream_t stream);
 
