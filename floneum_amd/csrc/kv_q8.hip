@@ -560,7 +560,7 @@ int launch_q8_dequantize(const Q8ReadParams &p, hipStream_t stream) {
             q.n = (int)std::min<int64_t>(rows, p.n - i);
             q.x.codes += (int64_t)b * p.x.cs[0];
             q.x.scales += (int64_t)b * p.x.ss[0];
-            q.out += ((int64_t)b * p.os[0] + i * p.os[2]) * bytes;
+            q.out = (char *)p.out + ((int64_t)b * p.os[0] + i * p.os[2]) * bytes;
             q.row += i;
             if (p.lens) q.lens += b;
             Q8ReadDivisors div;
