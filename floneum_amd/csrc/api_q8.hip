@@ -291,6 +291,10 @@ static int validate_attention(const fhip_q8_attn_args *a) {
         set_error("q8_attention: more than 2^31-1 query rows in one call");
         return FHIP_ERR_UNSUPPORTED;
     }
+    if (Skv > 0x7fffffffu - 4096) {  // (the kernels look a few tiles ahead in 32 bits)
+        set_error("q8_attention: more than 2^31-4097 keys");
+        return FHIP_ERR_UNSUPPORTED;
+    }
     return FHIP_OK;
 }
 

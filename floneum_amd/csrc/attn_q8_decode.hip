@@ -1,7 +1,7 @@
 // Attention over the 8-bit cache for few query rows: every code is read from memory once and straight into the registers that feed the
 // matrix cores; no LDS in the loop.
 //
-// A workgroup of four wavefronts serves CB blocks of 16 columns ((query row, head of the group) pairs of one KV head) over one share of
+// A workgroup of four wavefronts serves 16 columns ((query row, head of the group) pairs of one KV head) over one share of
 // the keys; a wavefront takes 32 keys a step.  S^T[key][column] = K Q^T and O^T[dim][column] += V^T P^T on v_mfma_f32_16x16x32_f16.
 // Lane (n = lane % 16, g = lane / 16):
 //   K operand  lane n of 16-key tile u holds key 8 (n / 4) + 4 u + n % 4, dims 64 s + 16 g .. + 15: one 16-byte load is two
@@ -15,8 +15,13 @@
 // to f16's upper range: f16 and bf16 queries fit one term exactly (to 2^-29 of the row's largest element), f32 ones take two (22 bits).
 // The value scale vs_j, in [2^(e_j - 1), 2^e_j), goes with the probability: with the running maximum M of s_j + e_j,
 //   p_j = 2^(s_j + e_j - M + 15) 2^-e_j,  w_j = p_j vs_j <= 2^15,  out = sum w_j c_j / sum p_j
-// which holds whatever the scales' range (a first token with values of almost nothing).  w is rounded to 11 bits (relative 2^-12, to 2^-29 of the largest) for 16-bit tensors and
-// taken as two terms for f32.
+// which holds whatever the scales' range (a first token with values of almost nothing).  w is rounded to 11 bits (relative 2^-12, to 2^-29 of the
+// largest) for 16-bit tensors and taken as two terms for f32.
+//
+// Bound by the bytes of codes and scales where there are many: 157 us for 16 ragged sequences of up to 16384 keys, 32 heads of 96 (e4m3, 5.2 TB/s),
+// 33 us with the joining for 16 of 4096, 8 KV heads of 128 (134 MB).  One sequence is bound by a chain of latencies: 10 us for 4096 keys, about half of it the
+// launch of the second kernel and its reads (one kernel whose last workgroup joins the shares took 97 us: the order it needs between XCDs
+// writes back and drops their L2).  Two steps of keys in flight against one: 39 -> 33 us; non-temporal loads: no change.
 #include <algorithm>
 
 #include "q8.h"
@@ -49,11 +54,11 @@ __device__ __forceinline__ float quads_sum(float x) {
     x += xor16(x);
     return x + xor32(x);
 }
-template <int DV, int TERMS, int FMT, int CB, bool MASK, bool BLOCKS>
+template <int DV, int TERMS, int FMT, bool MASK, bool BLOCKS>
 __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8AttnParams p) {
     request_arguments<Q8AttnParams>();
     using Dims = Q8Dims<DV>;
-    constexpr int VW = Dims::VW, KS = Dims::KS, TILES = Dims::TILES, COLS = 16 * CB, NBUF = DV <= 128 ? 2 : 1;
+    constexpr int VW = Dims::VW, KS = Dims::KS, TILES = Dims::TILES, COLS = 16, NBUF = DV <= 128 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float lds_acc[4][16][DV + 4];
     __shared__ float lds_m[4][COLS], lds_l[4][COLS];
 
@@ -72,14 +77,10 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     const int64_t lo64 = vis.lo + (int64_t)split * chunk;
     const int lo = (int)min(lo64, (int64_t)vis.hi), hi = (int)min((int64_t)vis.hi, lo64 + chunk);
 
-    float4_t acc[CB][TILES];
-    float m[CB], l[CB];
+    float4_t acc[TILES];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int cbk = 0; cbk < CB; cbk++) {
-        m[cbk] = -INFINITY, l[cbk] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < TILES; t++) acc[cbk][t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int t = 0; t < TILES; t++) acc[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
     const uint8_t *const kbase = p.k.codes + (int64_t)b * p.k.cs[0] + (int64_t)kvh * p.k.cs[1];
     const uint8_t *const vbase = p.v.codes + (int64_t)b * p.v.cs[0] + (int64_t)kvh * p.v.cs[1];
@@ -93,10 +94,10 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     const int kkey = 8 * (n >> 2) + (n & 3), vkey = 8 * g;  // the lane's first key of a step
 
     // queries: column c is row c / G, head c % G of the group
-    half8_t q[CB][TERMS][KS][2];
-    float colscale[CB];
-    int limit[CB], start[CB];  // keys [start, limit) of the column
-    int row[CB];
+    half8_t q[TERMS][KS][2];
+    float colscale;
+    int limit, start;  // keys [start, limit) of the column
+    int row;
     // What a wavefront holds of a step's keys.  Steps are loaded NBUF ahead, without a branch (behind one the compiler would wait for all
     // loads): the last step of a share starts 32 keys before its end and leaves out those of the step before, and steps beyond it load that
     // one again.  A tensor has at least 32 rows here.
@@ -175,12 +176,10 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                 if (vs[i] != vs[i]) ks[i] = vs[i], vs[i] = 1.0f;
         }
         // scores
-        float sc[CB][8];
+        float sc[8];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            float4_t s4[CB];
-#pragma unroll
-            for (int cbk = 0; cbk < CB; cbk++) s4[cbk] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            float4_t s4 = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -193,15 +192,11 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                         kf[4 * w] = y[0], kf[4 * w + 1] = y[1], kf[4 * w + 2] = z[0], kf[4 * w + 3] = z[1];
                     }
 #pragma unroll
-                    for (int cbk = 0; cbk < CB; cbk++)
-#pragma unroll
-                        for (int t = TERMS - 1; t >= 0; t--)
-                            s4[cbk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[cbk][t][s][a], s4[cbk], 0, 0, 0);
+                    for (int t = TERMS - 1; t >= 0; t--)
+                        s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[t][s][a], s4, 0, 0, 0);
                 }
 #pragma unroll
-            for (int cbk = 0; cbk < CB; cbk++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) sc[cbk][4 * u + r] = s4[cbk][r];
+            for (int r = 0; r < 4; r++) sc[4 * u + r] = s4[r];
         }
         load_k(x, next);
 #pragma unroll
@@ -210,19 +205,18 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
             exf[i] = (float)e;
             back[i] = __builtin_ldexpf(1.0f, -e);
         }
-        half8_t pw[CB][TERMS];
-#pragma unroll
-        for (int cbk = 0; cbk < CB; cbk++) {
+        half8_t pw[TERMS];
+        {
             float top = -INFINITY;
             if constexpr (!MASK) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) sc[cbk][i] = __builtin_fmaf(sc[cbk][i], ks[i] * colscale[cbk], exf[i]);
+                for (int i = 0; i < 8; i++) sc[i] = __builtin_fmaf(sc[i], ks[i] * colscale, exf[i]);
                 // the step reaches beyond what some column sees
-                if (__builtin_amdgcn_ballot_w64(at + 32 > limit[cbk] || at < start[cbk] || at < k0) != 0) {
+                if (__builtin_amdgcn_ballot_w64(at + 32 > limit || at < start || at < k0) != 0) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int key = at + vkey + i;
-                        if (key >= limit[cbk] || key < start[cbk] || key < k0) sc[cbk][i] = -INFINITY;
+                        if (key >= limit || key < start || key < k0) sc[i] = -INFINITY;
                     }
                 }
             } else {
@@ -230,32 +224,32 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                 for (int i = 0; i < 8; i++) {
                     const int key = at + vkey + i;
                     float add = -INFINITY;
-                    if (key < limit[cbk] && key >= k0)
-                        add = q8_load_any(p.mask, (p.mask_kind == FHIP_MASK_QK ? row[cbk] : b) * p.ms0 + key * p.ms1, p.q_dtype);
-                    const float s = q8_with_mask(sc[cbk][i] * (ks[i] * colscale[cbk]), add * Q8_LOG2E);
-                    sc[cbk][i] = add == -INFINITY ? -INFINITY : s + exf[i];
+                    if (key < limit && key >= k0)
+                        add = q8_load_any(p.mask, (p.mask_kind == FHIP_MASK_QK ? row : b) * p.ms0 + key * p.ms1, p.q_dtype);
+                    const float s = q8_with_mask(sc[i] * (ks[i] * colscale), add * Q8_LOG2E);
+                    sc[i] = add == -INFINITY ? -INFINITY : s + exf[i];
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, sc[cbk][i]);
-            top = fmaxf(m[cbk], quads_max(top));
+            for (int i = 0; i < 8; i++) top = fmaxf(top, sc[i]);
+            top = fmaxf(m, quads_max(top));
             const float ref = top == -INFINITY ? 0.0f : top - 15.0f;
-            if (__builtin_amdgcn_ballot_w64(top > m[cbk]) != 0) {
-                const float f = __builtin_amdgcn_exp2f(m[cbk] - (top == -INFINITY ? 0.0f : top));
-                m[cbk] = top;
-                l[cbk] *= f;
+            if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+                const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+                m = top;
+                l *= f;
 #pragma unroll
-                for (int t = 0; t < TILES; t++) acc[cbk][t] *= f;
+                for (int t = 0; t < TILES; t++) acc[t] *= f;
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float e = __builtin_amdgcn_exp2f(sc[cbk][i] - ref) * back[i];
-                l[cbk] += e;
+                const float e = __builtin_amdgcn_exp2f(sc[i] - ref) * back[i];
+                l += e;
                 float w = e * vs[i];
                 if constexpr (TERMS == 2) asm("" : "+v"(w));  // (both terms from the same rounded w: the product is not contracted into them)
                 const half_t hi16 = (half_t)w;
-                pw[cbk][0][i] = hi16;
-                if constexpr (TERMS == 2) pw[cbk][1][i] = (half_t)(w - (float)hi16);
+                pw[0][i] = hi16;
+                if constexpr (TERMS == 2) pw[1][i] = (half_t)(w - (float)hi16);
             }
         }
         load_scales(x, next);
@@ -284,26 +278,23 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int cbk = 0; cbk < CB; cbk++)
-#pragma unroll
-                    for (int y = TERMS - 1; y >= 0; y--)
-                        acc[cbk][4 * w + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[t], pw[cbk][y], acc[cbk][4 * w + t], 0, 0, 0);
+                for (int y = TERMS - 1; y >= 0; y--)
+                    acc[4 * w + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[t], pw[y], acc[4 * w + t], 0, 0, 0);
         }
         load_v(x, next);
     };
 
-    Q8Query8<TERMS> raw[CB][KS][2];
-#pragma unroll
-    for (int cbk = 0; cbk < CB; cbk++) {
-        const int c = min(c0 + cbk * 16 + n, NC - 1);
-        row[cbk] = c / p.G;
-        const int64_t base = (int64_t)b * p.qs[0] + (int64_t)(kvh * p.G + c - row[cbk] * p.G) * p.qs[1] + (int64_t)row[cbk] * p.qs[2];
+    Q8Query8<TERMS> raw[KS][2];
+    {
+        const int c = min(c0 + n, NC - 1);
+        row = c / p.G;
+        const int64_t base = (int64_t)b * p.qs[0] + (int64_t)(kvh * p.G + c - row * p.G) * p.qs[1] + (int64_t)row * p.qs[2];
         if (p.q_vec) {
 #pragma unroll
-            for (int s = 0; s < 2 * KS; s++) raw[cbk][s >> 1][s & 1].load(p, base, 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+            for (int s = 0; s < 2 * KS; s++) raw[s >> 1][s & 1].load(p, base, 64 * (s >> 1) + 16 * g + 8 * (s & 1));
         } else {
 #pragma unroll
-            for (int s = 0; s < 2 * KS; s++) raw[cbk][s >> 1][s & 1].gather(p, base, 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+            for (int s = 0; s < 2 * KS; s++) raw[s >> 1][s & 1].gather(p, base, 64 * (s >> 1) + 16 * g + 8 * (s & 1));
         }
     }
     Step steps[NBUF];
@@ -316,21 +307,20 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
             load_v(steps[i], k0 + 128 * i);
         }
     }
-#pragma unroll
-    for (int cbk = 0; cbk < CB; cbk++) {
+    {
         if (TERMS == 1 && p.q_dtype == FHIP_F16 && p.scale != 0.0f) {  // as they are
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int a = 0; a < 2; a++) q[cbk][0][s][a] = raw[cbk][s][a].halves(p, 64 * s + 16 * g + 8 * a);
-            colscale[cbk] = q8_score_scale(p, 0);
+                for (int a = 0; a < 2; a++) q[0][s][a] = raw[s][a].halves(p, 64 * s + 16 * g + 8 * a);
+            colscale = q8_score_scale(p, 0);
         } else {
             float x[KS][2][8], top = 0.0f;
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
                 for (int a = 0; a < 2; a++) {
-                    raw[cbk][s][a].widen(p, 64 * s + 16 * g + 8 * a, x[s][a]);
+                    raw[s][a].widen(p, 64 * s + 16 * g + 8 * a, x[s][a]);
 #pragma unroll
                     for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[s][a][e]));
                 }
@@ -343,14 +333,14 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                     for (int e = 0; e < 8; e++) {
                         half_t high, low;
                         q8_query_terms<TERMS>(p, x[s][a][e], shift, high, low);
-                        q[cbk][0][s][a][e] = high;
-                        if constexpr (TERMS == 2) q[cbk][1][s][a][e] = low;
+                        q[0][s][a][e] = high;
+                        if constexpr (TERMS == 2) q[1][s][a][e] = low;
                     }
-            colscale[cbk] = q8_score_scale(p, shift);
+            colscale = q8_score_scale(p, shift);
         }
-        const int64_t at = vis.pos0 + row[cbk];
-        limit[cbk] = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);
-        start[cbk] = (int)(p.window > 0 ? min((int64_t)hi, max((int64_t)0, at - p.window + 1)) : 0);
+        const int64_t at = vis.pos0 + row;
+        limit = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);
+        start = (int)(p.window > 0 ? min((int64_t)hi, max((int64_t)0, at - p.window + 1)) : 0);
     }
 
     while (k0 < hi) {
@@ -362,33 +352,29 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         }
     }
 
-    // the four wavefronts' states, one column block at a time
-#pragma unroll
-    for (int cbk = 0; cbk < CB; cbk++) {
-        l[cbk] = quads_sum(l[cbk]);
-        if (g == 0) lds_m[wave][cbk * 16 + n] = m[cbk], lds_l[wave][cbk * 16 + n] = l[cbk];
-    }
-#pragma unroll
-    for (int cbk = 0; cbk < CB; cbk++) {
+    // the four wavefronts' states
+    l = quads_sum(l);
+    if (g == 0) lds_m[wave][n] = m, lds_l[wave][n] = l;
+    {
         lds_barrier();  // (the loads of steps beyond the last one may still be on their way)
 #pragma unroll
         for (int w = 0; w < VW; w++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float4_t v = {acc[cbk][4 * w][r], acc[cbk][4 * w + 1][r], acc[cbk][4 * w + 2][r], acc[cbk][4 * w + 3][r]};
+                const float4_t v = {acc[4 * w][r], acc[4 * w + 1][r], acc[4 * w + 2][r], acc[4 * w + 3][r]};
                 *(float4_t *)&lds_acc[wave][n][Dims::dim(4 * g + r, w, 0)] = v;
             }
         lds_barrier();
-        const int col = threadIdx.x >> 4, sub = threadIdx.x & 15, c = c0 + cbk * 16 + col;
+        const int col = threadIdx.x >> 4, sub = threadIdx.x & 15, c = c0 + col;
         if (c < NC) {
             float M = -INFINITY, L = 0.0f, f[4];
 #pragma unroll
-            for (int x = 0; x < 4; x++) M = fmaxf(M, lds_m[x][cbk * 16 + col]);
+            for (int x = 0; x < 4; x++) M = fmaxf(M, lds_m[x][col]);
             const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                f[x] = __builtin_amdgcn_exp2f(lds_m[x][cbk * 16 + col] - ref);
-                L += lds_l[x][cbk * 16 + col] * f[x];
+                f[x] = __builtin_amdgcn_exp2f(lds_m[x][col] - ref);
+                L += lds_l[x][col] * f[x];
             }
             const int at = c / p.G;
             const int64_t o = (int64_t)b * p.os[0] + (int64_t)(kvh * p.G + c - at * p.G) * p.os[1] + (int64_t)at * p.os[2];
@@ -526,10 +512,10 @@ static int launch_decode_dims(const Q8AttnParams &p, const Q8AttnPlan &plan, hip
     const int64_t y = std::min<int64_t>(units, 32768), z = (units + y - 1) / y;
     const dim3 grid(p.nsplit, (unsigned)y, (unsigned)z);
     const bool blocks = p.k.log2_block > 0;
-    if (p.mask && blocks) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1, true, true>), grid, dim3(256), 0, stream, p);
-    else if (p.mask) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1, true, false>), grid, dim3(256), 0, stream, p);
-    else if (blocks) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1, false, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, 1, false, false>), grid, dim3(256), 0, stream, p);
+    if (p.mask && blocks) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, true, true>), grid, dim3(256), 0, stream, p);
+    else if (p.mask) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, true, false>), grid, dim3(256), 0, stream, p);
+    else if (blocks) hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, false, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((q8_decode_kernel<DV, TERMS, FMT, false, false>), grid, dim3(256), 0, stream, p);
     FHIP_HIP_CHECK(hipGetLastError());
     return p.nsplit > 1 ? launch_q8_merge(p, stream) : FHIP_OK;
 }

@@ -7,6 +7,13 @@
 // so that probabilities go from the scores' registers to the operand's without leaving their lane.  A lane holds 16 keys of each half of the tile;
 // their scales lie in one register of 16 lanes (a DPP row) and are broadcast by the multiplication that uses them.
 //
+// A tile costs a wavefront of 128 dims 32 products of 32 cycles and about 330 vector instructions, 32 of them exp2.  Both units are kept busy by one
+// wavefront: the next tile's scores are multiplied while this one's weights are made, this tile's values while the next one's scores are scaled and
+// the tile after them is widened into LDS.  The order is written down step by step (sched_barrier): left to itself the compiler puts the products
+// of a tile behind each other, each waiting for its piece of LDS (695 us against 660 for the prompt below).
+// Measured: 620 us for a causal prompt of 8192 f16 rows, 32 / 8 heads of 128, int8 (887 TFLOP/s of visible pairs; the matrix units are busy for 37 %
+// of the cycles, the vector units for 70 %, at 2.1 GHz); 159 us for 4 chunks of 512 bf16 rows over a window of 4096, e4m3.
+//
 // Numbers are brought to f16 as in the kernel for few rows (attn_q8_decode.hip): codes exactly, a column's q scaled by a power of two, one term for
 // 16-bit queries and two for f32.  The values' scales go with the probabilities, brought below 2^15 by a power of two E that follows the largest
 // scale met: w_j = p_j vs_j 2^(15 - E), out = 2^(E - 15) sum w_j c_j / sum p_j.
@@ -38,17 +45,20 @@ __device__ __forceinline__ half8_t q8_widen8_pairs(half2_t a, half2_t b, half2_t
     return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Waits: `WAVES_PER_SIMD` wavefronts share a SIMD's registers.
 template <int DV, int TERMS, int FMT, int WAVES, bool MASK>
 __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kernel(Q8AttnParams p) {
     request_arguments<Q8AttnParams>();
-    constexpr int COLS = 32 * WAVES, STEPS = DV / 16, DT = DV / 32, UNITS = DV / 16, CHUNKS = DV / 8;
-    // LDS, 16-byte chunks: K [key][chunk of 8 dims], V [dim][chunk of 8 keys]; the chunk is turned by the row so that 16 rows' pieces lie in
-    // different banks
-    __shared__ __attribute__((aligned(16))) half_t lds_k[2][Q8_TILE * DV];
-    __shared__ __attribute__((aligned(16))) half_t lds_v[2][Q8_TILE * DV];
-    auto k_at = [](int key, int chunk) { return (key * CHUNKS + (chunk ^ (DV % 128 == 0 ? key & 15 : (key >> 1) & 7))) * 8; };
-    auto v_at = [](int dim, int chunk) { return (dim * 8 + (chunk ^ (((dim >> 1) ^ (dim >> 4)) & 7))) * 8; };
+        // 16-bit queries: a column's reference is at most 2^SLACK behind its maximum, so that sums shrink once in many tiles (666 -> 649 us for a prompt
+    // of 8192); half a step of the smallest weights is 2^-35 of the largest scale.  f32 takes none of it.
+    constexpr int SLACK = TERMS == 1 ? 4 : 0;
+    // pieces of LDS in flight: two ahead of their products, one for f32, whose registers are full (71 us against 73)
+    constexpr int RG = TERMS == 1 ? 3 : 2;
+    constexpr int COLS = 32 * WAVES, STEPS = DV / 16, DT = DV / 32, UNITS = DV / 16;
+    // LDS: K [key][dim], V [dim][key]; a row's last 16 bytes are left over, so that 16 rows' pieces lie in different banks and every piece is at a
+    // constant distance from the lane's first
+    constexpr int KP = DV + 8, VP = Q8_TILE + 8;
+    __shared__ __attribute__((aligned(16))) half_t lds_k[2][Q8_TILE * KP];
+    __shared__ __attribute__((aligned(16))) half_t lds_v[2][DV * VP];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
     const int NC = p.G * p.Sq, units = p.B * p.Hkv;
@@ -124,68 +134,72 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
     const uint8_t *const vbase = p.v.codes + (int64_t)b * p.v.cs[0] + (int64_t)kvh * p.v.cs[1];
     const float *const kscale = p.k.scales + (int64_t)b * p.k.ss[0] + (int64_t)kvh * p.k.ss[1];
     const float *const vscale = p.v.scales + (int64_t)b * p.v.ss[0] + (int64_t)kvh * p.v.ss[1];
-    const int pitch = (p.D + 15) & ~15, krow = (int)p.k.cs[2], vrow = (int)p.v.cs[2];
+    const int pitch = (p.D + 15) & ~15;
+    const uint32_t krow = (uint32_t)p.k.cs[2], vrow = (uint32_t)p.v.cs[2];
 
-    // staging: 256 lanes move a tile's keys and 256 its values (the same ones in workgroups of four wavefronts)
-    constexpr int KN = 4 * DV / 256 > 0 ? 4 * DV / 256 : 1, VN = (2 * DV + 255) / 256;
-    const int sid = threadIdx.x & 255;
-    const bool moves_k = WAVES == 4 || wave >= 4, moves_v = WAVES == 4 || wave < 4;
+    // Staging: pieces of 16 bytes of the keys, 4 keys x 4 dims of the values.  Where a tile has fewer of them than there are lanes, the first half
+    // of the lanes moves keys, the second values.
+    constexpr int LANES = 64 * WAVES, PIECES = 4 * DV, KN = (PIECES + LANES - 1) / LANES;
+    const bool moves_k = PIECES >= LANES || wave < WAVES / 2, moves_v = PIECES >= LANES || wave >= WAVES / 2;
+    const int sid = PIECES >= LANES ? threadIdx.x : threadIdx.x % PIECES;
+    // of the values a wavefront takes 8 groups of keys by 8 of dims, which meet few banks
+    auto value_group = [](int u) { return 8 * ((u >> 6) & 1) + (u >> 3 & 7); };
+    auto value_dims = [](int u) { return 8 * (u >> 7) + (u & 7); };
     uint4_t ksrc[KN];
-    uint32_t vsrc[VN][8];
+    uint32_t vsrc[KN][4];
     // Rows beyond the share are loaded as its last one (what lies there may be anything, 8-bit NaN among it); pieces beyond a row from its start:
     // q is 0 there, and such dims of v are not written.
-    auto load_tile = [&](int k0) {
-        const int last = hi - 1 - k0;
-        if (moves_k) {
-            const uint8_t *const r = kbase + (int64_t)k0 * krow;
+    auto load_keys = [&](int at) {
+        const int k0 = min(at, hi - 1);
+        const uint32_t last = min(hi - 1 - k0, Q8_TILE - 1);
+        if (!moves_k) return;
+        const uint8_t *const r = kbase + (int64_t)k0 * krow;
 #pragma unroll
-            for (int i = 0; i < KN; i++) {
-                const int u = sid + 256 * i, key = u / UNITS, off = 16 * (u % UNITS);
-                ksrc[i] = *(const uint4_t *)(r + (uint32_t)(min(key, last) * krow + (off < pitch ? off : 0)));
-            }
-        }
-        if (moves_v) {
-            const uint8_t *const r = vbase + (int64_t)k0 * vrow;
-#pragma unroll
-            for (int i = 0; i < VN; i++) {
-                const int u = sid + 256 * i;
-                if (2 * DV % 256 != 0 && u >= 2 * DV) continue;
-                const int kg = u / (DV / 4), off = 4 * (u % (DV / 4)), base = 16 * (kg >> 1) + 4 * (kg & 1);
-                const uint32_t o = off < pitch ? off : 0;
-#pragma unroll
-                for (int e = 0; e < 8; e++) vsrc[i][e] = *(const uint32_t *)(r + (uint32_t)(min(base + (e & 3) + 8 * (e >> 2), last) * vrow + o));
-            }
+        for (int i = 0; i < KN; i++) {
+            const int u = sid + LANES * i, off = 16 * (u % UNITS);
+            ksrc[i] = *(const uint4_t *)(r + (min((uint32_t)(u / UNITS) * krow, last * krow) + (off < pitch ? off : 0)));
         }
     };
-    auto store_tile = [&](int buf) {
-        if (moves_k) {
+    auto load_values = [&](int at) {
+        const int k0 = min(at, hi - 1);
+        const uint32_t last = min(hi - 1 - k0, Q8_TILE - 1);
+        if (!moves_v) return;
+        const uint8_t *const r = vbase + (int64_t)k0 * vrow;
 #pragma unroll
-            for (int i = 0; i < KN; i++) {
-                const int u = sid + 256 * i, key = u / UNITS, chunk = 2 * (u % UNITS);
+        for (int i = 0; i < KN; i++) {
+            const int u = sid + LANES * i, off = 4 * value_dims(u);
+            const uint32_t o = off < pitch ? off : 0, at0 = 4 * value_group(u) * vrow;
 #pragma unroll
-                for (int e = 0; e < 2; e++)
-                    *(half8_t *)&lds_k[buf][k_at(key, chunk + e)] =
-                        q8_widen8_pairs(q8_pair_low<FMT>(ksrc[i][2 * e]), q8_pair_high<FMT>(ksrc[i][2 * e]), q8_pair_low<FMT>(ksrc[i][2 * e + 1]),
-                                        q8_pair_high<FMT>(ksrc[i][2 * e + 1]));
-            }
+            for (int e = 0; e < 4; e++) vsrc[i][e] = *(const uint32_t *)(r + (min(at0 + e * vrow, last * vrow) + o));
         }
-        if (moves_v) {
+    };
+    auto store_keys = [&](int buf) {
+        if (!moves_k) return;
 #pragma unroll
-            for (int i = 0; i < VN; i++) {
-                const int u = sid + 256 * i;
-                if (2 * DV % 256 != 0 && u >= 2 * DV) continue;
-                const int kg = u / (DV / 4), dim = 4 * (u % (DV / 4));
-                half2_t x[4][4];  // [dim][pair of keys]
+        for (int i = 0; i < KN; i++) {
+            const int u = sid + LANES * i, key = u / UNITS, chunk = 2 * (u % UNITS);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t a = vsrc[i][2 * e], c2 = vsrc[i][2 * e + 1];
-                    const uint32_t t01 = __builtin_amdgcn_perm(c2, a, 0x05010400u), t23 = __builtin_amdgcn_perm(c2, a, 0x07030602u);
-                    x[0][e] = q8_pair_low<FMT>(t01), x[1][e] = q8_pair_high<FMT>(t01);
-                    x[2][e] = q8_pair_low<FMT>(t23), x[3][e] = q8_pair_high<FMT>(t23);
-                }
+            for (int e = 0; e < 2; e++)
+                *(half8_t *)&lds_k[buf][key * KP + 8 * (chunk + e)] =
+                    q8_widen8_pairs(q8_pair_low<FMT>(ksrc[i][2 * e]), q8_pair_high<FMT>(ksrc[i][2 * e]), q8_pair_low<FMT>(ksrc[i][2 * e + 1]),
+                                    q8_pair_high<FMT>(ksrc[i][2 * e + 1]));
+        }
+    };
+    auto store_values = [&](int buf) {
+        if (!moves_v) return;
 #pragma unroll
-                for (int t = 0; t < 4; t++) *(half8_t *)&lds_v[buf][v_at(dim + t, kg)] = q8_widen8_pairs(x[t][0], x[t][1], x[t][2], x[t][3]);
+        for (int i = 0; i < KN; i++) {
+            const int u = sid + LANES * i, g = value_group(u), dim = 4 * value_dims(u), chunk = 2 * (g >> 2) + (g & 1), part = (g >> 1) & 1;
+            half2_t x[4][2];  // [dim][pair of keys]
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint32_t a = vsrc[i][2 * e], c2 = vsrc[i][2 * e + 1];
+                const uint32_t t01 = __builtin_amdgcn_perm(c2, a, 0x05010400u), t23 = __builtin_amdgcn_perm(c2, a, 0x07030602u);
+                x[0][e] = q8_pair_low<FMT>(t01), x[1][e] = q8_pair_high<FMT>(t01);
+                x[2][e] = q8_pair_low<FMT>(t23), x[3][e] = q8_pair_high<FMT>(t23);
             }
+#pragma unroll
+            for (int t = 0; t < 4; t++) *(half4_t *)&lds_v[buf][(dim + t) * VP + 8 * chunk + 4 * part] = half4_t{x[t][0][0], x[t][0][1], x[t][1][0], x[t][1][1]};
         }
     };
     // the scales of the lane's keys, one of 16 per lane of a row: key 32 u + 8 (i / 4) + 4 h + i % 4 in lane i
@@ -199,116 +213,177 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
         }
     };
 
-    if (lo < hi) {
-        load_tile(lo);
-        load_scales(lo);
-        store_tile(0);
-    }
-    lds_barrier();
-    int buf = 0;
-    for (int k0 = lo; k0 < hi; k0 += Q8_TILE, buf ^= 1) {
-        const bool more = k0 + Q8_TILE < hi;
-        if (more) load_tile(k0 + Q8_TILE);
-        float kf[2], vf[2];
-        int e = E;
+    // A tile's steps: its scores; scores times the keys' scales, masked, and their largest; weights; values.  Matrix products of a tile are STEPS2
+    // pieces read from LDS, of the keys (S) and again of the values (V).
+    constexpr int STEPS2 = DV / 8;
+    float16_t s[2], next[2];
+    half8_t piece[RG];
+    float kf[2], vf[2], nf[2];  // scales of the keys and values of the next tile (nf), and of this one's values (vf)
+    float top;
+    int e = E;
+    auto read_key = [&](int buf, auto ic) {
+        constexpr int i = decltype(ic)::value;
+        piece[i % RG] = *(const half8_t *)&lds_k[buf][(32 * (i % 2) + n) * KP + 8 * (i / 2 * 2 + h)];
+    };
+    auto read_value = [&](int buf, auto ic) {
+        constexpr int i = decltype(ic)::value;
+        piece[(STEPS2 + i) % RG] = *(const half8_t *)&lds_v[buf][(32 * (i % DT) + n) * VP + 8 * (i / DT * 2 + h)];
+    };
+    auto score = [&](auto ic) {
+        constexpr int i = decltype(ic)::value, u = i % 2;
+        if constexpr (i < 2)
+#pragma unroll
+            for (int r = 0; r < 16; r++) next[u][r] = 0.0f;
+#pragma unroll
+        for (int x = TERMS - 1; x >= 0; x--) next[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(piece[i % RG], q[x][i / 2], next[u], 0, 0, 0);
+    };
+    auto take_scales = [&]() {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             // NaN among the values' scales goes by way of the scores, where rows that a mask hides are taken out
             const bool lost = vs[u] != vs[u];
-            kf[u] = lost ? vs[u] : ks[u], vf[u] = lost ? 0.0f : vs[u];
-            e = max(e, vf[u] > 0.0f ? __builtin_amdgcn_frexp_expf(vf[u]) : -200);
+            kf[u] = lost ? vs[u] : ks[u], nf[u] = lost ? 0.0f : vs[u];
+            e = max(e, nf[u] > 0.0f ? __builtin_amdgcn_frexp_expf(nf[u]) : -200);
         }
-        e = wave_reduce_i(e, [](int x, int y) { return x > y ? x : y; });
-        float grown = 1.0f;
-        if (e > E) grown = __builtin_ldexpf(1.0f, max(E - e, -1000)), E = e;
-#pragma unroll
-        for (int u = 0; u < 2; u++) vf[u] = __builtin_ldexpf(vf[u], 15 - E);
-        if (more) load_scales(k0 + Q8_TILE);
-
-        float16_t s[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[u][r] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < STEPS; i++) {
-                const half8_t a = *(const half8_t *)&lds_k[buf][k_at(32 * u + n, 2 * i + h)];
-#pragma unroll
-                for (int x = TERMS - 1; x >= 0; x--) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[x][i], s[u], 0, 0, 0);
-            }
-        }
-        // times the keys' scales; with a mask in the log2 domain, else before the column's scale (which is positive)
-        float top = -INFINITY;
+    };
+    // score i (of 32) times its key's scale; with a mask in the log2 domain, else before the column's scale (which is positive)
+    auto scaled = [&](int k0, auto ic) {
+        constexpr int i = decltype(ic)::value, u = i / 16, r = i % 16;
+        const int key = 32 * u + 8 * (r / 4) + r % 4;
+        float t = row_lane<r>(kf[u]) * next[u][r];
         if constexpr (MASK) {
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                q8_each<16>([&](auto i) {
-                    constexpr int r = decltype(i)::value;
-                    const int key = k0 + 32 * u + 8 * (r / 4) + 4 * h + r % 4;
-                    float add = -INFINITY;
-                    if (key < limit) add = q8_load_any(p.mask, mask_row + key * p.ms1, p.q_dtype);
-                    const float t = q8_with_mask(row_lane<r>(kf[u]) * s[u][r] * colscale, add * Q8_LOG2E);
-                    s[u][r] = add == -INFINITY ? -INFINITY : t;
-                });
-        } else {
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                q8_each<16>([&](auto i) {
-                    constexpr int r = decltype(i)::value;
-                    s[u][r] = row_lane<r>(kf[u]) * s[u][r];
-                });
-            if (__builtin_amdgcn_ballot_w64(k0 + Q8_TILE > limit || k0 < start) != 0) {
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-                    q8_each<16>([&](auto i) {
-                        constexpr int r = decltype(i)::value;
-                        const int key = 32 * u + 8 * (r / 4) + r % 4;
-                        if (key >= limit - k0 - 4 * h || key < start - k0 - 4 * h) s[u][r] = -INFINITY;
-                    });
-            }
+            float add = -INFINITY;
+            if (key < limit - k0 - 4 * h) add = q8_load_any(p.mask, mask_row + (k0 + key + 4 * h) * p.ms1, p.q_dtype);
+            t = add == -INFINITY ? -INFINITY : q8_with_mask(t * colscale, add * Q8_LOG2E);
         }
-        const float g = MASK ? 1.0f : colscale;
+        s[u][r] = t;
+    };
+    // what the column does not see, and the largest score
+    auto largest = [&](int k0) {
+        if (!MASK && __builtin_amdgcn_ballot_w64(k0 + Q8_TILE > limit || k0 < start) != 0) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int key = 32 * u + 8 * (r / 4) + r % 4;
+                    if (key >= limit - k0 - 4 * h || key < start - k0 - 4 * h) s[u][r] = -INFINITY;
+                }
+        }
+        top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[u][r]);
-        top = fmaxf(top, xor32(top)) * g;
-        top = fmaxf(m, top);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        if (__builtin_amdgcn_ballot_w64(top > m || grown != 1.0f) != 0) {
+    };
+    const float g = MASK ? 1.0f : colscale;
+    half8_t pw[TERMS][4];
+    float ref = 0.0f;
+    auto weight = [&](auto ic) {
+        constexpr int i = decltype(ic)::value, u = i / 16, r = i % 16;
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], g, -ref));
+        l += x;
+        float w = row_lane<r>(vf[u]) * x;
+        if constexpr (TERMS == 2) asm("" : "+v"(w));  // (both terms from the same rounded w: the product is not contracted into them)
+        const half_t high = (half_t)w;
+        pw[0][2 * u + r / 8][r % 8] = high;
+        if constexpr (TERMS == 2) pw[1][2 * u + r / 8][r % 8] = (half_t)(w - (float)high);
+    };
+    auto value = [&](auto ic) {
+        constexpr int i = decltype(ic)::value, t = i % DT;
+#pragma unroll
+        for (int x = TERMS - 1; x >= 0; x--) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(piece[(STEPS2 + i) % RG], pw[x][i / DT], acc[t], 0, 0, 0);
+    };
+    // the part of 32 numbers that goes with step `i` of STEPS2
+    auto portion = [&](auto ic, auto &&f) {
+        constexpr int i = decltype(ic)::value, from = 32 * i / STEPS2, to = 32 * (i + 1) / STEPS2;
+        q8_each<to - from>([&](auto j) { f(std::integral_constant<int, from + decltype(j)::value>()); });
+    };
+#define IC(n) std::integral_constant<int, n>()
+
+    if (lo < hi) {
+        load_keys(lo);
+        load_values(lo);
+        load_scales(lo);
+        store_keys(0);
+        store_values(0);
+        take_scales();
+        load_keys(lo + Q8_TILE);
+        load_values(lo + Q8_TILE);
+        load_scales(lo + Q8_TILE);
+        lds_barrier();
+        q8_each<STEPS2>([&](auto i) {
+            read_key(0, i);
+            score(i);
+        });
+        store_keys(1);
+        load_keys(lo + 2 * Q8_TILE);
+        q8_each<32>([&](auto i) { scaled(lo, i); });
+        lds_barrier();
+    }
+    // the maximum and the scales' largest exponent follow; what was added so far shrinks with them
+    auto settle = [&](int k0) {
+        largest(k0);
+        float grown = 1.0f;
+        if (__builtin_amdgcn_ballot_w64(e > E) != 0) {
+            e = wave_reduce_i(e, [](int x, int y) { return x > y ? x : y; });
+            grown = __builtin_ldexpf(1.0f, max(E - e, -1000)), E = e;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) vf[u] = __builtin_ldexpf(nf[u], 15 - SLACK - E);
+        top = fmaxf(m, fmaxf(top, xor32(top)) * g);
+        if (__builtin_amdgcn_ballot_w64(top > m + SLACK || grown != 1.0f) != 0) {
+            ref = top == -INFINITY ? 0.0f : top;
             const float shrink = __builtin_amdgcn_exp2f(m - ref);
             m = top;
             l *= shrink;
 #pragma unroll
             for (int t = 0; t < DT; t++) acc[t] *= shrink * grown;
         }
-        half8_t pw[TERMS][4];
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-            q8_each<16>([&](auto i) {
-                constexpr int r = decltype(i)::value;
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], g, -ref));
-                l += x;
-                float w = row_lane<r>(vf[u]) * x;
-                if constexpr (TERMS == 2) asm("" : "+v"(w));  // (both terms from the same rounded w: the product is not contracted into them)
-                const half_t high = (half_t)w;
-                pw[0][2 * u + r / 8][r % 8] = high;
-                if constexpr (TERMS == 2) pw[1][2 * u + r / 8][r % 8] = (half_t)(w - (float)high);
-            });
-#pragma unroll
-        for (int t = 0; t < DT; t++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const half8_t a = *(const half8_t *)&lds_v[buf][v_at(32 * t + n, 2 * j + h)];
-#pragma unroll
-                for (int x = TERMS - 1; x >= 0; x--) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pw[x][j], acc[t], 0, 0, 0);
-            }
-        if (more) store_tile(buf ^ 1);
+    };
+    int buf = 0, k0 = lo;
+    for (; k0 + Q8_TILE < hi; k0 += Q8_TILE, buf ^= 1) {
+        read_key(buf ^ 1, IC(0));
+        if constexpr (RG == 3) read_key(buf ^ 1, IC(1));
+        settle(k0);
+        // the next tile's scores beside this one's weights
+        q8_each<STEPS2>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            __builtin_amdgcn_sched_barrier(0);
+            score(ic);
+            if constexpr (i + RG - 1 < STEPS2) read_key(buf ^ 1, IC(i + RG - 1));
+            else read_value(buf, IC(i + RG - 1 - STEPS2));
+            portion(ic, weight);
+        });
+        // this tile's values beside the scaling of the next one's scores and the staging
+        q8_each<STEPS2>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            __builtin_amdgcn_sched_barrier(0);
+            value(ic);
+            if constexpr (i + RG - 1 < STEPS2) read_value(buf, IC(i + RG - 1));
+            if constexpr (i == 0) take_scales();
+            if constexpr (!MASK) portion(ic, [&](auto j) { scaled(k0 + Q8_TILE, j); });
+            if constexpr (i == 1) load_scales(k0 + 2 * Q8_TILE);
+            if constexpr (i == 2) store_keys(buf);
+            if constexpr (i == STEPS2 / 2 - 1) load_keys(k0 + 3 * Q8_TILE);
+            if constexpr (i == STEPS2 / 2) store_values(buf ^ 1);
+            if constexpr (i == STEPS2 - 2) load_values(k0 + 2 * Q8_TILE);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (MASK) q8_each<32>([&](auto j) { scaled(k0 + Q8_TILE, j); });
         lds_barrier();
     }
+    if (k0 < hi) {
+        settle(k0);
+        q8_each<32>(weight);
+        q8_each<STEPS2>([&](auto i) {
+            read_value(buf, i);
+            value(i);
+        });
+    }
+#undef IC
     l += xor32(l);
     if (c0 + wave * 32 + n >= NC) return;
-    const float up = __builtin_ldexpf(1.0f, max(E, -140) - 15);
+    const float up = __builtin_ldexpf(1.0f, max(E, -140) - 15 + SLACK);
     const int64_t o = (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)row * p.os[2];
     const int64_t part = ((int64_t)bg * p.nsplit + split) * NC + c;
     // (sum / l) 2^(E - 15): the quotient first, which stays in range

@@ -99,7 +99,8 @@ def attention_bound(out, mass, top, p, q, k, scale, v_scales, fmt, dtype, out_dt
     sums = eps * (n / 32 + 256)
     # The products of a row's probabilities and scales are brought to f16 with the largest at 2^14 or more.  Below 2^-14 an f16 has a fixed step of
     # 2^-24, so the rounding of such a product (or of the second term of a larger one) is up to half of that, 2^-39 of the largest, and there are as
-    # many as keys, each times a code.
+    # many as keys, each times a code.  16-bit queries may have a reference of up to 2^4 below the row's maximum, with the largest product that reference
+    # allows still below 2^15: a row's largest is then at 2^10 or more, and half a step 2^-35 of it.
     weight = np.nan_to_num(np.nan_to_num(p) * np.repeat(v_scales, group, 1)[:, :, None, :]).max(-1, keepdims=True, initial=0.0)
-    floor = 2.0 ** -39 * n * q8.LARGEST[fmt] * weight
+    floor = 2.0 ** (-39 if dtype == fa.F32 else -35) * n * q8.LARGEST[fmt] * weight
     return HALF_STEP[out_dtype] * np.abs(out) + (2 * score + rounding + 2 * sums) * mass + floor + 1e-30

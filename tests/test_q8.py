@@ -139,6 +139,7 @@ def mask(shape, ptr=FAKE):
     (dict(analytic=fa.CAnalyticMask(1, 1, 0, -1)), fa.ERR_INVALID_ARG, "window"),
     (dict(analytic=fa.CAnalyticMask(1, 1, 1 << 62, 0)), fa.ERR_INVALID_ARG, "2\\^61"),
     (dict(q_positions=FAKE), fa.ERR_INVALID_ARG, "q_positions"),
+    (dict(k=t8([2, 2, (1 << 31) - 4096, 64]), v=t8([2, 2, (1 << 31) - 4096, 64])), fa.ERR_UNSUPPORTED, "keys"),
 ])
 def test_attention_refuses(change, code, text):
     rc, message = status(attn(**change))
