@@ -48,7 +48,7 @@ __device__ __forceinline__ half8_t q8_widen8_pairs(half2_t a, half2_t b, half2_t
 template <int DV, int TERMS, int FMT, int WAVES, bool MASK>
 __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kernel(Q8AttnParams p) {
     request_arguments<Q8AttnParams>();
-        // 16-bit queries: a column's reference is at most 2^SLACK behind its maximum, so that sums shrink once in many tiles (666 -> 649 us for a prompt
+    // 16-bit queries: a column's reference is at most 2^SLACK behind its maximum, so that sums shrink once in many tiles (666 -> 649 us for a prompt
     // of 8192); half a step of the smallest weights is 2^-35 of the largest scale.  f32 takes none of it.
     constexpr int SLACK = TERMS == 1 ? 4 : 0;
     // pieces of LDS in flight: two ahead of their products, one for f32, whose registers are full (71 us against 73)

@@ -488,7 +488,8 @@ typedef struct {
 
 /* Arguments of fhip_q8_append.  Zero-initialise, then fill. */
 typedef struct {
-    fhip_q8_tensor k;             /* where the rows go: the whole memory that may be written             */
+    fhip_q8_tensor k;             /* where the rows go: the whole memory that may be written (rows of a block that lie in
+                                     front of a view with first > 0 would not be coded again with it)  */
     fhip_q8_tensor v;
     uint64_t row;                 /* place of the first new row                                        */
     const int32_t *lens;          /* optional device [B]: sequence b's first new row goes to row + lens[b], and its position in

@@ -342,3 +342,45 @@ def test_rows_behind_32_bits(device):
     want = q8.read_back(q8.encode(k, s[..., None], INT8), s, INT8, 1)
     assert np.array_equal(x.dequantize(row=rows - 3).to_numpy(), want)
     assert np.array_equal(x.narrow(2, rows - 2, 2).dequantize().to_numpy(), want[:, :, 1:])
+
+
+@pytest.mark.parametrize("n", [3, 5000])
+@pytest.mark.parametrize("normed", [False, True])
+def test_strides_of_64_bits(device, normed, n):
+    """Batch strides beyond 31 bits (of a batch of one, which never steps) change nothing."""
+    rng = np.random.default_rng(n)
+    shape = (1, 8, n, 128)
+    tensors = [upload(device, normals(rng, shape, F16), F16) for _ in range(3)]
+    far = [fa.Tensor(t.buffer, F16, shape, [1 << 40] + list(t.strides[1:])) for t in tensors]
+    norm = fa.RmsNorm(np.linspace(0.5, 1.5, 128, dtype=np.float32), None, 1e-6, F32, device) if normed else None
+    rope = fa.RopeCache(128, n, 10000.0, device)
+    got = []
+    for (q, k, v), wide in ((tensors, False), (far, True)):
+        k8, v8 = (fa.Q8Tensor.empty(device, shape, fa.Q8Format(INT8), 1) for _ in range(2))
+        if wide:
+            k8, v8 = (fa.Q8Tensor(x.codes, x.scales, shape, x.format, 1, (1 << 40,) + x.strides[1:], 0, (1 << 40,) + x.scale_strides[1:]) for x in (k8, v8))
+        out = k8.append(v8, k, v, 0, rope=rope, k_norm=norm, q=q, q_norm=norm)
+        got.append([out.to_numpy(), k8.dequantize().to_numpy(), v8.dequantize().to_numpy()])
+    for near, far_ in zip(*got):
+        assert np.array_equal(near, far_)
+
+
+@pytest.mark.parametrize("B, rows", [(1, (1 << 25) + 41), (5, 1 << 23)])
+def test_reading_back_in_parts(device, B, rows):
+    """More than 2^30 pieces of eight codes, of one sequence and of five (which share their rows): a launch takes no more."""
+    D = 256
+    x = fa.Q8Tensor.empty(device, (1, 1, rows, D), fa.Q8Format.INT8, 1)
+    rng = np.random.default_rng(3)
+    places = [0, min(1 << 25, rows) - 2, rows - 4]
+    for at in places:
+        t = upload(device, normals(rng, (1, 1, 4, D), F32), F32)
+        x.append(x, t, t, min(at, rows - 4))
+    whole = fa.Q8Tensor(x.codes, x.scales, (B, 1, rows, D), x.format, 1, (0,) + x.strides[1:], 0, (0,) + x.scale_strides[1:])
+    out = whole.dequantize(fa.F16)
+    for at in places:
+        at = min(at, rows - 4)
+        want = x.narrow(2, at, 4).dequantize(fa.F16).to_numpy()
+        assert np.abs(want).max() > 0
+        for b in range(B):
+            part = fa.Tensor(out.buffer, fa.F16, (1, 1, 4, D), (4 * D, 4 * D, D, 1), (b * rows + at) * D)
+            assert np.array_equal(part.to_numpy(), want)
