@@ -12,7 +12,7 @@
 // the tile after them is widened into LDS.  The order is written down step by step (sched_barrier): left to itself the compiler puts the products
 // of a tile behind each other, each waiting for its piece of LDS (695 us against 660 for the prompt below).
 // Measured: 620 us for a causal prompt of 8192 f16 rows, 32 / 8 heads of 128, int8 (887 TFLOP/s of visible pairs; the matrix units are busy for 37 %
-// of the cycles, the vector units for 70 %, at 2.1 GHz); 159 us for 4 chunks of 512 bf16 rows over a window of 4096, e4m3.
+// of the cycles, the vector units for 63 %, at 2.1 GHz); 159 us for 4 chunks of 512 bf16 rows over a window of 4096, e4m3.
 //
 // Numbers are brought to f16 as in the kernel for few rows (attn_q8_decode.hip): codes exactly, a column's q scaled by a power of two, one term for
 // 16-bit queries and two for f32.  The values' scales go with the probabilities, brought below 2^15 by a power of two E that follows the largest

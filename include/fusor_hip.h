@@ -548,9 +548,9 @@ int fhip_q8_attention_workspace_bytes(const fhip_q8_attn_args *args, int32_t com
  * cases of fhip_flash_attention: rows whose keys are all masked come out NaN, no keys at all give zeros.  Scores, softmax
  * statistics and sums are f32; codes enter the matrix products exactly, f32 queries and probabilities as two 16-bit terms
  * each (f32 precision), 16-bit queries exactly and their probabilities rounded to 11 bits.  Products of probability and value
- * scale below 2^-40 (16-bit queries: 2^-35) of the largest scale that the row's keys bring are lost; finite mask values below
- * -2^22 / log2(e) count as that.  Rows of the cache that a mask hides by position or length may hold anything.  Asynchronous on
- * `s`; may be captured. */
+ * scale below 2^-40 (16-bit queries: 2^-35) of the largest scale among the keys that the call's rows see are lost; finite mask
+ * values below -2^22 / log2(e) count as that.  Rows of the cache that a mask hides by position or length may hold anything.
+ * Asynchronous on `s`; may be captured. */
 int fhip_q8_attention(fhip_stream *s, const fhip_q8_attn_args *args);
 
 /* Growable 8-bit cache of keys and values: fhip_kv_cache with the same observable lengths and growth (the allocation grows to

@@ -242,6 +242,18 @@ def test_scales_far_apart(device, dtype):
     c.check(out_dtype=F32)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D, Sq, Skv", [(64, 40, 700), (128, 300, 449), (256, 33, 1500), (192, 65, 64), (128, 64, 65)])
+def test_rising_maximum(device, dtype, D, Sq, Skv):
+    """Scores that grow along the keys, slowly enough that a row's maximum moves a little in every tile; then values' scales that grow."""
+    c = Call(device, 1, 4, 2, Sq, Skv, D, dtype, INT8, 1)
+    c.k_state[1][:] *= np.linspace(0.25, 8.0, Skv, dtype=np.float32)
+    c.check(out_dtype=F32)
+    c.v_state[1][:] *= np.exp2(np.linspace(-3.0, 3.0, Skv, dtype=np.float32))
+    offset = max(0, Skv - Sq)
+    c.check(hidden=positions_mask(Sq, Skv, [offset]), analytic=(True, offset, 0), out_dtype=F32)
+
+
 def test_queries_of_any_size(device):
     for power in (-140, -100, 0, 60):
         c = Call(device, 1, 2, 2, 2, 64, 64, F32, INT8, 1)
