@@ -19,9 +19,10 @@
 // largest) for 16-bit tensors and taken as two terms for f32.
 //
 // Bound by the bytes of codes and scales where there are many: 157 us for 16 ragged sequences of up to 16384 keys, 32 heads of 96 (e4m3, 5.2 TB/s),
-// 33 us with the joining for 16 of 4096, 8 KV heads of 128 (134 MB).  One sequence is bound by a chain of latencies: 10 us for 4096 keys, about half of it the
-// launch of the second kernel and its reads (one kernel whose last workgroup joins the shares took 97 us: the order it needs between XCDs
-// writes back and drops their L2).  Two steps of keys in flight against one: 39 -> 33 us; non-temporal loads: no change.
+// 33 us with the joining for 16 of 4096, 8 KV heads of 128 (134 MB).  One sequence is bound by a chain of latencies: 10 us for 4096 keys, 8 of the
+// main kernel and 3 of the joining where each stands alone (one kernel whose last workgroup joins the shares took 97 us: the order it needs
+// between XCDs writes back and drops their L2).  Two steps of keys in flight without a branch, against one behind one: 58 -> 35 us for the 16
+// sequences, with the joining by lanes side by side; non-temporal loads: no change.
 #include <algorithm>
 
 #include "q8.h"

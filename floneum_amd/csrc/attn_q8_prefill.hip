@@ -11,8 +11,9 @@
 // wavefront: the next tile's scores are multiplied while this one's weights are made, this tile's values while the next one's scores are scaled and
 // the tile after them is widened into LDS.  The order is written down step by step (sched_barrier): left to itself the compiler puts the products
 // of a tile behind each other, each waiting for its piece of LDS (695 us against 660 for the prompt below).
-// Measured: 620 us for a causal prompt of 8192 f16 rows, 32 / 8 heads of 128, int8 (887 TFLOP/s of visible pairs; the matrix units are busy for 37 %
-// of the cycles, the vector units for 63 %, at 2.1 GHz); 159 us for 4 chunks of 512 bf16 rows over a window of 4096, e4m3.
+// Measured: 620 to 660 us, box to box, for a causal prompt of 8192 f16 rows, 32 / 8 heads of 128, int8 (830 to 890 TFLOP/s of visible pairs; the
+// matrix units are busy for 37 % of the cycles, the vector units for 63 %, at 2.1 GHz); 159 us for 4 chunks of 512 bf16 rows over a window of 4096,
+// e4m3; 70 us for 129 f32 rows on 8003 keys, whose queries of two terms fill the registers.
 //
 // Numbers are brought to f16 as in the kernel for few rows (attn_q8_decode.hip): codes exactly, a column's q scaled by a power of two, one term for
 // 16-bit queries and two for f32.  The values' scales go with the probabilities, brought below 2^15 by a power of two E that follows the largest
