@@ -433,8 +433,12 @@ Q8AttnPlan q8_prefill_plan(const Q8AttnParams &p) {
 template <int DV, int TERMS, int FMT, int WAVES, bool MASK>
 static int launch_prefill_waves(const Q8AttnParams &p, hipStream_t stream) {
     const int64_t NC = (int64_t)p.G * p.Sq, blocks = (NC + 32 * WAVES - 1) / (32 * WAVES);
-    hipLaunchKernelGGL((q8_prefill_kernel<DV, TERMS, FMT, WAVES, MASK>), dim3((unsigned)((int64_t)p.B * p.Hkv * blocks * p.nsplit)), dim3(64 * WAVES), 0,
-                       stream, p);
+    const int64_t workgroups = (int64_t)p.B * p.Hkv * blocks * p.nsplit;
+    if (workgroups * 64 * WAVES > UINT32_MAX) {
+        set_error("q8_attention: more query rows than a launch has lanes for");
+        return FHIP_ERR_UNSUPPORTED;
+    }
+    hipLaunchKernelGGL((q8_prefill_kernel<DV, TERMS, FMT, WAVES, MASK>), dim3((unsigned)workgroups), dim3(64 * WAVES), 0, stream, p);
     FHIP_HIP_CHECK(hipGetLastError());
     return p.nsplit > 1 ? launch_q8_merge(p, stream) : FHIP_OK;
 }

@@ -440,14 +440,16 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendParams p) {
     }
 }
 
-// slots: of a job per workgroup
+// slots: of a job per workgroup.  0: more than a launch may have (2^32 lanes)
 static uint32_t append_workgroups(Q8AppendParams &p, uint32_t slots) {
     uint32_t wgs = 0;
     for (int i = 0; i < p.jobs; i++) {
         p.first_wg[i] = wgs;
         wgs += (p.job[i].total + slots - 1) / slots;
     }
-    return wgs;
+    if (wgs < (1u << 24)) return wgs;
+    set_error("q8_append: more rows than a launch has lanes for");
+    return 0;
 }
 // t / d for t < 2^31 as the high half of t * m[0], shifted down by m[1] (m[0] = 0: d is 1): with 2^l >= d the factor ceil(2^(31 + l) / d) is off by less
 // than one in 2^l / d, which is too little to reach the next quotient (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994)
@@ -460,7 +462,7 @@ static void divisor(uint32_t d, uint32_t m[2]) {
     m[1] = l - 1;
 }
 template <int LPR, int RPG>
-static void launch_rows(Q8AppendParams &p, bool normed, hipStream_t stream) {
+static int launch_rows(Q8AppendParams &p, bool normed, hipStream_t stream) {
     for (int i = 0; i < p.jobs; i++) {  // a slot is RPG positions of a head
         Q8Rows &j = p.job[i];
         const uint32_t sequences = j.total / ((uint32_t)j.heads * j.span);
@@ -477,16 +479,22 @@ static void launch_rows(Q8AppendParams &p, bool normed, hipStream_t stream) {
         near = near && !far(j.out.ss[0]) && !far(j.out.ss[1]);
     }
     const dim3 grid(append_workgroups(p, 256 / LPR));
+    if (grid.x == 0) return FHIP_ERR_UNSUPPORTED;
     if (normed && near) hipLaunchKernelGGL((q8_append_rows_kernel<LPR, RPG, true, true>), grid, dim3(256), 0, stream, p);
     else if (normed) hipLaunchKernelGGL((q8_append_rows_kernel<LPR, RPG, true, false>), grid, dim3(256), 0, stream, p);
     else if (near) hipLaunchKernelGGL((q8_append_rows_kernel<LPR, RPG, false, true>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((q8_append_rows_kernel<LPR, RPG, false, false>), grid, dim3(256), 0, stream, p);
+    FHIP_HIP_CHECK(hipGetLastError());
+    return FHIP_OK;
 }
 template <int LPR, int RPG>
-static void launch_blocks(Q8AppendParams &p, bool normed, hipStream_t stream) {
+static int launch_blocks(Q8AppendParams &p, bool normed, hipStream_t stream) {
     const dim3 grid(append_workgroups(p, 256 / LPR * RPG));
+    if (grid.x == 0) return FHIP_ERR_UNSUPPORTED;
     if (normed) hipLaunchKernelGGL((q8_append_kernel<LPR, RPG, true>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((q8_append_kernel<LPR, RPG, false>), grid, dim3(256), 0, stream, p);
+    FHIP_HIP_CHECK(hipGetLastError());
+    return FHIP_OK;
 }
 template <int LPR>
 static int launch_append_lpr(Q8AppendParams &p, int max_block, bool rows_alone, bool normed, hipStream_t stream) {
@@ -496,18 +504,16 @@ static int launch_append_lpr(Q8AppendParams &p, int max_block, bool rows_alone, 
         for (int i = 0; i < p.jobs; i++) rows += p.job[i].total;
         // two positions per group of lanes where that still gives every CU eight workgroups (us, q, k and v of 8192 f16 rows of 32/8 heads at 128, with
         // one, two and four: 57, 52 and 72)
-        if (rows >= (uint64_t)GR * 2 * 2048) launch_rows<LPR, 2>(p, normed, stream);
-        else launch_rows<LPR, 1>(p, normed, stream);
-    } else if (max_block <= GR) {
-        launch_blocks<LPR, 1>(p, normed, stream);
-    } else if (max_block <= 2 * GR) {
-        launch_blocks<LPR, 2>(p, normed, stream);
-    } else if constexpr (LPR > 8) {  // 64 tokens on groups of 16 or 32 lanes
-        if (max_block <= 4 * GR) launch_blocks<LPR, 4>(p, normed, stream);
-        else if constexpr (LPR > 16) launch_blocks<LPR, 8>(p, normed, stream);
+        if (rows >= (uint64_t)GR * 2 * 2048) return launch_rows<LPR, 2>(p, normed, stream);
+        return launch_rows<LPR, 1>(p, normed, stream);
     }
-    FHIP_HIP_CHECK(hipGetLastError());
-    return FHIP_OK;
+    if (max_block <= GR) return launch_blocks<LPR, 1>(p, normed, stream);
+    if (max_block <= 2 * GR) return launch_blocks<LPR, 2>(p, normed, stream);
+    if constexpr (LPR > 8) {  // 64 tokens on groups of 16 or 32 lanes
+        if (max_block <= 4 * GR) return launch_blocks<LPR, 4>(p, normed, stream);
+        if constexpr (LPR > 16) return launch_blocks<LPR, 8>(p, normed, stream);
+    }
+    return FHIP_ERR_UNSUPPORTED;  // (no such block)
 }
 int launch_q8_append(Q8AppendParams &p, int max_block, bool rows_alone, bool normed, hipStream_t stream) {
     if (p.D <= 64) return launch_append_lpr<8>(p, max_block, rows_alone, normed, stream);

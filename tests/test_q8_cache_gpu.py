@@ -384,3 +384,14 @@ def test_reading_back_in_parts(device, B, rows):
         for b in range(B):
             part = fa.Tensor(out.buffer, fa.F16, (1, 1, 4, D), (4 * D, 4 * D, D, 1), (b * rows + at) * D)
             assert np.array_equal(part.to_numpy(), want)
+
+
+@pytest.mark.parametrize("block", [1, 16])
+def test_more_rows_than_a_launch_takes(device, block):
+    """A call whose rows would need 2^32 lanes and more is refused (all but the first rows would lie outside the cache)."""
+    row = upload(device, np.ones((1, 1, 1, 128), np.float32), F32)
+    many = fa.Tensor(row.buffer, F32, (1, 1, 1 << 29, 128), (0, 0, 0, 1))
+    k8, v8 = (fa.Q8Tensor.empty(device, (1, 1, 16, 128), fa.Q8Format(INT8), block) for _ in range(2))
+    with pytest.raises(fa.FhipError, match="lanes"):
+        k8.append(v8, many, many, 0, lens=fa.IntTensor(device, [0]))
+    assert not k8.dequantize().to_numpy().any()
