@@ -135,6 +135,7 @@ static int check_new_rows(const fhip_q8_append_args *a, AppendShape *s) {
     if (a->rope) {
         const fhip_rope_tables *r = a->rope;
         if (!r->cos || !r->sin) return invalid("rope: NULL tables");
+        if (r->table_rows == 0) return invalid("rope: tables without rows");  // (rows that are left out are read at position 0)
         if (r->table_rows > 0x7fffffffffffull || r->start_pos > r->table_rows || (!a->lens && s->n > r->table_rows - r->start_pos)) {
             set_error("rope: positions %llu..%llu exceed the %llu rows of the tables", (unsigned long long)r->start_pos,
                       (unsigned long long)(r->start_pos + s->n), (unsigned long long)r->table_rows);

@@ -512,8 +512,8 @@ typedef struct {
  * likewise without norm and rotation, q normalised and rotated into q_out (the counterpart of fhip_kv_cache_qkv_rope_append).  Keys that
  * were rotated and normalised are the f32 values that call rounds to its cache's type.  Rows whose place lies outside the view, or whose
  * position outside the tables, are left out (with `lens` only the device knows them), and so are rows from counts[b] on: neither the
- * cache nor q_out is written there.  Rows of a block behind the new ones count as absent: what they held is lost with the
- * scale.  Asynchronous on `s`; may be captured. */
+ * cache nor q_out is written there.  The tables hold one row at least.  Rows of a block behind the new ones count as absent: what they
+ * held is lost with the scale.  Asynchronous on `s`; may be captured. */
 int fhip_q8_append(fhip_stream *s, const fhip_q8_append_args *args);
 
 /* out[b,h,i,:] = row `row` + lens[b] + i of x (lens NULL: row + i), code * scale in f32, rounded to out_dtype.  out: [B, Hkv, n, D], any

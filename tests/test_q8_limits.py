@@ -1,0 +1,23 @@
+"""Sizes at which calls of the 8-bit cache are refused, without a GPU: the checks come before anything that touches the device, so stand-ins
+for handles and device pointers are never looked into."""
+import ctypes
+
+import pytest
+
+import floneum_amd as fa
+from test_q8 import FAKE, append, t4, t8  # noqa: F401
+
+
+def call(function, *args):
+    """(status, message) of a library call on a stand-in for a stream."""
+    stream = ctypes.create_string_buffer(64)
+    rc = getattr(fa.lib(), function)(ctypes.cast(stream, ctypes.c_void_p), *args)
+    return rc, fa.lib().fhip_last_error().decode() if rc else ""
+
+
+@pytest.mark.parametrize("lens", [None, FAKE])
+@pytest.mark.parametrize("n", [1, 3])
+def test_rope_tables_without_rows(lens, n):
+    """Rows whose position the tables do not hold are left out with device lengths, but there has to be a row to read in their place."""
+    rc, message = call("fhip_q8_append", ctypes.byref(append(n=n, rope=(FAKE, FAKE, 0, 0, 0), lens=lens)))
+    assert rc == fa.ERR_INVALID_ARG and "tables" in message
