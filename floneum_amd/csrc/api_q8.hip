@@ -520,7 +520,9 @@ int fhip_q8_cache_create(fhip_device *dev, fhip_q8_format format, uint32_t block
     *out = nullptr;
     int rc = check_format(format, block_tokens);
     if (rc) return rc;
-    if (max_sequence_len == 0 || max_sequence_len > 0x3fffffffull) return invalid("q8_cache_create: max_sequence_len must be in 1..2^30-1");
+    // (the window slides through whole blocks of twice as many rows and two blocks, numbered in 31 bits)
+    if (max_sequence_len == 0 || max_sequence_len > (1ull << 30) - 2 * Q8_MAX_BLOCK)
+        return invalid("q8_cache_create: max_sequence_len must be in 1..2^30-128");
     fhip_q8_cache *c = new (std::nothrow) fhip_q8_cache();
     if (!c) {
         set_error("out of host memory");

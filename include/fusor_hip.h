@@ -556,6 +556,7 @@ int fhip_q8_attention(fhip_stream *s, const fhip_q8_attn_args *args);
 /* Growable 8-bit cache of keys and values: fhip_kv_cache with the same observable lengths and growth (the allocation grows to
  * the next power of two; beyond max_sequence_len only the last max_sequence_len rows stay), k_all / v_all being 8-bit views. */
 typedef struct fhip_q8_cache fhip_q8_cache;
+/* max_sequence_len: 1 to 2^30 - 128 */
 int fhip_q8_cache_create(fhip_device *dev, fhip_q8_format format, uint32_t block_tokens, uint64_t max_sequence_len,
                          fhip_q8_cache **out);
 int fhip_q8_cache_destroy(fhip_q8_cache *c);

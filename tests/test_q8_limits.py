@@ -21,3 +21,13 @@ def test_rope_tables_without_rows(lens, n):
     """Rows whose position the tables do not hold are left out with device lengths, but there has to be a row to read in their place."""
     rc, message = call("fhip_q8_append", ctypes.byref(append(n=n, rope=(FAKE, FAKE, 0, 0, 0), lens=lens)))
     assert rc == fa.ERR_INVALID_ARG and "tables" in message
+
+
+@pytest.mark.parametrize("block", [1, 8, 16, 32, 64])
+def test_longest_cache(block):
+    """A cache slides through 2 * max_sequence_len rows in whole blocks and two blocks more, and every row's number has 31 bits."""
+    longest = (1 << 30) - 128
+    assert -(-2 * longest // block) * block + 2 * block < 1 << 31
+    dev, out = ctypes.cast(ctypes.create_string_buffer(4096), ctypes.c_void_p), ctypes.c_void_p()
+    assert fa.lib().fhip_q8_cache_create(dev, 0, block, longest + 1, ctypes.byref(out)) == fa.ERR_INVALID_ARG and not out.value
+    assert "2^30-128" in fa.lib().fhip_last_error().decode()
