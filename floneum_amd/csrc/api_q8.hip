@@ -383,6 +383,10 @@ int fhip_q8_dequantize(fhip_stream *s, const fhip_q8_tensor *x, uint64_t row, co
             set_error("output stride %d is 0 (overlapping writes)", i);
             return FHIP_ERR_INVALID_ARG;
         }
+    if ((uint64_t)os[1] * (os[3] / 8) > 0x7fffffffull) {  // (the heads of a row go in one launch)
+        set_error("q8_dequantize: 2^34 elements or more in a row of all heads");
+        return FHIP_ERR_UNSUPPORTED;
+    }
     Q8ReadParams p;
     memset(&p, 0, sizeof(p));
     p.x = view_of(*x);

@@ -559,14 +559,14 @@ int launch_q8_dequantize(const Q8ReadParams &p, hipStream_t stream) {
     const uint64_t per_row = (uint64_t)p.H * (p.D / 8), most_rows = std::max<uint64_t>(1, (1u << 30) / per_row);
     const int rows = (int)std::min<uint64_t>(p.n, most_rows), sequences = (int)std::max<uint64_t>(1, std::min<uint64_t>(p.B, most_rows / rows));
     const int64_t bytes = p.out_dtype == FHIP_F32 ? 4 : 2;
-    for (int b = 0; b < p.B; b += sequences)
+    for (int64_t b = 0; b < p.B; b += sequences)
         for (int64_t i = 0; i < p.n; i += rows) {
             Q8ReadParams q = p;
-            q.B = std::min(sequences, p.B - b);
+            q.B = (int)std::min<int64_t>(sequences, p.B - b);
             q.n = (int)std::min<int64_t>(rows, p.n - i);
-            q.x.codes += (int64_t)b * p.x.cs[0];
-            q.x.scales += (int64_t)b * p.x.ss[0];
-            q.out = (char *)p.out + ((int64_t)b * p.os[0] + i * p.os[2]) * bytes;
+            q.x.codes += b * p.x.cs[0];
+            q.x.scales += b * p.x.ss[0];
+            q.out = (char *)p.out + (b * p.os[0] + i * p.os[2]) * bytes;
             q.row += i;
             if (p.lens) q.lens += b;
             Q8ReadDivisors div;

@@ -31,3 +31,11 @@ def test_longest_cache(block):
     dev, out = ctypes.cast(ctypes.create_string_buffer(4096), ctypes.c_void_p), ctypes.c_void_p()
     assert fa.lib().fhip_q8_cache_create(dev, 0, block, longest + 1, ctypes.byref(out)) == fa.ERR_INVALID_ARG and not out.value
     assert "2^30-128" in fa.lib().fhip_last_error().decode()
+
+
+@pytest.mark.parametrize("heads, D", [(1 << 28, 64), ((1 << 31) // 9 + 1, 72), (1 << 26, 256), (1 << 30, 256)])
+def test_reading_back_rows_of_too_many_heads(heads, D):
+    """A launch numbers the pieces of eight elements in 31 bits and takes at least a row of all heads."""
+    x, out = t8([1, heads, 1, D], stride=(0, 0, 256), scale_stride=(0, 0)), t4([1, heads, 1, D])
+    rc, message = call("fhip_q8_dequantize", ctypes.byref(x), 0, None, ctypes.byref(out), 0)
+    assert rc == fa.ERR_UNSUPPORTED and "2^34" in message
