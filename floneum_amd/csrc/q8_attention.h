@@ -123,9 +123,13 @@ __device__ __forceinline__ void q8_query_terms(const Q8AttnParams &p, float x, i
     high = (half_t)v;
     if constexpr (TERMS == 2) low = (half_t)(v - (float)high);
 }
-// what takes a product of such a query with codes times their scale to the log2 domain
+// What takes a product of such a query with codes times their scale to the log2 domain, rounded once.  Never 0, which has no product with the
+// -infinity of a hidden key, nor infinite, which has none with 0: a row that would need less than the least f32 has scores of next to nothing all the
+// same.
 __device__ __forceinline__ float q8_score_scale(const Q8AttnParams &p, int shift) {
-    return __builtin_ldexpf((p.scale != 0.0f ? __builtin_fabsf(p.scale) : 1.0f) * Q8_LOG2E, -shift);
+    const float factor = p.scale != 0.0f ? __builtin_fabsf(p.scale) : 1.0f;
+    const float g = __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(factor) * Q8_LOG2E, __builtin_amdgcn_frexp_expf(factor) - shift);
+    return fminf(fmaxf(g, 0x1p-149f), 3.402823466e38f);
 }
 
 }  // namespace fhip

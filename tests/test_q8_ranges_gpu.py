@@ -1,0 +1,49 @@
+"""Attention over the 8-bit cache where numbers are near the ends of f32's range, on both kernels (few rows and many), against the same in
+64 bits."""
+import numpy as np
+import pytest
+
+import floneum_amd as fa
+from oracle import q8
+from q8_helpers import rounded, upload, upload_q8
+from test_q8_attention_gpu import Call, positions_mask
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = fa.F32, fa.F16, fa.BF16
+INT8, E4M3 = q8.INT8, q8.E4M3
+
+
+def times_power(x, power):
+    """x * 2^power in f32 (in two steps: the power alone may have no f32)."""
+    half = power // 2
+    return (x * np.float32(2.0 ** half) * np.float32(2.0 ** (power - half))).astype(np.float32)
+
+
+# ---- scores -------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("power, scale", [(-140, None), (-145, 2.0 ** -20), (0, 1e-44), (-100, 2.0 ** -60), (-30, 2.0 ** -126)])
+@pytest.mark.parametrize("D, Sq, Skv", [(64, 40, 65), (128, 130, 130), (256, 40, 200), (64, 2, 65)])
+def test_queries_of_almost_nothing(device, dtype, power, scale, D, Sq, Skv):
+    """Queries, or a factor of the scores, that leave scores of nothing: every key that a row sees weighs the same, hidden ones nothing."""
+    c = Call(device, 1, 4, 2, Sq, Skv, D, dtype, INT8, 1)
+    c.q = rounded(times_power(c.q, max(power, -131) if dtype == BF16 else power), dtype)  # (bf16 ends at 2^-133)
+    c.scale = c.scale if scale is None else scale
+    c.check()
+    at = Skv - Sq
+    c.check(positions_mask(Sq, Skv, [at]), analytic=(True, at, 0))
+    c.check(positions_mask(Sq, Skv, [at], 20), analytic=(True, at, 20))
+    c.check(np.broadcast_to(np.arange(Skv) >= 50, (1, 1, Sq, Skv)), kv_lens=fa.IntTensor(device, [50]))
+    m = np.where(positions_mask(Sq, Skv, [at])[0, 0], -np.inf, 0.0).astype(np.float32)
+    c.check(positions_mask(Sq, Skv, [at]), mask=(upload(device, m, dtype), fa.MaskKind.QKMask))
+
+
+@pytest.mark.parametrize("Sq, Skv", [(2, 300), (40, 65), (130, 200)])
+def test_the_largest_factor(device, Sq, Skv):
+    """A factor of the scores whose product with log2 e is beyond f32, with keys and queries whose products are that small."""
+    c = Call(device, 1, 4, 2, Sq, Skv, 64, F32, INT8, 1)
+    c.q = times_power(c.q, -60)
+    c.k_state[1][:] = times_power(c.k_state[1], -70)
+    c.scale = 3.2e38
+    c.check()
