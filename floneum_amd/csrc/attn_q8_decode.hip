@@ -97,6 +97,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     // queries: column c is row c / G, head c % G of the group
     half8_t q[TERMS][KS][2];
     float colscale;
+    bool tiny = false;  // a column of queries below 2^-75: 2^64 of its factor go with the keys' scales, with which alone it would end beyond f32's normal range
     int limit, start;  // keys [start, limit) of the column
     int row;
     // What a wavefront holds of a step's keys.  Steps are loaded NBUF ahead, without a branch (behind one the compiler would wait for all
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         spread_scale8(x.ks, p.k, k0);
         spread_scale8(x.vs, p.v, k0);
         float exf[8], back[8], vs[8], ks[8];  // e_j, 2^-e_j
-        bool lost = false;
+        bool lost = tiny;
 #pragma unroll
         for (int i = 0; i < 8; i++) ks[i] = x.ks[i], vs[i] = x.vs[i];
 #pragma unroll
@@ -173,8 +174,10 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         // NaN among the values' scales goes by way of the scores, where rows that a mask hides are taken out
         if (__builtin_amdgcn_ballot_w64(lost) != 0) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < 8; i++) {
+                if (tiny) ks[i] *= 0x1p-64f;
                 if (vs[i] != vs[i]) ks[i] = vs[i], vs[i] = 1.0f;
+            }
         }
         // scores
         float sc[8];
@@ -337,7 +340,8 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                         q[0][s][a][e] = high;
                         if constexpr (TERMS == 2) q[1][s][a][e] = low;
                     }
-            colscale = q8_score_scale(p, shift);
+            tiny = shift > 90;
+            colscale = q8_score_scale(p, tiny ? shift - 64 : shift);
         }
         const int64_t at = vis.pos0 + row;
         limit = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);

@@ -82,7 +82,7 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
     const int c = min(c0 + wave * 32 + n, NC - 1);
     const int row = c / p.G, head = kvh * p.G + c % p.G;
     half8_t q[TERMS][STEPS];
-    float colscale;
+    int shift = 0;
     {  // lane half h holds dims 16 i + 8 h .. + 7 of step i
         const int64_t base = (int64_t)b * p.qs[0] + (int64_t)head * p.qs[1] + (int64_t)row * p.qs[2];
         Q8Query8<TERMS> raw[STEPS];
@@ -96,7 +96,6 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
         if (TERMS == 1 && p.q_dtype == FHIP_F16 && p.scale != 0.0f) {  // as they are
 #pragma unroll
             for (int i = 0; i < STEPS; i++) q[0][i] = raw[i].halves(p, 16 * i + 8 * h);
-            colscale = q8_score_scale(p, 0);
         } else {
             float x[STEPS][8], top = 0.0f;
 #pragma unroll
@@ -105,7 +104,7 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
 #pragma unroll
                 for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[i][e]));
             }
-            const int shift = q8_query_shift(fmaxf(top, xor32(top)));
+            shift = q8_query_shift(fmaxf(top, xor32(top)));
 #pragma unroll
             for (int i = 0; i < STEPS; i++)
 #pragma unroll
@@ -115,9 +114,12 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
                     q[0][i][e] = high;
                     if constexpr (TERMS == 2) q[1][i][e] = low;
                 }
-            colscale = q8_score_scale(p, shift);
         }
     }
+    // Products of codes and queries, below 2^33, are multiplied by the keys' scales (2^-100 to 2^121) first and by the column's factor afterwards: 2^-26 of it
+    // goes with the former, so that no product of finite numbers passes f32's range (2^-10 where queries of 2^85 and more have a factor near its end)
+    const int ahead = __builtin_amdgcn_ballot_w64(shift < -70) != 0 ? 10 : 26;
+    const float colscale = q8_score_scale(p, shift - ahead), down = __builtin_ldexpf(1.0f, -ahead);
     const int64_t at = vis.pos0 + row;
     const int limit = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);
     const int start = (int)(p.window > 0 ? min((int64_t)hi, max((int64_t)0, at - p.window + 1)) : 0);
@@ -128,7 +130,9 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
     for (int t = 0; t < DT; t++)
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[t][r] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
+    // the column's reference, from which its weights are counted (never -infinity: a row without a key has no weights, but no difference of infinities
+    // either), their sum, and the largest exponent of the values' scales (of the wavefront)
+    float m = -3.402823466e38f, l = 0.0f;
     int E = -200;
 
     const uint8_t *const kbase = p.k.codes + (int64_t)b * p.k.cs[0] + (int64_t)kvh * p.k.cs[1];
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
         for (int u = 0; u < 2; u++) {
             // NaN among the values' scales goes by way of the scores, where rows that a mask hides are taken out
             const bool lost = vs[u] != vs[u];
-            kf[u] = lost ? vs[u] : ks[u], nf[u] = lost ? 0.0f : vs[u];
+            kf[u] = (lost ? vs[u] : ks[u]) * down, nf[u] = lost ? 0.0f : vs[u];
             e = max(e, nf[u] > 0.0f ? __builtin_amdgcn_frexp_expf(nf[u]) : -200);
         }
     };
@@ -278,10 +282,9 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
     };
     const float g = MASK ? 1.0f : colscale;
     half8_t pw[TERMS][4];
-    float ref = 0.0f;
     auto weight = [&](auto ic) {
         constexpr int i = decltype(ic)::value, u = i / 16, r = i % 16;
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], g, -ref));
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], g, -m));
         l += x;
         float w = row_lane<r>(vf[u]) * x;
         if constexpr (TERMS == 2) asm("" : "+v"(w));  // (both terms from the same rounded w: the product is not contracted into them)
@@ -326,15 +329,14 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
         largest(k0);
         float grown = 1.0f;
         if (__builtin_amdgcn_ballot_w64(e > E) != 0) {
-            e = wave_reduce_i(e, [](int x, int y) { return x > y ? x : y; });
+            e = __builtin_amdgcn_readfirstlane(wave_reduce_i(e, [](int x, int y) { return x > y ? x : y; }));
             grown = __builtin_ldexpf(1.0f, max(E - e, -1000)), E = e;
         }
 #pragma unroll
         for (int u = 0; u < 2; u++) vf[u] = __builtin_ldexpf(nf[u], 15 - SLACK - E);
         top = fmaxf(m, fmaxf(top, xor32(top)) * g);
         if (__builtin_amdgcn_ballot_w64(top > m + SLACK || grown != 1.0f) != 0) {
-            ref = top == -INFINITY ? 0.0f : top;
-            const float shrink = __builtin_amdgcn_exp2f(m - ref);
+            const float shrink = __builtin_amdgcn_exp2f(m - top);
             m = top;
             l *= shrink;
 #pragma unroll

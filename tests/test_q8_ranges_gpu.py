@@ -47,3 +47,30 @@ def test_the_largest_factor(device, Sq, Skv):
     c.k_state[1][:] = times_power(c.k_state[1], -70)
     c.scale = 3.2e38
     c.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("fmt, block", [(INT8, 1), (E4M3, 16)])
+@pytest.mark.parametrize("D, Sq, Skv", [(64, 2, 300), (128, 1, 64), (64, 40, 65), (128, 130, 300), (256, 40, 90)])
+@pytest.mark.parametrize("power", [-90, 90, 112, 125])
+def test_keys_and_queries_far_apart(device, dtype, fmt, block, D, Sq, Skv, power):
+    """Scores of ordinary size from keys that are 2^power times the ordinary and queries that are as much smaller."""
+    c = Call(device, 1, 4, 2, Sq, Skv, D, dtype, fmt, block)
+    c.q = rounded(times_power(c.q, -power), dtype)
+    c.k_state[1][:] = times_power(c.k_state[1], power)
+    c.check(out_dtype=F32)
+    at = Skv - Sq
+    c.check(positions_mask(Sq, Skv, [at]), analytic=(True, at, 0), out_dtype=F32)
+    m = np.where(positions_mask(Sq, Skv, [at])[0, 0], -np.inf, 0.0).astype(np.float32)
+    c.check(positions_mask(Sq, Skv, [at]), mask=(upload(device, m, dtype), fa.MaskKind.QKMask), out_dtype=F32)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("Sq", [2, 40])
+def test_keys_of_every_size_at_once(device, dtype, Sq):
+    """Keys of 2^110 in front of, beside and behind ordinary ones, which the queries are small enough to see."""
+    c = Call(device, 1, 4, 2, Sq, 400, 64, dtype, INT8, 1)
+    power = 110 if dtype == F32 else 8
+    c.q = rounded(times_power(c.q, -power), dtype)
+    c.k_state[1][:, :, 3:350:7] = times_power(c.k_state[1][:, :, 3:350:7], power)
+    c.check(out_dtype=F32)
