@@ -384,15 +384,17 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
             const int at = c / p.G;
             const int64_t o = (int64_t)b * p.os[0] + (int64_t)(kvh * p.G + c - at * p.G) * p.os[1] + (int64_t)at * p.os[2];
             const int64_t share = ((int64_t)bg * p.nsplit + split) * NC + c;
-            const float inv = 1.0f / L;
+            // (of a share without a key that the column sees: zeros, which count for nothing)
+            const float inv = p.nsplit > 1 && L == 0.0f ? 0.0f : 1.0f / L;
             for (int d = 4 * sub; d < p.D; d += 64) {
                 float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int x = 0; x < 4; x++) v += *(const float4_t *)&lds_acc[x][col][d] * f[x];
+                v *= inv;
                 if (p.nsplit > 1) {
                     *(float4_t *)(p.partials + share * DV + d) = v;
                 } else {
-                    q8_store4_any(p, o + d * p.os[3], v * inv);
+                    q8_store4_any(p, o + d * p.os[3], v);
                 }
             }
             if (p.nsplit > 1 && sub == 0) {
@@ -403,9 +405,9 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     }
 }
 
-// Joins the shares of a (batch, kv head, column): groups of lanes, four dims a lane, add up every GROUPS-th share.  Bound by one memory latency after
-// another, so up to 64 shares are requested at once: a lane's sums of its shares, and by every wavefront the shares' maxima and sums, one a lane, whose
-// weights it keeps to itself.
+// Joins the shares of a (batch, kv head, column), which are means of their keys' values (sums of values near f32's end would pass it), by their parts of
+// the weights' sum: groups of lanes, four dims a lane, add up every GROUPS-th share.  Bound by one memory latency after another, so up to 64 shares are
+// requested at once: a lane's shares, and by every wavefront the shares' maxima and sums, one a lane, whose parts it keeps to itself.
 template <int DV, bool FEW>
 __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
     request_arguments<Q8AttnParams>();
@@ -420,16 +422,14 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
     const int group = tid / LPG, d = 4 * (tid % LPG);
     const float *const part = p.partials + first * DV + (d < p.D ? d : 0);
     float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-    float L;
     if constexpr (FEW) {
         const float2_at8_t own = *(const float2_at8_t *)(ml + 2 * (first + (int64_t)min(lane, p.nsplit - 1) * NC));
         float4_t x[MOST];
 #pragma unroll
         for (int i = 0; i < MOST; i++) x[i] = *(const float4_t *)(part + min(group + i * GROUPS, p.nsplit - 1) * step);
         const float M = wave_max(own[0]), ref = M == -INFINITY ? 0.0f : M;
-        const float f = lane < p.nsplit ? __builtin_amdgcn_exp2f(own[0] - ref) : 0.0f;
-        weight[64 * wave + lane] = f;
-        L = wave_sum(own[1] * f);
+        const float part_l = lane < p.nsplit ? own[1] * __builtin_amdgcn_exp2f(own[0] - ref) : 0.0f;
+        weight[64 * wave + lane] = part_l * (1.0f / wave_sum(part_l));
         wave_lds_sync();
 #pragma unroll
         for (int i = 0; i < MOST; i++)
@@ -448,19 +448,19 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
         __syncthreads();
         M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         const float ref = M == -INFINITY ? 0.0f : M;
-        L = 0.0f;
+        float L = 0.0f;
 #pragma unroll
         for (int i = 0; i < Q8_MAX_SHARES / 256; i++) {
-            const float f = __builtin_amdgcn_exp2f(m[i] - ref);
-            if (tid + 256 * i < p.nsplit) weight[tid + 256 * i] = f;
-            L += l[i] * f;
+            const float part_l = l[i] * __builtin_amdgcn_exp2f(m[i] - ref);
+            if (tid + 256 * i < p.nsplit) weight[tid + 256 * i] = part_l;
+            L += part_l;
         }
         L = wave_sum(L);
         if (lane == 0) red[4 + wave] = L;
         __syncthreads();
-        L = (red[4] + red[5]) + (red[6] + red[7]);
+        const float inv = 1.0f / ((red[4] + red[5]) + (red[6] + red[7]));
 #pragma unroll 4
-        for (int s = group; s < p.nsplit; s += GROUPS) v += *(const float4_t *)(part + s * step) * weight[s];
+        for (int s = group; s < p.nsplit; s += GROUPS) v += *(const float4_t *)(part + s * step) * (weight[s] * inv);
     }
     *(float4_t *)&sums[group][d] = v;
     __syncthreads();
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
 #pragma unroll
     for (int g = 1; g < GROUPS; g++) v += *(const float4_t *)&sums[g][d];
     const int b = (int)(bg / p.Hkv), row = c / p.G, head = (int)(bg - b * p.Hkv) * p.G + c - row * p.G;
-    q8_store4_any(p, (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)row * p.os[2] + d * p.os[3], v * (1.0f / L));
+    q8_store4_any(p, (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)row * p.os[2] + d * p.os[3], v);
 }
 
 static int q8_padded_dim(int D) { return (D + 63) / 64 * 64; }

@@ -389,8 +389,8 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
     const float up = __builtin_ldexpf(1.0f, max(E, -140) - 15 + SLACK);
     const int64_t o = (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)row * p.os[2];
     const int64_t part = ((int64_t)bg * p.nsplit + split) * NC + c;
-    // (sum / l) 2^(E - 15): the quotient first, which stays in range
-    const float inv = p.nsplit > 1 ? 1.0f : 1.0f / l;
+    // (sum / l) 2^(E - 15): the quotient first, which stays in range (of a share without a key that the column sees: zeros, which count for nothing)
+    const float inv = p.nsplit > 1 && l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -398,10 +398,10 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
             const int d = 32 * t + 2 * r + 4 * h;
             if (d >= p.D) continue;
             float4_t v = {acc[t][r], acc[t][r + 1], acc[t][r + 2], acc[t][r + 3]};
+            v = v * inv * up;
             if (p.nsplit > 1) {
-                *(float4_t *)(p.partials + part * DV + d) = v * up;
+                *(float4_t *)(p.partials + part * DV + d) = v;
             } else {
-                v = v * inv * up;
                 q8_store4_any(p, o + d * p.os[3], v);
             }
         }

@@ -86,7 +86,7 @@ struct Q8AttnParams {
     float scale;
     // keys in shares: `nsplit` per (batch, kv head, column block), each of at least `min_chunk` keys
     int32_t nsplit, min_chunk;
-    float *partials;   // [units][nsplit][16 * column blocks][padded D] sums, then as many (m, l)
+    float *partials;   // [B * Hkv][nsplit][G * Sq][padded D] means of the shares' values, then as many (m, l): largest score and sum of the weights
     int32_t cus;
 };
 struct Q8AttnPlan {

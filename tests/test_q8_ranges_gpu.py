@@ -74,3 +74,13 @@ def test_keys_of_every_size_at_once(device, dtype, Sq):
     c.q = rounded(times_power(c.q, -power), dtype)
     c.k_state[1][:, :, 3:350:7] = times_power(c.k_state[1][:, :, 3:350:7], power)
     c.check(out_dtype=F32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D, Sq, Skv", [(64, 1, 4000), (64, 40, 3000), (128, 33, 2500), (256, 2, 3000), (64, 40, 60)])
+def test_values_near_the_largest(device, dtype, D, Sq, Skv):
+    """Values whose sum over a share of the keys is beyond f32, and whose mean is not."""
+    c = Call(device, 1, 4, 2, Sq, Skv, D, dtype, INT8, 1)
+    c.v_state[0][:] = np.abs(c.v_state[0].view(np.int8)).view(np.uint8)  # (sums do not cancel)
+    c.v_state[1][:] = times_power(c.v_state[1], 121)
+    c.check(out_dtype=F32)
