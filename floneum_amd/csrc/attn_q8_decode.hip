@@ -13,10 +13,11 @@
 //
 // Codes are whole f16 numbers, so the products are exact up to the f32 accumulation.  A column's q is scaled by a power of two
 // to f16's upper range: f16 and bf16 queries fit one term exactly (to 2^-29 of the row's largest element), f32 ones take two (22 bits).
-// The value scale vs_j, in [2^(e_j - 1), 2^e_j), goes with the probability: with the running maximum M of s_j + e_j,
-//   p_j = 2^(s_j + e_j - M + 15) 2^-e_j,  w_j = p_j vs_j <= 2^15,  out = sum w_j c_j / sum p_j
-// which holds whatever the scales' range (a first token with values of almost nothing).  w is rounded to 11 bits (relative 2^-12, to 2^-29 of the
-// largest) for 16-bit tensors and taken as two terms for f32.
+// The value scale vs_j, in [2^(e_j - 1), 2^e_j), goes with the probability, which the sum of the weights takes without it: with the running maxima
+// M of s_j and X of s_j - M + e_j,
+//   p_j = 2^(s_j - M),  w_j = p_j vs_j 2^(15 - X) <= 2^15,  out = 2^(X - 15) sum w_j c_j / sum p_j
+// which holds whatever the scales' range (a first token with values of almost nothing, rows of zeros beside large ones: X >= -99, the exponent of the
+// least scale).  w is rounded to 11 bits (relative 2^-12, to 2^-29 of the largest) for 16-bit tensors and taken as two terms for f32.
 //
 // Bound by the bytes of codes and scales where there are many: 157 us for 16 ragged sequences of up to 16384 keys, 32 heads of 96 (e4m3, 5.2 TB/s),
 // 33 us with the joining for 16 of 4096, 8 KV heads of 128 (134 MB).  One sequence is bound by a chain of latencies: 10 us for 4096 keys, 8 of the
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     using Dims = Q8Dims<DV>;
     constexpr int VW = Dims::VW, KS = Dims::KS, TILES = Dims::TILES, COLS = 16, NBUF = DV <= 128 ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float lds_acc[4][16][DV + 4];
-    __shared__ float lds_m[4][COLS], lds_l[4][COLS];
+    __shared__ float lds_m[4][COLS], lds_fit[4][COLS], lds_l[4][COLS];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int NC = p.G * p.Sq, blocks = (NC + COLS - 1) / COLS;
@@ -79,7 +80,8 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     const int lo = (int)min(lo64, (int64_t)vis.hi), hi = (int)min((int64_t)vis.hi, lo64 + chunk);
 
     float4_t acc[TILES];
-    float m = -INFINITY, l = 0.0f;
+    // the largest score so far (never -infinity), the largest of scores less that plus the exponents of the values' scales, 2^(15 - fit), the weights' sum
+    float m = -3.402823466e38f, fit = -100.0f, lift = 0x1p115f, l = 0.0f;
 #pragma unroll
     for (int t = 0; t < TILES; t++) acc[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         const int at = first_key(k0), next = k0 + NBUF * 128;
         spread_scale8(x.ks, p.k, k0);
         spread_scale8(x.vs, p.v, k0);
-        float exf[8], back[8], vs[8], ks[8];  // e_j, 2^-e_j
+        float exf[8], vs[8], ks[8];  // (exf: e_j)
         bool lost = tiny;
 #pragma unroll
         for (int i = 0; i < 8; i++) ks[i] = x.ks[i], vs[i] = x.vs[i];
@@ -204,17 +206,13 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         }
         load_k(x, next);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int e = __builtin_amdgcn_frexp_expf(fmaxf(vs[i], Q8_LEAST_SCALE));
-            exf[i] = (float)e;
-            back[i] = __builtin_ldexpf(1.0f, -e);
-        }
+        for (int i = 0; i < 8; i++) exf[i] = (float)__builtin_amdgcn_frexp_expf(fmaxf(vs[i], Q8_LEAST_SCALE));
         half8_t pw[TERMS];
         {
             float top = -INFINITY;
             if constexpr (!MASK) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) sc[i] = __builtin_fmaf(sc[i], ks[i] * colscale, exf[i]);
+                for (int i = 0; i < 8; i++) sc[i] *= ks[i] * colscale;
                 // the step reaches beyond what some column sees
                 if (__builtin_amdgcn_ballot_w64(at + 32 > limit || at < start || at < k0) != 0) {
 #pragma unroll
@@ -231,25 +229,32 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                     if (key < limit && key >= k0)
                         add = q8_load_any(p.mask, (p.mask_kind == FHIP_MASK_QK ? row : b) * p.ms0 + key * p.ms1, p.q_dtype);
                     const float s = q8_with_mask(sc[i] * (ks[i] * colscale), add * Q8_LOG2E);
-                    sc[i] = add == -INFINITY ? -INFINITY : s + exf[i];
+                    sc[i] = add == -INFINITY ? -INFINITY : s;
                 }
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) top = fmaxf(top, sc[i]);
             top = fmaxf(m, quads_max(top));
-            const float ref = top == -INFINITY ? 0.0f : top - 15.0f;
-            if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
-                const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
-                m = top;
-                l *= f;
+            float most = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                sc[i] -= top;
+                most = fmaxf(most, sc[i] + exf[i]);
+            }
+            most = fmaxf(fmaxf(fit + (m - top), -100.0f), quads_max(most));
+            if (__builtin_amdgcn_ballot_w64(top > m || most > fit) != 0) {
+                const float f = __builtin_amdgcn_exp2f((m - top) + (fit - most));
+                l *= __builtin_amdgcn_exp2f(m - top);
+                m = top, fit = most;
+                lift = __builtin_amdgcn_exp2f(15.0f - fit);
 #pragma unroll
                 for (int t = 0; t < TILES; t++) acc[t] *= f;
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float e = __builtin_amdgcn_exp2f(sc[i] - ref) * back[i];
+                const float e = __builtin_amdgcn_exp2f(sc[i]);
                 l += e;
-                float w = e * vs[i];
+                float w = e * vs[i] * lift;
                 if constexpr (TERMS == 2) asm("" : "+v"(w));  // (both terms from the same rounded w: the product is not contracted into them)
                 const half_t hi16 = (half_t)w;
                 pw[0][i] = hi16;
@@ -359,7 +364,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
 
     // the four wavefronts' states
     l = quads_sum(l);
-    if (g == 0) lds_m[wave][n] = m, lds_l[wave][n] = l;
+    if (g == 0) lds_m[wave][n] = m, lds_fit[wave][n] = fit, lds_l[wave][n] = l;
     {
         lds_barrier();  // (the loads of steps beyond the last one may still be on their way)
 #pragma unroll
@@ -372,25 +377,28 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         lds_barrier();
         const int col = threadIdx.x >> 4, sub = threadIdx.x & 15, c = c0 + col;
         if (c < NC) {
-            float M = -INFINITY, L = 0.0f, f[4];
+            float M = -INFINITY, most = -INFINITY, L = 0.0f, f[4];
 #pragma unroll
             for (int x = 0; x < 4; x++) M = fmaxf(M, lds_m[x][col]);
-            const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                f[x] = __builtin_amdgcn_exp2f(lds_m[x][col] - ref);
-                L += lds_l[x][col] * f[x];
+                f[x] = lds_m[x][col] - M;
+                L += lds_l[x][col] * __builtin_amdgcn_exp2f(f[x]);
+                f[x] += lds_fit[x][col];
+                most = fmaxf(most, f[x]);
             }
+#pragma unroll
+            for (int x = 0; x < 4; x++) f[x] = __builtin_amdgcn_exp2f(f[x] - most);
             const int at = c / p.G;
             const int64_t o = (int64_t)b * p.os[0] + (int64_t)(kvh * p.G + c - at * p.G) * p.os[1] + (int64_t)at * p.os[2];
             const int64_t share = ((int64_t)bg * p.nsplit + split) * NC + c;
             // (of a share without a key that the column sees: zeros, which count for nothing)
-            const float inv = p.nsplit > 1 && L == 0.0f ? 0.0f : 1.0f / L;
+            const float inv = p.nsplit > 1 && L == 0.0f ? 0.0f : 1.0f / L, up = __builtin_amdgcn_exp2f(most - 15.0f);
             for (int d = 4 * sub; d < p.D; d += 64) {
                 float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int x = 0; x < 4; x++) v += *(const float4_t *)&lds_acc[x][col][d] * f[x];
-                v *= inv;
+                v = v * inv * up;
                 if (p.nsplit > 1) {
                     *(float4_t *)(p.partials + share * DV + d) = v;
                 } else {

@@ -76,6 +76,42 @@ def test_keys_of_every_size_at_once(device, dtype, Sq):
     c.check(out_dtype=F32)
 
 
+# ---- weights ------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D, Sq, Skv", [(64, 1, 40), (128, 2, 300), (256, 1, 2000), (64, 40, 65), (128, 130, 300), (256, 40, 200)])
+@pytest.mark.parametrize("power", [40, 50, 90, 115])
+def test_zero_values_beside_large_ones(device, dtype, D, Sq, Skv, power):
+    """Keys whose values are all zero, as a row of zeros is coded, count in the sum of the weights."""
+    c = Call(device, 1, 4, 2, Sq, Skv, D, dtype, INT8, 1)
+    codes, scales = c.v_state
+    codes[:, :, ::2], scales[:, :, ::2] = 0, q8.LEAST_SCALE
+    scales[:, :, 1::2] = times_power(scales[:, :, 1::2], power)
+    c.check(out_dtype=F32)
+    at = Skv - Sq
+    c.check(positions_mask(Sq, Skv, [at]), analytic=(True, at, 0), out_dtype=F32)
+    codes[:, :, :Skv - 3], scales[:, :, :Skv - 3] = 0, q8.LEAST_SCALE  # all but the last
+    c.check(out_dtype=F32)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_many_zero_values(device, dtype):
+    """More keys with values of nothing than the largest weight of one fits into f32, in one share, in front of ordinary ones."""
+    keys, zeros, D = 300_000, 290_000, 8
+    rng = np.random.default_rng(5)
+    codes = [rng.integers(-127, 128, (1, 1, keys, D)).astype(np.int8).view(np.uint8) for _ in range(2)]
+    scales = [np.full((1, 1, keys), 1 / 127, np.float32) for _ in range(2)]
+    codes[1][:, :, :zeros], scales[1][:, :, :zeros] = 0, q8.LEAST_SCALE
+    B, Hkv = 16, 32  # units enough that the keys are not shared out
+    one = [upload_q8(device, *s, fa.Q8Format.INT8, 1) for s in zip(codes, scales)]
+    k, v = (fa.Q8Tensor(t.codes, t.scales, (B, Hkv, keys, D), t.format, 1, (0, 0, t.strides[2]), 0, (0, 0)) for t in one)
+    got = upload(device, np.zeros((B, Hkv, 1, D)), dtype).flash_attention(k, v, 1.0, out_dtype=F32).to_numpy().astype(np.float64)
+    value = codes[1].view(np.int8).astype(np.float64)[0, 0] * scales[1].astype(np.float64)[0, 0][:, None]
+    want, mass = value.sum(0) / keys, np.abs(value).sum(0) / keys
+    # weights that are all alike, rounded once (2^-11 at most) times the scale, and sums of so many in f32, a lane's 1 / 16th of them
+    assert (np.abs(got - want) <= (2.0 ** -11 + 2.0 ** -24 * keys / 16) * mass).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("D, Sq, Skv", [(64, 1, 4000), (64, 40, 3000), (128, 33, 2500), (256, 2, 3000), (64, 40, 60)])
 def test_values_near_the_largest(device, dtype, D, Sq, Skv):
