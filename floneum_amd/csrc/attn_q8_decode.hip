@@ -168,17 +168,15 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         spread_scale8(x.ks, p.k, k0);
         spread_scale8(x.vs, p.v, k0);
         float exf[8], vs[8], ks[8];  // (exf: e_j)
-        bool lost = tiny;
+        uint32_t top_scale = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) ks[i] = x.ks[i], vs[i] = x.vs[i];
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) lost = lost || __builtin_isunordered(vs[i], vs[i + 1]);
-        // NaN among the values' scales goes by way of the scores, where rows that a mask hides are taken out
-        if (__builtin_amdgcn_ballot_w64(lost) != 0) {
+        for (int i = 0; i < 8; i++) ks[i] = x.ks[i], vs[i] = x.vs[i], top_scale = max(top_scale, __float_as_uint(vs[i]));
+        // What is no number among the values' scales (infinity and, as bits, all beyond it) goes by way of the scores, where rows that a mask hides are taken out
+        if (__builtin_amdgcn_ballot_w64(tiny || top_scale >= 0x7f800000u) != 0) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 if (tiny) ks[i] *= 0x1p-64f;
-                if (vs[i] != vs[i]) ks[i] = vs[i], vs[i] = 1.0f;
+                if (__float_as_uint(vs[i]) >= 0x7f800000u) ks[i] = __uint_as_float(0x7fc00000u), vs[i] = 0.0f;
             }
         }
         // scores

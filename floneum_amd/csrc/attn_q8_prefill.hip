@@ -245,9 +245,8 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
     auto take_scales = [&]() {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            // NaN among the values' scales goes by way of the scores, where rows that a mask hides are taken out
-            const bool lost = vs[u] != vs[u];
-            kf[u] = (lost ? vs[u] : ks[u]) * down, nf[u] = lost ? 0.0f : vs[u];
+            // what is no number among the values' scales goes by way of the scores, where rows that a mask hides are taken out
+            kf[u] = __builtin_fmaf(vs[u], 0.0f, ks[u] * down), nf[u] = vs[u] < INFINITY ? vs[u] : 0.0f;
             e = max(e, nf[u] > 0.0f ? __builtin_amdgcn_frexp_expf(nf[u]) : -200);
         }
     };

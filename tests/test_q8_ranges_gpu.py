@@ -120,3 +120,41 @@ def test_values_near_the_largest(device, dtype, D, Sq, Skv):
     c.v_state[0][:] = np.abs(c.v_state[0].view(np.int8)).view(np.uint8)  # (sums do not cancel)
     c.v_state[1][:] = times_power(c.v_state[1], 121)
     c.check(out_dtype=F32)
+
+
+# ---- rows that may hold anything ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("anything", [np.inf, -np.inf, np.nan, 3.4e38])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("block", [1, 16])
+@pytest.mark.parametrize("Sq", [1, 4, 70])
+def test_scales_of_anything_behind_the_last_row(device, anything, dtype, block, Sq):
+    lens = [160, 16, 32, 96]
+    c = Call(device, len(lens), 4, 2, Sq, 200, 64, dtype, E4M3, block)
+    for b, n in enumerate(lens):
+        for codes, scales in (c.k_state, c.v_state):
+            codes[b, :, n:], scales[b, :, n // block:] = 0x7F, anything
+    hidden = np.broadcast_to(np.arange(200) >= np.asarray(lens)[:, None, None, None], (len(lens), 1, Sq, 200))
+    got = upload(device, c.q, dtype).flash_attention(*c.tensors(), c.scale, kv_lens=fa.IntTensor(device, lens)).to_numpy()
+    for b, n in enumerate(lens):
+        for codes, scales in (c.k_state, c.v_state):
+            codes[b, :, n:], scales[b, :, n // block:] = 0, 1.0
+    c.check(hidden, got=got)
+
+
+@pytest.mark.parametrize("anything", [np.inf, np.nan])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("Sq, Skv", [(4, 100), (40, 130)])
+def test_scales_of_anything_on_rows_to_come(device, anything, dtype, Sq, Skv):
+    """The last key, which only the last query row sees, is nothing to the others."""
+    c = Call(device, 1, 4, 2, Sq, Skv, 64, dtype, INT8, 1)
+    for state in (c.k_state, c.v_state):
+        state[1][:, :, Skv - 1] = anything
+    got = upload(device, c.q, dtype).flash_attention(*c.tensors(), c.scale, analytic=(True, Skv - Sq, 0)).to_numpy().astype(np.float64)
+    assert not np.isfinite(got[:, :, Sq - 1]).any()
+    got[:, :, Sq - 1] = np.nan
+    for state in (c.k_state, c.v_state):
+        state[1][:, :, Skv - 1] = 1.0
+    hidden = positions_mask(Sq, Skv, [Skv - Sq])
+    hidden[:, :, Sq - 1] = True
+    c.check(hidden, got=got)
