@@ -40,12 +40,11 @@ __device__ __forceinline__ void q8_store4_any(const Q8AttnParams &p, int64_t idx
     }
 }
 
-// Score and additive mask (both times log2 e).  What a finite mask value puts below -2^22 (the type's lowest value, which overflows in the
-// log2 domain) counts as that: the exponent of the value's scale, which the kernel for few rows adds next, has to keep its weight beside it, and
-// a row whose keys are all that far down weighs them alike, as f32 scores that vanish beside the mask do.
+// Score and additive mask (both times log2 e).  A finite mask value hides nothing: what overflows in the log2 domain (the type's lowest value) counts as
+// the least f32, and a row whose keys are all that far down weighs them alike, as f32 scores that vanish beside the mask do.
 __device__ __forceinline__ float q8_with_mask(float s, float add) {
     const float t = s + add;
-    return t < -0x1p22f ? -0x1p22f : t;
+    return t < -3.402823466e38f ? -3.402823466e38f : t;
 }
 
 // The keys [lo, hi) that some row of row0 .. row1 sees, from the analytic mask and the lengths.

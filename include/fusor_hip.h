@@ -549,7 +549,8 @@ int fhip_q8_attention_workspace_bytes(const fhip_q8_attn_args *args, int32_t com
  * statistics and sums are f32; codes enter the matrix products exactly, f32 queries and probabilities as two 16-bit terms
  * each (f32 precision), 16-bit queries exactly and their probabilities rounded to 11 bits.  Products of probability and value
  * scale below 2^-40 (16-bit queries: 2^-35) of the largest scale among the keys that the call's rows see are lost; finite mask
- * values below -2^22 / log2(e) count as that.  Rows of the cache that a mask hides by position or length may hold anything.
+ * values below -2^128 / log2(e) (-2.36e38) count as the type's lowest.  Rows of the cache that a mask hides by position or length may
+ * hold anything, but for 8-bit NaN codes among the rows that some query row of the call sees.
  * Asynchronous on `s`; may be captured. */
 int fhip_q8_attention(fhip_stream *s, const fhip_q8_attn_args *args);
 

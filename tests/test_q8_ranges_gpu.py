@@ -122,6 +122,23 @@ def test_values_near_the_largest(device, dtype, D, Sq, Skv):
     c.check(out_dtype=F32)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D, Sq", [(64, 1), (64, 5), (128, 40), (256, 33)])
+@pytest.mark.parametrize("base, step", [(-2.0 ** 24, 2.0 ** 20), (-2.0 ** 30, 2.0 ** 27), (-2.0 ** 100, 2.0 ** 97), (-2.0 ** 127, 2.0 ** 125)])
+def test_low_masks_in_their_order(device, dtype, D, Sq, base, step):
+    """Rows whose keys a finite mask puts far down weigh those that it puts down the least."""
+    Skv = 200
+    c = Call(device, 2, 4, 2, Sq, Skv, D, dtype, INT8, 1)
+    c.q[:] = 0.0
+    m = np.full((Sq, Skv), base, np.float32)
+    m[:, 100:] += np.float32(step)
+    m[:, 7] = np.finfo(np.float32).min if dtype == F32 else -3.3895314e38
+    m[:, 9] = -np.inf
+    hidden = np.zeros((1, 1, Sq, Skv), bool)
+    hidden[..., :100] = True
+    c.check(hidden, mask=(upload(device, m, dtype), fa.MaskKind.QKMask))
+
+
 # ---- rows that may hold anything ------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("anything", [np.inf, -np.inf, np.nan, 3.4e38])
