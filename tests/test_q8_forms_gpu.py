@@ -1,0 +1,100 @@
+"""Forms of the 8-bit attention kernels that only some calls reach: workgroups of eight wavefronts, and mask tensors at every padded head
+size, format and block."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import floneum_amd as fa
+from oracle import q8
+from q8_helpers import rounded, upload
+from test_q8 import attn
+from test_q8_attention_gpu import Call, positions_mask
+
+F32, F16, BF16 = fa.F32, fa.F16, fa.BF16
+INT8, E4M3 = q8.INT8, q8.E4M3
+
+
+def workspace(B, Hkv, D, dtype):
+    need = ctypes.c_size_t()
+    a = attn(B=B, H=Hkv, Hkv=Hkv, Sq=65, Skv=300, D=D, dtype=dtype)
+    assert fa.lib().fhip_q8_attention_workspace_bytes(ctypes.byref(a), 256, ctypes.byref(need)) == fa.OK
+    return need.value
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [64, 72, 128])
+def test_where_eight_wavefronts_begin(D, dtype):
+    """Workgroups of 256 columns that fill the chip, one on each of its 256 CUs, have eight wavefronts and leave the keys whole; one KV head less, and
+    those of 128 columns have room for two shares of the keys."""
+    assert workspace(8, 32, D, dtype) == 0 and workspace(16, 16, D, dtype) == 0
+    assert workspace(1, 255, D, dtype) > 0 and workspace(8, 31, D, dtype) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("fmt", [INT8, E4M3])
+@pytest.mark.parametrize("D", [40, 64, 72, 128])
+@pytest.mark.parametrize("H, Sq, Skv", [(32, 65, 65), (64, 40, 130), (32, 33, 64)])
+def test_eight_wavefronts(device, H, Sq, Skv, D, fmt, dtype):
+    B, Hkv = 8, 32
+    assert B * Hkv >= device.compute_units
+    c = Call(device, B, H, Hkv, Sq, Skv, D, dtype, fmt, 1)
+    at = Skv - Sq
+    c.check(positions_mask(Sq, Skv, [at]), analytic=(True, at, 0))
+    c.check(positions_mask(Sq, Skv, [at], 17), analytic=(True, at, 17))
+    lens = [Skv, 0, 1, 31, 33, 64, 65, Skv - 1]
+    hidden = np.broadcast_to(np.arange(Skv) >= np.asarray(lens)[:, None, None, None], (B, 1, Sq, Skv))
+    c.check(hidden, kv_lens=fa.IntTensor(device, lens))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, fmt, D", [(F16, INT8, 128), (BF16, E4M3, 128), (F32, INT8, 128), (F16, E4M3, 64), (F32, E4M3, 64), (BF16, INT8, 72)])
+def test_eight_wavefronts_over_several_tiles(device, dtype, fmt, D):
+    """Tiles that are staged while others are multiplied, blocks of columns that end inside a wavefront, sequences at positions of their own."""
+    B, Hkv, Sq, Skv = 8, 32, 300, 337
+    c = Call(device, B, Hkv, Hkv, Sq, Skv, D, dtype, fmt, 1, first=0)
+    starts = [37, 0, 5, 36, 20, 1, 30, 12]
+    c.check(positions_mask(Sq, Skv, starts), analytic=(True, 0, 0), q_positions=fa.IntTensor(device, starts))
+    lens = [s + Sq for s in starts]
+    c.check(positions_mask(Sq, Skv, starts, 100, lens), analytic=(True, 0, 100), q_positions=fa.IntTensor(device, starts),
+            kv_lens=fa.IntTensor(device, lens))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_eight_wavefronts_in_blocks(device, dtype):
+    """Scales of blocks of 16 rows that begin inside one, grouped heads, one sequence of several blocks of columns."""
+    Hkv, Sq, Skv = 32, 1100, 90
+    c = Call(device, 1, 2 * Hkv, Hkv, Sq, Skv, 64, dtype, INT8, 16, first=5)
+    assert Hkv * -(-2 * Sq // 256) >= device.compute_units
+    c.check()
+    c.check(positions_mask(Sq, Skv, [0]), analytic=(True, 0, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("fmt", [INT8, E4M3])
+@pytest.mark.parametrize("block, first", [(1, 0), (16, 5)])
+@pytest.mark.parametrize("D", [64, 80, 128, 192, 256])
+@pytest.mark.parametrize("Sq, Skv", [(2, 100), (40, 100), (33, 65), (70, 300)])
+def test_mask_tensors(device, Sq, Skv, D, block, first, fmt, dtype):
+    B = 2
+    c = Call(device, B, 4, 2, Sq, Skv, D, dtype, fmt, block, first=first)
+    low = {F32: -3.4028235e38, F16: -65504.0, BF16: -3.3895314e38}[dtype]
+    m = rounded(c.rng.standard_normal((Sq, Skv)).astype(np.float32), dtype)
+    m[:, 7], m[-1, 20:] = -np.inf, -np.inf
+    m[0, 40:60] = low
+    m[1] = -np.inf                              # a row without a key
+    hidden = np.broadcast_to(np.isinf(m), (B, 1, Sq, Skv))
+    add = np.where(np.isinf(m), 0.0, np.maximum(m.astype(np.float64), -1e4))
+    c.check(hidden, add, mask=(upload(device, m, dtype), fa.MaskKind.QKMask))
+    c.check(hidden, add, mask=(upload(device, m, dtype, (1, 0)), fa.MaskKind.QKMask))
+    pad = np.zeros((B, Skv), np.float32)
+    pad[0, :9], pad[1, 50:] = -np.inf, -np.inf  # padded on the left and on the right
+    pad[0, 30] = -0.5
+    c.check(np.isinf(pad)[:, None, None], np.where(np.isinf(pad), 0.0, pad)[:, None, None], mask=(upload(device, pad, dtype), fa.MaskKind.BatchKeyMask))
+    lens = [0, 64]
+    hidden = np.isinf(pad)[:, None, None] | (np.arange(Skv) >= np.asarray(lens)[:, None, None, None])
+    c.check(hidden, np.where(np.isinf(pad), 0.0, pad)[:, None, None], mask=(upload(device, pad, dtype), fa.MaskKind.BatchKeyMask),
+            kv_lens=fa.IntTensor(device, lens))
