@@ -393,12 +393,15 @@ bool describe_q8(PyObject *t, fhip_q8_tensor *c, PyObject *device) {
 
 // q8_narrow(tensor, dim, start, length): a Q8Tensor, or None
 PyObject *q8_narrow(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 4 || Py_TYPE(a[0]) != q8.type) Py_RETURN_NONE;
+    const Ref codes(Py_XNewRef(slot(q8, a[0], 0))), scales(Py_XNewRef(slot(q8, a[0], 1))), format(Py_XNewRef(slot(q8, a[0], 3))),
+        block_tokens(Py_XNewRef(slot(q8, a[0], 4))), row_steps(Py_XNewRef(slot(q8, a[0], 5))), block_steps(Py_XNewRef(slot(q8, a[0], 7)));
     uint32_t dim, start, length, shape[4], block, first;
     int64_t strides[3], steps[2];
     uint64_t offset, scale_offset;
-    if (n != 4 || Py_TYPE(a[0]) != q8.type || !as_narrow(a[1], &dim) || dim > 2 || !as_narrow(a[2], &start) || !as_narrow(a[3], &length) ||
-        !numbers<4>(slot(q8, a[0], 2), shape) || (uint64_t)start + length > shape[dim] || !numbers<3>(slot(q8, a[0], 5), strides) ||
-        !numbers<2>(slot(q8, a[0], 7), steps) || !as_narrow(slot(q8, a[0], 4), &block) || block == 0 || !as_u64(slot(q8, a[0], 6), &offset) ||
+    if (!codes.o || !scales.o || !format.o || !as_narrow(a[1], &dim) || dim > 2 || !as_narrow(a[2], &start) || !as_narrow(a[3], &length) ||
+        !numbers<4>(slot(q8, a[0], 2), shape) || (uint64_t)start + length > shape[dim] || !numbers<3>(row_steps.o, strides) ||
+        !numbers<2>(block_steps.o, steps) || !as_narrow(block_tokens.o, &block) || block == 0 || !as_u64(slot(q8, a[0], 6), &offset) ||
         !as_u64(slot(q8, a[0], 8), &scale_offset) || !as_narrow(slot(q8, a[0], 9), &first))
         Py_RETURN_NONE;
     shape[dim] = length;
@@ -412,8 +415,7 @@ PyObject *q8_narrow(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Ref extents(tuple4(shape, nullptr)), at(PyLong_FromUnsignedLongLong(offset)), scale_at(PyLong_FromUnsignedLongLong(scale_offset)),
         place(PyLong_FromUnsignedLong(first));
     if (!extents.o || !at.o || !scale_at.o || !place.o) return nullptr;
-    PyObject *const values[10] = {slot(q8, a[0], 0), slot(q8, a[0], 1), extents.o, slot(q8, a[0], 3), slot(q8, a[0], 4),
-                                  slot(q8, a[0], 5), at.o, slot(q8, a[0], 7), scale_at.o, place.o};
+    PyObject *const values[10] = {codes.o, scales.o, extents.o, format.o, block_tokens.o, row_steps.o, at.o, block_steps.o, scale_at.o, place.o};
     return instance(q8, 10, values);
 }
 

@@ -39,3 +39,14 @@ def test_reading_back_rows_of_too_many_heads(heads, D):
     x, out = t8([1, heads, 1, D], stride=(0, 0, 256), scale_stride=(0, 0)), t4([1, heads, 1, D])
     rc, message = call("fhip_q8_dequantize", ctypes.byref(x), 0, None, ctypes.byref(out), 0)
     assert rc == fa.ERR_UNSUPPORTED and "2^34" in message
+
+
+@pytest.mark.parametrize("missing", ["codes", "scales", "shape", "format", "block_tokens", "strides", "offset", "scale_strides", "scale_offset", "first"])
+def test_parts_of_a_tensor_that_lacks_something(missing):
+    class Memory:
+        device, ptr = None, FAKE
+    fa.lib()
+    x = fa.Q8Tensor(Memory(), Memory(), (2, 3, 100, 72), fa.Q8Format.INT8, 16)
+    delattr(x, missing)
+    with pytest.raises(AttributeError, match=missing):
+        x.narrow(2, 1, 2)
