@@ -1017,6 +1017,8 @@ class Q8Tensor:
                 if done != OK:
                     check(done)
                 return q_out
+        if v_cache.device is not self.device:
+            raise AssertionError("Cannot mix tensors of different devices")
         a, q_out, keep = _q8_append_args(self.device, k, v, lens, counts, rope, start_pos, interleaved, k_norm, q, q_norm, q_out)
         a.k, a.v, a.row = self._c(), v_cache._c(), int(row)
         check(lib().fhip_q8_append(self.device.stream, ctypes.byref(a)))

@@ -50,3 +50,19 @@ def test_parts_of_a_tensor_that_lacks_something(missing):
     delattr(x, missing)
     with pytest.raises(AttributeError, match=missing):
         x.narrow(2, 1, 2)
+
+
+@pytest.mark.parametrize("with_native", [True, False])
+def test_caches_of_two_devices(monkeypatch, with_native):
+    """Keys and values of an append lie on one device, as everything else of a call."""
+    class Memory:
+        def __init__(self, device):
+            self.device, self.ptr = device, FAKE
+    fa.lib()
+    if not with_native:
+        monkeypatch.setattr(fa, "_native", None)
+    here, there = object(), object()
+    keys, values = (fa.Q8Tensor(Memory(d), Memory(d), (1, 2, 10, 64), fa.Q8Format.INT8, 1) for d in (here, there))
+    rows = fa.Tensor(Memory(here), fa.F16, (1, 2, 3, 64))
+    with pytest.raises(AssertionError, match="different devices"):
+        keys.append(values, rows, rows)
