@@ -7,7 +7,7 @@ import pytest
 
 import floneum_amd as fa
 from oracle import q8
-from q8_helpers import rounded, upload
+from q8_helpers import download_q8, random_cache, rounded, upload, upload_q8
 from test_q8 import attn
 from test_q8_attention_gpu import Call, positions_mask
 
@@ -98,3 +98,29 @@ def test_mask_tensors(device, Sq, Skv, D, block, first, fmt, dtype):
     hidden = np.isinf(pad)[:, None, None] | (np.arange(Skv) >= np.asarray(lens)[:, None, None, None])
     c.check(hidden, np.where(np.isinf(pad), 0.0, pad)[:, None, None], mask=(upload(device, pad, dtype), fa.MaskKind.BatchKeyMask),
             kv_lens=fa.IntTensor(device, lens))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [INT8, E4M3])
+@pytest.mark.parametrize("block, n", [(1, 1), (1, 3), (8, 1), (8, 3), (64, 5)])
+def test_rows_written_over(device, fmt, block, n):
+    """New rows in front of others: those of the same block are lost with its scale, those of later blocks (with blocks of one token, all) stay as they
+    were, bit for bit, and so do the blocks in front."""
+    rng = np.random.default_rng(block + n)
+    B, H, rows, D, at = 2, 2, 200, 64, 66
+    state = [random_cache(rng, B, H, rows, D, fmt, block) for _ in range(2)]
+    k8, v8 = (upload_q8(device, *s, fa.Q8Format(fmt), block) for s in state)
+    new = [rng.standard_normal((B, H, n, D)).astype(np.float32) * np.float32(4) for _ in range(2)]
+    k8.append(v8, upload(device, new[0], F32), upload(device, new[1], F32), at)
+    end = -(-(at + n) // block)  # the first block behind the new rows
+    for t, (codes, scales), x in zip((k8, v8), state, new):
+        got, got_scales = download_q8(t)
+        want, want_scales = codes.copy(), scales.copy()
+        for b in range(B):
+            for h in range(H):
+                q8.append_rows(want[b, h], want_scales[b, h], x[b, h], at, fmt, block)
+        assert np.array_equal(got_scales, want_scales)
+        assert np.array_equal(got[:, :, end * block:], codes[:, :, end * block:]) and np.array_equal(got_scales[:, :, end:], scales[:, :, end:])
+        assert np.array_equal(got[:, :, :at // block * block], codes[:, :, :at // block * block])
+        written = q8.code_values(got[:, :, at:at + n], fmt), q8.code_values(want[:, :, at:at + n], fmt)
+        assert np.array_equal(*written)

@@ -66,3 +66,11 @@ def test_caches_of_two_devices(monkeypatch, with_native):
     rows = fa.Tensor(Memory(here), fa.F16, (1, 2, 3, 64))
     with pytest.raises(AssertionError, match="different devices"):
         keys.append(values, rows, rows)
+
+
+def test_both_caches_are_called_alike():
+    """A program changes to the 8-bit cache by the class it creates: the steps of both take the same arguments."""
+    import inspect
+    for name in ("append", "append_rope", "qkv_rope_append"):
+        wide, narrow = (list(inspect.signature(getattr(c, name)).parameters) for c in (fa.KvCache, fa.Q8KvCache))
+        assert wide == narrow, name
