@@ -329,7 +329,10 @@ static void fill_attention(const fhip_q8_attn_args *a, int cus, Q8AttnParams *p)
     p->cus = cus > 0 ? cus : 256;
 }
 
-// Few columns ((query row, head of the group) pairs) per KV head: the kernel that streams the codes into registers (32 rows at a time).
+// Few columns ((query row, head of the group) pairs) per KV head: the kernel that streams the codes into registers (32 rows at a time).  It takes 16 columns
+// per workgroup and the codes once for each of them (us, few and many, recorded calls: 8 sequences of 4096 keys, 32/8 heads at 128, f16, 16 columns 22 and
+// 32, 32 columns 31 and 33, 48 columns 49 and 35; 8 of 4001, 16/4 at 256, bf16, 32 columns 28 and 47, 48 columns 51 and 49; 16 of 2000, 32/32 at 64, 48
+// columns 66 and 121).
 static Q8AttnPlan attention_plan(const Q8AttnParams &p) {
     return (int64_t)p.G * p.Sq <= 32 && p.Skv >= 32 ? q8_decode_plan(p) : q8_prefill_plan(p);
 }

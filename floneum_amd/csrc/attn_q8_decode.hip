@@ -17,10 +17,11 @@
 // M of s_j and X of s_j - M + e_j,
 //   p_j = 2^(s_j - M),  w_j = p_j vs_j 2^(15 - X) <= 2^15,  out = 2^(X - 15) sum w_j c_j / sum p_j
 // which holds whatever the scales' range (a first token with values of almost nothing, rows of zeros beside large ones: X >= -99, the exponent of the
-// least scale).  w is rounded to 11 bits (relative 2^-12, to 2^-29 of the largest) for 16-bit tensors and taken as two terms for f32.
+// least scale).  w is rounded to 11 bits (relative 2^-12, to 2^-29 of the largest) for 16-bit tensors, whose output is rounded as much once more (error
+// against 64 bits 2.9e-4 in f16 where f32 weights leave 2.1e-4, 1.7e-3 either way in bf16), and taken as two terms for f32 (2.9e-7).
 //
-// Bound by the bytes of codes and scales where there are many: 157 us for 16 ragged sequences of up to 16384 keys, 32 heads of 96 (e4m3, 5.2 TB/s),
-// 33 us with the joining for 16 of 4096, 8 KV heads of 128 (134 MB).  One sequence is bound by a chain of latencies: 10 us for 4096 keys, 8 of the
+// Bound by the bytes of codes and scales where there are many: 156 us for 16 ragged sequences of up to 16384 keys, 32 heads of 96 (e4m3, 5.2 TB/s),
+// 33.6 us with the joining for 16 of 4096, 8 KV heads of 128 (134 MB).  One sequence is bound by a chain of latencies: 10 us for 4096 keys, 8 of the
 // main kernel and 3 of the joining where each stands alone (one kernel whose last workgroup joins the shares took 97 us: the order it needs
 // between XCDs writes back and drops their L2).  Two steps of keys in flight without a branch, against one behind one: 58 -> 35 us for the 16
 // sequences, with the joining by lanes side by side; non-temporal loads: no change.
@@ -504,7 +505,8 @@ Q8AttnPlan q8_decode_plan(const Q8AttnParams &p) {
     const int64_t units = (int64_t)p.B * p.Hkv * ((NC + 15) / 16);
     int64_t seen = p.Skv;
     if (p.window > 0) seen = std::min<int64_t>(seen, p.window + p.Sq - 1);
-    // As many workgroups as the chip holds at once; four times as many shorter shares where the sequences have lengths of their own, which the
+    // As many workgroups as the chip holds at once (us, for one, two, three and four per CU, recorded calls: 16 sequences of 4096 keys, 32/8 heads at 128, f16,
+    // 28, 30, 34, 32; 3 of 14000 29, 28, 26, 28; 8 of 4001, 16/4 at 256, 22, 22, 32, 32); four times as many shorter shares where the sequences have lengths of their own, which the
     // host does not know: the long ones are spread (us, 16 of 128 to 16384 keys, 32/32 heads at 96: shares for 2, 4, 8 and 16 workgroups
     // per CU 209, 189, 175 and 188).
     const int64_t target = (p.kv_lens || p.q_positions ? 8 : 2) * (int64_t)p.cus;

@@ -12,12 +12,15 @@
 // the tile after them is widened into LDS.  The order is written down step by step (sched_barrier): left to itself the compiler puts the products
 // of a tile behind each other, each waiting for its piece of LDS (695 us against 660 for the prompt below).
 // Measured: 620 to 660 us, box to box, for a causal prompt of 8192 f16 rows, 32 / 8 heads of 128, int8 (830 to 890 TFLOP/s of visible pairs; the
-// matrix units are busy for 37 % of the cycles, the vector units for 63 %, at 2.1 GHz); 159 us for 4 chunks of 512 bf16 rows over a window of 4096,
-// e4m3; 70 us for 129 f32 rows on 8003 keys, whose queries of two terms fill the registers.
+// matrix units are busy for 37 % of the cycles, the vector units for 57 %); 156 us for 4 chunks of 512 bf16 rows over a window of 4096, e4m3; 68 us for
+// 129 f32 rows on 8003 keys, whose queries of two terms fill the registers.  Mask tensors walk all keys and spill at 128 dims: 299 us for 2048 f16 rows
+// under a causal one, against 75 under the analytic mask.
 //
 // Numbers are brought to f16 as in the kernel for few rows (attn_q8_decode.hip): codes exactly, a column's q scaled by a power of two, one term for
 // 16-bit queries and two for f32.  The values' scales go with the probabilities, brought below 2^15 by a power of two E that follows the largest
-// scale met: w_j = p_j vs_j 2^(15 - E), out = 2^(E - 15) sum w_j c_j / sum p_j.
+// scale met: w_j = p_j vs_j 2^(15 - E), out = 2^(E - 15) sum w_j c_j / sum p_j.  16-bit tensors' w is rounded to 11 bits, one term: the output's own rounding
+// is as large (error against 64 bits 2.9e-4 in f16 where f32 weights leave 2.0e-4, 1.7e-3 either way in bf16), and a second term would double the
+// values' products.
 #include <algorithm>
 #include <utility>
 
@@ -417,13 +420,20 @@ Q8AttnPlan q8_prefill_plan(const Q8AttnParams &p) {
     plan.prefill = true;
     const int64_t NC = (int64_t)p.G * p.Sq, units = (int64_t)p.B * p.Hkv;
     const int dv = q8_padded_dim(p.D);
-    // workgroups of eight wavefronts where they fill the chip, of four otherwise
+    // Workgroups of eight wavefronts where they fill the chip, of four otherwise: a tile that is widened once serves twice the columns (us, eight and
+    // four, f16, recorded calls: causal prompt of 8192 rows, 32/8 heads at 128, 621 and 654; 4 chunks of 512 on 4607 keys 173 and 188; 8 sequences of 65 rows on
+    // 300, 32/32 heads, 19 and 36; below one round: 1000 causal rows 66 and 62, 1500 of 32/32 heads 58 and 49).  Where it does not pay: causal prompts of about
+    // one round of workgroups, whose last rows set the time (2048 rows 74 and 65, 2300 83 and 74).
     plan.waves = dv <= 128 && !p.mask && units * ((NC + 255) / 256) >= p.cus ? 8 : 4;
     const int cols = 32 * plan.waves;
     const int64_t groups = units * ((NC + cols - 1) / cols);
+    // as many workgroups as the chip holds at once (us, for one, two and three per CU, 129 causal rows on 8003 keys: 32/8 heads at 128, f16 52, 46, 50, f32 82, 69,
+    // 80; 16/4 at 256, which a CU holds one of, 57, 66, 84; 200 on 4000 at 64 22, 24, 24)
     const int64_t target = (plan.waves == 8 || dv > 128 ? 1 : 2) * (int64_t)p.cus;
     int64_t seen = p.Skv;
     if (p.window > 0) seen = std::min<int64_t>(seen, p.window + p.Sq - 1);
+    // (us, for shares of 64, 128, 256 and 512 keys at least, f16 at 128: 16 rows on 3000 keys, 32/8 heads, 18, 15, 16, 22, 40 on 1000 17, 16, 18, 24; calls of few
+    // workgroups would take shorter ones, 64 rows on 500 keys of 4/2 heads at 64 10, 11, 13, 16)
     plan.min_chunk = 256;
     int64_t ns = std::min(target / std::max<int64_t>(groups, 1), (seen + plan.min_chunk - 1) / plan.min_chunk);
     plan.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(ns, 256));

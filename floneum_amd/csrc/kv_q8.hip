@@ -147,8 +147,9 @@ __device__ __forceinline__ void q8_norm_rows(const Q8Rows &J, float (&x)[RPG][8]
 // eight elements each, the two pieces of four whose pairs the rotation turns.  Groups of lanes take RPG positions of a head each, consecutive groups
 // the heads of those positions, which share their rows of the tables and, in a model's projections, lie together; the positions lie together in the
 // cache.  Where a row joins earlier ones and raises the scale (of a block's k-th row one time in k), its lanes code those again, one after the other.
-// Bound: bytes for prompts, instructions nearly as much (an exact quotient and its codes): 53 us for q, k and v of 8192 f16 rows of 32 / 8 heads at 128
-// (188 MB, 3.5 TB/s); one chain of latencies for a token (3.8 us for one sequence, 7.2 us with norms over 128 sequences).
+// Bound: memory for prompts, 53 us for q, k and v of 8192 f16 rows of 32 / 8 heads at 128 (188 MB, 3.5 TB/s; 41 us where the caches hold them): wavefronts
+// wait for 74 % of their cycles, the vector units (an exact quotient and its codes) are busy for 55 %; one chain of latencies for a token (3.8 us for one
+// sequence, 7 to 8 us with norms over 64 sequences).
 __device__ __forceinline__ uint32_t q8_divided(uint32_t t, const uint32_t m[2]) { return m[0] ? __umulhi(t, m[0]) >> m[1] : t; }
 
 struct Q8RowPlace {
@@ -293,6 +294,8 @@ __global__ __launch_bounds__(256) void q8_append_rows_kernel(Q8AppendParams p) {
 // the rotation turns.  Slots of a job run over (batch, head, place): with blocks of more than one token the places start at the
 // block that the first new row falls into, so that a block lies in one workgroup, which alone reads its old scale, finds the new one and codes its
 // rows, earlier ones included if the scale has grown.
+// Measured with 8192 f16 rows from the caches (q, k and v, floor 38 us; rows alone take 41 and 44): 57, 58, 56 and 68 us into blocks of 8, 16, 32 and 64 at
+// 128 dims, 32 / 8 heads; 58, 55, 69 and 121 at 256, 16 / 4 heads, where a lane holds up to eight rows and registers leave two wavefronts per SIMD.
 template <int LPR, int RPG, bool NORM>
 __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendParams p) {
     constexpr int GR = 256 / LPR, W = GR * RPG, PITCH = LPR * 8 + 4;
