@@ -100,7 +100,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
     // queries: column c is row c / G, head c % G of the group
     half8_t q[TERMS][KS][2];
     float colscale;
-    bool tiny = false;  // a column of queries below 2^-75: 2^64 of its factor go with the keys' scales, with which alone it would end beyond f32's normal range
+    bool tiny, vast;  // a column's factor that alone would end beyond f32's normal range: 2^64 of it, or 2^-64, go with the keys' scales
     int limit, start;  // keys [start, limit) of the column
     int row;
     // What a wavefront holds of a step's keys.  Steps are loaded NBUF ahead, without a branch (behind one the compiler would wait for all
@@ -173,10 +173,10 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
 #pragma unroll
         for (int i = 0; i < 8; i++) ks[i] = x.ks[i], vs[i] = x.vs[i], top_scale = max(top_scale, __float_as_uint(vs[i]));
         // What is no number among the values' scales (infinity and, as bits, all beyond it) goes by way of the scores, where rows that a mask hides are taken out
-        if (__builtin_amdgcn_ballot_w64(tiny || top_scale >= 0x7f800000u) != 0) {
+        if (__builtin_amdgcn_ballot_w64(tiny || vast || top_scale >= 0x7f800000u) != 0) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                if (tiny) ks[i] *= 0x1p-64f;
+                if (tiny || vast) ks[i] *= tiny ? 0x1p-64f : 0x1p64f;
                 if (__float_as_uint(vs[i]) >= 0x7f800000u) ks[i] = __uint_as_float(0x7fc00000u), vs[i] = 0.0f;
             }
         }
@@ -316,12 +316,12 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
         }
     }
     {
+        int shift = 0;
         if (TERMS == 1 && p.q_dtype == FHIP_F16 && p.scale != 0.0f) {  // as they are
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
                 for (int a = 0; a < 2; a++) q[0][s][a] = raw[s][a].halves(p, 64 * s + 16 * g + 8 * a);
-            colscale = q8_score_scale(p, 0);
         } else {
             float x[KS][2][8], top = 0.0f;
 #pragma unroll
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
 #pragma unroll
                     for (int e = 0; e < 8; e++) top = fmaxf(top, __builtin_fabsf(x[s][a][e]));
                 }
-            const int shift = q8_query_shift(quads_max(top));
+            shift = q8_query_shift(quads_max(top));
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -344,9 +344,10 @@ __global__ __launch_bounds__(256, DV == 64 ? 3 : 2) void q8_decode_kernel(Q8Attn
                         q[0][s][a][e] = high;
                         if constexpr (TERMS == 2) q[1][s][a][e] = low;
                     }
-            tiny = shift > 90;
-            colscale = q8_score_scale(p, tiny ? shift - 64 : shift);
         }
+        const int exponent = q8_score_exponent(p, shift);
+        tiny = exponent < -75, vast = exponent > 100;
+        colscale = q8_score_scale(p, shift - (tiny ? 64 : vast ? -64 : 0));
         const int64_t at = vis.pos0 + row;
         limit = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);
         start = (int)(p.window > 0 ? min((int64_t)hi, max((int64_t)0, at - p.window + 1)) : 0);

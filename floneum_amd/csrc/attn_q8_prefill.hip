@@ -120,8 +120,8 @@ __global__ __launch_bounds__(64 * WAVES, DV <= 128 ? 2 : 1) void q8_prefill_kern
         }
     }
     // Products of codes and queries, below 2^33, are multiplied by the keys' scales (2^-100 to 2^121) first and by the column's factor afterwards: 2^-26 of it
-    // goes with the former, so that no product of finite numbers passes f32's range (2^-10 where queries of 2^85 and more have a factor near its end)
-    const int ahead = __builtin_amdgcn_ballot_w64(shift < -70) != 0 ? 10 : 26;
+    // goes with the former, so that no product of finite numbers passes f32's range, or as much as the wavefront's largest factor leaves room for
+    const int ahead = min(26, 126 - __builtin_amdgcn_readfirstlane(wave_reduce_i(q8_score_exponent(p, shift), [](int x, int y) { return x > y ? x : y; })));
     const float colscale = q8_score_scale(p, shift - ahead), down = __builtin_ldexpf(1.0f, -ahead);
     const int64_t at = vis.pos0 + row;
     const int limit = (int)(p.causal ? max((int64_t)0, min((int64_t)hi, at + 1)) : hi);

@@ -125,10 +125,13 @@ __device__ __forceinline__ void q8_query_terms(const Q8AttnParams &p, float x, i
 // What takes a product of such a query with codes times their scale to the log2 domain, rounded once.  Never 0, which has no product with the
 // -infinity of a hidden key, nor infinite, which has none with 0: a row that would need less than the least f32 has scores of next to nothing all the
 // same.
+__device__ __forceinline__ float q8_score_factor(const Q8AttnParams &p) { return p.scale != 0.0f ? __builtin_fabsf(p.scale) : 1.0f; }
 __device__ __forceinline__ float q8_score_scale(const Q8AttnParams &p, int shift) {
-    const float factor = p.scale != 0.0f ? __builtin_fabsf(p.scale) : 1.0f;
+    const float factor = q8_score_factor(p);
     const float g = __builtin_ldexpf(__builtin_amdgcn_frexp_mantf(factor) * Q8_LOG2E, __builtin_amdgcn_frexp_expf(factor) - shift);
     return fminf(fmaxf(g, 0x1p-149f), 3.402823466e38f);
 }
+// it is below 2 to this plus 1
+__device__ __forceinline__ int q8_score_exponent(const Q8AttnParams &p, int shift) { return __builtin_amdgcn_frexp_expf(q8_score_factor(p)) - shift; }
 
 }  // namespace fhip

@@ -49,6 +49,32 @@ def test_the_largest_factor(device, Sq, Skv):
     c.check()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("Sq, Skv", [(2, 300), (40, 65), (130, 200)])
+def test_large_factors_of_the_least_products(device, dtype, Sq, Skv):
+    """Scores of ordinary size from the least queries of f16, keys of the least scale and a factor of 2^120."""
+    c = Call(device, 1, 4, 2, Sq, Skv, 64, dtype, INT8, 1)
+    c.q = np.sign(c.q).astype(np.float32) * np.float32(2.0 ** -24)
+    c.k_state = np.sign(c.k_state[0].view(np.int8)).astype(np.int8).view(np.uint8), np.full_like(c.k_state[1], q8.LEAST_SCALE)
+    c.scale = 2.0 ** 120
+    c.check()
+    at = Skv - Sq
+    c.check(positions_mask(Sq, Skv, [at]), analytic=(True, at, 0))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("Sq, Skv", [(2, 300), (40, 65), (130, 200)])
+def test_the_least_factors_of_large_products(device, dtype, Sq, Skv):
+    """Scores of ordinary size from large queries of f16, keys of 2^123 and a factor that is no normal f32."""
+    c = Call(device, 1, 4, 2, Sq, Skv, 64, dtype, INT8, 1)
+    c.q = rounded(c.q * np.float32(2.0 ** 12), dtype)
+    c.k_state[1][:] = times_power(c.k_state[1], 123)
+    c.scale = float(np.float32(1.37 * 2.0 ** -139))
+    c.check()
+    at = Skv - Sq
+    c.check(positions_mask(Sq, Skv, [at]), analytic=(True, at, 0))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("fmt, block", [(INT8, 1), (E4M3, 16)])
 @pytest.mark.parametrize("D, Sq, Skv", [(64, 2, 300), (128, 1, 64), (64, 40, 65), (128, 130, 300), (256, 40, 90)])
