@@ -430,14 +430,19 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
     const int group = tid / LPG, d = 4 * (tid % LPG);
     const float *const part = p.partials + first * DV + (d < p.D ? d : 0);
     float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    // parts of the sum are counted in 16 times the power of two above the number of keys (weights of the many-row kernel reach 16), so that no sum of means
+    // times parts is larger than a mean; their own sum, which takes two reductions more, is needed at the end only
+    const float down = __builtin_ldexpf(1.0f, __builtin_clz(p.Skv) - 36);
+    float L;
     if constexpr (FEW) {
         const float2_at8_t own = *(const float2_at8_t *)(ml + 2 * (first + (int64_t)min(lane, p.nsplit - 1) * NC));
         float4_t x[MOST];
 #pragma unroll
         for (int i = 0; i < MOST; i++) x[i] = *(const float4_t *)(part + min(group + i * GROUPS, p.nsplit - 1) * step);
         const float M = wave_max(own[0]), ref = M == -INFINITY ? 0.0f : M;
-        const float part_l = lane < p.nsplit ? own[1] * __builtin_amdgcn_exp2f(own[0] - ref) : 0.0f;
-        weight[64 * wave + lane] = part_l * (1.0f / wave_sum(part_l));
+        const float f = lane < p.nsplit ? own[1] * down * __builtin_amdgcn_exp2f(own[0] - ref) : 0.0f;
+        weight[64 * wave + lane] = f;
+        L = wave_sum(f);
         wave_lds_sync();
 #pragma unroll
         for (int i = 0; i < MOST; i++)
@@ -456,19 +461,19 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
         __syncthreads();
         M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         const float ref = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f;
+        L = 0.0f;
 #pragma unroll
         for (int i = 0; i < Q8_MAX_SHARES / 256; i++) {
-            const float part_l = l[i] * __builtin_amdgcn_exp2f(m[i] - ref);
-            if (tid + 256 * i < p.nsplit) weight[tid + 256 * i] = part_l;
-            L += part_l;
+            const float f = l[i] * down * __builtin_amdgcn_exp2f(m[i] - ref);
+            if (tid + 256 * i < p.nsplit) weight[tid + 256 * i] = f;
+            L += f;
         }
         L = wave_sum(L);
         if (lane == 0) red[4 + wave] = L;
         __syncthreads();
-        const float inv = 1.0f / ((red[4] + red[5]) + (red[6] + red[7]));
+        L = (red[4] + red[5]) + (red[6] + red[7]);
 #pragma unroll 4
-        for (int s = group; s < p.nsplit; s += GROUPS) v += *(const float4_t *)(part + s * step) * (weight[s] * inv);
+        for (int s = group; s < p.nsplit; s += GROUPS) v += *(const float4_t *)(part + s * step) * weight[s];
     }
     *(float4_t *)&sums[group][d] = v;
     __syncthreads();
@@ -476,7 +481,7 @@ __global__ __launch_bounds__(256) void q8_merge_kernel(Q8AttnParams p) {
 #pragma unroll
     for (int g = 1; g < GROUPS; g++) v += *(const float4_t *)&sums[g][d];
     const int b = (int)(bg / p.Hkv), row = c / p.G, head = (int)(bg - b * p.Hkv) * p.G + c - row * p.G;
-    q8_store4_any(p, (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)row * p.os[2] + d * p.os[3], v);
+    q8_store4_any(p, (int64_t)b * p.os[0] + (int64_t)head * p.os[1] + (int64_t)row * p.os[2] + d * p.os[3], v * (1.0f / L));
 }
 
 static int q8_padded_dim(int D) { return (D + 63) / 64 * 64; }
