@@ -511,10 +511,10 @@ Q8AttnPlan q8_decode_plan(const Q8AttnParams &p) {
     const int64_t units = (int64_t)p.B * p.Hkv * ((NC + 15) / 16);
     int64_t seen = p.Skv;
     if (p.window > 0) seen = std::min<int64_t>(seen, p.window + p.Sq - 1);
-    // As many workgroups as the chip holds at once (us, for one, two, three and four per CU, recorded calls: 16 sequences of 4096 keys, 32/8 heads at 128, f16,
-    // 28, 30, 34, 32; 3 of 14000 29, 28, 26, 28; 8 of 4001, 16/4 at 256, 22, 22, 32, 32); four times as many shorter shares where the sequences have lengths of their own, which the
-    // host does not know: the long ones are spread (us, 16 of 128 to 16384 keys, 32/32 heads at 96: shares for 2, 4, 8 and 16 workgroups
-    // per CU 209, 189, 175 and 188).
+    // As many workgroups as the chip holds at once (us, for one, two, three and four per CU, recorded calls: 16 sequences of 4096 keys, 32/8 heads at 128,
+    // f16, 28, 30, 34, 32; 3 of 14000 29, 28, 26, 28; 8 of 4001, 16/4 at 256, 22, 22, 32, 32); four times as many shorter shares where the sequences have
+    // lengths of their own, which the host does not know: the long ones are spread (us, 16 of 128 to 16384 keys, 32/32 heads at 96: shares for 2, 4, 8 and
+    // 16 workgroups per CU 209, 189, 175 and 188).
     const int64_t target = (p.kv_lens || p.q_positions ? 8 : 2) * (int64_t)p.cus;
     plan.min_chunk = 128;
     int64_t ns = std::min((target + units - 1) / units, (seen + 127) / 128);

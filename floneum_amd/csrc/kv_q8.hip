@@ -26,6 +26,12 @@ __device__ __forceinline__ float4_t q8_load4(const void *p, int64_t idx, int dty
     }
     return v;
 }
+// rows of the rotation's tables, which begin at any f32
+__device__ __forceinline__ float4_t q8_load_turn(const float *p) {
+    typedef float float4_at4_t __attribute__((ext_vector_type(4), aligned(4)));
+    const float4_at4_t v = *(const float4_at4_t *)p;
+    return float4_t{v[0], v[1], v[2], v[3]};
+}
 __device__ __forceinline__ float q8_round_through(float v, int dtype) {
     if (dtype == FHIP_F16) return (float)(half_t)v;
     if (dtype == FHIP_BF16) return to_float(from_float<bf16_t>(v));
@@ -248,8 +254,8 @@ __global__ __launch_bounds__(256) void q8_append_rows_kernel(Q8AppendParams p) {
                 }
             }
             if (J.mode != 2) {
-                tc[u] = *(const float4_t *)(p.cos + r[u].pos * half + 4 * j);
-                ts[u] = *(const float4_t *)(p.sin + r[u].pos * half + 4 * j);
+                tc[u] = q8_load_turn(p.cos + r[u].pos * half + 4 * j);
+                ts[u] = q8_load_turn(p.sin + r[u].pos * half + 4 * j);
             }
         }
     }
@@ -375,7 +381,7 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendParams p) {
 #pragma unroll
         for (int u = 0; u < RPG; u++) {
             if (!fresh[u] || !lane_on) continue;
-            const float4_t c = *(const float4_t *)(p.cos + pos[u] * half + 4 * j), s = *(const float4_t *)(p.sin + pos[u] * half + 4 * j);
+            const float4_t c = q8_load_turn(p.cos + pos[u] * half + 4 * j), s = q8_load_turn(p.sin + pos[u] * half + 4 * j);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int a = J.mode == 0 ? e : 2 * e, o = J.mode == 0 ? 4 + e : 2 * e + 1;

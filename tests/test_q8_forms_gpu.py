@@ -124,3 +124,32 @@ def test_rows_written_over(device, fmt, block, n):
         assert np.array_equal(got[:, :, :at // block * block], codes[:, :, :at // block * block])
         written = q8.code_values(got[:, :, at:at + n], fmt), q8.code_values(want[:, :, at:at + n], fmt)
         assert np.array_equal(*written)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("block, n", [(1, 7), (16, 1), (16, 40)])
+def test_tables_at_any_f32(device, block, n, interleaved):
+    """Rotation tables that begin at any f32, as the wide cache's calls take them: the same bits as tables at the start of their memory."""
+    from q8_helpers import _bytes_to
+    rng = np.random.default_rng(n)
+    B, H, D = 2, 2, 72
+    rope = fa.RopeCache(D, 100, 10000.0, device)
+    k, v = (upload(device, rng.standard_normal((B, H, n, D)), F32) for _ in range(2))
+    q = upload(device, rng.standard_normal((B, 4, n, D)), F32)
+    got = []
+    for ahead in (0, 1, 3):
+        memory = [_bytes_to(device, np.concatenate([np.full(ahead, 9, np.float32), t.ravel(), np.full(4, 9, np.float32)]))
+                  for t in (rope.cos_host, rope.sin_host)]
+        tables = fa.CRopeTables(*(m.ptr + 4 * ahead for m in memory), 100, 5, int(interleaved))
+        k8, v8 = (fa.Q8Tensor.empty(device, (B, H, 60, D), fa.Q8Format.INT8, block) for _ in range(2))
+        out = fa.Tensor.empty(device, q.shape, F32)
+        a = fa.CQ8AppendArgs()
+        a.k, a.v, a.row, a.rope = k8._c(), v8._c(), 3, ctypes.pointer(tables)
+        a.k_new, a.v_new, a.in_dtype = k._c4(), v._c4(), F32
+        a.q, a.q_out, a.q_dtype, a.q_out_dtype = q._c4(), out._c4(), F32, F32
+        fa.check(fa.lib().fhip_q8_append(device.stream, ctypes.byref(a)))
+        got.append([out.to_numpy(), *download_q8(k8), *download_q8(v8)])
+    for other in got[1:]:
+        assert all(np.array_equal(x, y) for x, y in zip(got[0], other))
+    assert np.array_equal(got[0][0], q8.rope(q.to_numpy(), rope.cos_host[5:5 + n], rope.sin_host[5:5 + n], interleaved))
