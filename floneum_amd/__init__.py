@@ -125,6 +125,13 @@ class CQ8AttnArgs(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class CContextAttnArgs(ctypes.Structure):
+    _fields_ = [("q", CTensor4), ("out", CTensor4), ("k", CTensor4), ("v", CTensor4), ("prefix_k", CTensor4), ("prefix_v", CTensor4),
+                ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int), ("scale", ctypes.c_float), ("causal", ctypes.c_int32),
+                ("q_pos_offset", ctypes.c_int64), ("window", ctypes.c_int64), ("sinks", ctypes.c_int64), ("kv_lens", ctypes.c_void_p),
+                ("q_positions", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
 SYMBOLS = {
     "fhip_last_error": (ctypes.c_char_p, []),
     "fhip_version": (ctypes.c_char_p, []),
@@ -200,6 +207,9 @@ SYMBOLS = {
     "fhip_q8_attention_validate": (ctypes.c_int, [ctypes.POINTER(CQ8AttnArgs)]),
     "fhip_q8_attention_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(CQ8AttnArgs), ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
     "fhip_q8_attention": (ctypes.c_int, [_P, ctypes.POINTER(CQ8AttnArgs)]),
+    "fhip_context_attention_validate": (ctypes.c_int, [ctypes.POINTER(CContextAttnArgs)]),
+    "fhip_context_attention_workspace_bytes": (ctypes.c_int, [ctypes.POINTER(CContextAttnArgs), ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
+    "fhip_context_attention": (ctypes.c_int, [_P, ctypes.POINTER(CContextAttnArgs)]),
     "fhip_q8_cache_create": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, _PP]),
     "fhip_q8_cache_destroy": (ctypes.c_int, [_P]),
     "fhip_q8_cache_reset": (ctypes.c_int, [_P]),
@@ -608,7 +618,7 @@ class Tensor:
 
     # -- the operator -------------------------------------------------------------------------------
     def flash_attention(self, k, v, scale, mask=None, *, analytic=None, kv_lens=None, out_dtype=None,
-                        force_kernel=KERNEL_AUTO, out=None, q_positions=None):
+                        force_kernel=KERNEL_AUTO, out=None, q_positions=None, sinks=None, prefix=None):
         """fusor::Tensor<4,D>::flash_attention(&self, k, v, scale, mask) -> Self.
 
         self [B,H,Sq,D]; k, v [B,Hkv,Skv,D]; mask = None or (Tensor<2>, MaskKind).  Keyword-only
@@ -618,8 +628,15 @@ class Tensor:
         where the reference panics.
 
         k and v may be an 8-bit cache's (Q8Tensor): fhip_q8_attention, which also takes `q_positions`, a
-        device int32 [B] tensor added to the analytic mask's q_pos_offset, sequence by sequence."""
+        device int32 [B] tensor added to the analytic mask's q_pos_offset, sequence by sequence.
+
+        `sinks` and `prefix` (either, or both): fhip_context_attention.  `sinks`: so many first keys stay visible under the
+        analytic mask's window.  `prefix` = (keys, values) [1,Hkv,P,D] that the whole batch shares, in front of every
+        sequence's own k and v; positions count from its first key, `kv_lens` the own keys alone.  Both take `q_positions`
+        and no mask tensor."""
         L = _LIB or lib()
+        if sinks is not None or prefix is not None:
+            return _context_attention(self, k, v, scale, mask, analytic, kv_lens, q_positions, sinks, prefix, out_dtype, force_kernel, out)
         if type(k) is Q8Tensor or type(v) is Q8Tensor:
             return _q8_attention(self, k, v, scale, mask, analytic, kv_lens, q_positions, out_dtype, force_kernel, out)
         if q_positions is not None:
@@ -1111,6 +1128,49 @@ def _q8_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, out_dtyp
     if need.value:
         a.workspace, a.workspace_bytes = dev.workspace(need.value)
     check(lib().fhip_q8_attention(dev.stream, ctypes.byref(a)))
+    return out
+
+
+def _context_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, sinks, prefix, out_dtype, force_kernel, out):
+    if type(k) is Q8Tensor or type(v) is Q8Tensor:
+        raise InvalidArgument(ERR_INVALID_ARG, "sinks and prefix are for keys and values of q's type")
+    if mask is not None:
+        raise InvalidArgument(ERR_INVALID_ARG, "sinks and prefix go with the analytic mask, not with a mask tensor")
+    if force_kernel != KERNEL_AUTO:
+        raise InvalidArgument(ERR_INVALID_ARG, "force_kernel does not apply to sinks and prefix")
+    pk, pv = (None, None) if prefix is None else prefix
+    inputs = [k, v] if prefix is None else [k, v, pk, pv]
+    dev = q.device
+    if not all(t.device is dev for t in inputs):
+        raise AssertionError("Cannot mix tensors of different devices")
+    if not all(len(t.shape) == 4 for t in [q] + inputs):
+        raise InvalidArgument(ERR_INVALID_ARG, "flash_attention takes rank-4 tensors")
+    if not all(t.dtype == q.dtype for t in inputs):
+        raise InvalidArgument(ERR_INVALID_ARG, "q, k, v and the prefix must share one element type")
+    if out is None:
+        out = Tensor.empty(dev, q.shape, q.dtype if out_dtype is None else out_dtype)
+    elif out_dtype is not None and out_dtype != out.dtype:
+        raise InvalidArgument(ERR_INVALID_ARG, "out_dtype differs from out's")
+    elif out.device is not dev:
+        raise AssertionError("Cannot mix tensors of different devices")
+    a = CContextAttnArgs()
+    a.q, a.out, a.k, a.v = q._c4(), out._c4(), k._c4(), v._c4()
+    if prefix is not None:
+        a.prefix_k, a.prefix_v = pk._c4(), pv._c4()
+    a.dtype, a.out_dtype, a.scale = q.dtype, out.dtype, float(np.float32(scale))
+    if isinstance(analytic, CAnalyticMask):
+        if analytic.enabled:
+            a.causal, a.q_pos_offset, a.window = analytic.causal, analytic.q_pos_offset, analytic.window
+    elif analytic is not None:
+        causal, off, window = analytic
+        a.causal, a.q_pos_offset, a.window = 1 if causal else 0, int(off), int(window or 0)
+    a.sinks = 0 if sinks is None else int(sinks)
+    a.kv_lens, a.q_positions = _lens_ptr(kv_lens, q.shape[0], "kv_lens"), _lens_ptr(q_positions, q.shape[0], "q_positions")
+    need = ctypes.c_size_t()
+    check(lib().fhip_context_attention_workspace_bytes(ctypes.byref(a), dev.compute_units, ctypes.byref(need)))
+    if need.value:
+        a.workspace, a.workspace_bytes = dev.workspace(need.value)
+    check(lib().fhip_context_attention(dev.stream, ctypes.byref(a)))
     return out
 
 

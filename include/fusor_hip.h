@@ -571,6 +571,43 @@ int fhip_q8_cache_allocated_seq_len(const fhip_q8_cache *c, uint64_t *len);
 int fhip_q8_cache_append(fhip_q8_cache *c, fhip_stream *s, const fhip_q8_append_args *args, fhip_q8_tensor *k_all,
                          fhip_q8_tensor *v_all);
 
+/* ---- attention over a context in two parts ---------------------------------------------------------
+ * Keys that come in two parts: a prefix that the whole batch shares (one instruction or document in front of many questions), held
+ * once, and every sequence's own; and a sliding window whose first tokens stay visible.  Each alone or both.  The reference has
+ * neither: there a shared prefix is copied into every sequence's cache, and such a window is a mask tensor with two runs of zeros per
+ * row, which fhip_flash_attention adds value by value over all keys.
+ * Keys are numbered through both parts: key j < P is row j of the prefix, the others row j - P of the sequence's own.  Query row i
+ * of sequence b stands at position p = q_pos_offset + q_positions[b] + i and sees
+ *   j < P + kv_lens[b]  and  (not causal or j <= p)  and  (window == 0 or j + window > p or j < sinks) */
+typedef struct {
+    fhip_tensor4 q;        /* [B, H,   Sq,  D] of dtype, any strides                                    */
+    fhip_tensor4 out;      /* the same shape, of out_dtype (dtype, or FHIP_F32)                         */
+    fhip_tensor4 k;        /* [B, Hkv, Skv, D] the sequences' own keys; v: their values                 */
+    fhip_tensor4 v;
+    fhip_tensor4 prefix_k; /* [1, Hkv, P, D] the shared prefix; all zero: none                          */
+    fhip_tensor4 prefix_v;
+    fhip_dtype dtype;
+    fhip_dtype out_dtype;
+    float scale;
+    int32_t causal;
+    int64_t q_pos_offset;
+    int64_t window;             /* 0: none                                                               */
+    int64_t sinks;              /* first keys that the window does not hide                              */
+    const int32_t *kv_lens;     /* optional device [B]: own keys that count (below 0: none, above Skv: all) */
+    const int32_t *q_positions; /* optional device [B], with causal or window; the contents of both may change between replays */
+    void *workspace;
+    size_t workspace_bytes;
+} fhip_context_attn_args;
+
+/* Host-only check of the arguments: the status and message that fhip_context_attention would return. */
+int fhip_context_attention_validate(const fhip_context_attn_args *args);
+/* Bytes of device workspace (16-byte aligned) the call needs on a device of `compute_units`; 0: none. */
+int fhip_context_attention_workspace_bytes(const fhip_context_attn_args *args, int32_t compute_units, size_t *bytes);
+/* out = softmax(q k^T * scale over the visible keys) v, with the head mapping, accumulation and special cases of fhip_flash_attention: rows that
+ * see no key come out NaN, no keys at all (P + Skv == 0) give zeros.  Rows of k, v and the prefix that no query row of the call sees may hold
+ * anything.  Asynchronous on `s`; may be captured.  Calls that share a workspace must not overlap. */
+int fhip_context_attention(fhip_stream *s, const fhip_context_attn_args *args);
+
 /* Library version string, e.g. "fusor-hip 0.1 (gfx950)". */
 const char *fhip_version(void);
 

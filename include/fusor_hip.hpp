@@ -532,6 +532,45 @@ inline Tensor<4> flash_attention(const Tensor<4> &q, const Q8Tensor &k, const Q8
     return out;
 }
 
+/// What flash_attention_context takes beside q, k, v and the scale; see fhip_context_attn_args.
+struct Context {
+    const Tensor<4> *prefix_k = nullptr, *prefix_v = nullptr;  ///< [1, Hkv, P, D], both or neither
+    bool causal = true;
+    int64_t q_pos_offset = 0, window = 0, sinks = 0;
+    const int32_t *kv_lens = nullptr, *q_positions = nullptr;  ///< device, [B]
+};
+
+/// q.flash_attention(k, v, scale) with a prefix that the batch shares, and with a window whose first tokens stay visible
+/// (fhip_context_attention)
+inline Tensor<4> flash_attention_context(const Tensor<4> &q, const Tensor<4> &k, const Tensor<4> &v, float scale, const Context &context) {
+    const Device &dev = q.device();
+    if (!context.prefix_k != !context.prefix_v) throw Panic("a prefix has keys and values");
+    for (const Tensor<4> *t : {&k, &v, context.prefix_k, context.prefix_v}) {
+        if (!t) continue;
+        if (!dev.same(t->device())) throw Panic("Cannot mix tensors of different devices");
+        if (t->dtype() != q.dtype()) throw Panic("q, k, v and the prefix must share one element type");
+    }
+    uint32_t shape[4];
+    for (int i = 0; i < 4; i++) shape[i] = q.shape()[i];
+    Tensor<4> out = Tensor<4>::empty(dev, q.dtype(), shape);
+    fhip_context_attn_args a{};
+    a.q = q.c4(), a.out = out.c4(), a.k = k.c4(), a.v = v.c4();
+    if (context.prefix_k) a.prefix_k = context.prefix_k->c4(), a.prefix_v = context.prefix_v->c4();
+    a.dtype = a.out_dtype = (fhip_dtype)q.dtype();
+    a.scale = scale;
+    a.causal = context.causal;
+    a.q_pos_offset = context.q_pos_offset, a.window = context.window, a.sinks = context.sinks;
+    a.kv_lens = context.kv_lens, a.q_positions = context.q_positions;
+    size_t need = 0;
+    check(fhip_context_attention_workspace_bytes(&a, dev.info().compute_units, &need));
+    if (need) {
+        a.workspace = dev.workspace(need);
+        a.workspace_bytes = dev.workspace_bytes();
+    }
+    check(fhip_context_attention(dev.stream(), &a));
+    return out;
+}
+
 /// fusor::RopeCache (fusor-ml/fusor/src/composite/rope.rs:180-265): [context_length, head_dim/2] f32
 /// cos/sin tables on the device, applied by one fused kernel per tensor.
 class RopeCache {

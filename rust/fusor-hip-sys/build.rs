@@ -28,6 +28,8 @@ const SOURCES: &[&str] = &[
     "kv_q8.hip",
     "attn_q8_decode.hip",
     "attn_q8_prefill.hip",
+    "api_context.hip",
+    "attn_context_any.hip",
 ];
 
 // the flags floneum_amd/build.py uses; packed-f32 VALU forms are kept out of the generated code on purpose

@@ -206,6 +206,29 @@ pub struct fhip_q8_attn_args {
     pub workspace_bytes: usize,
 }
 
+/// Arguments of one attention call over a context in two parts.  Zero-initialise, then fill.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct fhip_context_attn_args {
+    pub q: fhip_tensor4,
+    pub out: fhip_tensor4,
+    pub k: fhip_tensor4,
+    pub v: fhip_tensor4,
+    pub prefix_k: fhip_tensor4,
+    pub prefix_v: fhip_tensor4,
+    pub dtype: fhip_dtype,
+    pub out_dtype: fhip_dtype,
+    pub scale: f32,
+    pub causal: i32,
+    pub q_pos_offset: i64,
+    pub window: i64,
+    pub sinks: i64,
+    pub kv_lens: *const i32,
+    pub q_positions: *const i32,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: usize,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy)]
 pub struct fhip_device_info {
@@ -465,6 +488,11 @@ unsafe extern "C" {
         v_all: *mut fhip_q8_tensor,
     ) -> c_int;
 
+    // attention over a context in two parts
+    pub fn fhip_context_attention_validate(args: *const fhip_context_attn_args) -> c_int;
+    pub fn fhip_context_attention_workspace_bytes(args: *const fhip_context_attn_args, compute_units: i32, bytes: *mut usize) -> c_int;
+    pub fn fhip_context_attention(s: *mut fhip_stream, args: *const fhip_context_attn_args) -> c_int;
+
     pub fn fhip_version() -> *const c_char;
 }
 
@@ -481,4 +509,5 @@ const _: () = {
     assert!(core::mem::size_of::<fhip_q8_tensor>() == 104);
     assert!(core::mem::size_of::<fhip_q8_append_args>() == 528);
     assert!(core::mem::size_of::<fhip_q8_attn_args>() == 448);
+    assert!(core::mem::size_of::<fhip_context_attn_args>() == 456);
 };

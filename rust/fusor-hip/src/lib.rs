@@ -408,6 +408,57 @@ impl<D: HipDataType> HipTensor<4, D> {
         check(unsafe { fhip_q8_attention(dev.stream(), &a) }).expect("flash_attention_q8");
         out
     }
+
+    /// [`HipTensor::flash_attention`] under a causal mask and a window of `window` keys (0: none) whose first `sinks` keys stay
+    /// visible, behind a `prefix` (keys, values) `[1, kv_heads, p, head_dim]` that the whole batch shares (`fhip_context_attention`).
+    /// The first query row stands at position `q_pos_offset`, counted from the prefix's first key.
+    pub fn flash_attention_context(
+        &self,
+        k: &Self,
+        v: &Self,
+        scale: f32,
+        prefix: Option<(&Self, &Self)>,
+        q_pos_offset: usize,
+        window: usize,
+        sinks: usize,
+    ) -> Self {
+        let dev = self.device().clone();
+        let out = Self::uninit(&dev, self.shape).expect("output allocation");
+        let mut a: fhip_context_attn_args = unsafe { std::mem::zeroed() };
+        a.q = self.as_ffi();
+        a.out = out.as_ffi();
+        a.k = k.as_ffi();
+        a.v = v.as_ffi();
+        if let Some((pk, pv)) = prefix {
+            a.prefix_k = pk.as_ffi();
+            a.prefix_v = pv.as_ffi();
+        }
+        a.dtype = D::FHIP_DTYPE;
+        a.out_dtype = D::FHIP_DTYPE;
+        a.scale = scale;
+        a.causal = 1;
+        a.q_pos_offset = q_pos_offset as i64;
+        a.window = window as i64;
+        a.sinks = sinks as i64;
+        let mut need = 0usize;
+        check(unsafe { fhip_context_attention_workspace_bytes(&a, dev.compute_units(), &mut need) }).expect("workspace query");
+        let mut ws = dev.0.workspace.lock().unwrap();
+        if need > ws.1 {
+            unsafe {
+                if !ws.0.is_null() {
+                    fhip_stream_synchronize(dev.stream());
+                    fhip_free(dev.raw(), ws.0);
+                }
+                let mut p = ptr::null_mut();
+                check(fhip_malloc(dev.raw(), need, &mut p)).expect("workspace allocation");
+                *ws = (p, need);
+            }
+        }
+        a.workspace = ws.0;
+        a.workspace_bytes = ws.1;
+        check(unsafe { fhip_context_attention(dev.stream(), &a) }).expect("flash_attention_context");
+        out
+    }
 }
 
 impl<D: HipDataType> HipTensor<2, D> {
