@@ -124,13 +124,16 @@ int fhip_context_attention_workspace_bytes(const fhip_context_attn_args *args, i
     *bytes = 0;
     const int rc = validate_context(args);
     if (rc || empty(args->q.shape)) return rc;
-    (void)compute_units;
+    if (args->k.shape[2] == 0 && args->prefix_k.shape[2] == 0) return FHIP_OK;
+    ContextParams p;
+    fill_context(args, compute_units, &p);
+    *bytes = context_plan(p, args->dtype).bytes;
     return FHIP_OK;
 }
 
 int fhip_context_attention(fhip_stream *s, const fhip_context_attn_args *args) {
     if (!s) return invalid("stream is NULL");
-    const int rc = validate_context(args);
+    int rc = validate_context(args);
     if (rc || empty(args->q.shape)) return rc;
     FHIP_HIP_CHECK(hipSetDevice(s->dev->ordinal));
     if (args->k.shape[2] == 0 && args->prefix_k.shape[2] == 0) {  // no keys at all: zeros, as fhip_flash_attention
@@ -139,7 +142,16 @@ int fhip_context_attention(fhip_stream *s, const fhip_context_attn_args *args) {
     }
     ContextParams p;
     fill_context(args, s->dev->prop.multiProcessorCount, &p);
-    return launch_context_any(p, args->dtype, s->s);
+    const ContextPlan plan = context_plan(p, args->dtype);
+    if (plan.any) return launch_context_any(p, args->dtype, s->s);
+    if (plan.bytes && (!args->workspace || ((uintptr_t)args->workspace & 15) != 0 || args->workspace_bytes < plan.bytes)) {
+        set_error("context_attention: needs %zu bytes of 16-byte aligned workspace, got %zu", plan.bytes, args->workspace ? args->workspace_bytes : 0);
+        return FHIP_ERR_WORKSPACE;
+    }
+    p.partials = (float *)args->workspace;
+    p.slots = plan.slots, p.pf_pitch = p.D + 4;
+    rc = launch_context_rows(p, plan.rows, args->dtype, s->s);
+    return rc || plan.slots == 1 ? rc : launch_context_merge(p, args->dtype, s->s);
 }
 
 }  // extern "C"

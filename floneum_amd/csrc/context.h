@@ -17,6 +17,34 @@ struct ContextParams : AttnParams {
     int32_t slots;
 };
 
+// The kernel for few rows.  A job streams one part's keys for columns, (query row, head of the group) pairs of a KV head: of one sequence
+// (its own keys), or of all of them (the prefix).
+struct ContextRowsJob {
+    int32_t prefix;  // else the sequences' own keys
+    int32_t units;   // KV heads, times the batch for own keys
+    int32_t blocks;  // column blocks of a unit
+    int32_t nsplit, chunk;  // shares of the visible keys, `chunk` keys each
+    int32_t slot0;
+};
+struct ContextRows {
+    ContextRowsJob job[2];
+    int32_t second;  // first workgroup of job[1]
+    int32_t total;   // workgroups
+    int32_t columns; // of a workgroup: 16 or 32
+};
+
+// What a call runs.
+struct ContextPlan {
+    bool any;  // the kernel that takes every call, alone
+    ContextRows rows;
+    int slots;
+    size_t bytes;  // of workspace
+};
+ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype);
+
 int launch_context_any(const ContextParams &p, fhip_dtype dtype, hipStream_t stream);
+bool context_rows_takes(const ContextParams &p, fhip_dtype dtype);
+int launch_context_rows(const ContextParams &p, const ContextRows &rows, fhip_dtype dtype, hipStream_t stream);
+int launch_context_merge(const ContextParams &p, fhip_dtype dtype, hipStream_t stream);
 
 }  // namespace fhip

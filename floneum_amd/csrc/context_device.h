@@ -5,6 +5,8 @@
 
 namespace fhip {
 
+constexpr float CONTEXT_LOG2E = 1.4426950408889634f;
+
 // Keys are numbered through both parts: j < P is row j of the prefix, the others row j - P of the sequence's own.  A row sees
 // [0, first) and [lo, hi), with first <= lo <= hi.
 struct ContextRow {
@@ -19,6 +21,32 @@ __device__ __forceinline__ ContextRow context_row(const ContextParams &p, int b,
     r.lo = p.window > 0 ? (int)min((int64_t)r.hi, max(at - p.window + 1, (int64_t)0)) : 0;
     r.first = min(p.sinks, r.lo);
     return r;
+}
+// the same within one part, in rows of that part
+__device__ __forceinline__ ContextRow context_row_of(const ContextParams &p, bool prefix, int b, int row) {
+    ContextRow r = context_row(p, b, row);
+    if (prefix) r.first = min(r.first, p.P), r.lo = min(r.lo, p.P), r.hi = min(r.hi, p.P);
+    else r.first = max(r.first - p.P, 0), r.lo = max(r.lo - p.P, 0), r.hi = max(r.hi - p.P, 0);
+    return r;
+}
+
+// What some row of several sees: [0, first) and [lo, hi) again.  Rows that see nothing do not count.
+struct ContextSpan {
+    int first, lo, hi;
+    // visible keys in order: key v, or v + gap from `first` on
+    __device__ __forceinline__ int keys() const { return first + max(hi - lo, 0); }
+    __device__ __forceinline__ int gap() const { return lo - first; }
+};
+// of the rows that the lanes of a wavefront hold
+__device__ __forceinline__ ContextSpan context_span(const ContextRow &r) {
+    const bool none = r.first == 0 && r.lo >= r.hi;
+    ContextSpan s;
+    s.first = __builtin_amdgcn_readfirstlane(wave_reduce_i(r.first, [](int x, int y) { return max(x, y); }));
+    s.lo = __builtin_amdgcn_readfirstlane(wave_reduce_i(none ? 0x7fffffff : r.lo, [](int x, int y) { return min(x, y); }));
+    s.hi = __builtin_amdgcn_readfirstlane(wave_reduce_i(none ? 0 : r.hi, [](int x, int y) { return max(x, y); }));
+    s.lo = max(s.lo, s.first);
+    if (s.hi < s.lo) s.hi = s.lo = s.first;
+    return s;
 }
 
 }  // namespace fhip

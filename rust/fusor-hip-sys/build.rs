@@ -30,6 +30,8 @@ const SOURCES: &[&str] = &[
     "attn_q8_prefill.hip",
     "api_context.hip",
     "attn_context_any.hip",
+    "attn_context_rows.hip",
+    "context_plan.hip",
 ];
 
 // the flags floneum_amd/build.py uses; packed-f32 VALU forms are kept out of the generated code on purpose
