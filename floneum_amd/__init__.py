@@ -1153,6 +1153,12 @@ def _context_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, sin
         raise InvalidArgument(ERR_INVALID_ARG, "out_dtype differs from out's")
     elif out.device is not dev:
         raise AssertionError("Cannot mix tensors of different devices")
+    if _native is not None:
+        done = _native.context_attention(q, k, v, scale, analytic, kv_lens, q_positions, sinks, prefix, out)
+        if done is not None:
+            if done != OK:
+                check(done)
+            return out
     a = CContextAttnArgs()
     a.q, a.out, a.k, a.v = q._c4(), out._c4(), k._c4(), v._c4()
     if prefix is not None:

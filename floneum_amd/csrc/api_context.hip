@@ -150,7 +150,8 @@ int fhip_context_attention(fhip_stream *s, const fhip_context_attn_args *args) {
     }
     p.partials = (float *)args->workspace;
     p.slots = plan.slots, p.pf_pitch = p.D + 4;
-    rc = launch_context_rows(p, plan.rows, args->dtype, s->s);
+    for (int i = 0; i < plan.tile_launches && !rc; i++) rc = launch_context_tiles(p, plan.tiles[i], args->dtype, s->s);
+    if (!rc && plan.rows.total) rc = launch_context_rows(p, plan.rows, args->dtype, s->s);
     return rc || plan.slots == 1 ? rc : launch_context_merge(p, args->dtype, s->s);
 }
 

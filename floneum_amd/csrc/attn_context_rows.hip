@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
 #pragma unroll
     for (int cb = 0; cb < CB; cb++) {
         at[cb] = column_at(p, w.b, w.g, w.c0 + min(j + 16 * cb, w.columns - 1));
-        seen[cb] = context_row_of(p, w.prefix, at[cb].b, at[cb].row);
+        seen[cb] = context_row(p, at[cb].b, at[cb].row).of(p, w.prefix);
         if (!(w.prefix && p.window == 0)) {
             const ContextSpan s = context_span(seen[cb]);
             if (cb == 0) {
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
 #pragma unroll
     for (int cb = 0; cb < CB; cb++) {
         at[cb] = column_at(p, w.b, w.g, w.c0 + min(j + 16 * cb, w.columns - 1));
-        seen[cb] = context_row_of(p, w.prefix, at[cb].b, at[cb].row);
+        seen[cb] = context_row(p, at[cb].b, at[cb].row).of(p, w.prefix);
         if (!(w.prefix && p.window == 0)) {
             const ContextSpan s = context_span(seen[cb]);
             if (cb == 0) {

@@ -1,0 +1,64 @@
+// Attention over a context in two parts on the 256-row kernel of the 16-bit matrix cores (attn_prefill_mfma_kernel.h), head dims to 128: prompts and
+// chunks under a window with first tokens, behind a prefix, and the rows of a whole batch on the prefix that it shares.
+#include <type_traits>
+
+#include "attn_prefill_mfma_kernel.h"
+#include "context.h"
+
+namespace fhip {
+
+bool context_tiles_takes(const ContextParams &p, fhip_dtype dtype) {
+    if (dtype == FHIP_F32 || p.D > 128 || !context_rows_takes(p, dtype)) return false;
+    if (!(p.scale > 0.0f && p.scale * PF_LOG2E < 2.0f)) return false;
+    // queries are read in pieces of 16 bytes
+    if ((uintptr_t)p.q % 16 != 0 || p.qs[3] != 1) return false;
+    for (int i = 0; i < 3; i++)
+        if (p.qs[i] % 8 != 0) return false;
+    // keys and values through 32-bit buffer offsets: rows that do not overlap, less than 2 GiB of a tensor's head
+    auto fits = [&](int64_t row, int64_t rows) { return row >= p.D && rows * row * 2 < 0x7fffffff - 65536; };
+    if (p.Skv > 0 && !(fits(p.ks[2], p.Skv) && fits(p.vs[2], p.Skv))) return false;
+    return p.P == 0 || (fits(p.pks[1], p.P) && fits(p.pvs[1], p.P));
+}
+
+template <typename T>
+static void launch_type(const ContextParams &p, bool half, hipStream_t stream) {
+    const int bm = half ? PF_BM / 2 : PF_BM, nqb = (p.rows + bm - 1) / bm;
+    const dim3 grid((unsigned)((int64_t)p.units * nqb * p.pf_nsplit)), block(64 * PF_WAVES);
+    const int bytes = p.out_f32 ? 4 : 2;
+    int out_vec = p.os[3] == 1 && (uintptr_t)p.out % 16 == 0;
+    for (int i = 0; i < 3; i++)
+        if (p.os[i] * bytes % 16 != 0) out_vec = 0;
+    auto run = [&](auto dim, auto contracted, auto padded) {
+        constexpr int DIM = decltype(dim)::value, QDIM = decltype(contracted)::value;
+        constexpr bool PAD = decltype(padded)::value;
+        if (p.with_prefix && p.with_own) {
+            ContextBoth both;
+            (ContextParams &)both = p;
+            hipLaunchKernelGGL((prefill_mfma_kernel<T, DIM, QDIM, PAD, false, ContextBoth>), grid, block, 0, stream, both, nqb, out_vec);
+        } else if (half) hipLaunchKernelGGL((prefill_mfma_kernel<T, DIM, QDIM, PAD, true, ContextParams>), grid, block, 0, stream, p, nqb, out_vec);
+        else hipLaunchKernelGGL((prefill_mfma_kernel<T, DIM, QDIM, PAD, false, ContextParams>), grid, block, 0, stream, p, nqb, out_vec);
+    };
+    using std::integral_constant;
+    using std::true_type;
+    using std::false_type;
+    if (p.D == 64) run(integral_constant<int, 64>{}, integral_constant<int, 64>{}, false_type{});
+    else if (p.D == 96) run(integral_constant<int, 96>{}, integral_constant<int, 96>{}, false_type{});
+    else if (p.D == 128) run(integral_constant<int, 128>{}, integral_constant<int, 128>{}, false_type{});
+    else if (p.D < 64) run(integral_constant<int, 64>{}, integral_constant<int, 64>{}, true_type{});
+    else if (p.D <= 80) run(integral_constant<int, 96>{}, integral_constant<int, 80>{}, true_type{});
+    else if (p.D < 96) run(integral_constant<int, 96>{}, integral_constant<int, 96>{}, true_type{});
+    else run(integral_constant<int, 128>{}, integral_constant<int, 128>{}, true_type{});
+}
+
+int launch_context_tiles(const ContextParams &p0, const ContextTilesLaunch &how, fhip_dtype dtype, hipStream_t stream) {
+    ContextParams p = p0;
+    p.fold = how.fold, p.with_prefix = how.with_prefix, p.with_own = how.with_own;
+    p.units = how.units, p.rows = how.rows;
+    p.pf_nsplit = how.shares, p.pf_chunk = how.chunk, p.slot0 = how.slot0;
+    if (dtype == FHIP_F16) launch_type<half_t>(p, how.half, stream);
+    else launch_type<bf16_t>(p, how.half, stream);
+    FHIP_HIP_CHECK(hipGetLastError());
+    return FHIP_OK;
+}
+
+}  // namespace fhip

@@ -15,7 +15,14 @@ struct ContextParams : AttnParams {
     // shares of the keys: every (sequence, head, query row) has `slots` places in `partials`, each pf_pitch floats: D values, the
     // reference exponent (base 2) and the sum of the weights
     int32_t slots;
+    // tiled kernels: what a launch takes.  Rows of a KV head are stacked, see context_tiles.h; the tiles of their visible keys are dealt to
+    // pf_nsplit shares of pf_chunk tiles.
+    int32_t fold;        // rows of all sequences together (on the prefix alone)
+    int32_t with_prefix, with_own;
+    int32_t units, rows; // KV heads (times the batch, if not folded), stacked rows of each
+    int32_t slot0;
 };
+struct ContextBoth : ContextParams {};  // of a launch that takes both parts
 
 // The kernel for few rows.  A job streams one part's keys for columns, (query row, head of the group) pairs of a KV head: of one sequence
 // (its own keys), or of all of them (the prefix).
@@ -33,10 +40,21 @@ struct ContextRows {
     int32_t columns; // of a workgroup: 16 or 32
 };
 
-// What a call runs.
+// A launch of a tiled kernel, see ContextParams.
+struct ContextTilesLaunch {
+    int32_t fold, with_prefix, with_own;
+    int32_t units, rows;
+    int32_t half;            // 128 stacked rows per workgroup instead of 256
+    int32_t shares, chunk;   // of the visible tiles
+    int32_t slot0;
+};
+
+// What a call runs, in this order, and the merge where a row has several places.
 struct ContextPlan {
     bool any;  // the kernel that takes every call, alone
-    ContextRows rows;
+    int32_t tile_launches;
+    ContextTilesLaunch tiles[2];
+    ContextRows rows;  // total 0: none
     int slots;
     size_t bytes;  // of workspace
 };
@@ -45,6 +63,8 @@ ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype);
 int launch_context_any(const ContextParams &p, fhip_dtype dtype, hipStream_t stream);
 bool context_rows_takes(const ContextParams &p, fhip_dtype dtype);
 int launch_context_rows(const ContextParams &p, const ContextRows &rows, fhip_dtype dtype, hipStream_t stream);
+bool context_tiles_takes(const ContextParams &p, fhip_dtype dtype);
+int launch_context_tiles(const ContextParams &p, const ContextTilesLaunch &how, fhip_dtype dtype, hipStream_t stream);
 int launch_context_merge(const ContextParams &p, fhip_dtype dtype, hipStream_t stream);
 
 }  // namespace fhip

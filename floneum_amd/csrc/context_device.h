@@ -11,6 +11,10 @@ constexpr float CONTEXT_LOG2E = 1.4426950408889634f;
 // [0, first) and [lo, hi), with first <= lo <= hi.
 struct ContextRow {
     int first, lo, hi;
+    __device__ __forceinline__ ContextRow of(const ContextParams &p, bool prefix) const;  // within one part, in rows of that part
+    __device__ __forceinline__ ContextRow uniform() const {
+        return {__builtin_amdgcn_readfirstlane(first), __builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi)};
+    }
 };
 __device__ __forceinline__ ContextRow context_row(const ContextParams &p, int b, int row) {
     const int own = p.kv_lens ? min(max(p.kv_lens[b], 0), p.Skv) : p.Skv;
@@ -22,12 +26,9 @@ __device__ __forceinline__ ContextRow context_row(const ContextParams &p, int b,
     r.first = min(p.sinks, r.lo);
     return r;
 }
-// the same within one part, in rows of that part
-__device__ __forceinline__ ContextRow context_row_of(const ContextParams &p, bool prefix, int b, int row) {
-    ContextRow r = context_row(p, b, row);
-    if (prefix) r.first = min(r.first, p.P), r.lo = min(r.lo, p.P), r.hi = min(r.hi, p.P);
-    else r.first = max(r.first - p.P, 0), r.lo = max(r.lo - p.P, 0), r.hi = max(r.hi - p.P, 0);
-    return r;
+__device__ __forceinline__ int part_row(const ContextParams &p, bool prefix, int key) { return prefix ? min(key, p.P) : max(key - p.P, 0); }
+__device__ __forceinline__ ContextRow ContextRow::of(const ContextParams &p, bool prefix) const {
+    return {part_row(p, prefix, first), part_row(p, prefix, lo), part_row(p, prefix, hi)};
 }
 
 // What some row of several sees: [0, first) and [lo, hi) again.  Rows that see nothing do not count.
@@ -36,6 +37,12 @@ struct ContextSpan {
     // visible keys in order: key v, or v + gap from `first` on
     __device__ __forceinline__ int keys() const { return first + max(hi - lo, 0); }
     __device__ __forceinline__ int gap() const { return lo - first; }
+    // the first visible key and the one behind the last (of a span that has some)
+    __device__ __forceinline__ int begin() const { return first > 0 ? 0 : lo; }
+    __device__ __forceinline__ int end() const { return lo < hi ? hi : first; }
+    __device__ __forceinline__ ContextSpan of(const ContextParams &p, bool prefix) const {
+        return {part_row(p, prefix, first), part_row(p, prefix, lo), part_row(p, prefix, hi)};
+    }
 };
 // of the rows that the lanes of a wavefront hold
 __device__ __forceinline__ ContextSpan context_span(const ContextRow &r) {

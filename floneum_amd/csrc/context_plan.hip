@@ -38,30 +38,97 @@ static int64_t workgroups_of(const ContextRowsJob &job) {
     return job.blocks == 1 ? shares : div_up(shares, 8) * 8 * job.blocks;
 }
 
+// Time of a launch of the tiled kernel in us, from the constants of prefill_mfma_time (attn_prefill_mfma.hip): rounds of workgroups that walk their tiles,
+// the longest where they fit one round, the mean otherwise.
+static double tiles_time(const ContextParams &p, const ContextTilesLaunch &how) {
+    const int bm = how.half ? 128 : 256;
+    const int64_t blocks = div_up(how.rows, bm), wgs = (int64_t)how.units * blocks * how.shares, rounds = div_up(wgs, p.cus);
+    const double dims = p.D <= 64 ? 1.0 : p.D <= 96 ? 1.43 : 1.86;
+    const int64_t tiles = how.chunk;
+    return 4.6 + rounds * (how.half ? 5.3 + 0.356 * dims * tiles : 3.9 + 0.579 * dims * tiles);
+}
+static ContextTilesLaunch tiles_launch(const ContextParams &p, bool fold, bool with_prefix, bool with_own, bool parked) {
+    ContextTilesLaunch best, how;
+    memset(&how, 0, sizeof(how));
+    how.fold = fold, how.with_prefix = with_prefix, how.with_own = with_own;
+    how.units = fold ? p.Hkv : p.B * p.Hkv;
+    how.rows = (fold ? p.B : 1) * p.G * p.Sq;
+    double least = 0.0;
+    memset(&best, 0, sizeof(best));
+    for (const bool half : {false, true}) {
+        if (half && with_prefix && with_own) break;  // (the form of 128 rows takes one part)
+        how.half = half;
+        const int64_t positions = std::min<int64_t>(p.Sq, (half ? 128 : 256) / p.G + 2);
+        int64_t keys = 0;
+        if (with_prefix) keys += most_visible(p, p.P, fold ? p.Sq : positions, p.sinks);
+        if (with_own) keys += most_visible(p, p.Skv, positions, std::max<int64_t>((int64_t)p.sinks - p.P, 0));
+        if (with_prefix && with_own && p.causal && p.window > 0) keys = std::min(keys, p.window + positions + p.sinks);
+        const int64_t tiles = std::max<int64_t>(div_up(keys, 64), 1);
+        const int64_t wgs = (int64_t)how.units * div_up(how.rows, half ? 128 : 256);
+        for (int64_t shares = 1; shares <= tiles; shares++) {
+            if (shares > 1 && wgs * shares > 2 * p.cus) break;
+            how.chunk = (int32_t)div_up(tiles, shares);
+            how.shares = (int32_t)div_up(tiles, how.chunk);
+            double us = tiles_time(p, how);
+            if (how.shares > 1 || parked) us += 0.488e-6 * (double)p.B * p.H * p.Sq * how.shares * (p.D + 4) * sizeof(float);
+            if (how.shares > 1 && !parked) us += 3.0;
+            if (least == 0.0 || us < 0.98 * least) least = us, best = how;
+        }
+    }
+    return best;
+}
+
 ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     ContextPlan plan;
     memset(&plan, 0, sizeof(plan));
     plan.any = true;
     if (!context_rows_takes(p, dtype)) return plan;
-    const int64_t most = (int64_t)p.G * p.Sq * (p.P > 0 ? p.B : 1);
-    ContextRows &rows = plan.rows;
-    rows.columns = most > 16 && p.D <= 128 ? 32 : 16;
-    const int step = dtype == FHIP_F32 ? 64 : 128;
-    const int64_t target = (int64_t)p.cus * (p.D > 128 ? 1 : 2);
-    int jobs = 0;
-    int64_t total = 0, slots = 0;
-    for (const bool prefix : {true, false}) {
-        if ((prefix ? p.P : p.Skv) == 0) continue;
-        ContextRowsJob job = rows_job(p, prefix, rows.columns, step, target);
-        job.slot0 = (int32_t)slots;
-        slots += job.nsplit;
-        if (jobs == 1) rows.second = (int32_t)total;
-        rows.job[jobs++] = job;
-        total += workgroups_of(job);
+    const bool tiles = context_tiles_takes(p, dtype);
+    const int64_t each = (int64_t)p.G * p.Sq;  // columns of a sequence and KV head
+    // rows of all sequences meet the prefix together where they see one run of it
+    const bool can_fold = p.P > 0 && p.B > 1 && (p.window == 0 || !p.q_positions);
+    const bool own_by_rows = !tiles || each <= 32;
+    bool prefix_by_rows = p.P > 0 && (!tiles || (own_by_rows && (each * p.B <= 32 || !can_fold)));
+    int64_t slots = 0;
+    auto add_tiles = [&](bool fold, bool with_prefix, bool with_own, bool parked) {
+        ContextTilesLaunch &how = plan.tiles[plan.tile_launches++];
+        how = tiles_launch(p, fold, with_prefix, with_own, parked);
+        how.slot0 = (int32_t)slots;
+        slots += how.shares;
+    };
+    if (p.P > 0 && !prefix_by_rows) {
+        if (own_by_rows) add_tiles(p.B > 1, true, false, p.Skv > 0);
+        else if (can_fold && each < 128) add_tiles(true, true, false, true), add_tiles(false, false, true, true);
+        else add_tiles(false, true, p.Skv > 0, false);
+    } else if (!own_by_rows) {
+        add_tiles(false, false, true, false);
     }
-    if (jobs == 1) rows.second = (int32_t)total;
-    if (total > 0x7fffffff || slots > 0x7fffffff) return plan;
-    rows.total = (int32_t)total;
+    if (own_by_rows) {
+        ContextRows &rows = plan.rows;
+        const int64_t most = each * (prefix_by_rows ? p.B : 1);
+        rows.columns = most > 16 && p.D <= 128 ? 32 : 16;
+        const int step = dtype == FHIP_F32 ? 64 : 128;
+        const int64_t target = (int64_t)p.cus * (p.D > 128 ? 1 : 2);
+        int jobs = 0;
+        int64_t total = 0;
+        for (const bool prefix : {true, false}) {
+            if (prefix ? !prefix_by_rows : p.Skv == 0) continue;
+            ContextRowsJob job = rows_job(p, prefix, rows.columns, step, target);
+            job.slot0 = (int32_t)slots;
+            slots += job.nsplit;
+            if (jobs == 1) rows.second = (int32_t)total;
+            rows.job[jobs++] = job;
+            total += workgroups_of(job);
+        }
+        if (jobs == 1) rows.second = (int32_t)total;
+        if (total > 0x7fffffff) return plan;
+        rows.total = (int32_t)total;
+    }
+    for (int i = 0; i < plan.tile_launches; i++) {
+        const ContextTilesLaunch &how = plan.tiles[i];
+        if ((int64_t)how.units * div_up(how.rows, how.half ? 128 : 256) * how.shares > 0x7fffffff) return plan;
+    }
+    if (slots > 0x7fffffff) return plan;
     plan.any = false;
     plan.slots = (int)slots;
     if (slots > 1) plan.bytes = (size_t)p.B * p.H * p.Sq * (size_t)slots * (size_t)(p.D + 4) * sizeof(float);

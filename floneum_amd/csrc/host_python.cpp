@@ -583,6 +583,54 @@ PyObject *q8_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return PyLong_FromLong(rc);
 }
 
+// ---- attention over a context in two parts ------------------------------------------------------------------------------------
+
+// context_attention(q, k, v, scale, analytic, kv_lens, q_positions, sinks, prefix, out): the library's status, or None
+PyObject *context_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    if (n != 10 || Py_TYPE(a[0]) != tensor.type || !slot(tensor, a[0], 0)) Py_RETURN_NONE;
+    const Ref memory(Py_NewRef(slot(tensor, a[0], 0)));
+    Ref device(PyObject_GetAttr(memory.o, n_device));
+    fhip_context_attn_args args;
+    memset(&args, 0, sizeof(args));
+    int32_t dtype, other[2], out_dtype;
+    void *stream;
+    uint64_t cus;
+    if (!device.o || !describe<4>(a[0], &args.q, &dtype, nullptr) || !describe<4>(a[1], &args.k, &other[0], device.o) ||
+        !describe<4>(a[2], &args.v, &other[1], device.o) || other[0] != dtype || other[1] != dtype ||
+        !describe<4>(a[9], &args.out, &out_dtype, device.o) || !PyFloat_Check(a[3]) || !(std::fabs(PyFloat_AS_DOUBLE(a[3])) < 1e38)) {
+        not_plain();
+        Py_RETURN_NONE;
+    }
+    args.dtype = (fhip_dtype)dtype, args.out_dtype = (fhip_dtype)out_dtype, args.scale = (float)PyFloat_AS_DOUBLE(a[3]);
+    if (a[4] != Py_None) {
+        fhip_analytic_mask mask;
+        if (!analytic_of(a[4], &mask)) Py_RETURN_NONE;
+        if (mask.enabled) args.causal = mask.causal, args.q_pos_offset = mask.q_pos_offset, args.window = mask.window;
+    }
+    if (a[8] != Py_None) {
+        if (!PyTuple_CheckExact(a[8]) || PyTuple_GET_SIZE(a[8]) != 2 || !describe<4>(PyTuple_GET_ITEM(a[8], 0), &args.prefix_k, &other[0], device.o) ||
+            !describe<4>(PyTuple_GET_ITEM(a[8], 1), &args.prefix_v, &other[1], device.o) || other[0] != dtype || other[1] != dtype)
+            Py_RETURN_NONE;
+    }
+    if ((a[5] != Py_None && !lens_of(a[5], args.q.shape[0], &args.kv_lens)) ||
+        (a[6] != Py_None && !lens_of(a[6], args.q.shape[0], &args.q_positions)) || (a[7] != Py_None && !as_i64(a[7], &args.sinks)) ||
+        !attr_handle(device.o, n_stream, &stream) || !attr_u64(device.o, n_compute_units, &cus))
+        Py_RETURN_NONE;
+    size_t need = 0;
+    int rc = fhip_context_attention_workspace_bytes(&args, (int32_t)cus, &need);
+    if (rc == FHIP_OK && need) {
+        const int got = workspace_of(device.o, need, &args.workspace, &args.workspace_bytes);
+        if (got < 0) return nullptr;
+        if (got == 0) Py_RETURN_NONE;
+    }
+    if (rc == FHIP_OK) {
+        Py_BEGIN_ALLOW_THREADS
+        rc = fhip_context_attention((fhip_stream *)stream, &args);
+        Py_END_ALLOW_THREADS
+    }
+    return PyLong_FromLong(rc);
+}
+
 bool find(Slots *s, PyObject *type, int n, const char *const *names) {
     s->type = (PyTypeObject *)type;
     for (int i = 0; i < n; i++) {
@@ -626,6 +674,7 @@ PyMethodDef methods[] = {
     {"q8_dequantize", (PyCFunction)(void *)q8_dequantize, METH_FASTCALL, nullptr},
     {"q8_append", (PyCFunction)(void *)q8_append, METH_FASTCALL, nullptr},
     {"q8_cache_append", (PyCFunction)(void *)q8_cache_append, METH_FASTCALL, nullptr},
+    {"context_attention", (PyCFunction)(void *)context_attention, METH_FASTCALL, nullptr},
     {"q8_attention", (PyCFunction)(void *)q8_attention, METH_FASTCALL, nullptr},
     {"bind", (PyCFunction)(void *)bind, METH_FASTCALL, nullptr},
     {"attention", (PyCFunction)(void *)attention, METH_FASTCALL, nullptr},

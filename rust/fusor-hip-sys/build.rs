@@ -31,6 +31,7 @@ const SOURCES: &[&str] = &[
     "api_context.hip",
     "attn_context_any.hip",
     "attn_context_rows.hip",
+    "attn_context_tiles.hip",
     "context_plan.hip",
 ];
 
