@@ -51,12 +51,11 @@ static void launch_type(const ContextParams &p, bool half, hipStream_t stream) {
 }
 
 int launch_context_tiles(const ContextParams &p0, const ContextTilesLaunch &how, fhip_dtype dtype, hipStream_t stream) {
+    if (dtype == FHIP_F32) return launch_context_terms(p0, how, stream);
     ContextParams p = p0;
-    p.fold = how.fold, p.with_prefix = how.with_prefix, p.with_own = how.with_own;
-    p.units = how.units, p.rows = how.rows;
-    p.pf_nsplit = how.shares, p.pf_chunk = how.chunk, p.slot0 = how.slot0;
-    if (dtype == FHIP_F16) launch_type<half_t>(p, how.half, stream);
-    else launch_type<bf16_t>(p, how.half, stream);
+    set_tiles_launch(p, how);
+    if (dtype == FHIP_F16) launch_type<half_t>(p, how.rows_per_group == 128, stream);
+    else launch_type<bf16_t>(p, how.rows_per_group == 128, stream);
     FHIP_HIP_CHECK(hipGetLastError());
     return FHIP_OK;
 }

@@ -44,10 +44,16 @@ struct ContextRows {
 struct ContextTilesLaunch {
     int32_t fold, with_prefix, with_own;
     int32_t units, rows;
-    int32_t half;            // 128 stacked rows per workgroup instead of 256
+    int32_t rows_per_group;  // stacked rows of a workgroup
+    int32_t key_groups;      // wavefronts of a workgroup that share its rows, see the kernels
     int32_t shares, chunk;   // of the visible tiles
     int32_t slot0;
 };
+inline void set_tiles_launch(ContextParams &p, const ContextTilesLaunch &how) {
+    p.fold = how.fold, p.with_prefix = how.with_prefix, p.with_own = how.with_own;
+    p.units = how.units, p.rows = how.rows;
+    p.pf_nsplit = how.shares, p.pf_chunk = how.chunk, p.slot0 = how.slot0;
+}
 
 // What a call runs, in this order, and the merge where a row has several places.
 struct ContextPlan {
@@ -65,6 +71,8 @@ bool context_rows_takes(const ContextParams &p, fhip_dtype dtype);
 int launch_context_rows(const ContextParams &p, const ContextRows &rows, fhip_dtype dtype, hipStream_t stream);
 bool context_tiles_takes(const ContextParams &p, fhip_dtype dtype);
 int launch_context_tiles(const ContextParams &p, const ContextTilesLaunch &how, fhip_dtype dtype, hipStream_t stream);
+bool context_terms_takes(const ContextParams &p, fhip_dtype dtype);
+int launch_context_terms(const ContextParams &p, const ContextTilesLaunch &how, hipStream_t stream);
 int launch_context_merge(const ContextParams &p, fhip_dtype dtype, hipStream_t stream);
 
 }  // namespace fhip
