@@ -11,7 +11,7 @@ SOURCES = ["api.hip", "attn_generic.hip", "attn_decode.hip", "attn_prefill_mfma.
            "attn_prefill_f32.hip", "attn_prefill_f32_terms.hip",
            "kv_cache.hip", "mask_intervals.hip", "rope.hip", "calibration.hip",
            "api_q8.hip", "kv_q8.hip", "attn_q8_decode.hip", "attn_q8_prefill.hip",
-           "api_context.hip", "attn_context_any.hip", "attn_context_rows.hip", "attn_context_tiles.hip", "attn_context_terms.hip", "context_plan.hip"]
+           "api_context.hip", "attn_context_any.hip", "attn_context_rows.hip", "attn_context_tiles.hip", "attn_context_wide.hip", "attn_context_terms.hip", "context_plan.hip"]
 LIB = os.path.join(HERE, "libfusor_hip.so")
 HOST = os.path.join(HERE, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))  # (no other interpreter takes it for its own)
 STATIC = os.path.join(HERE, "libfusor_hip.a")

@@ -1,5 +1,5 @@
-// Attention over a context in two parts on the 256-row kernel of the 16-bit matrix cores (attn_prefill_mfma_kernel.h), head dims to 128: prompts and
-// chunks under a window with first tokens, behind a prefix, and the rows of a whole batch on the prefix that it shares.
+// Attention over a context in two parts on the tiled kernels of the 16-bit matrix cores: prompts and chunks under a window with first tokens, behind a
+// prefix, and the rows of a whole batch on the prefix that it shares.  Here the 256-row kernel (attn_prefill_mfma_kernel.h), head dims to 128.
 #include <type_traits>
 
 #include "attn_prefill_mfma_kernel.h"
@@ -8,8 +8,9 @@
 namespace fhip {
 
 bool context_tiles_takes(const ContextParams &p, fhip_dtype dtype) {
-    if (dtype == FHIP_F32 || p.D > 128 || !context_rows_takes(p, dtype)) return false;
-    if (!(p.scale > 0.0f && p.scale * PF_LOG2E < 2.0f)) return false;
+    if (dtype == FHIP_F32 || !context_rows_takes(p, dtype)) return false;
+    // (in bf16 Q takes the power of two of the scale: up to 1, and above head_dim 128 not so small that elements leave the normal range)
+    if (!(p.scale > 0.0f && p.scale * PF_LOG2E < 2.0f) || (p.D > 128 && p.scale * PF_LOG2E < 0.00390625f)) return false;
     // queries are read in pieces of 16 bytes
     if ((uintptr_t)p.q % 16 != 0 || p.qs[3] != 1) return false;
     for (int i = 0; i < 3; i++)
@@ -52,6 +53,7 @@ static void launch_type(const ContextParams &p, bool half, hipStream_t stream) {
 
 int launch_context_tiles(const ContextParams &p0, const ContextTilesLaunch &how, fhip_dtype dtype, hipStream_t stream) {
     if (dtype == FHIP_F32) return launch_context_terms(p0, how, stream);
+    if (p0.D > 128) return launch_context_wide(p0, how, dtype, stream);
     ContextParams p = p0;
     set_tiles_launch(p, how);
     if (dtype == FHIP_F16) launch_type<half_t>(p, how.rows_per_group == 128, stream);

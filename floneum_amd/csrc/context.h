@@ -72,6 +72,7 @@ int launch_context_rows(const ContextParams &p, const ContextRows &rows, fhip_dt
 bool context_tiles_takes(const ContextParams &p, fhip_dtype dtype);
 int launch_context_tiles(const ContextParams &p, const ContextTilesLaunch &how, fhip_dtype dtype, hipStream_t stream);
 bool context_terms_takes(const ContextParams &p, fhip_dtype dtype);
+int launch_context_wide(const ContextParams &p, const ContextTilesLaunch &how, fhip_dtype dtype, hipStream_t stream);  // one part
 int launch_context_terms(const ContextParams &p, const ContextTilesLaunch &how, hipStream_t stream);
 int launch_context_merge(const ContextParams &p, fhip_dtype dtype, hipStream_t stream);
 

@@ -41,18 +41,19 @@ static int64_t workgroups_of(const ContextRowsJob &job) {
     return job.blocks == 1 ? shares : div_up(shares, 8) * 8 * job.blocks;
 }
 
-// Time of a launch of the 256-row kernel in us, from the constants of prefill_mfma_time (attn_prefill_mfma.hip): rounds of workgroups that walk their tiles of
-// 64 keys.
+// Time of a launch of the 16-bit kernels in us, from the constants of prefill_mfma_time (attn_prefill_mfma.hip) and prefill_wide_time
+// (attn_prefill_mfma_wide.hip): rounds of workgroups that walk their tiles of 64 keys, above head_dim 128 32.
 static double tiles_time(const ContextParams &p, const ContextTilesLaunch &how, int64_t keys) {
     const int64_t wgs = (int64_t)how.units * div_up(how.rows, how.rows_per_group) * how.shares, rounds = div_up(wgs, p.cus);
+    if (p.D > 128) return 5.0 + rounds * (6.5 + 0.70 * div_up(div_up(keys, how.shares), 32));
     const double dims = p.D <= 64 ? 1.0 : p.D <= 96 ? 1.43 : 1.86, tiles = (double)div_up(div_up(keys, how.shares), 64);
     return 4.6 + rounds * (how.rows_per_group == 128 ? 5.3 + 0.356 * dims * tiles : 3.9 + 0.579 * dims * tiles);
 }
 static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype, bool fold, bool with_prefix, bool with_own, bool parked) {
     const bool f32 = dtype == FHIP_F32, both = with_prefix && with_own;
-    const int tile = f32 ? 32 : 64;
-    // (rows per workgroup, key groups); of the 16-bit kernel the form of 128 rows takes one part
-    static const int FORMS[2][3][2] = {{{256, 1}, {128, 2}, {0, 0}}, {{128, 1}, {128, 2}, {64, 2}}};
+    const int tile = f32 || p.D > 128 ? 32 : 64;
+    // (rows per workgroup, key groups); to head_dim 128 the 16-bit form of 128 rows takes one part
+    static const int FORMS[3][3][2] = {{{256, 1}, {128, 2}, {0, 0}}, {{128, 1}, {0, 0}, {0, 0}}, {{128, 1}, {128, 2}, {64, 2}}};
     ContextTilesLaunch best, how;
     memset(&how, 0, sizeof(how));
     how.fold = fold, how.with_prefix = with_prefix, how.with_own = with_own;
@@ -60,8 +61,8 @@ static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype,
     how.rows = (fold ? p.B : 1) * p.G * p.Sq;
     best = how;
     double least = 0.0;
-    for (const auto &form : FORMS[f32]) {
-        if (form[0] == 0 || (!f32 && form[0] == 128 && both) || (f32 && p.D > 128 && form[1] > 1)) continue;
+    for (const auto &form : FORMS[f32 ? 2 : p.D > 128 ? 1 : 0]) {
+        if (form[0] == 0 || (!f32 && p.D <= 128 && form[0] == 128 && both) || (f32 && p.D > 128 && form[1] > 1)) continue;
         how.rows_per_group = form[0], how.key_groups = form[1];
         const int64_t positions = std::min<int64_t>(p.Sq, form[0] / p.G + 2);
         int64_t keys = 0;
@@ -100,6 +101,7 @@ ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     // rows of all sequences meet the prefix together where they see one run of it
     const bool can_fold = p.P > 0 && p.B > 1 && (p.window == 0 || !p.q_positions);
     const bool own_by_rows = !tiles || each <= (dtype == FHIP_F32 ? 64 : 32);
+    const bool one_part = dtype != FHIP_F32 && p.D > 128;  // the tiled kernel takes one part per launch
     bool prefix_by_rows = p.P > 0 && (!tiles || (own_by_rows && (each * p.B <= (dtype == FHIP_F32 ? 64 : 32) || !can_fold)));
     int64_t slots = 0;
     auto add_tiles = [&](bool fold, bool with_prefix, bool with_own, bool parked) {
@@ -110,7 +112,8 @@ ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     };
     if (p.P > 0 && !prefix_by_rows) {
         if (own_by_rows) add_tiles(p.B > 1, true, false, p.Skv > 0);
-        else if (can_fold && each < 128) add_tiles(true, true, false, true), add_tiles(false, false, true, true);
+        else if ((can_fold && each < 128) || (one_part && p.Skv > 0))
+            add_tiles(can_fold, true, false, true), add_tiles(false, false, true, true);
         else add_tiles(false, true, p.Skv > 0, false);
     } else if (!own_by_rows) {
         add_tiles(false, false, true, false);

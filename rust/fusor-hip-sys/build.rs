@@ -32,6 +32,7 @@ const SOURCES: &[&str] = &[
     "attn_context_any.hip",
     "attn_context_rows.hip",
     "attn_context_tiles.hip",
+    "attn_context_wide.hip",
     "attn_context_terms.hip",
     "context_plan.hip",
 ];
