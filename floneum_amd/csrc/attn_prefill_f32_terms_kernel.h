@@ -450,11 +450,8 @@ __global__ __launch_bounds__(64 * U * KG, D > 128 || (KG == 2 && U == 2 && D > 6
     typename std::conditional<BOTH, ContextBothTiles<PT_BN>, ContextTiles<PT_BN>>::type tiles;
     if constexpr (CTX) {
         total_rows = p.rows;
-        const int last = p.rows - 1;
-        row_at = stacked_row(p, b, g, min(query, last));
-        sees = context_row(p, row_at.b, row_at.row);
-        wave_sees = stacked_span(p, b, min(qw0, last), min(qw0 + 31, last), lane);
-        wg_sees = stacked_span(p, b, min(q0, last), min(q0 + bm - 1, last), lane).some;
+        row_at = stacked_row(p, b, g, min(query, p.rows - 1));
+        stacked_spans<32 * U>(p, b, q0, qw0, lane, row_at, wave_sees, wg_sees, sees);
         if constexpr (!BOTH) {
             const bool prefix = p.with_prefix != 0;
             sees = sees.of(p, prefix), wave_sees = wave_sees.of(p, prefix), wg_sees = wg_sees.of(p, prefix);

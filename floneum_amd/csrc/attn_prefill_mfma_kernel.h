@@ -192,11 +192,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void prefill_mfma_kernel(P p, int
     typename std::conditional<BOTH, ContextBothTiles<PF_BN>, ContextTiles<PF_BN>>::type tiles;
     if constexpr (CTX) {
         total_rows = p.rows;
-        const int last = p.rows - 1;
-        row_at = stacked_row(p, b, g, min(query, last));
-        sees = context_row(p, row_at.b, row_at.row);
-        wave_sees = stacked_span(p, b, min(qw0, last), min(qw0 + 31, last), lane);
-        wg_sees = stacked_span(p, b, q0, min(q0 + BM - 1, last), lane).some;
+        row_at = stacked_row(p, b, g, min(query, p.rows - 1));
+        stacked_spans<BM>(p, b, q0, qw0, lane, row_at, wave_sees, wg_sees, sees);
         if constexpr (!BOTH) {
             const bool prefix = p.with_prefix != 0;
             sees = sees.of(p, prefix), wave_sees = wave_sees.of(p, prefix), wg_sees = wg_sees.of(p, prefix);

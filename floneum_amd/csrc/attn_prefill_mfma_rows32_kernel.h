@@ -149,12 +149,11 @@ __global__ __launch_bounds__(256, 1) void prefill_mfma_wide_rows32_kernel(P p, i
     ContextTiles<R32_KEYS> tiles;
     if constexpr (CTX) {
         total_rows = p.rows;
-        const int last = p.rows - 1;
         const bool prefix = p.with_prefix != 0;
-        row_at = stacked_row(p, b, g, min(query, last));
-        sees = context_row(p, row_at.b, row_at.row).of(p, prefix);
-        all_see = stacked_span(p, b, min(qw0, last), min(qw0 + 31, last), lane).of(p, prefix).all;
-        wg_sees = stacked_span(p, b, q0, min(q0 + R32_BM - 1, last), lane).some.of(p, prefix);
+        StackedSpan wave_sees;
+        row_at = stacked_row(p, b, g, min(query, p.rows - 1));
+        stacked_spans<R32_BM>(p, b, q0, qw0, lane, row_at, wave_sees, wg_sees, sees);
+        sees = sees.of(p, prefix), all_see = wave_sees.all.of(p, prefix), wg_sees = wg_sees.of(p, prefix);
         tiles.set(p, wg_sees, ksplit);
         key_end = wg_sees.end();
     } else {

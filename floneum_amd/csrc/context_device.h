@@ -16,16 +16,23 @@ struct ContextRow {
         return {__builtin_amdgcn_readfirstlane(first), __builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi)};
     }
 };
-__device__ __forceinline__ ContextRow context_row(const ContextParams &p, int b, int row) {
-    const int own = p.kv_lens ? min(max(p.kv_lens[b], 0), p.Skv) : p.Skv;
-    const int64_t at = p.q_pos_offset + (p.q_positions ? p.q_positions[b] : 0) + row;
-    ContextRow r;
-    r.hi = p.P + own;
-    if (p.causal) r.hi = (int)min((int64_t)r.hi, max(at + 1, (int64_t)0));
-    r.lo = p.window > 0 ? (int)min((int64_t)r.hi, max(at - p.window + 1, (int64_t)0)) : 0;
-    r.first = min(p.sinks, r.lo);
-    return r;
+// what a sequence brings
+struct ContextSequence {
+    int keys;    // of both parts
+    int64_t at;  // position of its first row
+    __device__ __forceinline__ ContextRow row(const ContextParams &p, int i) const {
+        ContextRow r;
+        r.hi = p.causal ? (int)min((int64_t)keys, max(at + i + 1, (int64_t)0)) : keys;
+        r.lo = p.window > 0 ? (int)min((int64_t)r.hi, max(at + i - p.window + 1, (int64_t)0)) : 0;
+        r.first = min(p.sinks, r.lo);
+        return r;
+    }
+};
+__device__ __forceinline__ ContextSequence context_sequence(const ContextParams &p, int b) {
+    const int own = p.kv_lens ? p.kv_lens[b] : p.Skv, start = p.q_positions ? p.q_positions[b] : 0;
+    return {p.P + min(max(own, 0), p.Skv), p.q_pos_offset + start};
 }
+__device__ __forceinline__ ContextRow context_row(const ContextParams &p, int b, int row) { return context_sequence(p, b).row(p, row); }
 __device__ __forceinline__ int part_row(const ContextParams &p, bool prefix, int key) { return prefix ? min(key, p.P) : max(key - p.P, 0); }
 __device__ __forceinline__ ContextRow ContextRow::of(const ContextParams &p, bool prefix) const {
     return {part_row(p, prefix, first), part_row(p, prefix, lo), part_row(p, prefix, hi)};

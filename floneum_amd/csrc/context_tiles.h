@@ -24,30 +24,60 @@ struct StackedSpan {
         return {some.of(p, prefix), all.of(p, prefix)};
     }
 };
-__device__ __forceinline__ StackedSpan stacked_span(const ContextParams &p, int b, int r0, int r1, int lane) {
-    StackedSpan s;
+// Of the wavefront's 32 rows from qw0 on and of the workgroup's BM rows from q0 on; sees: of the lane's row, qw0 + lane % 32.  What the sequences bring is
+// asked for once and together: each time it is waited for costs a launch of few tiles a memory latency.
+template <int BM>
+__device__ __forceinline__ void stacked_spans(const ContextParams &p, int b, int q0, int qw0, int lane, const StackedRow &at, StackedSpan &wave, ContextSpan &wg,
+                                              ContextRow &sees) {
+    const int last = p.rows - 1;
     if (b >= 0) {  // a sequence's rows: both ends move forward with the row
-        const ContextRow x = context_row(p, b, p.G == 1 ? r0 : r0 / p.G).uniform(), y = context_row(p, b, p.G == 1 ? r1 : r1 / p.G).uniform();
-        s.some.first = y.first, s.some.lo = max(x.lo, y.first), s.some.hi = max(y.hi, s.some.lo);
-        s.all = ContextRow{x.first, y.lo, x.hi};
-        return s;
+        const ContextSequence s = context_sequence(p, b);
+        auto query = [&](int r) __attribute__((always_inline)) { return p.G == 1 ? min(r, last) : min(r, last) / p.G; };
+        auto between = [&](int r0, int r1) __attribute__((always_inline)) {
+            const ContextRow x = s.row(p, query(r0)).uniform(), y = s.row(p, query(r1)).uniform();
+            const int lo = max(x.lo, y.first);
+            return StackedSpan{{y.first, lo, max(y.hi, lo)}, {x.first, y.lo, x.hi}};
+        };
+        sees = s.row(p, at.row);
+        wave = between(qw0, qw0 + 31);
+        wg = between(q0, q0 + BM - 1).some;
+        return;
     }
-    ContextRow all = {0x7fffffff, 0, 0x7fffffff};
-    int first = 0, lo = 0x7fffffff, hi = 0;
-    for (int r = r0 + lane; r <= r1; r += 64) {
-        const StackedRow at = stacked_row(p, -1, 0, r);
-        const ContextRow x = context_row(p, at.b, at.row);
-        all.first = min(all.first, x.first), all.lo = max(all.lo, x.lo), all.hi = min(all.hi, x.hi);
-        first = max(first, x.first), hi = max(hi, x.hi);
-        if (x.first > 0 || x.lo < x.hi) lo = min(lo, x.lo);
+    constexpr int N = (BM + 63) / 64;
+    ContextSequence s[N], mine = context_sequence(p, at.b);
+    int row[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const StackedRow x = stacked_row(p, -1, 0, min(q0 + min(lane + 64 * i, BM - 1), last));
+        row[i] = x.row, s[i] = context_sequence(p, x.b);
     }
     auto least = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(wave_reduce_i(x, [](int a, int c) { return min(a, c); })); };
     auto most = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(wave_reduce_i(x, [](int a, int c) { return max(a, c); })); };
-    s.all = ContextRow{least(all.first), most(all.lo), least(all.hi)};
-    s.some.first = most(first);
-    s.some.lo = max(least(lo), s.some.first), s.some.hi = max(most(hi), s.some.lo);
-    if (s.some.lo == 0x7fffffff) s.some.lo = s.some.hi = 0;
-    return s;
+    sees = mine.row(p, at.row);
+    if (p.window == 0) {  // [0, hi) each
+        int hi = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) hi = max(hi, s[i].row(p, row[i]).hi);
+        wg = {0, 0, most(hi)};
+        wave = {{0, 0, most(sees.hi)}, {0, 0, least(sees.hi)}};
+        return;
+    }
+    int first = 0, lo = 0x7fffffff, hi = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const ContextRow x = s[i].row(p, row[i]);
+        first = max(first, x.first), hi = max(hi, x.hi);
+        if (x.first > 0 || x.lo < x.hi) lo = min(lo, x.lo);
+    }
+    auto span = [&](int f, int l, int h) __attribute__((always_inline)) {
+        ContextSpan r;
+        r.first = most(f), r.lo = max(least(l), r.first), r.hi = max(most(h), r.lo);
+        if (r.lo == 0x7fffffff) r.lo = r.hi = 0;
+        return r;
+    };
+    wg = span(first, lo, hi);
+    wave.some = span(sees.first, sees.first > 0 || sees.lo < sees.hi ? sees.lo : 0x7fffffff, sees.hi);
+    wave.all = ContextRow{least(sees.first), most(sees.lo), least(sees.hi)};
 }
 
 // The tiles of KEYS keys that hold what some row sees, in order.  Tiles start at multiples of KEYS rows of their tensor, and none is listed twice.
