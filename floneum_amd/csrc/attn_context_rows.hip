@@ -1,9 +1,9 @@
 // Attention over a context in two parts for few query rows: every visible key and value is read once per column block, straight from memory
 // into registers and from there through LDS to the matrix cores; what no row sees is not touched.
 //
-// Columns are (query row, head of the group) pairs that share a KV head.  A workgroup of four wavefronts serves 16 or 32 of them over one
-// share of one part's visible keys, 32 keys (f32: 16) per wavefront and step:
-//   own keys   columns of one sequence; the visible rows of its cache, first tokens and window, are numbered without the gap between them
+// Columns are (query row, head of the group) pairs that share a KV head.  A workgroup of four wavefronts serves 16 or 32 of them over one share of one
+// part's visible keys, which are numbered without the gap between first tokens and window, a tile of 32 (f32: 16) per wavefront and step:
+//   own keys   columns of one sequence
 //   prefix     columns of all sequences, so that the prefix is read once for the batch
 // Both go in one launch, the prefix's workgroups first.
 //   S^T[key][column] = K Q^T           v_mfma_f32_16x16x32 of the tensors' type, f32: v_mfma_f32_16x16x4_f32
@@ -18,7 +18,11 @@
 namespace fhip {
 
 constexpr int CR_WAVES = 4;
+constexpr int CR_NT = 2;                   // streamed past the caches (measured against plain loads: 16 ragged sequences, 232 MB, 51.0 us and 57.4)
+constexpr uint64_t CR_FAR = 1 << 25;  // bytes between rows up to which a tile's offsets stay in 31 bits
 typedef uint32_t uint2r_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) char *lds_t;
+#define CR_LDS(type, at) ((__attribute__((address_space(3))) type *)(at))
 
 template <typename T>
 struct RowsMma;
@@ -56,20 +60,19 @@ __device__ __forceinline__ float column_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Rows that no column sees may hold anything, NaN among it, which 0 x NaN would bring into the result: where a step has such rows, their values are
-// cleared in LDS.  Bits of keys that some column of the 16 lanes sees:
+// bits of keys that some column of the 16 lanes sees
 __device__ __forceinline__ uint32_t any_column(uint32_t x) {
     x |= (uint32_t)dpp_mov_i<DPP_QUAD_XOR1>((int)x);
     x |= (uint32_t)dpp_mov_i<DPP_QUAD_XOR2>((int)x);
     x |= (uint32_t)dpp_mov_i<DPP_ROW_HALF_MIRROR>((int)x);
     return x | (uint32_t)dpp_mov_i<DPP_ROW_MIRROR>((int)x);
 }
-// 16 lanes clear a row of BYTES
+// 16 lanes clear a row of BYTES in LDS
 template <int BYTES>
-__device__ __forceinline__ void clear_row(__attribute__((address_space(3))) char *row, int lane) {
+__device__ __forceinline__ void clear_row(lds_t row, int lane) {
 #pragma unroll
     for (int at = 0; at < BYTES; at += 256)
-        if (at + 16 * lane < BYTES) *(__attribute__((address_space(3))) uint4_t *)(row + at + 16 * lane) = uint4_t{0, 0, 0, 0};
+        if (at + 16 * lane < BYTES) *CR_LDS(uint4_t, row + at + 16 * lane) = uint4_t{0, 0, 0, 0};
 }
 
 // where a column's row of q, of the result and of the partials is
@@ -125,152 +128,63 @@ __device__ __forceinline__ void park_nothing(const ContextParams &p, const RowsW
     ws[p.D + 1] = 0.0f;
 }
 
-// Joins the wavefronts' states, [wave][COLS][D + 2] floats of LDS, and writes the share or the result.
-template <typename T, int COLS>
-__device__ __forceinline__ void join_waves(const ContextParams &p, const RowsWork &w, const float *states, int pitch) {
-    const int D = p.D, pieces = D / 4;
-    const bool vec = p.os[3] == 1;
-    for (int i = threadIdx.x; i < w.columns * pieces; i += 64 * CR_WAVES) {
-        const int column = i / pieces, d = 4 * (i - column * pieces);
-        float m = -INFINITY;
+// Four dims of a column's result, or of its share.
+template <typename T>
+__device__ __forceinline__ void write_column(const ContextParams &p, const RowsWork &w, int column, int d, float m, float l, float4_t o) {
+    const ColumnAt at = column_at(p, w.b, w.g, column);
+    if (p.slots > 1) {
+        float *ws = p.partials + ((((int64_t)at.b * p.H + at.h) * p.Sq + at.row) * p.slots + w.slot) * p.pf_pitch;
+        *(float4_t *)(ws + d) = o;
+        if (d == 0) ws[p.D] = m, ws[p.D + 1] = l;
+        return;
+    }
+    const int64_t to = at.b * p.os[0] + at.h * p.os[1] + at.row * p.os[2] + d * p.os[3];
 #pragma unroll
-        for (int wave = 0; wave < CR_WAVES; wave++) m = fmaxf(m, states[(wave * COLS + column) * pitch + pitch - 2]);
-        const float reference = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f;
-        float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int wave = 0; wave < CR_WAVES; wave++) {
-            const float *src = states + (wave * COLS + column) * pitch;
-            const float weight = __builtin_amdgcn_exp2f(src[pitch - 2] - reference);
-            l += weight * src[pitch - 1];
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[e] += weight * src[d + e];
+    for (int e = 0; e < 4; e++) o[e] /= l;  // no visible key: 0 / 0 = NaN
+    const bool f32 = sizeof(T) == 4 || p.out_f32;
+    char *const out = (char *)p.out + to * (f32 ? 4 : 2);
+    if (p.os[3] == 1 && ((uintptr_t)out & (f32 ? 15 : 7)) == 0) {
+        if (f32) {
+            *(float4_t *)out = o;
+        } else if constexpr (sizeof(T) == 2) {
+            const T four[4] = {from_float<T>(o[0]), from_float<T>(o[1]), from_float<T>(o[2]), from_float<T>(o[3])};
+            uint2r_t bits;
+            __builtin_memcpy(&bits, four, 8);
+            *(uint2r_t *)out = bits;
         }
-        const ColumnAt at = column_at(p, w.b, w.g, w.c0 + column);
-        if (p.slots > 1) {
-            float *ws = p.partials + ((((int64_t)at.b * p.H + at.h) * p.Sq + at.row) * p.slots + w.slot) * p.pf_pitch;
-            *(float4_t *)(ws + d) = o;
-            if (d == 0) ws[D] = m, ws[D + 1] = l;
-            continue;
-        }
-        const int64_t to = at.b * p.os[0] + at.h * p.os[1] + at.row * p.os[2] + d * p.os[3];
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] /= l;  // no visible key: 0 / 0 = NaN
-        const bool f32 = sizeof(T) == 4 || p.out_f32;
-        char *const out = (char *)p.out + to * (f32 ? 4 : 2);
-        if (vec && ((uintptr_t)out & (f32 ? 15 : 7)) == 0) {
-            if (f32) {
-                *(float4_t *)out = o;
-            } else if constexpr (sizeof(T) == 2) {
-                const T four[4] = {from_float<T>(o[0]), from_float<T>(o[1]), from_float<T>(o[2]), from_float<T>(o[3])};
-                uint2r_t bits;
-                __builtin_memcpy(&bits, four, 8);
-                *(uint2r_t *)out = bits;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (f32) ((float *)p.out)[to + e * p.os[3]] = o[e];
-                else ((T *)p.out)[to + e * p.os[3]] = from_float<T>(o[e]);
-            }
+        for (int e = 0; e < 4; e++) {
+            if (f32) ((float *)p.out)[to + e * p.os[3]] = o[e];
+            else ((T *)p.out)[to + e * p.os[3]] = from_float<T>(o[e]);
         }
     }
 }
 
-#define CR_LDS(type, at) ((__attribute__((address_space(3))) type *)(lds + (at)))
-
-// DP: head_dim rounded up to a multiple of 32.  The dims behind head_dim read the row's first ones again; Q is zero there, and such dims of
-// the result are not written.
+// A wavefront's columns and their state.  DP: head_dim rounded up to a multiple of 32; Q is zero in the dims behind head_dim, and such dims of the result
+// are not written.
+// Rows that no column sees may hold anything, NaN among it, which 0 x NaN would bring into the result: in tiles with such rows their values are
+// cleared in LDS.
 template <typename T, int DP, int CB>
-__global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_kernel(ContextParams p, ContextRows rows) {
-    request_arguments<ContextParams, ContextRows>();
+struct Columns {
     typedef typename RowsMma<T>::vec8 vec8;
-    constexpr int KEYS = 32, COLS = 16 * CB;
-    constexpr int KP = DP * 2 + 16, VP = DP * 2 + 32;  // row pitches in LDS: 4 and 8 banks apart
-    constexpr int K_BYTES = KEYS * KP, WAVE_BYTES = K_BYTES + KEYS * VP;
-    constexpr int CPR = DP / 8, LOADS = KEYS * CPR / 64;  // 16-byte pieces of a row; loads per lane and tensor
-    constexpr int KB = DP / 32, NB = DP / 16;
-    constexpr int STATE = DP + 2, STATE_BYTES = CR_WAVES * COLS * STATE * 4;
-    __shared__ __attribute__((aligned(16))) char smem[CR_WAVES * WAVE_BYTES > STATE_BYTES ? CR_WAVES * WAVE_BYTES : STATE_BYTES];
-
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 15, q4 = lane >> 4;
-    auto lds = (__attribute__((address_space(3))) char *)smem + wave * WAVE_BYTES;
-    const RowsWork w = rows_work(p, rows);
-    if (w.none) return;
-
-    // the lane's columns and what they see
-    ColumnAt at[CB];
-    ContextRow seen[CB];
-    ContextSpan span;
-    if (w.prefix && p.window == 0) span = ContextSpan{0, 0, p.P};  // (not asked of the sequences' positions, which are a memory latency away)
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-        at[cb] = column_at(p, w.b, w.g, w.c0 + min(j + 16 * cb, w.columns - 1));
-        seen[cb] = context_row(p, at[cb].b, at[cb].row).of(p, w.prefix);
-        if (!(w.prefix && p.window == 0)) {
-            const ContextSpan s = context_span(seen[cb]);
-            if (cb == 0) {
-                span = s;
-            } else {
-                const int lo = s.keys() == 0 ? span.lo : span.keys() == 0 ? s.lo : min(span.lo, s.lo);
-                span.hi = max(span.hi, s.hi), span.first = max(span.first, s.first), span.lo = max(lo, span.first);
-            }
-        }
-    }
-    const int v_lo = w.split * w.chunk, v_hi = w.last ? span.keys() : min(v_lo + w.chunk, span.keys()), first = span.first, gap = span.gap();
-    if (v_lo >= v_hi && p.slots > 1) {
-        park_nothing(p, w);
-        return;
-    }
-    bool alike = true;
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) alike = alike && seen[cb].first >= first && seen[cb].lo <= span.lo && seen[cb].hi >= span.hi;
-    alike = __builtin_amdgcn_ballot_w64(!alike) == 0;  // every column sees the whole share
-
-    const uint16_t *const k = w.prefix ? (const uint16_t *)p.pk + w.g * p.pks[0] : (const uint16_t *)p.k + w.b * p.ks[0] + w.g * p.ks[1];
-    const uint16_t *const v = w.prefix ? (const uint16_t *)p.pv + w.g * p.pvs[0] : (const uint16_t *)p.v + w.b * p.vs[0] + w.g * p.vs[1];
-    const int64_t k_row = w.prefix ? p.pks[1] : p.ks[2], v_row = w.prefix ? p.pvs[1] : p.vs[2];
-
+    static constexpr int KEYS = 32;
+    static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 32;  // row pitches in LDS: 4 and 8 banks apart
+    static constexpr int KB = DP / 32, NB = DP / 16;
+    vec8 q[CB][KB];
     float4_t o[CB][NB];
     float m[CB], l[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++) o[cb][nb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        m[cb] = -INFINITY, l[cb] = 0.0f;
-    }
-
-    // Visible keys are numbered v; the tile behind the one in LDS is on its way in registers.  Rows behind the share's last key repeat it.
-    uint4_t kst[LOADS], vst[LOADS];
-    auto load_tile = [&](int base) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < LOADS; u++) {
-            const int piece = lane + 64 * u, row = piece / CPR, col = 8 * (piece % CPR), x = min(base + row, v_hi - 1);
-            const int key = x + (x >= first ? gap : 0), dim = col < p.D ? col : 0;
-            kst[u] = __builtin_nontemporal_load((const uint4_t *)(k + key * k_row + dim));
-            vst[u] = __builtin_nontemporal_load((const uint4_t *)(v + key * v_row + dim));
-        }
-    };
-    auto store_tile = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < LOADS; u++) {
-            const int piece = lane + 64 * u, row = piece / CPR, col = piece % CPR;
-            *CR_LDS(uint4_t, row * KP + col * 16) = kst[u];
-            *CR_LDS(uint4_t, K_BYTES + row * VP + col * 16) = vst[u];
-        }
-    };
+    ContextRow seen[CB];
 
     // Q^T operand: column j, dims 32 kb + 8 q4 .. + 7
-    vec8 q[CB][KB];
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-        const uint16_t *from = (const uint16_t *)p.q + at[cb].b * p.qs[0] + at[cb].h * p.qs[1] + at[cb].row * p.qs[2];
+    __device__ __forceinline__ void load_q(const ContextParams &p, int cb, const ColumnAt &at, bool used, int q4) {
+        const uint16_t *from = (const uint16_t *)p.q + at.b * p.qs[0] + at.h * p.qs[1] + at.row * p.qs[2];
         const bool whole = p.qs[3] == 1 && ((uintptr_t)from & 15) == 0;
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
             const int dim = 32 * kb + 8 * q4;
             uint4_t raw = {0, 0, 0, 0};
-            if (j + 16 * cb < w.columns && dim < p.D) {
+            if (used && dim < p.D) {
                 if (whole) {
                     raw = *(const uint4_t *)(from + dim);
                 } else {
@@ -281,17 +195,17 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
             q[cb][kb] = __builtin_bit_cast(vec8, raw);
         }
     }
-    const float scale2 = p.scale * CONTEXT_LOG2E;
-
-    constexpr int STEP = CR_WAVES * KEYS;
-    int base = v_lo + wave * KEYS;
-    if (base < v_hi) load_tile(base);
-    for (; base < v_hi; base += STEP) {
-        wave_lds_sync();  // the previous step's reads precede these writes
-        store_tile();
-        wave_lds_sync();
-        if (base + STEP < v_hi) load_tile(base + STEP);
-
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int cb = 0; cb < CB; cb++) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) o[cb][nb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            m[cb] = -INFINITY, l[cb] = 0.0f;
+        }
+    }
+    // The tile of visible keys base .. in LDS; whole: every column sees all of it.
+    __device__ __forceinline__ void step(lds_t k, lds_t v, int base, int end, int first, int gap, bool whole, float scale2, int lane) {
+        const int j = lane & 15, q4 = lane >> 4;
         float4_t s[CB][2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -299,13 +213,12 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
             for (int cb = 0; cb < CB; cb++) s[cb][t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
-                const uint4_t raw = *CR_LDS(uint4_t, (16 * t + j) * KP + (32 * kb + 8 * q4) * 2);
+                const uint4_t raw = *CR_LDS(uint4_t, k + (16 * t + j) * KP + (32 * kb + 8 * q4) * 2);
 #pragma unroll
                 for (int cb = 0; cb < CB; cb++) s[cb][t] = RowsMma<T>::mfma(__builtin_bit_cast(vec8, raw), q[cb][kb], s[cb][t]);
             }
         }
         vec8 weights[CB];
-        const bool whole = alike && base + KEYS <= v_hi;
         uint32_t used = 0;  // the lane's keys that some column sees
 #pragma unroll
         for (int cb = 0; cb < CB; cb++) {
@@ -317,7 +230,7 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int n = base + 16 * (e >> 2) + 4 * q4 + (e & 3), key = n + (n >= first ? gap : 0);
-                    const bool sees = n < v_hi && key < seen[cb].hi && (key >= seen[cb].lo || key < seen[cb].first);
+                    const bool sees = n < end && key < seen[cb].hi && (key >= seen[cb].lo || key < seen[cb].first);
                     x[e] = sees ? x[e] : -INFINITY;
                     used |= sees ? 1u << e : 0u;
                 }
@@ -349,11 +262,11 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
             used = any_column(used);
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (!(used >> e & 1)) clear_row<DP * 2>(lds + K_BYTES + (16 * (e >> 2) + 4 * q4 + (e & 3)) * VP, j);
+                if (!(used >> e & 1)) clear_row<DP * 2>(v + (16 * (e >> 2) + 4 * q4 + (e & 3)) * VP, j);
             wave_lds_sync();
         }
         // the transposing load hands lane i of 16 V[row .. row + 3][dim + i]
-        const int v_at = K_BYTES + (4 * q4 + (j >> 2)) * VP + 8 * (j & 3);
+        const lds_t v_at = v + (4 * q4 + (j >> 2)) * VP + 8 * (j & 3);
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             const short4_t a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(CR_LDS(short4_t, v_at + nb * 32));
@@ -364,113 +277,41 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
             for (int cb = 0; cb < CB; cb++) o[cb][nb] = RowsMma<T>::mfma(values, weights[cb], o[cb][nb]);
         }
     }
-
-    __syncthreads();  // the states take the tiles' place
-    float *const states = (float *)smem;
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
+    // dims of column 16 cb + j to `to`, [DP], then the reference and the sum
+    __device__ __forceinline__ void park(float *to, int cb, int q4) {
         const float sum = column_sum(l[cb]);
-        float *const to = states + (wave * COLS + j + 16 * cb) * STATE;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int r = 0; r < 4; r++) to[16 * nb + 4 * q4 + r] = o[cb][nb][r];
         if (q4 == 0) to[DP] = m[cb], to[DP + 1] = sum;
     }
-    __syncthreads();
-    join_waves<T, COLS>(p, w, states, STATE);
-}
+};
 
-// The same for f32 tensors: 16 keys per wavefront and step.  Contraction slot (c, i, q4) of K Q^T is dim 16 c + 4 q4 + i, so that one 16-byte read of
-// a row feeds four matrix steps; slot (i, q4) of V^T P^T is key 4 q4 + i, whose weight the lane already holds, and row n of output block (nb, e)
-// is dim 16 VW nb + VW n + e, so that one read of a row feeds VW steps.  The step's share of O forms on its own and is added once (one
-// rounding at the size of the sum).
+// The same for f32 tensors: 16 keys per tile.  Contraction slot (c, i, q4) of K Q^T is dim 16 c + 4 q4 + i, so that one 16-byte read of a row feeds
+// four matrix steps; slot (i, q4) of V^T P^T is key 4 q4 + i, whose weight the lane already holds, and row n of output block (nb, e) is dim
+// 16 VW nb + VW n + e, so that one read of a row feeds VW steps.  The tile's share of O forms on its own and is added once (one rounding at the
+// size of the sum).
 template <int DP, int CB>
-__global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_f32_kernel(ContextParams p, ContextRows rows) {
-    request_arguments<ContextParams, ContextRows>();
-    constexpr int KEYS = 16, COLS = 16 * CB;
-    constexpr int KP = DP * 4 + 16, K_BYTES = KEYS * KP, WAVE_BYTES = 2 * K_BYTES;
-    constexpr int CPR = DP / 4, LOADS = KEYS * CPR / 64, KC = DP / 16, VW = DP % 64 == 0 ? 4 : 2, NB = DP / (16 * VW);
-    constexpr int STATE = DP + 2, STATE_BYTES = CR_WAVES * COLS * STATE * 4;
+struct Columns<float, DP, CB> {
+    static constexpr int KEYS = 16;
+    static constexpr int KP = DP * 4 + 16, VP = KP;
+    static constexpr int KC = DP / 16, VW = DP % 64 == 0 ? 4 : 2, NB = DP / (16 * VW);
     typedef float vrow_t __attribute__((ext_vector_type(VW)));
-    __shared__ __attribute__((aligned(16))) char smem[CR_WAVES * WAVE_BYTES > STATE_BYTES ? CR_WAVES * WAVE_BYTES : STATE_BYTES];
-
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 15, q4 = lane >> 4;
-    auto lds = (__attribute__((address_space(3))) char *)smem + wave * WAVE_BYTES;
-    const RowsWork w = rows_work(p, rows);
-    if (w.none) return;
-
-    ColumnAt at[CB];
-    ContextRow seen[CB];
-    ContextSpan span;
-    if (w.prefix && p.window == 0) span = ContextSpan{0, 0, p.P};
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-        at[cb] = column_at(p, w.b, w.g, w.c0 + min(j + 16 * cb, w.columns - 1));
-        seen[cb] = context_row(p, at[cb].b, at[cb].row).of(p, w.prefix);
-        if (!(w.prefix && p.window == 0)) {
-            const ContextSpan s = context_span(seen[cb]);
-            if (cb == 0) {
-                span = s;
-            } else {
-                const int lo = s.keys() == 0 ? span.lo : span.keys() == 0 ? s.lo : min(span.lo, s.lo);
-                span.hi = max(span.hi, s.hi), span.first = max(span.first, s.first), span.lo = max(lo, span.first);
-            }
-        }
-    }
-    const int v_lo = w.split * w.chunk, v_hi = w.last ? span.keys() : min(v_lo + w.chunk, span.keys()), first = span.first, gap = span.gap();
-    if (v_lo >= v_hi && p.slots > 1) {
-        park_nothing(p, w);
-        return;
-    }
-    bool alike = true;
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) alike = alike && seen[cb].first >= first && seen[cb].lo <= span.lo && seen[cb].hi >= span.hi;
-    alike = __builtin_amdgcn_ballot_w64(!alike) == 0;
-
-    const float *const k = w.prefix ? (const float *)p.pk + w.g * p.pks[0] : (const float *)p.k + w.b * p.ks[0] + w.g * p.ks[1];
-    const float *const v = w.prefix ? (const float *)p.pv + w.g * p.pvs[0] : (const float *)p.v + w.b * p.vs[0] + w.g * p.vs[1];
-    const int64_t k_row = w.prefix ? p.pks[1] : p.ks[2], v_row = w.prefix ? p.pvs[1] : p.vs[2];
-
+    float4_t q[CB][KC];
     float4_t o[CB][NB][VW];
     float m[CB], l[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-            for (int e = 0; e < VW; e++) o[cb][nb][e] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        m[cb] = -INFINITY, l[cb] = 0.0f;
-    }
-    float4_t kst[LOADS], vst[LOADS];
-    auto load_tile = [&](int base) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < LOADS; u++) {
-            const int piece = lane + 64 * u, row = piece / CPR, col = 4 * (piece % CPR), x = min(base + row, v_hi - 1);
-            const int key = x + (x >= first ? gap : 0), dim = col < p.D ? col : 0;
-            kst[u] = __builtin_nontemporal_load((const float4_t *)(k + key * k_row + dim));
-            vst[u] = __builtin_nontemporal_load((const float4_t *)(v + key * v_row + dim));
-        }
-    };
-    auto store_tile = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < LOADS; u++) {
-            const int piece = lane + 64 * u, row = piece / CPR, col = piece % CPR;
-            *CR_LDS(float4_t, row * KP + col * 16) = kst[u];
-            *CR_LDS(float4_t, K_BYTES + row * KP + col * 16) = vst[u];
-        }
-    };
+    ContextRow seen[CB];
+
     // Q^T operand: column j, dims 16 c + 4 q4 .. + 3
-    float4_t q[CB][KC];
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-        const float *from = (const float *)p.q + at[cb].b * p.qs[0] + at[cb].h * p.qs[1] + at[cb].row * p.qs[2];
+    __device__ __forceinline__ void load_q(const ContextParams &p, int cb, const ColumnAt &at, bool used, int q4) {
+        const float *from = (const float *)p.q + at.b * p.qs[0] + at.h * p.qs[1] + at.row * p.qs[2];
         const bool whole = p.qs[3] == 1 && ((uintptr_t)from & 15) == 0;
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const int dim = 16 * c + 4 * q4;
             q[cb][c] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            if (j + 16 * cb < w.columns && dim < p.D) {
+            if (used && dim < p.D) {
                 if (whole) {
                     q[cb][c] = *(const float4_t *)(from + dim);
                 } else {
@@ -480,30 +321,30 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
             }
         }
     }
-    const float scale2 = p.scale * CONTEXT_LOG2E;
-
-    constexpr int STEP = CR_WAVES * KEYS;
-    int base = v_lo + wave * KEYS;
-    if (base < v_hi) load_tile(base);
-    for (; base < v_hi; base += STEP) {
-        wave_lds_sync();
-        store_tile();
-        wave_lds_sync();
-        if (base + STEP < v_hi) load_tile(base + STEP);
-
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int cb = 0; cb < CB; cb++) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int e = 0; e < VW; e++) o[cb][nb][e] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            m[cb] = -INFINITY, l[cb] = 0.0f;
+        }
+    }
+    __device__ __forceinline__ void step(lds_t k, lds_t v, int base, int end, int first, int gap, bool whole, float scale2, int lane) {
+        const int j = lane & 15, q4 = lane >> 4;
         float4_t s[CB];
 #pragma unroll
         for (int cb = 0; cb < CB; cb++) s[cb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < KC; c++) {
-            const float4_t a = *CR_LDS(float4_t, j * KP + (16 * c + 4 * q4) * 4);
+            const float4_t a = *CR_LDS(float4_t, k + j * KP + (16 * c + 4 * q4) * 4);
 #pragma unroll
             for (int cb = 0; cb < CB; cb++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) s[cb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], q[cb][c][i], s[cb], 0, 0, 0);
         }
         float x[CB][4];
-        const bool whole = alike && base + KEYS <= v_hi;
         uint32_t used = 0;
 #pragma unroll
         for (int cb = 0; cb < CB; cb++) {
@@ -514,7 +355,7 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int n = base + 4 * q4 + r, key = n + (n >= first ? gap : 0);
-                    const bool sees = n < v_hi && key < seen[cb].hi && (key >= seen[cb].lo || key < seen[cb].first);
+                    const bool sees = n < end && key < seen[cb].hi && (key >= seen[cb].lo || key < seen[cb].first);
                     x[cb][r] = sees ? x[cb][r] : -INFINITY;
                     used |= sees ? 1u << r : 0u;
                 }
@@ -542,14 +383,14 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
             used = any_column(used);
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                if (!(used >> r & 1)) clear_row<DP * 4>(lds + K_BYTES + (4 * q4 + r) * KP, j);
+                if (!(used >> r & 1)) clear_row<DP * 4>(v + (4 * q4 + r) * VP, j);
             wave_lds_sync();
         }
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             vrow_t a[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) a[i] = *CR_LDS(vrow_t, K_BYTES + (4 * q4 + i) * KP + (16 * VW * nb + VW * j) * 4);
+            for (int i = 0; i < 4; i++) a[i] = *CR_LDS(vrow_t, v + (4 * q4 + i) * VP + (16 * VW * nb + VW * j) * 4);
 #pragma unroll
             for (int cb = 0; cb < CB; cb++)
 #pragma unroll
@@ -561,13 +402,8 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
                 }
         }
     }
-
-    __syncthreads();
-    float *const states = (float *)smem;
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
+    __device__ __forceinline__ void park(float *to, int cb, int q4) {
         const float sum = column_sum(l[cb]);
-        float *const to = states + (wave * COLS + j + 16 * cb) * STATE;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -576,8 +412,132 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
                 for (int r = 0; r < 4; r++) to[16 * VW * nb + VW * (4 * q4 + r) + e] = o[cb][nb][e][r];
         if (q4 == 0) to[DP] = m[cb], to[DP + 1] = sum;
     }
+};
+
+// CB: blocks of 16 columns
+template <typename T, int DP, int CB>
+__global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_kernel(ContextParams p, ContextRows rows) {
+    request_arguments<ContextParams, ContextRows>();
+    typedef Columns<T, DP, CB> C;
+    constexpr int KEYS = C::KEYS, COLS = 16 * CB, ES = sizeof(T), STEP = CR_WAVES * KEYS;
+    constexpr int PER = 16 / ES, CPR = DP / PER, LOADS = KEYS * CPR / 64;  // elements of a 16-byte piece, pieces of a row, loads per lane and tensor
+    constexpr bool RUNS = 64 % CPR == 0 && ES == 2;
+    constexpr int WAVE_BYTES = KEYS * (C::KP + C::VP), STATE = DP + 2, STATE_BYTES = CR_WAVES * COLS * STATE * 4;
+    __shared__ __attribute__((aligned(16))) char smem[CR_WAVES * WAVE_BYTES > STATE_BYTES ? CR_WAVES * WAVE_BYTES : STATE_BYTES];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane & 15, q4 = lane >> 4;
+    const lds_t k_tile = (lds_t)smem + wave * WAVE_BYTES, v_tile = k_tile + KEYS * C::KP;
+    const RowsWork w = rows_work(p, rows);
+    if (w.none) return;
+
+    // the lane's columns and what they see
+    C columns;
+    ContextSpan span = {0, 0, p.P};  // (of a prefix without a window: not asked of the sequences' positions, which are a memory latency away)
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++) {
+        const ColumnAt at = column_at(p, w.b, w.g, w.c0 + min(j + 16 * cb, w.columns - 1));
+        columns.load_q(p, cb, at, j + 16 * cb < w.columns, q4);
+        columns.seen[cb] = context_row(p, at.b, at.row).of(p, w.prefix);
+        if (!(w.prefix && p.window == 0)) {
+            const ContextSpan s = context_span(columns.seen[cb]);
+            if (cb == 0) {
+                span = s;
+            } else {
+                const int lo = s.keys() == 0 ? span.lo : span.keys() == 0 ? s.lo : min(span.lo, s.lo);
+                span.hi = max(span.hi, s.hi), span.first = max(span.first, s.first), span.lo = max(lo, span.first);
+            }
+        }
+    }
+    const int first = span.first, gap = span.gap(), v_lo = w.split * w.chunk, v_hi = w.last ? span.keys() : min(v_lo + w.chunk, span.keys());
+    if (v_lo >= v_hi && p.slots > 1) {
+        park_nothing(p, w);
+        return;
+    }
+    bool alike = true;
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++)
+        alike = alike && columns.seen[cb].first >= first && columns.seen[cb].lo <= span.lo && columns.seen[cb].hi >= span.hi;
+    alike = __builtin_amdgcn_ballot_w64(!alike) == 0;  // every column sees the whole share
+    columns.clear();
+
+    const T *const k = w.prefix ? (const T *)p.pk + w.g * p.pks[0] : (const T *)p.k + w.b * p.ks[0] + w.g * p.ks[1];
+    const T *const v = w.prefix ? (const T *)p.pv + w.g * p.pvs[0] : (const T *)p.v + w.b * p.vs[0] + w.g * p.vs[1];
+    const int64_t k_row = (w.prefix ? p.pks[1] : p.ks[2]) * ES, v_row = (w.prefix ? p.pvs[1] : p.vs[2]) * ES;  // bytes
+
+    // The tile behind the one in LDS is on its way in registers.  A tile's rows are a buffer that starts at its first and ends with the share's last key:
+    // what lies behind reads as zero, without a clamp or an address per lane.  Rows that a load does not divide evenly, f32 rows (whose two forms
+    // together spill at 32 columns), rows far apart and the one tile within which the first tokens end have an address per lane, with the last
+    // key again behind it.
+    const int row = lane / CPR, col = lane % CPR;
+    const bool inside = col * PER < p.D, far = (uint64_t)k_row > CR_FAR || (uint64_t)v_row > CR_FAR;
+    const uint32_t k_at = inside ? row * (uint32_t)k_row + col * 16 : 0x7ffffff0u, v_at = inside ? row * (uint32_t)v_row + col * 16 : 0x7ffffff0u;
+    constexpr int ROWS = 64 / CPR;  // of a load
+    uint4_t kst[LOADS], vst[LOADS];
+    auto load_tile = [&](int base) __attribute__((always_inline)) {
+        if (!RUNS || far || (base < first && base + KEYS > first)) {
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                const int piece = lane + 64 * u, x = min(base + piece / CPR, v_hi - 1), dim = piece % CPR * PER < p.D ? piece % CPR * PER : 0;
+                const int64_t key = x + (x >= first ? gap : 0);
+                kst[u] = __builtin_nontemporal_load((const uint4_t *)((const char *)(k + dim) + key * k_row));
+                vst[u] = __builtin_nontemporal_load((const uint4_t *)((const char *)(v + dim) + key * v_row));
+            }
+        } else {
+            const int64_t key = base + (base >= first ? gap : 0);
+            const int left = min(v_hi - base, KEYS) - 1;
+            auto rows_from = [&](const T *from, int64_t bytes) __attribute__((always_inline)) {
+                const uint64_t at = (uint64_t)((const char *)from + key * bytes);
+                const uint32_t low = __builtin_amdgcn_readfirstlane((int)(uint32_t)at), high = __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32));
+                return __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)high << 32 | low), 0, __builtin_amdgcn_readfirstlane(left * (int)bytes + p.D * ES),
+                                                         0x00020000);
+            };
+            const auto k_rows = rows_from(k, k_row), v_rows = rows_from(v, v_row);
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                kst[u] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(k_rows, k_at + u * ROWS * (uint32_t)k_row, 0, CR_NT));
+                vst[u] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(v_rows, v_at + u * ROWS * (uint32_t)v_row, 0, CR_NT));
+            }
+        }
+    };
+    const float scale2 = p.scale * CONTEXT_LOG2E;
+    int base = v_lo + wave * KEYS;
+    if (base < v_hi) load_tile(base);
+    for (; base < v_hi; base += STEP) {
+        wave_lds_sync();  // the previous tile's reads precede these writes
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) {
+            const int piece = lane + 64 * u;
+            *CR_LDS(uint4_t, k_tile + piece / CPR * C::KP + piece % CPR * 16) = kst[u];
+            *CR_LDS(uint4_t, v_tile + piece / CPR * C::VP + piece % CPR * 16) = vst[u];
+        }
+        wave_lds_sync();
+        if (base + STEP < v_hi) load_tile(base + STEP);
+        columns.step(k_tile, v_tile, base, v_hi, first, gap, alike && base + KEYS <= v_hi, scale2, lane);
+    }
+
+    __syncthreads();  // the states take the tiles' place
+    float *const states = (float *)smem;
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++) columns.park(states + (wave * COLS + j + 16 * cb) * STATE, cb, q4);
     __syncthreads();
-    join_waves<float, COLS>(p, w, states, STATE);
+    const int pieces = p.D / 4;
+    for (int i = threadIdx.x; i < w.columns * pieces; i += 64 * CR_WAVES) {
+        const int column = i / pieces, d = 4 * (i - column * pieces);
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int x = 0; x < CR_WAVES; x++) m = fmaxf(m, states[(x * COLS + column) * STATE + DP]);
+        const float reference = m == -INFINITY ? 0.0f : m;
+        float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < CR_WAVES; x++) {
+            const float *src = states + (x * COLS + column) * STATE;
+            const float weight = __builtin_amdgcn_exp2f(src[DP] - reference);
+            l += weight * src[DP + 1];
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] += weight * src[d + e];
+        }
+        write_column<T>(p, w, w.c0 + column, d, m, l, o);
+    }
 }
 
 // ---- shares ---------------------------------------------------------------------------------------------------------------------------
@@ -714,8 +674,7 @@ static bool launch_rows_dims(const ContextParams &p, const ContextRows &rows, hi
     const dim3 grid((unsigned)rows.total), block(64 * CR_WAVES);
     auto run = [&](auto dims) {
         constexpr int DP = decltype(dims)::value;
-        if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((context_rows_f32_kernel<DP, CB>), grid, block, 0, stream, p, rows);
-        else hipLaunchKernelGGL((context_rows_kernel<T, DP, CB>), grid, block, 0, stream, p, rows);
+        hipLaunchKernelGGL((context_rows_kernel<T, DP, CB>), grid, block, 0, stream, p, rows);
         return true;
     };
     using std::integral_constant;
