@@ -20,25 +20,67 @@ static int64_t part_keys(const ContextParams &p, bool prefix) {
     if (prefix) return p.q_positions ? (int64_t)p.P : most_visible(p, p.P, p.Sq, p.sinks);
     return most_visible(p, p.Skv, p.Sq, std::max<int64_t>((int64_t)p.sinks - p.P, 0));
 }
-static ContextRowsJob rows_job(const ContextParams &p, bool prefix, int columns, int step, int64_t target) {
-    ContextRowsJob job;
-    job.prefix = prefix;
-    job.units = prefix ? p.Hkv : p.B * p.Hkv;
-    job.blocks = (int32_t)div_up((int64_t)(prefix ? p.B : 1) * p.G * p.Sq, columns);
-    const int64_t keys = part_keys(p, prefix);
-    const int64_t workgroups = (int64_t)job.units * job.blocks;
-    int64_t shares = std::min(div_up(target, std::max<int64_t>(workgroups, 1)), div_up(keys, step));
-    shares = std::max(shares, div_up(keys, 1024));
-    shares = std::max<int64_t>(shares, 1);
-    job.chunk = (int32_t)(div_up(div_up(keys, shares), step) * step);
-    job.chunk = std::max(job.chunk, step);
-    job.nsplit = (int32_t)std::max<int64_t>(div_up(keys, job.chunk), 1);
-    job.slot0 = 0;
-    return job;
-}
-static int64_t workgroups_of(const ContextRowsJob &job) {
-    const int64_t shares = (int64_t)job.units * job.nsplit;
-    return job.blocks == 1 ? shares : div_up(shares, 8) * 8 * job.blocks;
+// Writing shares' results and reading them again.
+static double partials_us(const ContextParams &p, int64_t slots) { return 0.488e-6 * (double)p.B * p.H * p.Sq * (double)slots * (p.D + 4) * sizeof(float); }
+
+// The launch for few rows: its jobs and their shares, and its time in us with the merge's.
+struct RowsPlan {
+    ContextRows rows;
+    int64_t slots;
+    double us;
+};
+static RowsPlan rows_launch(const ContextParams &p, fhip_dtype dtype, bool with_prefix, int64_t slots_before) {
+    const int64_t each = (int64_t)p.G * p.Sq, most = each * (with_prefix ? p.B : 1);
+    const bool f32 = dtype == FHIP_F32, two = most > 16 && p.D <= 128;
+    const int columns = two ? 32 : 16, step = f32 ? 64 : 128, size = f32 ? 4 : 2;
+    // Fitted to 101 calls at six lengths of the shares each; the shares it picks are 2 per cent slower than each call's best in the mean, 12 at most.
+    // A step of a workgroup, what all of them take in from the caches (f32 with 32 columns: as the matrix cores take it) and from memory, bytes per us,
+    // and workgroups per CU.  Where sequences differ in length, 0.3 of the longest share is left over at the end.
+    const double step_us = !f32 ? 0.35 + 0.0063 * p.D : two ? 0.20 + 0.0208 * p.D : 0.24 + 0.0119 * p.D;
+    const double cached = f32 ? (two ? 5.1e6 : 10e6) : 10.8e6, memory = 6.2e6;
+    const int64_t at_once = (int64_t)p.cus * (p.D > 128 ? 1 : p.D > 64 ? 2 : 3);
+    RowsPlan best;
+    memset(&best, 0, sizeof(best));  // (us 0: too many workgroups for a launch)
+    for (int steps = 1; steps <= 8; steps++) {
+        RowsPlan plan;
+        memset(&plan, 0, sizeof(plan));
+        plan.rows.columns = columns;
+        plan.slots = slots_before;
+        const int64_t chunk = (int64_t)steps * step;
+        int64_t total = 0, workgroups = 0, all_steps = 0, longest = 0;
+        double taken = 0.0, read = 0.0;
+        int jobs = 0;
+        for (const bool prefix : {true, false}) {
+            if (prefix ? !with_prefix : p.Skv == 0) continue;
+            ContextRowsJob &job = plan.rows.job[jobs];
+            const int64_t keys = part_keys(p, prefix);
+            job.prefix = prefix;
+            job.units = prefix ? p.Hkv : p.B * p.Hkv;
+            job.blocks = (int32_t)div_up(prefix ? most : each, columns);
+            job.chunk = (int32_t)chunk;
+            job.nsplit = (int32_t)std::max<int64_t>(div_up(keys, chunk), 1);
+            job.slot0 = (int32_t)plan.slots;
+            plan.slots += job.nsplit;
+            const int64_t shares = (int64_t)job.units * job.nsplit;
+            if (jobs++ == 1) plan.rows.second = (int32_t)total;
+            total += job.blocks == 1 ? shares : div_up(shares, 8) * 8 * job.blocks;
+            const int64_t walked = std::max<int64_t>(std::min<int64_t>(div_up(keys, step), steps), 1);
+            workgroups += shares * job.blocks;
+            all_steps += shares * job.blocks * walked;
+            longest = std::max(longest, walked);
+            taken += (double)job.units * job.blocks * keys * p.D * 2 * size;
+            read += (double)job.units * keys * p.D * 2 * size;
+        }
+        if (total > 0x7fffffff) continue;
+        if (jobs == 1) plan.rows.second = (int32_t)total;
+        plan.rows.total = (int32_t)total;
+        const double last = step_us * (double)longest, shared = f32 && two ? std::min(std::max((double)workgroups / p.cus, 1.0), 1.25) : 1.0;
+        plan.us = 2.7 + (double)div_up(workgroups, at_once) * (p.D > 128 ? 4.5 : 2.8) + (p.kv_lens || p.P > 0 ? 0.3 * last : 0.0) +
+                  std::max({shared * last, step_us * (double)all_steps / (double)at_once, taken / cached, read / memory});
+        if (plan.slots > 1) plan.us += 1.5 + partials_us(p, plan.slots - slots_before);
+        if (best.us == 0.0 || plan.us < best.us) best = plan;
+    }
+    return best;
 }
 
 // Time of a launch of the 16-bit kernels in us, from the constants of prefill_mfma_time (attn_prefill_mfma.hip) and prefill_wide_time
@@ -49,7 +91,7 @@ static double tiles_time(const ContextParams &p, const ContextTilesLaunch &how, 
     const double dims = p.D <= 64 ? 1.0 : p.D <= 96 ? 1.43 : 1.86, tiles = (double)div_up(div_up(keys, how.shares), 64);
     return 4.6 + rounds * (how.rows_per_group == 128 ? 5.3 + 0.356 * dims * tiles : 3.9 + 0.579 * dims * tiles);
 }
-static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype, bool fold, bool with_prefix, bool with_own, bool parked) {
+static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype, bool fold, bool with_prefix, bool with_own, bool parked, double *time) {
     const bool f32 = dtype == FHIP_F32, both = with_prefix && with_own;
     const int tile = f32 || p.D > 128 ? 32 : 64;
     // (rows per workgroup, key groups); to head_dim 128 the 16-bit form of 128 rows takes one part
@@ -83,11 +125,12 @@ static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype,
             } else {
                 us = tiles_time(p, how, keys);
             }
-            if (how.shares > 1 || parked) us += 0.488e-6 * (double)p.B * p.H * p.Sq * how.shares * (p.D + 4) * sizeof(float);
+            if (how.shares > 1 || parked) us += partials_us(p, how.shares);
             if (how.shares > 1 && !parked) us += 3.0;
             if (least == 0.0 || us < 0.98 * least) least = us, best = how;
         }
     }
+    *time = least;
     return best;
 }
 
@@ -102,42 +145,35 @@ ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     const bool can_fold = p.P > 0 && p.B > 1 && (p.window == 0 || !p.q_positions);
     const bool own_by_rows = !tiles || each <= (dtype == FHIP_F32 ? 64 : 32);
     const bool one_part = dtype != FHIP_F32 && p.D > 128;  // the tiled kernel takes one part per launch
-    bool prefix_by_rows = p.P > 0 && (!tiles || (own_by_rows && (each * p.B <= (dtype == FHIP_F32 ? 64 : 32) || !can_fold)));
     int64_t slots = 0;
+    double us = 0.0;
     auto add_tiles = [&](bool fold, bool with_prefix, bool with_own, bool parked) {
+        double time;
         ContextTilesLaunch &how = plan.tiles[plan.tile_launches++];
-        how = tiles_launch(p, dtype, fold, with_prefix, with_own, parked);
+        how = tiles_launch(p, dtype, fold, with_prefix, with_own, parked, &time);
         how.slot0 = (int32_t)slots;
         slots += how.shares;
+        us += time;
     };
-    if (p.P > 0 && !prefix_by_rows) {
-        if (own_by_rows) add_tiles(p.B > 1, true, false, p.Skv > 0);
-        else if ((can_fold && each < 128) || (one_part && p.Skv > 0))
-            add_tiles(can_fold, true, false, true), add_tiles(false, false, true, true);
-        else add_tiles(false, true, p.Skv > 0, false);
-    } else if (!own_by_rows) {
-        add_tiles(false, false, true, false);
-    }
     if (own_by_rows) {
-        ContextRows &rows = plan.rows;
-        const int64_t most = each * (prefix_by_rows ? p.B : 1);
-        rows.columns = most > 16 && p.D <= 128 ? 32 : 16;
-        const int step = dtype == FHIP_F32 ? 64 : 128;
-        const int64_t target = (int64_t)p.cus * (p.D > 128 ? 1 : 2);
-        int jobs = 0;
-        int64_t total = 0;
-        for (const bool prefix : {true, false}) {
-            if (prefix ? !prefix_by_rows : p.Skv == 0) continue;
-            ContextRowsJob job = rows_job(p, prefix, rows.columns, step, target);
-            job.slot0 = (int32_t)slots;
-            slots += job.nsplit;
-            if (jobs == 1) rows.second = (int32_t)total;
-            rows.job[jobs++] = job;
-            total += workgroups_of(job);
+        RowsPlan rows = rows_launch(p, dtype, p.P > 0, 0);
+        if (rows.us == 0.0) return plan;
+        if (p.P > 0 && tiles && can_fold) {
+            // rows of all sequences on the prefix: with the own keys' launch, or on tiles in one of their own
+            add_tiles(true, true, false, p.Skv > 0);
+            const RowsPlan own = rows_launch(p, dtype, false, slots);
+            if (p.Skv > 0) us += own.us;
+            if (us < rows.us) {
+                rows = own;
+            } else {
+                plan.tile_launches = 0, slots = 0;
+            }
         }
-        if (jobs == 1) rows.second = (int32_t)total;
-        if (total > 0x7fffffff) return plan;
-        rows.total = (int32_t)total;
+        if (plan.tile_launches == 0 || p.Skv > 0) plan.rows = rows.rows, slots = rows.slots;
+    } else if (p.P > 0 && ((can_fold && each < 128) || (one_part && p.Skv > 0))) {
+        add_tiles(can_fold, true, false, true), add_tiles(false, false, true, true);
+    } else {
+        add_tiles(false, p.P > 0, p.Skv > 0, false);
     }
     for (int i = 0; i < plan.tile_launches; i++) {
         const ContextTilesLaunch &how = plan.tiles[i];
