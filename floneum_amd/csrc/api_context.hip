@@ -111,6 +111,15 @@ static void fill_context(const fhip_context_attn_args *a, int cus, ContextParams
     p->cus = cus > 0 ? cus : 256;
 }
 
+static int run_plan(ContextParams &p, const ContextPlan &plan, fhip_dtype dtype, hipStream_t stream) {
+    if (plan.any) return launch_context_any(p, dtype, stream);
+    p.slots = plan.slots;
+    int rc = FHIP_OK;
+    for (int i = 0; i < plan.tile_launches && !rc; i++) rc = launch_context_tiles(p, plan.tiles[i], dtype, stream);
+    if (!rc && plan.rows.total) rc = launch_context_rows(p, plan.rows, dtype, stream);
+    return rc || plan.slots == 1 ? rc : launch_context_merge(p, dtype, stream);
+}
+
 }  // namespace fhip
 
 using namespace fhip;
@@ -127,7 +136,7 @@ int fhip_context_attention_workspace_bytes(const fhip_context_attn_args *args, i
     if (args->k.shape[2] == 0 && args->prefix_k.shape[2] == 0) return FHIP_OK;
     ContextParams p;
     fill_context(args, compute_units, &p);
-    *bytes = context_plan(p, args->dtype).bytes;
+    *bytes = context_call(p, args->dtype).bytes;
     return FHIP_OK;
 }
 
@@ -142,17 +151,20 @@ int fhip_context_attention(fhip_stream *s, const fhip_context_attn_args *args) {
     }
     ContextParams p;
     fill_context(args, s->dev->prop.multiProcessorCount, &p);
-    const ContextPlan plan = context_plan(p, args->dtype);
-    if (plan.any) return launch_context_any(p, args->dtype, s->s);
-    if (plan.bytes && (!args->workspace || ((uintptr_t)args->workspace & 15) != 0 || args->workspace_bytes < plan.bytes)) {
-        set_error("context_attention: needs %zu bytes of 16-byte aligned workspace, got %zu", plan.bytes, args->workspace ? args->workspace_bytes : 0);
+    const ContextCall call = context_call(p, args->dtype);
+    if (call.bytes && (!args->workspace || ((uintptr_t)args->workspace & 15) != 0 || args->workspace_bytes < call.bytes)) {
+        set_error("context_attention: needs %zu bytes of 16-byte aligned workspace, got %zu", call.bytes, args->workspace ? args->workspace_bytes : 0);
         return FHIP_ERR_WORKSPACE;
     }
-    p.partials = (float *)args->workspace;
-    p.slots = plan.slots, p.pf_pitch = p.D + 4;
-    for (int i = 0; i < plan.tile_launches && !rc; i++) rc = launch_context_tiles(p, plan.tiles[i], args->dtype, s->s);
-    if (!rc && plan.rows.total) rc = launch_context_rows(p, plan.rows, args->dtype, s->s);
-    return rc || plan.slots == 1 ? rc : launch_context_merge(p, args->dtype, s->s);
+    p.partials = (float *)args->workspace, p.pf_pitch = p.D + 4;
+    for (int i = 0; i < call.parts && !rc; i++) {
+        ContextParams part = p;
+        part.q = (const char *)p.q + call.first_row[i] * p.qs[2] * bytes_of(args->dtype);
+        part.out = (char *)p.out + call.first_row[i] * p.os[2] * bytes_of(args->out_dtype);
+        part.Sq = call.rows[i], part.q_pos_offset = p.q_pos_offset + call.first_row[i];
+        rc = run_plan(part, call.plan[i], args->dtype, s->s);
+    }
+    return rc;
 }
 
 }  // extern "C"

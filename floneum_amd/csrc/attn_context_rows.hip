@@ -18,8 +18,9 @@
 namespace fhip {
 
 constexpr int CR_WAVES = 4;
-constexpr int CR_NT = 2;                   // streamed past the caches (measured against plain loads: 16 ragged sequences, 232 MB, 51.0 us and 57.4)
-constexpr uint64_t CR_FAR = 1 << 25;  // bytes between rows up to which a tile's offsets stay in 31 bits
+constexpr int CR_STREAMED = 2;         // past the caches: own keys, which are read once (16 ragged sequences, 232 MB: 51.0 us, 57.4 without); a prefix is
+                                       // read once per block of columns (32 sequences on 8192 keys: 31.9 us, 35.4 streamed)
+constexpr uint64_t CR_FAR = 1 << 25;   // bytes between rows up to which a tile's offsets stay in 31 bits
 typedef uint32_t uint2r_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) char *lds_t;
 #define CR_LDS(type, at) ((__attribute__((address_space(3))) type *)(at))
@@ -492,11 +493,15 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
                                                          0x00020000);
             };
             const auto k_rows = rows_from(k, k_row), v_rows = rows_from(v, v_row);
+            auto pieces = [&](auto aux) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < LOADS; u++) {
-                kst[u] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(k_rows, k_at + u * ROWS * (uint32_t)k_row, 0, CR_NT));
-                vst[u] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(v_rows, v_at + u * ROWS * (uint32_t)v_row, 0, CR_NT));
-            }
+                for (int u = 0; u < LOADS; u++) {
+                    kst[u] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(k_rows, k_at + u * ROWS * (uint32_t)k_row, 0, decltype(aux)::value));
+                    vst[u] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(v_rows, v_at + u * ROWS * (uint32_t)v_row, 0, decltype(aux)::value));
+                }
+            };
+            if (w.prefix) pieces(std::integral_constant<int, 0>{});
+            else pieces(std::integral_constant<int, CR_STREAMED>{});
         }
     };
     const float scale2 = p.scale * CONTEXT_LOG2E;

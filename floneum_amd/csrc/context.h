@@ -63,8 +63,16 @@ struct ContextPlan {
     ContextRows rows;  // total 0: none
     int slots;
     size_t bytes;  // of workspace
+    double us;     // estimated
 };
-ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype);
+// A call, or its first query rows and then the others; both use the same workspace.
+struct ContextCall {
+    int parts;
+    int first_row[2], rows[2];
+    ContextPlan plan[2];
+    size_t bytes;
+};
+ContextCall context_call(const ContextParams &p, fhip_dtype dtype);
 
 int launch_context_any(const ContextParams &p, fhip_dtype dtype, hipStream_t stream);
 bool context_rows_takes(const ContextParams &p, fhip_dtype dtype);

@@ -33,9 +33,9 @@ static RowsPlan rows_launch(const ContextParams &p, fhip_dtype dtype, bool with_
     const int64_t each = (int64_t)p.G * p.Sq, most = each * (with_prefix ? p.B : 1);
     const bool f32 = dtype == FHIP_F32, two = most > 16 && p.D <= 128;
     const int columns = two ? 32 : 16, step = f32 ? 64 : 128, size = f32 ? 4 : 2;
-    // Fitted to 101 calls at six lengths of the shares each; the shares it picks are 2 per cent slower than each call's best in the mean, 12 at most.
+    // Fitted to 101 calls at six lengths of the shares each; the shares it picks are 1.5 per cent slower than each call's best in the mean, 12 at most.
     // A step of a workgroup, what all of them take in from the caches (f32 with 32 columns: as the matrix cores take it) and from memory, bytes per us,
-    // and workgroups per CU.  Where sequences differ in length, 0.3 of the longest share is left over at the end.
+    // and workgroups per CU.  0.3 of the longest share is left over at the end.
     const double step_us = !f32 ? 0.35 + 0.0063 * p.D : two ? 0.20 + 0.0208 * p.D : 0.24 + 0.0119 * p.D;
     const double cached = f32 ? (two ? 5.1e6 : 10e6) : 10.8e6, memory = 6.2e6;
     const int64_t at_once = (int64_t)p.cus * (p.D > 128 ? 1 : p.D > 64 ? 2 : 3);
@@ -75,7 +75,7 @@ static RowsPlan rows_launch(const ContextParams &p, fhip_dtype dtype, bool with_
         if (jobs == 1) plan.rows.second = (int32_t)total;
         plan.rows.total = (int32_t)total;
         const double last = step_us * (double)longest, shared = f32 && two ? std::min(std::max((double)workgroups / p.cus, 1.0), 1.25) : 1.0;
-        plan.us = 2.7 + (double)div_up(workgroups, at_once) * (p.D > 128 ? 4.5 : 2.8) + (p.kv_lens || p.P > 0 ? 0.3 * last : 0.0) +
+        plan.us = 2.7 + (double)div_up(workgroups, at_once) * (p.D > 128 ? 4.5 : 2.8) + 0.3 * last +
                   std::max({shared * last, step_us * (double)all_steps / (double)at_once, taken / cached, read / memory});
         if (plan.slots > 1) plan.us += 1.5 + partials_us(p, plan.slots - slots_before);
         if (best.us == 0.0 || plan.us < best.us) best = plan;
@@ -134,7 +134,7 @@ static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype,
     return best;
 }
 
-ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
+static ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     ContextPlan plan;
     memset(&plan, 0, sizeof(plan));
     plan.any = true;
@@ -146,7 +146,7 @@ ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     const bool own_by_rows = !tiles || each <= (dtype == FHIP_F32 ? 64 : 32);
     const bool one_part = dtype != FHIP_F32 && p.D > 128;  // the tiled kernel takes one part per launch
     int64_t slots = 0;
-    double us = 0.0;
+    double &us = plan.us;
     auto add_tiles = [&](bool fold, bool with_prefix, bool with_own, bool parked) {
         double time;
         ContextTilesLaunch &how = plan.tiles[plan.tile_launches++];
@@ -166,8 +166,10 @@ ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
             if (us < rows.us) {
                 rows = own;
             } else {
-                plan.tile_launches = 0, slots = 0;
+                plan.tile_launches = 0, slots = 0, us = rows.us;
             }
+        } else {
+            us = rows.us;
         }
         if (plan.tile_launches == 0 || p.Skv > 0) plan.rows = rows.rows, slots = rows.slots;
     } else if (p.P > 0 && ((can_fold && each < 128) || (one_part && p.Skv > 0))) {
@@ -185,6 +187,36 @@ ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     plan.slots = (int)slots;
     if (slots > 1) plan.bytes = (size_t)p.B * p.H * p.Sq * (size_t)slots * (size_t)(p.D + 4) * sizeof(float);
     return plan;
+}
+
+ContextCall context_call(const ContextParams &p, fhip_dtype dtype) {
+    ContextCall call;
+    memset(&call, 0, sizeof(call));
+    call.parts = 1, call.rows[0] = p.Sq;
+    call.plan[0] = context_plan(p, dtype);
+    // Where the last workgroup of each unit would hold few of its rows, these go to the kernel for few rows if that is estimated to take less: 8 x 257
+    // rows of 32 heads on a prefix of 8192 keys take 301 us instead of 369, 32 x 65 rows at head_dim 256 on 2048 138 instead of 179.
+    const int limit = dtype == FHIP_F32 ? 64 : 32;
+    if (!call.plan[0].any && call.plan[0].rows.total == 0) {
+        double least = call.plan[0].us;
+        const ContextPlan whole = call.plan[0];
+        for (int i = 0; i < whole.tile_launches; i++) {
+            const int64_t group = whole.tiles[i].rows_per_group, first = (int64_t)p.G * p.Sq / group * group / p.G, rest = p.Sq - first;
+            if (first == 0 || rest == 0 || rest * p.G > limit) continue;
+            ContextParams q = p;
+            q.Sq = (int)first;
+            const ContextPlan most = context_plan(q, dtype);
+            q.Sq = (int)rest, q.q_pos_offset += first;
+            const ContextPlan last = context_plan(q, dtype);
+            if (most.any || last.any || most.us + last.us >= least) continue;
+            least = most.us + last.us;
+            call.parts = 2;
+            call.rows[0] = call.first_row[1] = (int)first, call.rows[1] = (int)rest;
+            call.plan[0] = most, call.plan[1] = last;
+        }
+    }
+    call.bytes = std::max(call.plan[0].bytes, call.plan[1].bytes);
+    return call;
 }
 
 }  // namespace fhip
