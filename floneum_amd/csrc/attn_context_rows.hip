@@ -293,16 +293,16 @@ struct Columns {
 // four matrix steps; slot (i, q4) of V^T P^T is key 4 q4 + i, whose weight the lane already holds, and row n of output block (nb, e) is dim
 // 16 VW nb + VW n + e, so that one read of a row feeds VW steps.  The tile's share of O forms on its own and is added once (one rounding at the
 // size of the sum).
-template <int DP, int CB>
-struct Columns<float, DP, CB> {
+template <int DP>
+struct Columns<float, DP, 1> {
     static constexpr int KEYS = 16;
     static constexpr int KP = DP * 4 + 16, VP = KP;
     static constexpr int KC = DP / 16, VW = DP % 64 == 0 ? 4 : 2, NB = DP / (16 * VW);
     typedef float vrow_t __attribute__((ext_vector_type(VW)));
-    float4_t q[CB][KC];
-    float4_t o[CB][NB][VW];
-    float m[CB], l[CB];
-    ContextRow seen[CB];
+    float4_t q[KC];
+    float4_t o[NB][VW];
+    float m, l;
+    ContextRow seen[1];
 
     // Q^T operand: column j, dims 16 c + 4 q4 .. + 3
     __device__ __forceinline__ void load_q(const ContextParams &p, int cb, const ColumnAt &at, bool used, int q4) {
@@ -311,75 +311,65 @@ struct Columns<float, DP, CB> {
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const int dim = 16 * c + 4 * q4;
-            q[cb][c] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            q[c] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
             if (used && dim < p.D) {
                 if (whole) {
-                    q[cb][c] = *(const float4_t *)(from + dim);
+                    q[c] = *(const float4_t *)(from + dim);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) q[cb][c][e] = from[(dim + e) * p.qs[3]];
+                    for (int e = 0; e < 4; e++) q[c][e] = from[(dim + e) * p.qs[3]];
                 }
             }
         }
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int cb = 0; cb < CB; cb++) {
+        for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                for (int e = 0; e < VW; e++) o[cb][nb][e] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            m[cb] = -INFINITY, l[cb] = 0.0f;
-        }
+            for (int e = 0; e < VW; e++) o[nb][e] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        m = -INFINITY, l = 0.0f;
     }
     __device__ __forceinline__ void step(lds_t k, lds_t v, int base, int end, int first, int gap, bool whole, float scale2, int lane) {
         const int j = lane & 15, q4 = lane >> 4;
-        float4_t s[CB];
-#pragma unroll
-        for (int cb = 0; cb < CB; cb++) s[cb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        float4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const float4_t a = *CR_LDS(float4_t, k + j * KP + (16 * c + 4 * q4) * 4);
 #pragma unroll
-            for (int cb = 0; cb < CB; cb++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[cb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], q[cb][c][i], s[cb], 0, 0, 0);
+            for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], q[c][i], s, 0, 0, 0);
         }
-        float x[CB][4];
+        float x[4];
         uint32_t used = 0;
+        // element r is visible key base + 4 q4 + r
 #pragma unroll
-        for (int cb = 0; cb < CB; cb++) {
-            // element r is visible key base + 4 q4 + r
-#pragma unroll
-            for (int r = 0; r < 4; r++) x[cb][r] = s[cb][r] * scale2;
-            if (!whole) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int n = base + 4 * q4 + r, key = n + (n >= first ? gap : 0);
-                    const bool sees = n < end && key < seen[cb].hi && (key >= seen[cb].lo || key < seen[cb].first);
-                    x[cb][r] = sees ? x[cb][r] : -INFINITY;
-                    used |= sees ? 1u << r : 0u;
-                }
-            }
-            const float top = fmaxf(m[cb], column_max(fmaxf(fmaxf(x[cb][0], x[cb][1]), fmaxf(x[cb][2], x[cb][3]))));
-            if (__builtin_amdgcn_ballot_w64(top > m[cb]) != 0) {
-                const float moved = __builtin_amdgcn_exp2f(m[cb] - (top == -INFINITY ? 0.0f : top));
-                m[cb] = top;
-                l[cb] *= moved;
-#pragma unroll
-                for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                    for (int e = 0; e < VW; e++) o[cb][nb][e] *= moved;
-            }
-            const float reference = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f;
+        for (int r = 0; r < 4; r++) x[r] = s[r] * scale2;
+        if (!whole) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                x[cb][r] = __builtin_amdgcn_exp2f(x[cb][r] - reference);
-                sum += x[cb][r];
+                const int n = base + 4 * q4 + r, key = n + (n >= first ? gap : 0);
+                const bool sees = n < end && key < seen[0].hi && (key >= seen[0].lo || key < seen[0].first);
+                x[r] = sees ? x[r] : -INFINITY;
+                used |= sees ? 1u << r : 0u;
             }
-            l[cb] += sum;
         }
+        const float top = fmaxf(m, column_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))));
+        if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+            const float moved = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+            m = top;
+            l *= moved;
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int e = 0; e < VW; e++) o[nb][e] *= moved;
+        }
+        const float reference = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            x[r] = __builtin_amdgcn_exp2f(x[r] - reference);
+            sum += x[r];
+        }
+        l += sum;
         if (!whole) {
             used = any_column(used);
 #pragma unroll
@@ -393,25 +383,23 @@ struct Columns<float, DP, CB> {
 #pragma unroll
             for (int i = 0; i < 4; i++) a[i] = *CR_LDS(vrow_t, v + (4 * q4 + i) * VP + (16 * VW * nb + VW * j) * 4);
 #pragma unroll
-            for (int cb = 0; cb < CB; cb++)
+            for (int e = 0; e < VW; e++) {
+                float4_t share = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int e = 0; e < VW; e++) {
-                    float4_t share = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) share = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][e], x[cb][i], share, 0, 0, 0);
-                    o[cb][nb][e] += share;
-                }
+                for (int i = 0; i < 4; i++) share = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][e], x[i], share, 0, 0, 0);
+                o[nb][e] += share;
+            }
         }
     }
     __device__ __forceinline__ void park(float *to, int cb, int q4) {
-        const float sum = column_sum(l[cb]);
+        const float sum = column_sum(l);
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int e = 0; e < VW; e++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) to[16 * VW * nb + VW * (4 * q4 + r) + e] = o[cb][nb][e][r];
-        if (q4 == 0) to[DP] = m[cb], to[DP + 1] = sum;
+                for (int r = 0; r < 4; r++) to[16 * VW * nb + VW * (4 * q4 + r) + e] = o[nb][e][r];
+        if (q4 == 0) to[DP] = m, to[DP + 1] = sum;
     }
 };
 
@@ -422,7 +410,7 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
     typedef Columns<T, DP, CB> C;
     constexpr int KEYS = C::KEYS, COLS = 16 * CB, ES = sizeof(T), STEP = CR_WAVES * KEYS;
     constexpr int PER = 16 / ES, CPR = DP / PER, LOADS = KEYS * CPR / 64;  // elements of a 16-byte piece, pieces of a row, loads per lane and tensor
-    constexpr bool RUNS = 64 % CPR == 0 && ES == 2;
+    constexpr bool RUNS = 64 % CPR == 0;  // a load takes whole rows
     constexpr int WAVE_BYTES = KEYS * (C::KP + C::VP), STATE = DP + 2, STATE_BYTES = CR_WAVES * COLS * STATE * 4;
     __shared__ __attribute__((aligned(16))) char smem[CR_WAVES * WAVE_BYTES > STATE_BYTES ? CR_WAVES * WAVE_BYTES : STATE_BYTES];
 
@@ -466,9 +454,9 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_
     const int64_t k_row = (w.prefix ? p.pks[1] : p.ks[2]) * ES, v_row = (w.prefix ? p.pvs[1] : p.vs[2]) * ES;  // bytes
 
     // The tile behind the one in LDS is on its way in registers.  A tile's rows are a buffer that starts at its first and ends with the share's last key:
-    // what lies behind reads as zero, without a clamp or an address per lane.  Rows that a load does not divide evenly, f32 rows (whose two forms
-    // together spill at 32 columns), rows far apart and the one tile within which the first tokens end have an address per lane, with the last
-    // key again behind it.
+    // what lies behind reads as zero, without a clamp or an address per lane.  Rows that a load does not
+    // divide evenly, rows far apart and the one tile within which the first tokens end have an address per lane, with the last key again behind
+    // it.  (With addresses alone 64 f32 columns on 2048 keys at head_dim 128 take 25.4 us instead of 22.9.)
     const int row = lane / CPR, col = lane % CPR;
     const bool inside = col * PER < p.D, far = (uint64_t)k_row > CR_FAR || (uint64_t)v_row > CR_FAR;
     const uint32_t k_at = inside ? row * (uint32_t)k_row + col * 16 : 0x7ffffff0u, v_at = inside ? row * (uint32_t)v_row + col * 16 : 0x7ffffff0u;
@@ -694,7 +682,10 @@ static bool launch_rows_dims(const ContextParams &p, const ContextRows &rows, hi
 }
 template <typename T>
 static bool launch_rows_type(const ContextParams &p, const ContextRows &rows, hipStream_t stream) {
-    return rows.columns == 32 ? launch_rows_dims<T, 2>(p, rows, stream) : launch_rows_dims<T, 1>(p, rows, stream);
+    if constexpr (sizeof(T) == 2) {
+        if (rows.columns == 32) return launch_rows_dims<T, 2>(p, rows, stream);
+    }
+    return launch_rows_dims<T, 1>(p, rows, stream);
 }
 int launch_context_rows(const ContextParams &p, const ContextRows &rows, fhip_dtype dtype, hipStream_t stream) {
     const bool ran = dtype == FHIP_F32   ? launch_rows_type<float>(p, rows, stream)

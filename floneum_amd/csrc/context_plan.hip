@@ -29,15 +29,15 @@ struct RowsPlan {
     int64_t slots;
     double us;
 };
-static RowsPlan rows_launch(const ContextParams &p, fhip_dtype dtype, bool with_prefix, int64_t slots_before) {
+static RowsPlan rows_launch_of(const ContextParams &p, fhip_dtype dtype, bool with_prefix, int64_t slots_before, int columns) {
     const int64_t each = (int64_t)p.G * p.Sq, most = each * (with_prefix ? p.B : 1);
-    const bool f32 = dtype == FHIP_F32, two = most > 16 && p.D <= 128;
-    const int columns = two ? 32 : 16, step = f32 ? 64 : 128, size = f32 ? 4 : 2;
+    const bool f32 = dtype == FHIP_F32;
+    const int step = f32 ? 64 : 128, size = f32 ? 4 : 2;
     // Fitted to 101 calls at six lengths of the shares each; the shares it picks are 1.5 per cent slower than each call's best in the mean, 12 at most.
-    // A step of a workgroup, what all of them take in from the caches (f32 with 32 columns: as the matrix cores take it) and from memory, bytes per us,
+    // A step of a workgroup, what all of them take in from the caches and from memory, bytes per us,
     // and workgroups per CU.  0.3 of the longest share is left over at the end.
-    const double step_us = !f32 ? 0.35 + 0.0063 * p.D : two ? 0.20 + 0.0208 * p.D : 0.24 + 0.0119 * p.D;
-    const double cached = f32 ? (two ? 5.1e6 : 10e6) : 10.8e6, memory = 6.2e6;
+    const double step_us = f32 ? 0.24 + 0.0119 * p.D : 0.35 + 0.0063 * p.D, cached = f32 ? 10e6 : 10.8e6, memory = 6.2e6;
+    const double start_us = 2.7 + (columns == 32 ? 0.03 * p.D : 0.0);
     const int64_t at_once = (int64_t)p.cus * (p.D > 128 ? 1 : p.D > 64 ? 2 : 3);
     RowsPlan best;
     memset(&best, 0, sizeof(best));  // (us 0: too many workgroups for a launch)
@@ -74,13 +74,22 @@ static RowsPlan rows_launch(const ContextParams &p, fhip_dtype dtype, bool with_
         if (total > 0x7fffffff) continue;
         if (jobs == 1) plan.rows.second = (int32_t)total;
         plan.rows.total = (int32_t)total;
-        const double last = step_us * (double)longest, shared = f32 && two ? std::min(std::max((double)workgroups / p.cus, 1.0), 1.25) : 1.0;
-        plan.us = 2.7 + (double)div_up(workgroups, at_once) * (p.D > 128 ? 4.5 : 2.8) + 0.3 * last +
-                  std::max({shared * last, step_us * (double)all_steps / (double)at_once, taken / cached, read / memory});
+        const double last = step_us * (double)longest;
+        plan.us = start_us + (double)div_up(workgroups, at_once) * (p.D > 128 ? 4.5 : 2.8) + 0.3 * last +
+                  std::max({last, step_us * (double)all_steps / (double)at_once, taken / cached, read / memory});
         if (plan.slots > 1) plan.us += 1.5 + partials_us(p, plan.slots - slots_before);
         if (best.us == 0.0 || plan.us < best.us) best = plan;
     }
     return best;
+}
+
+// 32 columns halve what is taken in for a unit with so many, but the other part's few columns pay for them too: 32 sequences on 8192 keys at head_dim 128
+// take 26.2 us with 32 and 37.5 with 16, on 512 keys 18.0 and 14.9.  f32 tensors, which the matrix cores bound, take 16 (60 of 60 calls, up to a third).
+static RowsPlan rows_launch(const ContextParams &p, fhip_dtype dtype, bool with_prefix, int64_t slots_before) {
+    const RowsPlan one = rows_launch_of(p, dtype, with_prefix, slots_before, 16);
+    if ((int64_t)p.G * p.Sq * (with_prefix ? p.B : 1) <= 16 || p.D > 128 || dtype == FHIP_F32) return one;
+    const RowsPlan two = rows_launch_of(p, dtype, with_prefix, slots_before, 32);
+    return one.us < two.us ? one : two;
 }
 
 // Time of a launch of the 16-bit kernels in us, from the constants of prefill_mfma_time (attn_prefill_mfma.hip) and prefill_wide_time
