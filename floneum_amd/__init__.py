@@ -1147,6 +1147,9 @@ def _context_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, sin
         raise InvalidArgument(ERR_INVALID_ARG, "flash_attention takes rank-4 tensors")
     if not all(t.dtype == q.dtype for t in inputs):
         raise InvalidArgument(ERR_INVALID_ARG, "q, k, v and the prefix must share one element type")
+    lens_ptr, positions_ptr = _lens_ptr(kv_lens, q.shape[0], "kv_lens"), _lens_ptr(q_positions, q.shape[0], "q_positions")
+    if not all(t is None or t.buffer.device is dev for t in (kv_lens, q_positions)):
+        raise AssertionError("Cannot mix tensors of different devices")
     if out is None:
         out = Tensor.empty(dev, q.shape, q.dtype if out_dtype is None else out_dtype)
     elif out_dtype is not None and out_dtype != out.dtype:
@@ -1171,7 +1174,7 @@ def _context_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, sin
         causal, off, window = analytic
         a.causal, a.q_pos_offset, a.window = 1 if causal else 0, int(off), int(window or 0)
     a.sinks = 0 if sinks is None else int(sinks)
-    a.kv_lens, a.q_positions = _lens_ptr(kv_lens, q.shape[0], "kv_lens"), _lens_ptr(q_positions, q.shape[0], "q_positions")
+    a.kv_lens, a.q_positions = lens_ptr, positions_ptr
     need = ctypes.c_size_t()
     check(lib().fhip_context_attention_workspace_bytes(ctypes.byref(a), dev.compute_units, ctypes.byref(need)))
     if need.value:

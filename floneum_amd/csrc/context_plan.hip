@@ -120,7 +120,8 @@ static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype,
         if (with_prefix) keys += fold ? part_keys(p, true) : most_visible(p, p.P, positions, p.sinks);
         if (with_own) keys += most_visible(p, p.Skv, positions, std::max<int64_t>((int64_t)p.sinks - p.P, 0));
         if (both && p.causal && p.window > 0) keys = std::min(keys, p.window + positions + p.sinks);
-        const int64_t tiles = std::max<int64_t>(div_up(keys, tile), 1), wgs = (int64_t)how.units * div_up(how.rows, form[0]);
+        keys = std::max<int64_t>(keys, 1);
+        const int64_t tiles = div_up(keys, tile), wgs = (int64_t)how.units * div_up(how.rows, form[0]);
         for (int64_t shares = 1; shares <= tiles; shares++) {
             if (shares > 1 && wgs * shares > 3 * p.cus) break;
             how.chunk = (int32_t)div_up(tiles, shares);
@@ -182,7 +183,8 @@ static ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
         }
         if (plan.tile_launches == 0 || p.Skv > 0) plan.rows = rows.rows, slots = rows.slots;
     } else if (p.P > 0 && ((can_fold && each < 128) || (one_part && p.Skv > 0))) {
-        add_tiles(can_fold, true, false, true), add_tiles(false, false, true, true);
+        add_tiles(can_fold, true, false, p.Skv > 0);
+        if (p.Skv > 0) add_tiles(false, false, true, true);
     } else {
         add_tiles(false, p.P > 0, p.Skv > 0, false);
     }

@@ -126,3 +126,40 @@ def test_python_refusals():
                       (dict(sinks=1, out=_Stub((1, 2, 1, 64), device=object())), AssertionError)):
         with pytest.raises(error):
             q.flash_attention(k, k, 1.0, **kw)
+
+
+def test_python_lengths():
+    dev = object()
+    q, k = _Stub((2, 2, 1, 64), device=dev), _Stub((2, 2, 9, 64), device=dev)
+
+    def lens(n, device, dtype="i32"):
+        return type("L", (), dict(dtype=dtype, shape=(n,), offset=0, buffer=type("B", (), dict(ptr=FAKE, device=device))()))()
+
+    for kw, error in ((dict(kv_lens=lens(2, object())), AssertionError), (dict(q_positions=lens(2, object())), AssertionError),
+                      (dict(kv_lens=lens(3, dev)), fa.InvalidArgument), (dict(q_positions=lens(2, dev, "f32")), fa.InvalidArgument),
+                      (dict(kv_lens=np.zeros(2, np.int32)), fa.InvalidArgument)):
+        with pytest.raises(error):
+            q.flash_attention(k, k, 1.0, sinks=1, analytic=(True, 0, 4), **kw)
+
+
+@pytest.mark.parametrize("dtype", [fa.F32, fa.F16, fa.BF16])
+def test_workspaces_of_any_call(dtype):
+    """The size query answers for every shape within the limits, and asks for no more than a share of the keys that a call reads: a row's place holds
+    D + 4 floats and stands for 64 keys of D elements and more."""
+    rng = np.random.default_rng(3)
+    need = ctypes.c_size_t()
+
+    def drawn(lo, hi):
+        return int(round(np.exp(rng.uniform(np.log(lo), np.log(hi)))))
+
+    for _ in range(400):
+        Hkv, G, D = drawn(1, 64), drawn(1, 40), 8 * drawn(1, 32)
+        Skv, P = (drawn(1, 1 << 24) if rng.random() < 0.9 else 0 for _ in range(2))
+        Sq = drawn(1, 1 << 16)
+        B = drawn(1, max(1, min(1 << 16, ((1 << 31) - 1) // (Hkv * G * Sq))))
+        if B * Hkv * G * Sq >= 1 << 31:
+            continue
+        a = args(B=B, H=Hkv * G, Hkv=Hkv, Sq=Sq, Skv=Skv, P=P, D=D, dtype=dtype, out_dtype=dtype, window=drawn(1, 1 << 20) if rng.random() < 0.5 else 0,
+                 sinks=drawn(1, 200), causal=1, q_pos_offset=drawn(1, 1 << 24), kv_lens=FAKE if rng.random() < 0.5 else None)
+        assert fa.lib().fhip_context_attention_workspace_bytes(ctypes.byref(a), 256, ctypes.byref(need)) == fa.OK
+        assert need.value <= B * Hkv * G * Sq * 4 * (D + 4) * (2 + (Skv + 63) // 64 + (P + 63) // 64)
