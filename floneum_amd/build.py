@@ -51,9 +51,9 @@ def build(verbose=True):
     subprocess.check_call(["g++", "-std=c++17", "-O2", "-Wall", "-Wno-missing-field-initializers", "-fPIC", "-shared", "-fvisibility=hidden",
                            "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, "host_python.cpp"), "-o", HOST, "-L", HERE,
                            "-lfusor_hip", "-Wl,-rpath,$ORIGIN"])
-    # the C++ host mirror's test programs (need a GPU, started by tests/test_host_mirror_gpu.py and tests/test_q8_host_mirror_gpu.py)
+    # the C++ host mirror's test programs (need a GPU, each started by a test of its own)
     root = os.path.dirname(HERE)
-    for name in ("test_host_mirror", "test_host_mirror_q8"):
+    for name in ("test_host_mirror", "test_host_mirror_q8", "test_host_mirror_context"):
         cpp = os.path.join(root, "tests", "cpp", name + ".cpp")
         if os.path.exists(cpp):
             subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-I", os.path.join(root, "include"), cpp,
