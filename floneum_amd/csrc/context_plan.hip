@@ -144,16 +144,14 @@ static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype,
     return best;
 }
 
-static ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
+// The sequences' own keys in the kernel for few rows, or on tiles.
+static ContextPlan plan_with(const ContextParams &p, fhip_dtype dtype, bool tiles, bool own_by_rows) {
     ContextPlan plan;
     memset(&plan, 0, sizeof(plan));
     plan.any = true;
-    if (!context_rows_takes(p, dtype)) return plan;
-    const bool tiles = context_tiles_takes(p, dtype) || context_terms_takes(p, dtype);
     const int64_t each = (int64_t)p.G * p.Sq;  // columns of a sequence and KV head
     // rows of all sequences meet the prefix together where they see one run of it
     const bool can_fold = p.P > 0 && p.B > 1 && (p.window == 0 || !p.q_positions);
-    const bool own_by_rows = !tiles || each <= (dtype == FHIP_F32 ? 64 : 32);
     const bool one_part = dtype != FHIP_F32 && p.D > 128;  // the tiled kernel takes one part per launch
     int64_t slots = 0;
     double &us = plan.us;
@@ -198,6 +196,23 @@ static ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     plan.slots = (int)slots;
     if (slots > 1) plan.bytes = (size_t)p.B * p.H * p.Sq * (size_t)slots * (size_t)(p.D + 4) * sizeof(float);
     return plan;
+}
+static ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
+    if (!context_rows_takes(p, dtype)) {
+        ContextPlan any;
+        memset(&any, 0, sizeof(any));
+        any.any = true;
+        return any;
+    }
+    const bool tiles = context_tiles_takes(p, dtype) || context_terms_takes(p, dtype);
+    const int64_t each = (int64_t)p.G * p.Sq;
+    if (!tiles || each <= 16) return plan_with(p, dtype, tiles, true);
+    const ContextPlan many = plan_with(p, dtype, true, false);
+    if (each > 256) return many;
+    const ContextPlan few = plan_with(p, dtype, true, true);
+    // (252 calls of 20 to 256 columns: 1 per cent slower than the faster of the two in the mean, 30 at most; a limit of 32 columns, f32 64, is 6 per cent
+    // slower: 12 f16 rows of one sequence on 600 keys at head_dim 128 take 9.9 us here and 13.6 on tiles, 5 of 32 sequences at 256 on 4000 124 and 70)
+    return !few.any && (many.any || 0.9 * few.us < many.us) ? few : many;
 }
 
 ContextCall context_call(const ContextParams &p, fhip_dtype dtype) {
