@@ -39,8 +39,8 @@ SEED = 0xF10E0000
 # per configuration, the bytes and the SHA-256 of the kernel source they were measured on; a figure whose source
 # has changed since is not reported.  Written by --record-traffic from the counter CSVs.
 TRAFFIC_RECORD = os.path.join(ROOT, "profiles", "traffic.json")
-KERNEL_SOURCES = {"decode_splitkv": "attn_decode.hip", "prefill_mfma": "attn_prefill_mfma.hip",
-                  "prefill_f32": "attn_prefill_f32_terms.hip", "generic": "attn_generic.hip"}
+KERNEL_SOURCES = {"decode_splitkv": "attn_decode.hip", "prefill_mfma": "attn_prefill_mfma_kernel.h",
+                  "prefill_f32": "attn_prefill_f32_terms_kernel.h", "generic": "attn_generic.hip"}
 
 
 def source_hash(kernel, source=None):
@@ -778,7 +778,7 @@ def record_traffic(name, fetch_csv, write_csv):
         out["kernel_symbol"] = kname
     out["kernel"] = kernel
     # the file the kernel lives in (the wide-head 16-bit prefill kernels have files of their own)
-    out["source"] = "attn_prefill_mfma_rows32.hip" if "prefill_mfma_wide_rows32" in out["kernel_symbol"] else \
+    out["source"] = "attn_prefill_mfma_rows32_kernel.h" if "prefill_mfma_wide_rows32" in out["kernel_symbol"] else \
         "attn_prefill_mfma_rows64.hip" if "prefill_mfma_rows64" in out["kernel_symbol"] else \
         "attn_prefill_mfma_wide.hip" if "prefill_mfma_wide" in out["kernel_symbol"] else \
         "attn_prefill_f32.hip" if "prefill_f32" in out["kernel_symbol"] and "terms" not in out["kernel_symbol"] else \
