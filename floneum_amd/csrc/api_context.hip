@@ -115,7 +115,7 @@ static int run_plan(ContextParams &p, const ContextPlan &plan, fhip_dtype dtype,
     if (plan.any) return launch_context_any(p, dtype, stream);
     p.slots = plan.slots;
     int rc = FHIP_OK;
-    for (int i = 0; i < plan.tile_launches && !rc; i++) rc = launch_context_tiles(p, plan.tiles[i], dtype, stream);
+    if (plan.tiles.jobs) rc = launch_context_tiles(p, plan.tiles, dtype, stream);
     if (!rc && plan.rows.total) rc = launch_context_rows(p, plan.rows, dtype, stream);
     return rc || plan.slots == 1 ? rc : launch_context_merge(p, dtype, stream);
 }

@@ -3,7 +3,7 @@
 // pass from lane to lane.  Only keys that the row sees are touched.
 //   s_j = scale * q . k_j;  out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s), the maximum and the sums running, in f32
 // Bound: every key is read once per query row, a key per lane (rows of a tensor apart): 16 sequences of one token on 4112 visible f16 keys of
-// 32/8 heads at 128 take milliseconds where the kernel for few rows takes microseconds.
+// 32/8 heads at 128 take 4.0 ms, 8192 rows under a window of 4096 185 (the other kernels: 0.05 and 0.39).
 #include "context_device.h"
 
 namespace fhip {

@@ -1,5 +1,7 @@
 // Attention over one part of a context on the kernel of four 32-row wavefronts (attn_prefill_mfma_rows32_kernel.h): 16-bit tensors at head dims above 128,
 // padded with zeros up to 256.
+// Bound: ends of workgroups that walk few tiles (256 rows of 16 sequences on 4001 shared keys, 4 KV heads at 256: 22 us in 96 workgroups of eleven tiles;
+// more of them write more shares: 12.8 MB as it is).
 #include <type_traits>
 
 #include "attn_prefill_mfma_rows32_kernel.h"
@@ -8,22 +10,21 @@
 namespace fhip {
 
 template <typename T>
-static void launch_type(const ContextParams &p, hipStream_t stream) {
-    const int nqb = (p.rows + R32_BM - 1) / R32_BM;
-    const dim3 grid((unsigned)((int64_t)p.units * nqb * p.pf_nsplit)), block(256);
+static void launch_type(const ContextParams &p, const ContextTilesLaunch &how, hipStream_t stream) {
+    const dim3 grid((unsigned)how.total), block(256);
     const int bytes = p.out_f32 ? 4 : 2;
     int out_vec = p.os[3] == 1 && (uintptr_t)p.out % 16 == 0;
     for (int i = 0; i < 3; i++)
         if (p.os[i] * bytes % 16 != 0) out_vec = 0;
-    if (p.slots > 1) hipLaunchKernelGGL((prefill_mfma_wide_rows32_kernel<T, true, ContextParams>), grid, block, 0, stream, p, nqb, out_vec);
-    else hipLaunchKernelGGL((prefill_mfma_wide_rows32_kernel<T, false, ContextParams>), grid, block, 0, stream, p, nqb, out_vec);
+    if (p.slots > 1) hipLaunchKernelGGL((prefill_mfma_wide_rows32_kernel<T, true, ContextParams>), grid, block, 0, stream, p, 0, out_vec);
+    else hipLaunchKernelGGL((prefill_mfma_wide_rows32_kernel<T, false, ContextParams>), grid, block, 0, stream, p, 0, out_vec);
 }
 
 int launch_context_wide(const ContextParams &p0, const ContextTilesLaunch &how, fhip_dtype dtype, hipStream_t stream) {
     ContextParams p = p0;
     set_tiles_launch(p, how);
-    if (dtype == FHIP_F16) launch_type<half_t>(p, stream);
-    else launch_type<bf16_t>(p, stream);
+    if (dtype == FHIP_F16) launch_type<half_t>(p, how, stream);
+    else launch_type<bf16_t>(p, how, stream);
     FHIP_HIP_CHECK(hipGetLastError());
     return FHIP_OK;
 }

@@ -353,8 +353,14 @@ __global__ __launch_bounds__(64 * U * KG, D > 128 || (KG == 2 && U == 2 && D > 6
     // Workgroup -> (units, batch, kv head): the units of a KV head are its row blocks times the query heads that share it,
     // numbered heads first, so that U consecutive ones read the same keys; those with the most keys first.
     // (grid: shares of the keys, kv heads of the batch, workgroups per kv head)
-    const int nks = gridDim.x, nwg = gridDim.z;
+    int nks = gridDim.x, nwg = gridDim.z;
     int ksplit = blockIdx.x, rem = blockIdx.y, wz = blockIdx.z;
+    if constexpr (CTX) {  // (one dimension: two jobs)
+        const uint32_t place = tiles_work(p);
+        nks = p.job.shares, nwg = p.job.blocks;
+        const int id = place / nks;
+        ksplit = place % nks, wz = id / p.job.units, rem = id - wz * p.job.units;
+    }
     // The shares of a square prompt differ in length: workgroup wz + P of a share sees as many keys of it as workgroup wz of the next
     // one (P: level_pitch), so those with equal wz + share * P are a level, and the levels are numbered the longest first, without gaps.
     // Workgroups are dealt to the shader engines in turn, which a descending order evens out.  us at head_dim 256, in the grid's order
@@ -391,7 +397,7 @@ __global__ __launch_bounds__(64 * U * KG, D > 128 || (KG == 2 && U == 2 && D > 6
     const int unit_row = CTX ? unit : over_g(unit);  // 32-row block of the unit
     const int h = g * p.G + unit - unit_row * p.G;
     if constexpr (CTX)
-        if (p.fold) b = -1, g = rem;  // rows of all sequences
+        if (p.job.fold) b = -1, g = rem;  // rows of all sequences
     // rows of a tile beyond the sequence's own keys, or behind the last query's position, are never fetched (what they
     // hold, NaN included, must not reach the result as 0 x NaN in P . V)
     int key_end = !CTX && p.kv_lens ? min(p.Skv, max(p.kv_lens[b], 1)) : p.Skv;
@@ -449,11 +455,11 @@ __global__ __launch_bounds__(64 * U * KG, D > 128 || (KG == 2 && U == 2 && D > 6
     ContextSpan wg_sees;
     typename std::conditional<BOTH, ContextBothTiles<PT_BN>, ContextTiles<PT_BN>>::type tiles;
     if constexpr (CTX) {
-        total_rows = p.rows;
-        row_at = stacked_row(p, b, g, min(query, p.rows - 1));
+        total_rows = p.job.rows;
+        row_at = stacked_row(p, b, g, min(query, total_rows - 1));
         stacked_spans<32 * U>(p, b, q0, qw0, lane, row_at, wave_sees, wg_sees, sees);
         if constexpr (!BOTH) {
-            const bool prefix = p.with_prefix != 0;
+            const bool prefix = p.job.with_prefix != 0;
             sees = sees.of(p, prefix), wave_sees = wave_sees.of(p, prefix), wg_sees = wg_sees.of(p, prefix);
         }
         tiles.set(p, wg_sees, ksplit);
@@ -499,7 +505,7 @@ __global__ __launch_bounds__(64 * U * KG, D > 128 || (KG == 2 && U == 2 && D > 6
         own_k = part_rows((const T *)p.k + seq * p.ks[0] + g * p.ks[1], p.ks[2], BOTH ? wg_sees.of(p, false).end() : wg_sees.end());
         own_v = part_rows((const T *)p.v + seq * p.vs[0] + g * p.vs[1], p.vs[2], BOTH ? wg_sees.of(p, false).end() : wg_sees.end());
         if constexpr (!BOTH)
-            if (p.with_prefix) own_k = prefix_k, own_v = prefix_v;
+            if (p.job.with_prefix) own_k = prefix_k, own_v = prefix_v;
     }
     const int k_row = CTX ? own_k.bytes : (int)p.ks[2] * ES, v_row = CTX ? own_v.bytes : (int)p.vs[2] * ES;
     const auto k_rows = [&]() __attribute__((always_inline)) {

@@ -156,10 +156,14 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void prefill_mfma_kernel(P p, int
     const int pack = KS && !CTX ? p.pf_pack : 0;
     const int heads = pack ? p.H / 4 : p.H;  // head units per batch entry
     int bh_count = p.B * heads;
-    if constexpr (CTX) bh_count = p.units;
-    const int nks = max(p.pf_nsplit, 1);
-    const int ksplit = blockIdx.x % nks;  // which share of the keys (0 when the keys are not split over workgroups)
-    const int id = blockIdx.x / nks;
+    uint32_t place = blockIdx.x;
+    int nks = max(p.pf_nsplit, 1);
+    if constexpr (CTX) {
+        place = tiles_work(p);
+        bh_count = p.job.units, nqb = p.job.blocks, nks = p.job.shares;
+    }
+    const int ksplit = place % nks;  // which share of the keys (0 when the keys are not split over workgroups)
+    const int id = place / nks;
     const int qb = nqb - 1 - id / bh_count;
     int rem = id % bh_count;
     int b = rem / heads;
@@ -168,8 +172,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void prefill_mfma_kernel(P p, int
     else if ((p.H & 7) == 0) h = (h & 7) * (p.H >> 3) + (h >> 3);
     int g = h / p.G;
     if constexpr (CTX) {
-        b = p.fold ? -1 : rem / p.Hkv;  // (-1: rows of all sequences)
-        g = p.fold ? rem : rem - b * p.Hkv;
+        b = p.job.fold ? -1 : rem / p.Hkv;  // (-1: rows of all sequences)
+        g = p.job.fold ? rem : rem - b * p.Hkv;
     }
     // Rows of a tile beyond the sequence's own keys (kv_lens below the view's length: a ragged batch in one cache
     // allocation) read as zero (the buffers end there): what such rows hold, NaN included, must not reach the result as 0 x NaN in P . V.
@@ -191,11 +195,11 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void prefill_mfma_kernel(P p, int
     ContextSpan wg_sees;
     typename std::conditional<BOTH, ContextBothTiles<PF_BN>, ContextTiles<PF_BN>>::type tiles;
     if constexpr (CTX) {
-        total_rows = p.rows;
-        row_at = stacked_row(p, b, g, min(query, p.rows - 1));
+        total_rows = p.job.rows;
+        row_at = stacked_row(p, b, g, min(query, total_rows - 1));
         stacked_spans<BM>(p, b, q0, qw0, lane, row_at, wave_sees, wg_sees, sees);
         if constexpr (!BOTH) {
-            const bool prefix = p.with_prefix != 0;
+            const bool prefix = p.job.with_prefix != 0;
             sees = sees.of(p, prefix), wave_sees = wave_sees.of(p, prefix), wg_sees = wg_sees.of(p, prefix);
         }
         tiles.set(p, wg_sees, ksplit);
@@ -258,7 +262,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void prefill_mfma_kernel(P p, int
             prefix_end = wg_sees.of(p, true).end(), key_end = wg_sees.of(p, false).end();
         } else {
             key_end = wg_sees.end();
-            if (p.with_prefix) kg = prefix_kg, vg = prefix_vg, krow_bytes = prefix_krow_bytes, vrow_bytes = prefix_vrow_bytes, key_rows = p.P;
+            if (p.job.with_prefix) kg = prefix_kg, vg = prefix_vg, krow_bytes = prefix_krow_bytes, vrow_bytes = prefix_vrow_bytes, key_rows = p.P;
         }
     }
 

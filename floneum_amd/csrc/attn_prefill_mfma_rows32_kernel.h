@@ -121,10 +121,14 @@ __global__ __launch_bounds__(256, 1) void prefill_mfma_wide_rows32_kernel(P p, i
     // workgroup -> (query block, batch, head): long (late) query blocks first; consecutive workgroups land on
     // consecutive XCDs, so with H a multiple of 8 the heads are dealt so that an XCD works on neighbouring heads
     int bh_count = p.B * p.H;
-    if constexpr (CTX) bh_count = p.units;
-    const int nks = SPLIT ? max(p.pf_nsplit, 1) : 1;
-    const int ksplit = SPLIT ? blockIdx.x % nks : 0;  // which share of the keys
-    const int id = SPLIT ? blockIdx.x / nks : blockIdx.x;
+    uint32_t place = blockIdx.x;
+    int nks = SPLIT ? max(p.pf_nsplit, 1) : 1;
+    if constexpr (CTX) {
+        place = tiles_work(p);
+        bh_count = p.job.units, nqb = p.job.blocks, nks = p.job.shares;
+    }
+    const int ksplit = SPLIT ? place % nks : 0;  // which share of the keys
+    const int id = SPLIT ? place / nks : place;
     const int qb = nqb - 1 - id / bh_count;
     const int rem = id % bh_count;
     int b = rem / p.H;
@@ -132,8 +136,8 @@ __global__ __launch_bounds__(256, 1) void prefill_mfma_wide_rows32_kernel(P p, i
     if ((p.H & 7) == 0) h = (h & 7) * (p.H >> 3) + (h >> 3);
     int g = h / p.G;
     if constexpr (CTX) {
-        b = p.fold ? -1 : rem / p.Hkv;  // (-1: rows of all sequences)
-        g = p.fold ? rem : rem - b * p.Hkv;
+        b = p.job.fold ? -1 : rem / p.Hkv;  // (-1: rows of all sequences)
+        g = p.job.fold ? rem : rem - b * p.Hkv;
     }
     // rows of a tile beyond the sequence's own keys read as zero (the buffers end there)
     int key_end = !CTX && p.kv_lens ? min(p.Skv, max(p.kv_lens[b], 1)) : p.Skv;
@@ -148,10 +152,10 @@ __global__ __launch_bounds__(256, 1) void prefill_mfma_wide_rows32_kernel(P p, i
     ContextSpan wg_sees;
     ContextTiles<R32_KEYS> tiles;
     if constexpr (CTX) {
-        total_rows = p.rows;
-        const bool prefix = p.with_prefix != 0;
+        total_rows = p.job.rows;
+        const bool prefix = p.job.with_prefix != 0;
         StackedSpan wave_sees;
-        row_at = stacked_row(p, b, g, min(query, p.rows - 1));
+        row_at = stacked_row(p, b, g, min(query, total_rows - 1));
         stacked_spans<R32_BM>(p, b, q0, qw0, lane, row_at, wave_sees, wg_sees, sees);
         sees = sees.of(p, prefix), all_see = wave_sees.all.of(p, prefix), wg_sees = wg_sees.of(p, prefix);
         tiles.set(p, wg_sees, ksplit);
@@ -188,7 +192,7 @@ __global__ __launch_bounds__(256, 1) void prefill_mfma_wide_rows32_kernel(P p, i
     int krow_bytes = (int)p.ks[2] * 2, vrow_bytes = (int)p.vs[2] * 2, key_rows = p.Skv;
     if constexpr (CTX) {
         kg = (const uint16_t *)p.k + max(b, 0) * p.ks[0] + g * p.ks[1], vg = (const uint16_t *)p.v + max(b, 0) * p.vs[0] + g * p.vs[1];
-        if (p.with_prefix) {
+        if (p.job.with_prefix) {
             kg = (const uint16_t *)p.pk + g * p.pks[0], vg = (const uint16_t *)p.pv + g * p.pvs[0];
             krow_bytes = (int)p.pks[1] * 2, vrow_bytes = (int)p.pvs[1] * 2, key_rows = p.P;
         }

@@ -5,6 +5,15 @@
 
 namespace fhip {
 
+// A tiled kernel's rows and tiles: rows of a KV head are stacked, see context_tiles.h; the tiles of their visible keys are dealt to `shares` of `chunk`
+// tiles.
+struct ContextTilesJob {
+    int32_t fold;                   // rows of all sequences together (on the prefix alone)
+    int32_t with_prefix, with_own;
+    int32_t units, rows, blocks;    // KV heads (times the batch, if not folded), stacked rows of each, workgroups that these fill
+    int32_t shares, chunk;
+    int32_t slot0;                  // of the first share
+};
 // k, v, Skv, kv_lens of AttnParams are the sequences' own; q_pos_offset and window as there, positions counted from the prefix's first key.
 struct ContextParams : AttnParams {
     const void *pk, *pv;     // the prefix, [Hkv, P, D]
@@ -15,12 +24,9 @@ struct ContextParams : AttnParams {
     // shares of the keys: every (sequence, head, query row) has `slots` places in `partials`, each pf_pitch floats: D values, the
     // reference exponent (base 2) and the sum of the weights
     int32_t slots;
-    // tiled kernels: what a launch takes.  Rows of a KV head are stacked, see context_tiles.h; the tiles of their visible keys are dealt to
-    // pf_nsplit shares of pf_chunk tiles.
-    int32_t fold;        // rows of all sequences together (on the prefix alone)
-    int32_t with_prefix, with_own;
-    int32_t units, rows; // KV heads (times the batch, if not folded), stacked rows of each
-    int32_t slot0;
+    // tiled kernels: workgroups from `second` on take the other job
+    ContextTilesJob job, other;
+    int32_t second;
 };
 struct ContextBoth : ContextParams {};  // of a launch that takes both parts
 
@@ -40,26 +46,20 @@ struct ContextRows {
     int32_t columns; // of a workgroup: 16 or 32
 };
 
-// A launch of a tiled kernel, see ContextParams.
+// A launch of a tiled kernel.
 struct ContextTilesLaunch {
-    int32_t fold, with_prefix, with_own;
-    int32_t units, rows;
     int32_t rows_per_group;  // stacked rows of a workgroup
     int32_t key_groups;      // wavefronts of a workgroup that share its rows, see the kernels
-    int32_t shares, chunk;   // of the visible tiles
-    int32_t slot0;
+    int32_t jobs;            // 0: no launch
+    ContextTilesJob job[2];
+    int32_t second, total;   // workgroups of job[0], of both
 };
-inline void set_tiles_launch(ContextParams &p, const ContextTilesLaunch &how) {
-    p.fold = how.fold, p.with_prefix = how.with_prefix, p.with_own = how.with_own;
-    p.units = how.units, p.rows = how.rows;
-    p.pf_nsplit = how.shares, p.pf_chunk = how.chunk, p.slot0 = how.slot0;
-}
+inline void set_tiles_launch(ContextParams &p, const ContextTilesLaunch &how) { p.job = how.job[0], p.other = how.job[1], p.second = how.second; }
 
 // What a call runs, in this order, and the merge where a row has several places.
 struct ContextPlan {
     bool any;  // the kernel that takes every call, alone
-    int32_t tile_launches;
-    ContextTilesLaunch tiles[2];
+    ContextTilesLaunch tiles;
     ContextRows rows;  // total 0: none
     int slots;
     size_t bytes;  // of workspace

@@ -1,6 +1,7 @@
 // Attention over a context in two parts: which kernels a call runs, and in how many shares of its keys.
 #include <algorithm>
 #include <cstring>
+#include <initializer_list>
 
 #include "context.h"
 
@@ -92,56 +93,84 @@ static RowsPlan rows_launch(const ContextParams &p, fhip_dtype dtype, bool with_
     return one.us < two.us ? one : two;
 }
 
-// Time of a launch of the 16-bit kernels in us, from the constants of prefill_mfma_time (attn_prefill_mfma.hip) and prefill_wide_time
+// Time in us of a launch of the 16-bit kernels, from the constants of prefill_mfma_time (attn_prefill_mfma.hip) and prefill_wide_time
 // (attn_prefill_mfma_wide.hip): rounds of workgroups that walk their tiles of 64 keys, above head_dim 128 32.
-static double tiles_time(const ContextParams &p, const ContextTilesLaunch &how, int64_t keys) {
-    const int64_t wgs = (int64_t)how.units * div_up(how.rows, how.rows_per_group) * how.shares, rounds = div_up(wgs, p.cus);
-    if (p.D > 128) return 5.0 + rounds * (6.5 + 0.70 * div_up(div_up(keys, how.shares), 32));
-    const double dims = p.D <= 64 ? 1.0 : p.D <= 96 ? 1.43 : 1.86, tiles = (double)div_up(div_up(keys, how.shares), 64);
-    return 4.6 + rounds * (how.rows_per_group == 128 ? 5.3 + 0.356 * dims * tiles : 3.9 + 0.579 * dims * tiles);
+static double tiles_time(const ContextParams &p, int rows_per_group, int64_t workgroups, int64_t tiles) {
+    const double rounds = (double)div_up(workgroups, p.cus), dims = p.D <= 64 ? 1.0 : p.D <= 96 ? 1.43 : 1.86;
+    if (p.D > 128) return 5.0 + rounds * (6.5 + 0.70 * (double)tiles);
+    return 4.6 + rounds * (rows_per_group == 128 ? 5.3 + 0.356 * dims * (double)tiles : 3.9 + 0.579 * dims * (double)tiles);
 }
-static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype, bool fold, bool with_prefix, bool with_own, bool parked, double *time) {
-    const bool f32 = dtype == FHIP_F32, both = with_prefix && with_own;
+static ContextTilesJob tiles_job(const ContextParams &p, bool fold, bool with_prefix, bool with_own) {
+    ContextTilesJob job;
+    memset(&job, 0, sizeof(job));
+    job.fold = fold, job.with_prefix = with_prefix, job.with_own = with_own;
+    job.units = fold ? p.Hkv : p.B * p.Hkv;
+    job.rows = (fold ? p.B : 1) * p.G * p.Sq;
+    return job;
+}
+// The launch of one job, or of two that share the length of their shares; parked: other results of its rows are merged with its own anyway.
+static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype, std::initializer_list<ContextTilesJob> of, bool parked, double *time) {
+    const bool f32 = dtype == FHIP_F32;
     const int tile = f32 || p.D > 128 ? 32 : 64;
     // (rows per workgroup, key groups); to head_dim 128 the 16-bit form of 128 rows takes one part
     static const int FORMS[3][3][2] = {{{256, 1}, {128, 2}, {0, 0}}, {{128, 1}, {0, 0}, {0, 0}}, {{128, 1}, {128, 2}, {64, 2}}};
     ContextTilesLaunch best, how;
     memset(&how, 0, sizeof(how));
-    how.fold = fold, how.with_prefix = with_prefix, how.with_own = with_own;
-    how.units = fold ? p.Hkv : p.B * p.Hkv;
-    how.rows = (fold ? p.B : 1) * p.G * p.Sq;
     best = how;
+    how.jobs = (int32_t)of.size();
     double least = 0.0;
     for (const auto &form : FORMS[f32 ? 2 : p.D > 128 ? 1 : 0]) {
+        const bool both = of.begin()->with_prefix && of.begin()->with_own;
         if (form[0] == 0 || (!f32 && p.D <= 128 && form[0] == 128 && both) || (f32 && p.D > 128 && form[1] > 1)) continue;
         how.rows_per_group = form[0], how.key_groups = form[1];
         const int64_t positions = std::min<int64_t>(p.Sq, form[0] / p.G + 2);
-        int64_t keys = 0;
-        if (with_prefix) keys += fold ? part_keys(p, true) : most_visible(p, p.P, positions, p.sinks);
-        if (with_own) keys += most_visible(p, p.Skv, positions, std::max<int64_t>((int64_t)p.sinks - p.P, 0));
-        if (both && p.causal && p.window > 0) keys = std::min(keys, p.window + positions + p.sinks);
-        keys = std::max<int64_t>(keys, 1);
-        const int64_t tiles = div_up(keys, tile), wgs = (int64_t)how.units * div_up(how.rows, form[0]);
-        for (int64_t shares = 1; shares <= tiles; shares++) {
-            if (shares > 1 && wgs * shares > 3 * p.cus) break;
-            how.chunk = (int32_t)div_up(tiles, shares);
-            how.shares = (int32_t)div_up(tiles, how.chunk);
-            if (how.shares != shares) continue;
-            double us;
-            if (f32) {
-                const TermsCall call = {1, how.units, 1, how.rows, (int)keys, p.D, p.cus, false, 0, true, false};
-                us = prefill_f32_terms_time(call, {form[0] / 32, form[1]}, how.shares);
-                if (how.shares > 1) us -= prefill_f32_merge_time(call, how.shares);
-            } else {
-                us = tiles_time(p, how, keys);
+        int64_t tiles[2] = {0, 0}, keys_of[2] = {0, 0}, groups[2] = {0, 0};
+        for (int j = 0; j < how.jobs; j++) {
+            ContextTilesJob &job = how.job[j] = of.begin()[j];
+            int64_t keys = 0;
+            if (job.with_prefix) keys += job.fold ? part_keys(p, true) : most_visible(p, p.P, positions, p.sinks);
+            if (job.with_own) keys += most_visible(p, p.Skv, positions, std::max<int64_t>((int64_t)p.sinks - p.P, 0));
+            if (both && p.causal && p.window > 0) keys = std::min(keys, p.window + positions + p.sinks);
+            keys_of[j] = std::max<int64_t>(keys, 1), tiles[j] = div_up(keys_of[j], tile);
+            job.blocks = (int32_t)div_up(job.rows, form[0]);
+            groups[j] = (int64_t)job.units * job.blocks;
+        }
+        const int longest = tiles[1] > tiles[0];
+        for (int64_t shares = 1; shares <= tiles[longest]; shares++) {
+            const int64_t chunk = div_up(tiles[longest], shares);
+            if (div_up(tiles[longest], chunk) != shares) continue;
+            int64_t total = 0, slots = 0;
+            for (int j = 0; j < how.jobs; j++) {
+                ContextTilesJob &job = how.job[j];
+                job.chunk = (int32_t)chunk, job.shares = (int32_t)div_up(tiles[j], chunk);
+                job.slot0 = (int32_t)slots;
+                slots += job.shares;
+                if (j == 1) how.second = (int32_t)std::min<int64_t>(total, 0x7fffffff);
+                total += groups[j] * job.shares;
             }
-            if (how.shares > 1 || parked) us += partials_us(p, how.shares);
-            if (how.shares > 1 && !parked) us += 3.0;
+            if (shares > 1 && total > 3 * p.cus) break;
+            if (total > 0x7fffffff) break;
+            if (how.jobs == 1) how.second = (int32_t)total;
+            how.total = (int32_t)total;
+            double us;
+            if (!f32) {
+                us = tiles_time(p, form[0], total, chunk);
+            } else if (how.jobs == 1) {
+                const TermsCall call = {1, how.job[0].units, 1, how.job[0].rows, (int)keys_of[0], p.D, p.cus, false, 0, true, false};
+                us = prefill_f32_terms_time(call, {form[0] / 32, form[1]}, (int)shares);
+                if (shares > 1) us -= prefill_f32_merge_time(call, (int)shares);
+            } else {
+                if (total * form[0] > 0x7fffffff) break;
+                const TermsCall call = {1, 1, 1, (int)total * form[0], (int)chunk * tile, p.D, p.cus, false, 0, true, false};
+                us = prefill_f32_terms_time(call, {form[0] / 32, form[1]}, 1);
+            }
+            if (slots > 1 || parked) us += partials_us(p, slots);
+            if (slots > 1 && !parked) us += 3.0;
             if (least == 0.0 || us < 0.98 * least) least = us, best = how;
         }
     }
     *time = least;
-    return best;
+    return best;  // (of no jobs: too many workgroups for a launch)
 }
 
 // The sequences' own keys in the kernel for few rows, or on tiles.
@@ -154,42 +183,29 @@ static ContextPlan plan_with(const ContextParams &p, fhip_dtype dtype, bool tile
     const bool can_fold = p.P > 0 && p.B > 1 && (p.window == 0 || !p.q_positions);
     const bool one_part = dtype != FHIP_F32 && p.D > 128;  // the tiled kernel takes one part per launch
     int64_t slots = 0;
-    double &us = plan.us;
-    auto add_tiles = [&](bool fold, bool with_prefix, bool with_own, bool parked) {
-        double time;
-        ContextTilesLaunch &how = plan.tiles[plan.tile_launches++];
-        how = tiles_launch(p, dtype, fold, with_prefix, with_own, parked, &time);
-        how.slot0 = (int32_t)slots;
-        slots += how.shares;
-        us += time;
+    auto set_tiles = [&](std::initializer_list<ContextTilesJob> of, bool parked) {
+        plan.tiles = tiles_launch(p, dtype, of, parked, &plan.us);
+        slots = (int64_t)plan.tiles.job[0].shares + plan.tiles.job[1].shares;
+        return plan.tiles.jobs > 0;
     };
     if (own_by_rows) {
         RowsPlan rows = rows_launch(p, dtype, p.P > 0, 0);
         if (rows.us == 0.0) return plan;
-        if (p.P > 0 && tiles && can_fold) {
+        bool on_tiles = false;
+        if (p.P > 0 && tiles && can_fold && set_tiles({tiles_job(p, true, true, false)}, p.Skv > 0)) {
             // rows of all sequences on the prefix: with the own keys' launch, or on tiles in one of their own
-            add_tiles(true, true, false, p.Skv > 0);
             const RowsPlan own = rows_launch(p, dtype, false, slots);
-            if (p.Skv > 0) us += own.us;
-            if (us < rows.us) {
-                rows = own;
-            } else {
-                plan.tile_launches = 0, slots = 0, us = rows.us;
-            }
-        } else {
-            us = rows.us;
+            if (p.Skv > 0) plan.us += own.us;
+            on_tiles = plan.us < rows.us;
+            if (on_tiles) rows = own;
         }
-        if (plan.tile_launches == 0 || p.Skv > 0) plan.rows = rows.rows, slots = rows.slots;
+        if (!on_tiles) memset(&plan.tiles, 0, sizeof(plan.tiles)), plan.us = rows.us;
+        if (!on_tiles || p.Skv > 0) plan.rows = rows.rows, slots = rows.slots;
     } else if (p.P > 0 && ((can_fold && each < 128) || (one_part && p.Skv > 0))) {
-        add_tiles(can_fold, true, false, p.Skv > 0);
-        if (p.Skv > 0) add_tiles(false, false, true, true);
-    } else {
-        add_tiles(false, p.P > 0, p.Skv > 0, false);
-    }
-    for (int i = 0; i < plan.tile_launches; i++) {
-        const ContextTilesLaunch &how = plan.tiles[i];
-        if ((int64_t)how.units * div_up(how.rows, how.rows_per_group) * how.shares > 0x7fffffff) return plan;
-        if (dtype == FHIP_F32 && (how.units > 65535 || div_up(how.rows, how.rows_per_group) > 65535)) return plan;  // (dimensions of its grid)
+        const ContextTilesJob prefix = tiles_job(p, can_fold, true, false);
+        if (!(p.Skv > 0 ? set_tiles({prefix, tiles_job(p, false, false, true)}, false) : set_tiles({prefix}, false))) return plan;
+    } else if (!set_tiles({tiles_job(p, false, p.P > 0, p.Skv > 0)}, false)) {
+        return plan;
     }
     if (slots > 0x7fffffff) return plan;
     plan.any = false;
@@ -206,10 +222,10 @@ static ContextPlan context_plan(const ContextParams &p, fhip_dtype dtype) {
     }
     const bool tiles = context_tiles_takes(p, dtype) || context_terms_takes(p, dtype);
     const int64_t each = (int64_t)p.G * p.Sq;
-    if (!tiles || each <= 16) return plan_with(p, dtype, tiles, true);
+    const ContextPlan few = !tiles || each <= 256 ? plan_with(p, dtype, tiles, true) : ContextPlan();
+    if (!tiles || (each <= 16 && !few.tiles.jobs)) return few;
     const ContextPlan many = plan_with(p, dtype, true, false);
     if (each > 256) return many;
-    const ContextPlan few = plan_with(p, dtype, true, true);
     // (252 calls of 20 to 256 columns: 1 per cent slower than the faster of the two in the mean, 30 at most; a limit of 32 columns, f32 64, is 6 per cent
     // slower: 12 f16 rows of one sequence on 600 keys at head_dim 128 take 9.9 us here and 13.6 on tiles, 5 of 32 sequences at 256 on 4000 124 and 70)
     return !few.any && (many.any || 0.9 * few.us < many.us) ? few : many;
@@ -223,19 +239,14 @@ ContextCall context_call(const ContextParams &p, fhip_dtype dtype) {
     // Where the last workgroup of each unit would hold few of its rows, these go to the kernel for few rows if that is estimated to take less: 8 x 257
     // rows of 32 heads on a prefix of 8192 keys take 301 us instead of 369, 32 x 65 rows at head_dim 256 on 2048 138 instead of 179.
     const int limit = dtype == FHIP_F32 ? 64 : 32;
-    if (!call.plan[0].any && call.plan[0].rows.total == 0) {
-        double least = call.plan[0].us;
-        const ContextPlan whole = call.plan[0];
-        for (int i = 0; i < whole.tile_launches; i++) {
-            const int64_t group = whole.tiles[i].rows_per_group, first = (int64_t)p.G * p.Sq / group * group / p.G, rest = p.Sq - first;
-            if (first == 0 || rest == 0 || rest * p.G > limit) continue;
-            ContextParams q = p;
-            q.Sq = (int)first;
-            const ContextPlan most = context_plan(q, dtype);
-            q.Sq = (int)rest, q.q_pos_offset += first;
-            const ContextPlan last = context_plan(q, dtype);
-            if (most.any || last.any || most.us + last.us >= least) continue;
-            least = most.us + last.us;
+    const int64_t group = call.plan[0].tiles.rows_per_group, first = group ? (int64_t)p.G * p.Sq / group * group / p.G : 0, rest = p.Sq - first;
+    if (first > 0 && rest > 0 && rest * p.G <= limit && call.plan[0].rows.total == 0) {
+        ContextParams q = p;
+        q.Sq = (int)first;
+        const ContextPlan most = context_plan(q, dtype);
+        q.Sq = (int)rest, q.q_pos_offset += first;
+        const ContextPlan last = context_plan(q, dtype);
+        if (!most.any && !last.any && most.us + last.us < call.plan[0].us) {
             call.parts = 2;
             call.rows[0] = call.first_row[1] = (int)first, call.rows[1] = (int)rest;
             call.plan[0] = most, call.plan[1] = last;

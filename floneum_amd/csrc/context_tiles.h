@@ -1,8 +1,22 @@
 // Device code of the tiled kernels of attention over a context in two parts: which rows and which tiles of keys a workgroup takes.
 #pragma once
+#include <type_traits>
+
 #include "context_device.h"
 
 namespace fhip {
+
+// The workgroup's place in its job, which p.job is from here on.
+template <class P>
+__device__ __forceinline__ uint32_t tiles_work(P &p) {
+    if constexpr (!std::is_same<P, ContextBoth>::value) {
+        if ((int)blockIdx.x >= p.second) {
+            p.job = p.other;
+            return blockIdx.x - p.second;
+        }
+    }
+    return blockIdx.x;
+}
 
 // Stacked rows of a KV head: the heads of its group within a query row, query rows within a sequence, and where the rows of all sequences meet
 // the prefix together (fold) sequences behind each other.
@@ -29,7 +43,7 @@ struct StackedSpan {
 template <int BM>
 __device__ __forceinline__ void stacked_spans(const ContextParams &p, int b, int q0, int qw0, int lane, const StackedRow &at, StackedSpan &wave, ContextSpan &wg,
                                               ContextRow &sees) {
-    const int last = p.rows - 1;
+    const int last = p.job.rows - 1;
     if (b >= 0) {  // a sequence's rows: both ends move forward with the row
         const ContextSequence s = context_sequence(p, b);
         auto query = [&](int r) __attribute__((always_inline)) { return p.G == 1 ? min(r, last) : min(r, last) / p.G; };
@@ -101,9 +115,9 @@ struct ContextTiles {
     __device__ __forceinline__ void set(const ContextParams &p, const ContextSpan &s, int share) {
         const int n0 = (s.first + KEYS - 1) >> SHIFT, s1 = max(s.lo >> SHIFT, n0);
         const int n1 = s.hi > s.lo ? max(((s.hi + KEYS - 1) >> SHIFT) - s1, 0) : 0;
-        const int t0 = share * p.pf_chunk, left = n0 + n1 - t0;
+        const int t0 = share * p.job.chunk, left = n0 + n1 - t0;
         end0 = n0 - t0, from0 = KEYS * t0, from1 = KEYS * (s1 - n0 + t0);
-        count = max(share + 1 < p.pf_nsplit ? min(left, p.pf_chunk) : left, 0);
+        count = max(share + 1 < p.job.shares ? min(left, p.job.chunk) : left, 0);
     }
 };
 // Of both parts, keys numbered through them: the prefix's up to `first`, then either the prefix's from `lo` on or own ones up to `first`, then own ones
@@ -135,16 +149,16 @@ struct ContextBothTiles {
         if (own1) n1 = (b.first + KEYS - 1) >> SHIFT;
         else if (a.hi > a.lo) s1 = max(a.lo >> SHIFT, n0), n1 = max(((a.hi + KEYS - 1) >> SHIFT) - s1, 0);
         if (b.hi > b.lo) s2 = max(b.lo >> SHIFT, own1 ? n1 : 0), n2 = max(((b.hi + KEYS - 1) >> SHIFT) - s2, 0);
-        const int t0 = share * p.pf_chunk, left = n0 + n1 + n2 - t0;
+        const int t0 = share * p.job.chunk, left = n0 + n1 + n2 - t0;
         end0 = n0 - t0, end1 = n0 + n1 - t0;
         from0 = KEYS * t0, from1 = KEYS * (s1 - n0 + t0), from2 = KEYS * (s2 - n0 - n1 + t0);
-        count = max(share + 1 < p.pf_nsplit ? min(left, p.pf_chunk) : left, 0);
+        count = max(share + 1 < p.job.shares ? min(left, p.job.chunk) : left, 0);
     }
 };
 
 // Where this lane's row of the result, or of the shares, starts, in elements.
 __device__ __forceinline__ int64_t stacked_output(const ContextParams &p, const StackedRow &at, int share) {
-    if (p.slots > 1) return ((((int64_t)at.b * p.H + at.h) * p.Sq + at.row) * p.slots + p.slot0 + share) * p.pf_pitch;
+    if (p.slots > 1) return ((((int64_t)at.b * p.H + at.h) * p.Sq + at.row) * p.slots + p.job.slot0 + share) * p.pf_pitch;
     return at.b * p.os[0] + at.h * p.os[1] + at.row * p.os[2];
 }
 __device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
