@@ -1,7 +1,7 @@
 // Attention over one part of a context on the kernel of four 32-row wavefronts (attn_prefill_mfma_rows32_kernel.h): 16-bit tensors at head dims above 128,
 // padded with zeros up to 256.
-// Bound: ends of workgroups that walk few tiles (256 rows of 16 sequences on 4001 shared keys, 4 KV heads at 256: 22 us in 96 workgroups of eleven tiles;
-// more of them write more shares: 12.8 MB as it is).
+// Bound: ends of workgroups that walk few tiles, of a wavefront per SIMD: four rows of 16 sequences on 4001 shared and up to 600 own keys, 16/4 heads at 256,
+// 24 us in 232 workgroups of nine or ten tiles, a round, and 4.8 of merging (two launches for the two parts: 23 and, few rows, 15.5).
 #include <type_traits>
 
 #include "attn_prefill_mfma_rows32_kernel.h"

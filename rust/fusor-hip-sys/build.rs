@@ -73,8 +73,11 @@ fn compile(root: &Path, out_dir: &Path) {
         run(&mut cmd);
         objects.push(obj);
     }
-    for header in ["common.h", "device_utils.h", "attn_bounds.h"] {
-        println!("cargo:rerun-if-changed={}", csrc.join(header).display());
+    for entry in std::fs::read_dir(&csrc).unwrap() {
+        let header = entry.unwrap().path();
+        if header.extension().is_some_and(|e| e == "h") {
+            println!("cargo:rerun-if-changed={}", header.display());
+        }
     }
     let archive = out_dir.join("libfusor_hip.a");
     let _ = std::fs::remove_file(&archive);
