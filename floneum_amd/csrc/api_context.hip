@@ -78,8 +78,8 @@ static int validate_context(const fhip_context_attn_args *a) {
         set_error("head_dim %u > 512 has no kernel", qs[3]);
         return FHIP_ERR_UNSUPPORTED;
     }
-    if ((uint64_t)qs[1] * qs[2] > 0x7fffffffull || (uint64_t)qs[0] * qs[1] * qs[2] > 0x7fffffffull) {
-        set_error("context_attention: more than 2^31-1 query rows in one call");
+    if ((uint64_t)qs[1] * qs[2] > 0x7fffffffull - 4096 || (uint64_t)qs[0] * qs[1] * qs[2] > 0x7fffffffull - 4096) {
+        set_error("context_attention: more than 2^31-4097 query rows in one call");
         return FHIP_ERR_UNSUPPORTED;
     }
     if ((uint64_t)a->prefix_k.shape[2] + a->k.shape[2] > 0x7fffffffull - 4096) {  // (the kernels look a few tiles ahead in 32 bits)

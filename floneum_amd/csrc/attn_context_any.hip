@@ -15,7 +15,7 @@ template <typename T>
 __global__ __launch_bounds__(64 * CA_WAVES) void context_any_kernel(ContextParams p) {
     __shared__ float q_lds[CA_WAVES][64 * CA_DIMS];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, D = p.D;
-    const int64_t row = (int64_t)blockIdx.x * CA_WAVES + wave;
+    const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * CA_WAVES + wave;
     if (row >= (int64_t)p.B * p.H * p.Sq) return;  // (a whole wavefront, and no barrier follows)
     const int i = (int)(row % p.Sq), h = (int)(row / p.Sq % p.H), b = (int)(row / ((int64_t)p.Sq * p.H)), g = h / p.G;
 
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(64 * CA_WAVES) void context_any_kernel(ContextParam
 
 int launch_context_any(const ContextParams &p, fhip_dtype dtype, hipStream_t stream) {
     const int64_t rows = (int64_t)p.B * p.H * p.Sq;
-    const dim3 grid((unsigned)((rows + CA_WAVES - 1) / CA_WAVES)), block(64 * CA_WAVES);
+    const dim3 grid = rows_grid((rows + CA_WAVES - 1) / CA_WAVES), block(64 * CA_WAVES);
     if (dtype == FHIP_F32) hipLaunchKernelGGL(context_any_kernel<float>, grid, block, 0, stream, p);
     else if (dtype == FHIP_F16) hipLaunchKernelGGL(context_any_kernel<half_t>, grid, block, 0, stream, p);
     else hipLaunchKernelGGL(context_any_kernel<bf16_t>, grid, block, 0, stream, p);

@@ -549,7 +549,7 @@ __global__ __launch_bounds__(GROUPS > 1 ? LANES * GROUPS : 256) void context_mer
     constexpr int ROWS = GROUPS > 1 ? 1 : 256 / LANES, U = 8;
     __shared__ __attribute__((aligned(16))) float parts[GROUPS][GROUPS > 1 ? 4 * LANES : 4];
     __shared__ float states[GROUPS][2];
-    const uint32_t row = GROUPS > 1 ? blockIdx.x : blockIdx.x * ROWS + threadIdx.x / LANES;
+    const uint32_t row = GROUPS > 1 ? blockIdx.x : (blockIdx.y * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / LANES;
     if (GROUPS == 1 && row >= (uint32_t)(p.B * p.H * p.Sq)) return;
     const int group = GROUPS > 1 ? threadIdx.x / LANES : 0, D = p.D, lane_dim = 4 * (threadIdx.x % LANES), dim = lane_dim < D ? lane_dim : 0;
     const float *const from = p.partials + (int64_t)row * p.slots * p.pf_pitch;
@@ -632,7 +632,7 @@ static void merge_dims(const ContextParams &p, hipStream_t stream) {
         if (p.os[i] % 4 != 0) out_vec = 0;
     if (p.slots <= 8 || rows > 4L * p.cus) {
         constexpr int ROWS = 256 / LANES;
-        hipLaunchKernelGGL((context_merge_kernel<T, LANES, 1>), dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(256), 0, stream, p, out_vec);
+        hipLaunchKernelGGL((context_merge_kernel<T, LANES, 1>), rows_grid((rows + ROWS - 1) / ROWS), dim3(256), 0, stream, p, out_vec);
     } else if (p.slots <= 32) {
         hipLaunchKernelGGL((context_merge_kernel<T, LANES, 4>), dim3((unsigned)rows), dim3(LANES * 4), 0, stream, p, out_vec);
     } else {

@@ -56,6 +56,12 @@ struct ContextTilesLaunch {
 };
 inline void set_tiles_launch(ContextParams &p, const ContextTilesLaunch &how) { p.job = how.job[0], p.other = how.job[1], p.second = how.second; }
 
+// A launch has less than 2^32 threads in a dimension: the workgroups of one with a workgroup for every few rows in two.
+inline dim3 rows_grid(int64_t workgroups) {
+    const int64_t x = workgroups < 1 << 22 ? workgroups : 1 << 22;
+    return dim3((unsigned)x, (unsigned)((workgroups + x - 1) / x));
+}
+
 // What a call runs, in this order, and the merge where a row has several places.
 struct ContextPlan {
     bool any;  // the kernel that takes every call, alone

@@ -72,7 +72,7 @@ static RowsPlan rows_launch_of(const ContextParams &p, fhip_dtype dtype, bool wi
             taken += (double)job.units * job.blocks * keys * p.D * 2 * size;
             read += (double)job.units * keys * p.D * 2 * size;
         }
-        if (total > 0x7fffffff) continue;
+        if (total >= 1 << 24) continue;  // (2^32 threads)
         if (jobs == 1) plan.rows.second = (int32_t)total;
         plan.rows.total = (int32_t)total;
         const double last = step_us * (double)longest;
@@ -149,7 +149,7 @@ static ContextTilesLaunch tiles_launch(const ContextParams &p, fhip_dtype dtype,
                 total += groups[j] * job.shares;
             }
             if (shares > 1 && total > 3 * p.cus) break;
-            if (total > 0x7fffffff) break;
+            if (total >= 1 << 23) break;  // (2^32 threads)
             if (how.jobs == 1) how.second = (int32_t)total;
             how.total = (int32_t)total;
             double us;

@@ -163,3 +163,17 @@ def test_workspaces_of_any_call(dtype):
                  sinks=drawn(1, 200), causal=1, q_pos_offset=drawn(1, 1 << 24), kv_lens=FAKE if rng.random() < 0.5 else None)
         assert fa.lib().fhip_context_attention_workspace_bytes(ctypes.byref(a), 256, ctypes.byref(need)) == fa.OK
         assert need.value <= B * Hkv * G * Sq * 4 * (D + 4) * (2 + (Skv + 63) // 64 + (P + 63) // 64)
+
+
+def test_limits_of_rows():
+    """2^31 - 4097 rows at most: a workgroup's last row is counted in 32 bits."""
+    top = (1 << 31) - 4097
+    assert status(args(B=1, H=1, Hkv=1, Sq=top, D=8)) == (fa.OK, "")
+    for a in (args(B=1, H=1, Hkv=1, Sq=top + 1, D=8), args(B=1 << 10, H=1 << 10, Hkv=1, Sq=1 << 11, D=8)):
+        rc, message = status(a)
+        assert rc == fa.ERR_UNSUPPORTED and "query rows" in message
+    need = ctypes.c_size_t()
+    for Skv, P in ((1, 0), (1, 1), (0, 100), (100000, 5)):  # (rows times shares beyond what a launch takes: another kernel's)
+        for B, Sq in ((1, top), (top // 64, 64), (top, 1)):
+            a = args(B=B, H=1, Hkv=1, Sq=Sq, Skv=Skv, P=P, D=8)
+            assert fa.lib().fhip_context_attention_workspace_bytes(ctypes.byref(a), 256, ctypes.byref(need)) == fa.OK

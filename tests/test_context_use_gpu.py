@@ -340,3 +340,32 @@ def test_conversations_behind_one_instruction(device, dtype):
             got = upload(device, q, dtype).flash_attention(*keys, scale, analytic=(True, P + at, w), sinks=s, prefix=prefix).to_numpy()
             want, bound = definition(q, ks, vs, pk, pv, scale, visible(B, n, at + n, P, offset=P + at, window=w, sinks=s), dtype, dtype)
             assert (np.abs(np.asarray(got, np.float64) - want) <= bound).all(), (n, at, w)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Sq", [1, 40, 300])
+def test_a_prefix_of_no_rows(device, dtype, Sq):
+    c = Call(device, dtype, 2, 4, 2, Sq, 350, 0, 64, seed=15)
+    none = fa.Tensor.empty(device, (1, 2, 0, 64), dtype)
+    how = dict(offset=350 - Sq, window=70, sinks=2)
+    got = upload(device, c.q, dtype).flash_attention(*(upload(device, x, dtype) for x in (c.k, c.v)), c.scale, analytic=(True, 350 - Sq, 70), sinks=2,
+                                                     prefix=(none, none))
+    c.check(np.asarray(got.to_numpy(), np.float32), **how)
+
+
+def test_many_rows(device):
+    """More rows than a launch has in one dimension at a wavefront each: in the kernel that takes every call, and in a tiled one."""
+    for D in (12, 16):
+        B, H, Sq = 1 << 15, 4, 600
+        n = B * H * Sq
+        q = fa.Tensor.empty(device, (B, H, Sq, D), fa.F16)
+        fa.check(fa.lib().fhip_memset(device.stream, ctypes.c_void_p(q.buffer.ptr), 0, q.buffer.nbytes))
+        k = upload(device, np.ones((1, 1, 2, D)), fa.F16)
+        v = upload(device, np.broadcast_to(np.asarray([1.0, 3.0])[None, None, :, None], (1, 1, 2, D)), fa.F16)
+        whole = [fa.Tensor(t.buffer, fa.F16, (B, 1, 2, D), (0, *t.strides[1:])) for t in (k, v)]
+        out = q.flash_attention(*whole, 0.5, prefix=(k, v))  # (scores of nothing: the mean of 1, 3, 1, 3)
+        assert n * 64 > 1 << 32
+        for at in (0, n - 1, (1 << 26) + 5):
+            host = np.empty(D, np.float16)
+            fa.check(fa.lib().fhip_memcpy_d2h(device.stream, host.ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(out.buffer.ptr + at * D * 2), 2 * D))
+            assert (host == 2.0).all(), (D, at)
