@@ -2,7 +2,8 @@
 // into registers and from there through LDS to the matrix cores; what no row sees is not touched.
 //
 // Columns are (query row, head of the group) pairs that share a KV head.  A workgroup of four wavefronts serves 16 or 32 of them over one share of one
-// part's visible keys, which are numbered without the gap between first tokens and window, a tile of 32 (f32: 16) per wavefront and step:
+// part's visible keys, which are numbered without the gap between first tokens and window, a tile of 32 (f32, and above head_dim 128: 16) per wavefront
+// and step:
 //   own keys   columns of one sequence
 //   prefix     columns of all sequences, so that the prefix is read once for the batch
 // Both go in one launch, the prefix's workgroups first.
@@ -169,14 +170,15 @@ __device__ __forceinline__ void write_column(const ContextParams &p, const RowsW
     }
 }
 
-// A wavefront's columns and their state.  DP: head_dim rounded up to a multiple of 32; Q is zero in the dims behind head_dim, and such dims of the result
+// A wavefront's columns and their state.  Above head_dim 128 tiles of 16 keys leave room for a second workgroup on the CU (half of a second product's
+// contraction is then zero: 32 sequences of up to 1024 keys of 16/4 heads at 192 take 17.6 us instead of 23.1).  DP: head_dim rounded up to a multiple of 32; Q is zero in the dims behind head_dim, and such dims of the result
 // are not written.
 // Rows that no column sees may hold anything, NaN among it, which 0 x NaN would bring into the result: in tiles with such rows their values are
 // cleared in LDS.
 template <typename T, int DP, int CB>
 struct Columns {
     typedef typename RowsMma<T>::vec8 vec8;
-    static constexpr int KEYS = 32;
+    static constexpr int KEYS = DP > 128 ? 16 : 32, TB = KEYS / 16, E = 4 * TB;
     static constexpr int KP = DP * 2 + 16, VP = DP * 2 + 32;  // row pitches in LDS: 4 and 8 banks apart
     static constexpr int KB = DP / 32, NB = DP / 16;
     vec8 q[CB][KB];
@@ -214,9 +216,9 @@ struct Columns {
     // The tile of visible keys base .. in LDS; whole: every column sees all of it.
     __device__ __forceinline__ void step(lds_t k, lds_t v, int base, int end, int first, int gap, bool whole, float scale2, int lane) {
         const int j = lane & 15, q4 = lane >> 4;
-        float4_t s[CB][2];
+        float4_t s[CB][TB];
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int t = 0; t < TB; t++) {
 #pragma unroll
             for (int cb = 0; cb < CB; cb++) s[cb][t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -231,12 +233,12 @@ struct Columns {
 #pragma unroll
         for (int cb = 0; cb < CB; cb++) {
             // element (t, r) is visible key base + 16 t + 4 q4 + r
-            float x[8];
+            float x[E];
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = s[cb][e >> 2][e & 3] * scale2;
+            for (int e = 0; e < E; e++) x[e] = s[cb][e >> 2][e & 3] * scale2;
             if (!whole) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < E; e++) {
                     const int n = base + 16 * (e >> 2) + 4 * q4 + (e & 3), key = n + (n >= first ? gap : 0);
                     const bool sees = n < end && key < seen[cb].hi && (key >= seen[cb].lo || key < seen[cb].first);
                     x[e] = sees ? x[e] : -INFINITY;
@@ -245,7 +247,7 @@ struct Columns {
             }
             float top = x[0];
 #pragma unroll
-            for (int e = 1; e < 8; e++) top = fmaxf(top, x[e]);
+            for (int e = 1; e < E; e++) top = fmaxf(top, x[e]);
             top = fmaxf(m[cb], column_max(top));
             if (__builtin_amdgcn_ballot_w64(top > m[cb]) != 0) {
                 const float moved = __builtin_amdgcn_exp2f(m[cb] - (top == -INFINITY ? 0.0f : top));
@@ -257,19 +259,20 @@ struct Columns {
             const float reference = top == -INFINITY ? 0.0f : top;
             float sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
+            for (int e = 0; e < E; e++) {
                 x[e] = __builtin_amdgcn_exp2f(x[e] - reference);
                 sum += x[e];
             }
             l[cb] += sum;
-            // P^T operand: slot (q4, e) is key 4 q4 + e, or 16 + 4 q4 + e - 4 from e = 4 on
-            weights[cb] = __builtin_bit_cast(vec8, uint4_t{RowsMma<T>::pack2(x[0], x[1]), RowsMma<T>::pack2(x[2], x[3]),
-                                                           RowsMma<T>::pack2(x[4], x[5]), RowsMma<T>::pack2(x[6], x[7])});
+            // P^T operand: slot (q4, e) is key 4 q4 + e, or 16 + 4 q4 + e - 4 from e = 4 on (of 16 keys: zero)
+            uint4_t packed = {RowsMma<T>::pack2(x[0], x[1]), RowsMma<T>::pack2(x[2], x[3]), 0, 0};
+            if constexpr (TB == 2) packed[2] = RowsMma<T>::pack2(x[4], x[5]), packed[3] = RowsMma<T>::pack2(x[6], x[7]);
+            weights[cb] = __builtin_bit_cast(vec8, packed);
         }
         if (!whole) {
             used = any_column(used);
 #pragma unroll
-            for (int e = 0; e < 8; e++)
+            for (int e = 0; e < E; e++)
                 if (!(used >> e & 1)) clear_row<DP * 2>(v + (16 * (e >> 2) + 4 * q4 + (e & 3)) * VP, j);
             wave_lds_sync();
         }
@@ -278,8 +281,8 @@ struct Columns {
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             const short4_t a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(CR_LDS(short4_t, v_at + nb * 32));
-            const short4_t a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(CR_LDS(short4_t, v_at + 16 * VP + nb * 32));
-            const uint2r_t u0 = __builtin_bit_cast(uint2r_t, a0), u1 = __builtin_bit_cast(uint2r_t, a1);
+            uint2r_t u0 = __builtin_bit_cast(uint2r_t, a0), u1 = {0, 0};
+            if constexpr (TB == 2) u1 = __builtin_bit_cast(uint2r_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(CR_LDS(short4_t, v_at + 16 * VP + nb * 32)));
             const vec8 values = __builtin_bit_cast(vec8, uint4_t{u0[0], u0[1], u1[0], u1[1]});
 #pragma unroll
             for (int cb = 0; cb < CB; cb++) o[cb][nb] = RowsMma<T>::mfma(values, weights[cb], o[cb][nb]);
@@ -412,7 +415,7 @@ struct Columns<float, DP, 1> {
 
 // CB: blocks of 16 columns
 template <typename T, int DP, int CB>
-__global__ __launch_bounds__(64 * CR_WAVES, DP > 128 ? 1 : 2) void context_rows_kernel(ContextParams p, ContextRows rows) {
+__global__ __launch_bounds__(64 * CR_WAVES, DP > 128 && sizeof(T) == 4 ? 1 : 2) void context_rows_kernel(ContextParams p, ContextRows rows) {
     request_arguments<ContextParams, ContextRows>();
     typedef Columns<T, DP, CB> C;
     constexpr int KEYS = C::KEYS, COLS = 16 * CB, ES = sizeof(T), STEP = CR_WAVES * KEYS;

@@ -33,16 +33,17 @@ struct RowsPlan {
 static RowsPlan rows_launch_of(const ContextParams &p, fhip_dtype dtype, bool with_prefix, int64_t slots_before, int columns) {
     const int64_t each = (int64_t)p.G * p.Sq, most = each * (with_prefix ? p.B : 1);
     const bool f32 = dtype == FHIP_F32;
-    const int step = f32 ? 64 : 128, size = f32 ? 4 : 2;
-    // Fitted to 101 calls at six lengths of the shares each; the shares it picks are 1.5 per cent slower than each call's best in the mean, 12 at most.
+    const int step = f32 || p.D > 128 ? 64 : 128, size = f32 ? 4 : 2;
+    // Fitted to 101 calls at six lengths of the shares each, and 40 at eight above head_dim 128; the shares it picks are 1.5 per cent slower than each call's best in the mean, 12 at most.
     // A step of a workgroup, what all of them take in from the caches and from memory, bytes per us,
     // and workgroups per CU.  0.3 of the longest share is left over at the end.
-    const double step_us = f32 ? 0.24 + 0.0119 * p.D : 0.35 + 0.0063 * p.D, cached = f32 ? 10e6 : 10.8e6, memory = 6.2e6;
+    const double step_us = f32 ? 0.24 + 0.0119 * p.D : p.D > 128 ? 0.36 + 0.0028 * p.D : 0.35 + 0.0063 * p.D;
+    const double cached = f32 ? 10e6 : 10.8e6, memory = 6.2e6;  // (above head_dim 128 up to 14e6: tiles then pass for slower than they are)
     const double start_us = 2.7 + (columns == 32 ? 0.03 * p.D : 0.0);
-    const int64_t at_once = (int64_t)p.cus * (p.D > 128 ? 1 : p.D > 64 ? 2 : 3);
+    const int64_t at_once = (int64_t)p.cus * (p.D > 128 && f32 ? 1 : p.D > 64 ? 2 : 3);
     RowsPlan best;
     memset(&best, 0, sizeof(best));  // (us 0: too many workgroups for a launch)
-    for (int steps = 1; steps <= 8; steps++) {
+    for (int steps = 1; steps <= (f32 || p.D <= 128 ? 8 : 16); steps++) {
         RowsPlan plan;
         memset(&plan, 0, sizeof(plan));
         plan.rows.columns = columns;
@@ -76,7 +77,7 @@ static RowsPlan rows_launch_of(const ContextParams &p, fhip_dtype dtype, bool wi
         if (jobs == 1) plan.rows.second = (int32_t)total;
         plan.rows.total = (int32_t)total;
         const double last = step_us * (double)longest;
-        plan.us = start_us + (double)div_up(workgroups, at_once) * (p.D > 128 ? 4.5 : 2.8) + 0.3 * last +
+        plan.us = start_us + (double)div_up(workgroups, at_once) * (f32 && p.D > 128 ? 4.5 : 2.8) + 0.3 * last +
                   std::max({last, step_us * (double)all_steps / (double)at_once, taken / cached, read / memory});
         if (plan.slots > 1) plan.us += 1.5 + partials_us(p, plan.slots - slots_before);
         if (best.us == 0.0 || plan.us < best.us) best = plan;
