@@ -1,5 +1,5 @@
 // Attention over a context in two parts for few query rows: every visible key and value is read once per column block, straight from memory
-// into registers and from there through LDS to the matrix cores; what no row sees is not touched.
+// into registers and from there through LDS to the matrix cores; what lies outside the columns' windows is not touched.
 //
 // Columns are (query row, head of the group) pairs that share a KV head.  A workgroup of four wavefronts serves 16 or 32 of them over one share of one
 // part's visible keys, which are numbered without the gap between first tokens and window, a tile of 32 (f32, and above head_dim 128: 16) per wavefront
@@ -26,7 +26,7 @@
 namespace fhip {
 
 constexpr int CR_WAVES = 4;
-constexpr int CR_STREAMED = 2;         // past the caches: own keys, which are read once (16 ragged sequences, 232 MB: 51.0 us, 57.4 without); a prefix is
+constexpr int CR_STREAMED = 2;         // past the caches: own keys, which are read once (16 ragged sequences, 259 MB: 51.0 us, 57.4 without); a prefix is
                                        // read once per block of columns (32 sequences on 8192 keys: 31.9 us, 35.4 streamed)
 constexpr uint64_t CR_FAR = 1 << 25;   // bytes between rows up to which a tile's offsets stay in 31 bits
 typedef uint32_t uint2r_t __attribute__((ext_vector_type(2)));
