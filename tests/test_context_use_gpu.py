@@ -369,3 +369,26 @@ def test_many_rows(device):
             host = np.empty(D, np.float16)
             fa.check(fa.lib().fhip_memcpy_d2h(device.stream, host.ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(out.buffer.ptr + at * D * 2), 2 * D))
             assert (host == 2.0).all(), (D, at)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Sq", [1, 40, 200])
+@pytest.mark.parametrize("D", [64, 72, 256])
+def test_broadcast_inputs(device, dtype, Sq, D):
+    """Queries that heads share, keys that the batch or its heads share, one row of values for all keys."""
+    B, H, Hkv, Skv, P = 2, 4, 2, 210, 90
+    c = Call(device, dtype, B, H, Hkv, Sq, Skv, P, D, seed=16)
+    c.q[:] = c.q[:, :1]
+    c.k[:] = c.k[:1, :1]
+    c.v[:] = c.v[:1, :, :1]
+    c.pk[:] = c.pk[:1]
+    c.pv[:] = c.pv[:, :1]
+
+    def shared(x, *dims):
+        """x with one element of memory along `dims`."""
+        t = upload(device, x[tuple(slice(0, 1) if i in dims else slice(None) for i in range(4))], dtype)
+        return fa.Tensor(t.buffer, dtype, x.shape, [0 if i in dims else s for i, s in enumerate(t.strides)])
+
+    tensors = [shared(c.q, 1), shared(c.k, 0, 1), shared(c.v, 0, 2), shared(c.pk[None], 1), shared(c.pv[None], 2)]
+    for how in (dict(offset=P + Skv - Sq), dict(offset=P + Skv - Sq, window=150, sinks=5)):
+        c.check(c.run(tensors=tensors, **how), **how)
