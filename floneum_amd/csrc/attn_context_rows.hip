@@ -476,10 +476,13 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 && sizeof(T) == 4 ? 1 : 2) 
         if (!RUNS || far || (base < first && base + KEYS > first)) {
 #pragma unroll
             for (int u = 0; u < LOADS; u++) {
-                const int piece = lane + 64 * u, x = min(base + piece / CPR, v_hi - 1), dim = piece % CPR * PER < p.D ? piece % CPR * PER : 0;
+                const int piece = lane + 64 * u, x = min(base + piece / CPR, v_hi - 1);
+                const bool there = piece % CPR * PER < p.D;
+                const int dim = there ? piece % CPR * PER : 0;
                 const int64_t key = x + (x >= first ? gap : 0);
                 kst[u] = __builtin_nontemporal_load((const uint4_t *)((const char *)(k + dim) + key * k_row));
                 vst[u] = __builtin_nontemporal_load((const uint4_t *)((const char *)(v + dim) + key * v_row));
+                if (!there) kst[u] = uint4_t{0, 0, 0, 0};  // (they meet zeros of Q, and 0 x inf is NaN)
             }
         } else {
             const int64_t key = base + (base >= first ? gap : 0);
