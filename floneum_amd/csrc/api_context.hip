@@ -120,6 +120,29 @@ static int run_plan(ContextParams &p, const ContextPlan &plan, fhip_dtype dtype,
     return rc || plan.slots == 1 ? rc : launch_context_merge(p, dtype, stream);
 }
 
+// What a call that passes the checks runs on a device of `cus` compute units, for tests: of its up to two parts, behind each other, their query rows (0: no such
+// part), whether the kernel for every call takes them, rows per workgroup, key groups and jobs of the tiled launch, each job's {fold, with_prefix, with_own, shares},
+// the few-row launch's columns (0: no such launch), its jobs' {prefix, shares} (no job: 0 shares), and the places of a row in the workspace.
+constexpr int FORM_WORDS = 19;
+void context_forms(const fhip_context_attn_args *args, int cus, int32_t *forms) {
+    ContextParams p;
+    fill_context(args, cus, &p);
+    const ContextCall call = context_call(p, args->dtype);
+    memset(forms, 0, 2 * FORM_WORDS * sizeof(int32_t));
+    for (int i = 0; i < call.parts; i++) {
+        const ContextPlan &plan = call.plan[i];
+        int32_t *f = forms + i * FORM_WORDS;
+        *f++ = call.rows[i], *f++ = plan.any;
+        if (plan.any) continue;
+        *f++ = plan.tiles.rows_per_group, *f++ = plan.tiles.key_groups, *f++ = plan.tiles.jobs;
+        for (int j = 0; j < 2; j++, f += 4)
+            if (j < plan.tiles.jobs) f[0] = plan.tiles.job[j].fold, f[1] = plan.tiles.job[j].with_prefix, f[2] = plan.tiles.job[j].with_own, f[3] = plan.tiles.job[j].shares;
+        *f++ = plan.rows.total ? plan.rows.columns : 0;
+        for (const ContextRowsJob &job : plan.rows.job) *f++ = job.prefix, *f++ = plan.rows.total ? job.nsplit : 0;
+        *f = plan.slots;
+    }
+}
+
 }  // namespace fhip
 
 using namespace fhip;
