@@ -505,18 +505,20 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 && sizeof(T) == 4 ? 1 : 2) 
     const float scale2 = p.scale * CONTEXT_LOG2E;
     int base = v_lo + wave * KEYS;
     if (base < v_hi) load_tile(base);
-    // Pieces of K behind head_dim meet zeros of Q, and 0 x inf is NaN: they are cleared once and not written again.  (Asked of each piece where it is written:
-    // a choice made where it is loaded waits for the load, 16 f32 sequences of 2005 visible keys at head_dim 136 42.6 us instead of 37.3.)
-    auto there = [&](int piece) __attribute__((always_inline)) { return piece % CPR * PER < p.D; };
-#pragma unroll
-    for (int u = 0; u < LOADS; u++)
-        if (const int piece = lane + 64 * u; !there(piece)) *CR_LDS(uint4_t, k_tile + piece / CPR * C::KP + piece % CPR * 16) = uint4_t{0, 0, 0, 0};
     for (; base < v_hi; base += STEP) {
+        // Pieces of K behind head_dim meet zeros of Q, and 0 x inf is NaN.  (Cleared here and not where they are loaded, which would wait for the load: 16 f32
+        // sequences of 2005 visible keys at head_dim 136 42.6 us instead of 37.5.)
+        if (p.D < DP) {
+            asm volatile("");  // a branch
+#pragma unroll
+            for (int u = 0; u < LOADS; u++)
+                if ((lane + 64 * u) % CPR * PER >= p.D) kst[u] = uint4_t{0, 0, 0, 0};
+        }
         wave_lds_sync();  // the previous tile's reads precede these writes
 #pragma unroll
         for (int u = 0; u < LOADS; u++) {
             const int piece = lane + 64 * u;
-            if (there(piece)) *CR_LDS(uint4_t, k_tile + piece / CPR * C::KP + piece % CPR * 16) = kst[u];
+            *CR_LDS(uint4_t, k_tile + piece / CPR * C::KP + piece % CPR * 16) = kst[u];
             *CR_LDS(uint4_t, v_tile + piece / CPR * C::VP + piece % CPR * 16) = vst[u];
         }
         wave_lds_sync();
