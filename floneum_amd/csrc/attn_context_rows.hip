@@ -101,8 +101,7 @@ struct RowsWork {
     bool prefix;
     int b, g;         // b < 0: columns of all sequences
     int c0, columns;  // first column, columns in use
-    int slot, split, chunk;
-    bool last;        // share: takes all keys that are left
+    int slot, split, nsplit, chunk;
 };
 __device__ __forceinline__ RowsWork rows_work(const ContextParams &p, const ContextRows &rows) {
     const bool second = (int)blockIdx.x >= rows.second;
@@ -116,8 +115,7 @@ __device__ __forceinline__ RowsWork rows_work(const ContextParams &p, const Cont
     // (where sequences are short only the first shares have keys: they are spread over the XCDs as well)
     r.split = nsplit == 1 ? 0 : (int)((share - unit * nsplit + unit) % nsplit);
     r.slot = job.slot0 + r.split;
-    r.chunk = job.chunk;
-    r.last = r.split + 1 == job.nsplit;
+    r.nsplit = job.nsplit, r.chunk = job.chunk;
     r.prefix = job.prefix;
     const uint32_t b = unit / (uint32_t)p.Hkv;
     r.g = (int)(unit - b * p.Hkv);
@@ -447,7 +445,13 @@ __global__ __launch_bounds__(64 * CR_WAVES, DP > 128 && sizeof(T) == 4 ? 1 : 2) 
             }
         }
     }
-    const int first = span.first, gap = span.gap(), v_lo = w.split * w.chunk, v_hi = w.last ? span.keys() : min(v_lo + w.chunk, span.keys());
+    // Shares of `chunk` keys, or where these do not hold all of them of the length that does, in whole steps.  (In 32 bits without a sign: the last share may begin
+    // behind 2^31 keys.)
+    const int first = span.first, gap = span.gap();
+    const uint32_t keys = (uint32_t)span.keys();
+    uint32_t chunk = (uint32_t)w.chunk;
+    if (keys > chunk * (uint32_t)w.nsplit) chunk = ((keys + w.nsplit - 1) / w.nsplit + STEP - 1) / STEP * STEP;
+    const int v_lo = (int)min(w.split * chunk, keys), v_hi = (int)min(w.split * chunk + chunk, keys);
     if (v_lo >= v_hi && p.slots > 1) {
         park_nothing(p, w);
         return;

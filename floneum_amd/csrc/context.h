@@ -36,7 +36,7 @@ struct ContextRowsJob {
     int32_t prefix;  // else the sequences' own keys
     int32_t units;   // KV heads, times the batch for own keys
     int32_t blocks;  // column blocks of a unit
-    int32_t nsplit, chunk;  // shares of the visible keys, `chunk` keys each
+    int32_t nsplit, chunk;  // shares of the visible keys, `chunk` keys each (more where that is too little for all)
     int32_t slot0;
 };
 struct ContextRows {
