@@ -11,8 +11,13 @@ namespace fhip {
 
 bool context_tiles_takes(const ContextParams &p, fhip_dtype dtype) {
     if (dtype == FHIP_F32 || !context_rows_takes(p, dtype)) return false;
-    // (in bf16 Q takes the power of two of the scale: up to 1, and above head_dim 128 not so small that elements leave the normal range)
-    if (!(p.scale > 0.0f && p.scale * PF_LOG2E < 2.0f) || (p.D > 128 && p.scale * PF_LOG2E < 0.00390625f)) return false;
+    // In bf16 at the kernels' own widths Q takes the power of two of the factor of the scores: up to 1, so that no element leaves the type's range above, and not so small
+    // that elements in use leave the normal range below.  Elsewhere the factor multiplies f32 sums of products, which f16 elements leave below 2^40.  (8192 f16 rows of
+    // 32/8 heads at 128 under a window of 4096: 0.40 ms here, 1.3 in the kernel for few rows.)
+    const float factor = p.scale * PF_LOG2E;
+    const bool in_q = dtype == FHIP_BF16 && (p.D > 128 || p.D == 64 || p.D == 96 || p.D == 128);
+    if (!(p.scale > 0.0f && factor < (in_q ? 2.0f : 0x1p64f))) return false;
+    if (in_q && factor < (p.D > 128 ? 0x1p-8f : 0x1p-64f)) return false;
     // queries are read in pieces of 16 bytes
     if ((uintptr_t)p.q % 16 != 0 || p.qs[3] != 1) return false;
     for (int i = 0; i < 3; i++)

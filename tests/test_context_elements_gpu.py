@@ -28,3 +28,12 @@ def test_infinite_keys_at_padded_head_dims(device, dtype, D, window, sinks, Sq, 
     seen[:, :, [3, P + Skv - 2]] = False
     want, bound = definition(c.q, c.k, c.v, c.pk, c.pv, c.scale, seen, dtype, dtype)
     assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 72, 96, 128, 192, 256])
+@pytest.mark.parametrize("scale", [1e-44, 1e-39, 1e-30, 1e-15, 1e-4, 1.5, 40.0])
+@pytest.mark.parametrize("Sq", [2, 150])
+def test_any_scale(device, dtype, D, scale, Sq):
+    """Scales down to f32's smallest numbers (the weights are then all alike) and such as leave one key all of the weight."""
+    Call(device, dtype, 1, 4, 2, Sq, 200, 70, D, scale=scale, seed=D).both(offset=270 - Sq, window=190, sinks=3)

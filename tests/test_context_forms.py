@@ -33,3 +33,14 @@ def test_the_calls_reach_every_launch(calls, launches):
                 assert launch + part in reached, (launch, part)
             assert any(r.startswith(launch + "all prefix /; ") for r in reached), launch
     assert sum(" | " in form for *_, form in calls) >= 10
+
+
+@pytest.mark.parametrize("dtype", [fa.F16, fa.BF16])
+@pytest.mark.parametrize("D", [64, 72, 96, 104, 128])
+@pytest.mark.parametrize("scale", [1e-6, 0.1, 1.0, 1.5, 3.0, 1000.0])
+def test_scales_of_prompts(dtype, D, scale):
+    """Prompts of 16-bit tensors stay on the tiled kernel at every scale that it can form the scores with: all but, in bf16 at the widths of the kernel itself, such as
+    would raise elements of Q beyond the type."""
+    a = args(B=1, H=32, Hkv=8, Sq=8192, Skv=8192, D=D, dtype=dtype, out_dtype=dtype, window=4096, sinks=16, scale=scale)
+    raises = dtype == fa.BF16 and D in (64, 96, 128) and scale * 1.4426950408889634 >= 2.0
+    assert [bool(f.tiles) for f in forms(a)] == [not raises]
