@@ -19,6 +19,7 @@
 //   f32 columns              the matrix cores: 16 sequences on 4096 shared and 1500 own keys under a window 53 us
 //   one sequence             two launches that depend on each other, a chain of latencies each: 1028 visible f32 keys 6.9 and 3 us
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "context_device.h"
@@ -670,10 +671,10 @@ int launch_context_merge(const ContextParams &p, fhip_dtype dtype, hipStream_t s
 
 // ---- launch ---------------------------------------------------------------------------------------------------------------------------
 
-// Rows of keys and values are read in pieces of 16 bytes.
+// Rows of keys and values are read in pieces of 16 bytes; scores take one factor, scale times log2 e, which has to be a number.
 bool context_rows_takes(const ContextParams &p, fhip_dtype dtype) {
     const int per = dtype == FHIP_F32 ? 4 : 8;
-    if (p.D % 8 != 0 || p.D > 256) return false;
+    if (p.D % 8 != 0 || p.D > 256 || !std::isfinite(p.scale * CONTEXT_LOG2E)) return false;
     auto pieces = [&](const void *at, const int64_t *strides, int n) {
         if ((uintptr_t)at % 16 != 0 || strides[n - 1] != 1) return false;
         for (int i = 0; i + 1 < n; i++)

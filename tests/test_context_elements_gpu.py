@@ -37,3 +37,15 @@ def test_infinite_keys_at_padded_head_dims(device, dtype, D, window, sinks, Sq, 
 def test_any_scale(device, dtype, D, scale, Sq):
     """Scales down to f32's smallest numbers (the weights are then all alike) and such as leave one key all of the weight."""
     Call(device, dtype, 1, 4, 2, Sq, 200, 70, D, scale=scale, seed=D).both(offset=270 - Sq, window=190, sinks=3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 136])
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38])
+@pytest.mark.parametrize("Sq", [2, 150])
+def test_scales_at_the_end_of_f32(device, dtype, D, scale, Sq):
+    """Scales whose product with log2 e is beyond f32, on queries and keys small enough for it (in f16, which has no such elements, on queries of nothing)."""
+    c = Call(device, dtype, 1, 4, 2, Sq, 200, 70, D, scale=scale, std=3e-19 if dtype != fa.F16 else 1.0, lean=0.0, seed=D)
+    if dtype == fa.F16:
+        c.q[:] = 0.0
+    c.both(offset=270 - Sq, window=190, sinks=3)
