@@ -1131,14 +1131,29 @@ def _q8_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, out_dtyp
     return out
 
 
+def _int64(x, name):
+    # (a ctypes field would take the low 64 bits of any number)
+    try:
+        n = int(x)
+    except (TypeError, ValueError, OverflowError):
+        n = None
+    if n is None or n != x:
+        raise InvalidArgument(ERR_INVALID_ARG, f"{name} is not a whole number")
+    if not -1 << 63 <= n < 1 << 63:
+        raise InvalidArgument(ERR_INVALID_ARG, f"{name} does not fit 64 bits")
+    return n
+
+
 def _context_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, sinks, prefix, out_dtype, force_kernel, out):
-    if type(k) is Q8Tensor or type(v) is Q8Tensor:
+    if prefix is not None and not (isinstance(prefix, (tuple, list)) and len(prefix) == 2):
+        raise InvalidArgument(ERR_INVALID_ARG, "a prefix is a pair of keys and values")
+    pk, pv = (None, None) if prefix is None else prefix
+    if type(k) is Q8Tensor or type(v) is Q8Tensor or type(pk) is Q8Tensor or type(pv) is Q8Tensor:
         raise InvalidArgument(ERR_INVALID_ARG, "sinks and prefix are for keys and values of q's type")
     if mask is not None:
         raise InvalidArgument(ERR_INVALID_ARG, "sinks and prefix go with the analytic mask, not with a mask tensor")
     if force_kernel != KERNEL_AUTO:
         raise InvalidArgument(ERR_INVALID_ARG, "force_kernel does not apply to sinks and prefix")
-    pk, pv = (None, None) if prefix is None else prefix
     inputs = [k, v] if prefix is None else [k, v, pk, pv]
     dev = q.device
     if not all(t.device is dev for t in inputs):
@@ -1172,8 +1187,8 @@ def _context_attention(q, k, v, scale, mask, analytic, kv_lens, q_positions, sin
             a.causal, a.q_pos_offset, a.window = analytic.causal, analytic.q_pos_offset, analytic.window
     elif analytic is not None:
         causal, off, window = analytic
-        a.causal, a.q_pos_offset, a.window = 1 if causal else 0, int(off), int(window or 0)
-    a.sinks = 0 if sinks is None else int(sinks)
+        a.causal, a.q_pos_offset, a.window = 1 if causal else 0, _int64(off, "q_pos_offset"), _int64(window or 0, "window")
+    a.sinks = 0 if sinks is None else _int64(sinks, "sinks")
     a.kv_lens, a.q_positions = lens_ptr, positions_ptr
     need = ctypes.c_size_t()
     check(lib().fhip_context_attention_workspace_bytes(ctypes.byref(a), dev.compute_units, ctypes.byref(need)))
