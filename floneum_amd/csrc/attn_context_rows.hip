@@ -340,14 +340,19 @@ struct Columns<float, DP, 1> {
     }
     __device__ __forceinline__ void step(lds_t k, lds_t v, int base, int end, int first, int gap, bool whole, float scale2, int lane) {
         const int j = lane & 15, q4 = lane >> 4;
-        float4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+        // (in four sums: a single one would add up four times the roundings)
+        float4_t sums[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) sums[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             const float4_t a = *CR_LDS(float4_t, k + j * KP + (16 * c + 4 * q4) * 4);
 #pragma unroll
-            for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], q[c][i], s, 0, 0, 0);
+            for (int i = 0; i < 4; i++) sums[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], q[c][i], sums[i], 0, 0, 0);
         }
+        const float4_t s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
         float x[4];
+        bool hidden[4] = {false, false, false, false};
         uint32_t used = 0;
         // element r is visible key base + 4 q4 + r
 #pragma unroll
@@ -358,6 +363,7 @@ struct Columns<float, DP, 1> {
                 const int n = base + 4 * q4 + r, key = n + (n >= first ? gap : 0);
                 const bool sees = n < end && key < seen[0].hi && (key >= seen[0].lo || key < seen[0].first);
                 x[r] = sees ? x[r] : -INFINITY;
+                hidden[r] = !sees;
                 used |= sees ? 1u << r : 0u;
             }
         }
@@ -375,7 +381,9 @@ struct Columns<float, DP, 1> {
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            x[r] = __builtin_amdgcn_exp2f(x[r] - reference);
+            // (one rounding, at the size of the difference; a hidden key's stays -infinity)
+            const float d = __builtin_fmaf(s[r], scale2, -reference);
+            x[r] = __builtin_amdgcn_exp2f(hidden[r] ? -INFINITY : d);
             sum += x[r];
         }
         l += sum;
