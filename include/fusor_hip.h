@@ -605,7 +605,7 @@ int fhip_context_attention_validate(const fhip_context_attn_args *args);
 int fhip_context_attention_workspace_bytes(const fhip_context_attn_args *args, int32_t compute_units, size_t *bytes);
 /* out = softmax(q k^T * scale over the visible keys) v, with the head mapping, accumulation and special cases of fhip_flash_attention: rows that
  * see no key come out NaN, no keys at all (P + Skv == 0) give zeros.  Of 16-bit tensors the weights are rounded to their type for the product with the
- * values; scores, maxima and sums are f32's, and so is all of it for f32 tensors.  Rows of k, v and the prefix that no query row of the call sees may hold
+ * values, the rest is f32; f32 tensors are computed in f32 precision throughout.  Rows of k, v and the prefix that no query row of the call sees may hold
  * anything.  Asynchronous on `s`; may be captured.  Calls that share a workspace must not overlap. */
 int fhip_context_attention(fhip_stream *s, const fhip_context_attn_args *args);
 
