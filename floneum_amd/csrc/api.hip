@@ -232,8 +232,9 @@ static bool prefill_mfma_eligible(const fhip_attn_args *a) {
     if (!rows_vectorizable(a->q, 2) || !rows_vectorizable(a->k, 2) || !rows_vectorizable(a->v, 2)) return false;
     // in bf16 that kernel multiplies Q by the power-of-two part of scale * log2(e): the power must be at most 1 so that no
     // finite element can leave the type's range (f16 and the padded head dims are scaled in f32 only, and so is the wide-head
-    // kernel; f16 keeps the same limit)
+    // kernel; f16 keeps the same limit), and a power at all, which a subnormal number's exponent bits do not give
     if (exact && (!(a->scale > 0.0f) || !(a->scale * 1.4426950408889634f < 2.0f))) return false;
+    if (exact && a->dtype == FHIP_BF16 && a->scale * 1.4426950408889634f < 0x1p-126f) return false;
     // K/V rows are fetched through 32-bit buffer offsets: rows must not overlap and one (batch, kv
     // head) slice must span less than 2 GiB
     const uint64_t Skv = a->k.shape[2];
