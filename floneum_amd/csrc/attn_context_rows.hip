@@ -14,10 +14,11 @@
 //
 // Bound, and measured with inputs larger than the caches:
 //   many keys of their own   memory: 64 sequences of 4096 f16 keys of 32/8 heads at 128 stream 6.3 TB/s, 16 ragged ones 5.2, every byte once
-//   a prefix                 the caches, which hand out 10 to 11 TB/s: 32 sequences on 8192 shared and up to 1024 own keys 31.6 us, of which memory reads
-//                            107 MB, each byte once, and the column blocks 205 (fewer instructions per step change nothing)
-//   f32 columns              the matrix cores: 16 sequences on 4096 shared and 1500 own keys under a window 53 us
-//   one sequence             two launches that depend on each other, a chain of latencies each: 1028 visible f32 keys 6.9 and 3 us
+//   a prefix                 the caches: 32 sequences on 8192 shared and up to 1024 own keys 31.6 us; memory reads 109 MB, each byte once, the column blocks take in 205:
+//                            7.5 TB/s over the launch's 27.5 us, 10 while its one round of workgroups is whole (they live three quarters of it in the mean)
+//   f32 columns              16 sequences on 4096 shared and 1500 own keys under a window 53 us: two rounds of workgroups, about 700 with keys on 512 places.  The
+//                            matrix instructions hold a SIMD for 13 us of it, vector ones for 8; a wavefront waits 42 % of its time to issue and 31 % for memory and LDS
+//   one sequence             two launches that depend on each other, a chain of latencies each: 1028 visible f32 keys 7.0 and 3.2 us
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -93,7 +93,7 @@ static RowsPlan rows_launch_of(const ContextParams &p, fhip_dtype dtype, bool wi
 }
 
 // 32 columns halve what is taken in for a unit with so many, but the other part's few columns pay for them too: 32 sequences on 8192 keys at head_dim 128
-// take 26.2 us with 32 and 37.5 with 16, on 512 keys 18.0 and 14.9.  f32 tensors, which the matrix cores bound, take 16 (60 of 60 calls, up to a third).
+// take 26.2 us with 32 and 37.5 with 16, on 512 keys 18.0 and 14.9.  f32 tensors take 16 (faster in 60 of 60 calls, by up to a third).
 static RowsPlan rows_launch(const ContextParams &p, fhip_dtype dtype, bool with_prefix, int64_t slots_before) {
     const RowsPlan one = rows_launch_of(p, dtype, with_prefix, slots_before, 16);
     if ((int64_t)p.G * p.Sq * (with_prefix ? p.B : 1) <= 16 || p.D > 128 || dtype == FHIP_F32) return one;
