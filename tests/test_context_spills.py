@@ -1,5 +1,4 @@
-"""Registers that the tiled kernels of attention over a context in two parts spill (host only): to memory at most what their design notes say, and none in 16 bits to
-head_dim 128."""
+"""Registers that the tiled kernels of attention over a context in two parts spill (host only): to memory at most 16 in f32 and two above head_dim 128 in 16 bits, none below."""
 from test_kernel_registers import kernels  # noqa: F401
 
 
